@@ -1,0 +1,261 @@
+// Layer norm over the last axis, forward and backward, alone or behind the residual add in front of it (gfx950).
+//
+//   s = x + residual, rounded to the tensors' type (or s = x);   xhat = (s - mean(s)) / sqrt(var(s) + eps);   y = xhat * weight + bias
+//   dx = rstd (g - mean(g) - xhat mean(g xhat)) + ds,  g = dy * weight;   dweight = sum over rows of dy * xhat,  dbias = sum over rows of dy
+//
+// The norm is of the sum as it is stored: what the block goes on with, and what the backward pass reads.  Everything between a load and a
+// store is fp32: statistics, xhat, the sums over rows; results are rounded once.  The variance is the mean of the squared differences from
+// the mean, in a second run over registers, so rows far from zero lose nothing.
+//
+// A workgroup takes a row and runs over it three times (the second and third mostly from the caches); the weight's and bias' gradients are
+// added up by a thread a column, in a fixed order and without atomics, so that the same call gives the same bits.
+#pragma once
+#include "cascmm_common.h"
+
+namespace cascmm {
+
+struct NormParams {
+  const void* x;         // [rows][cols], row stride ldx (backward: the s that was normed)
+  const void* residual;  // forward: NULL or [rows][cols]
+  const void* weight;    // [cols] or NULL (ones)
+  const void* bias;      // [cols] or NULL (zeros)
+  void* y;               // forward: result; backward: dx
+  void* sum;             // forward with a residual: s
+  float* mean;           // [rows]; forward: written unless NULL; backward: read
+  float* rstd;
+  const void* dy;        // backward
+  const void* ds;        // backward: NULL or the gradient that reaches s past the norm
+  float* partials;       // backward: [workgroups][2][cols] sums for dweight, dbias; NULL: not wanted
+  int64_t rows, ldx, ldr, ldy, lds, lddy, ldds;
+  int cols, weight_f32;  // weight_f32: weight and bias are fp32 whatever the elements are
+  float eps, inv_cols;
+};
+
+// sum over the 64 lanes, in every lane: inside rows of sixteen by DPP moves, then the four rows in order
+template <int CTRL> __device__ __forceinline__ float norm_dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float norm_wave_sum(float v) {
+  v += norm_dpp<0xB1>(v);    // lane ^ 1
+  v += norm_dpp<0x4E>(v);    // lane ^ 2
+  v += norm_dpp<0x141>(v);   // the other four of eight
+  v += norm_dpp<0x140>(v);   // the other eight of sixteen
+  const int b = __builtin_bit_cast(int, v);
+  float s = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 0));
+  s += __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16));
+  s += __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 32));
+  s += __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48));
+  return s;
+}
+// N sums over the WPR waves of a workgroup.  `turn` counts the reductions: two sets of slots take turns, so one barrier each is enough
+// (a wave writes a set again only behind the barrier that all readers of it have passed).
+template <int WPR, int N> __device__ __forceinline__ void norm_sums(float (&v)[N], float* slots, int& turn) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = norm_wave_sum(v[i]);
+  if constexpr (WPR > 1) {
+    float* set = slots + (turn & 1) * (2 * WPR);
+    ++turn;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) set[i * WPR + (threadIdx.x >> 6)] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) s += set[i * WPR + w];
+      v[i] = s;
+    }
+  }
+}
+
+// 16 bytes of a row as fp32.  Rows start on element boundaries, not always on 16 bytes: the type says so to the compiler.
+template <int IODT> struct NormRow {
+  typedef typename IoType<IODT>::T E;
+  static constexpr int VEC = 16 / (int)sizeof(E);
+  typedef E chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
+  // chunk at column c of a row of `cols` (past the end: zeros)
+  static __device__ __forceinline__ chunk load(const E* row, int c, int cols) {
+    chunk v;
+    if (c + VEC <= cols) {
+      v = *(const chunk*)(row + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = c + e < cols ? row[c + e] : (E)0.f;
+    }
+    return v;
+  }
+  static __device__ __forceinline__ void store(E* row, int c, int cols, chunk v) {
+    if (c + VEC <= cols) {
+      *(chunk*)(row + c) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (c + e < cols) row[c + e] = v[e];
+    }
+  }
+  // a chunk of weight or bias
+  static __device__ __forceinline__ void load_weight(float (&w)[VEC], const void* p, int f32, int c, int cols, float otherwise) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) w[e] = otherwise;
+    if (!p) return;
+    if (f32 && sizeof(E) == 2) {
+      const float* q = (const float*)p;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = c + e < cols ? q[c + e] : 0.f;
+    } else {
+      const chunk v = load((const E*)p, c, cols);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = (float)v[e];
+    }
+  }
+};
+
+// A workgroup a row, three runs over it (the second and third mostly from the caches)
+constexpr int kNormWide = 1024;
+template <int IODT, bool ADD>
+__global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const NormParams p) {
+  typedef NormRow<IODT> R;
+  typedef typename R::E E;
+  typedef typename R::chunk chunk;
+  constexpr int VEC = R::VEC, WPR = kNormWide / 64, STEP = kNormWide * VEC;
+  __shared__ float slots[4 * WPR];
+  const int64_t row = blockIdx.x;
+  const int cols = p.cols, col0 = threadIdx.x * VEC;
+  const E* x = (const E*)p.x + row * p.ldx;
+  int turn = 0;
+  float total[1] = {0.f};
+  for (int64_t c = col0; c < cols; c += STEP) {
+    chunk v = R::load(x, (int)c, cols);
+    if constexpr (ADD) {
+      const chunk r = R::load((const E*)p.residual + row * p.ldr, (int)c, cols);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = (E)((float)v[e] + (float)r[e]);
+      R::store((E*)p.sum + row * p.lds, (int)c, cols, v);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) total[0] += (float)v[e];
+  }
+  // (a thread reads back what it has written itself)
+  const E* s = ADD ? (const E*)p.sum + row * p.lds : x;
+  norm_sums<WPR>(total, slots, turn);
+  const float mean = total[0] * p.inv_cols;
+  float square[1] = {0.f};
+  for (int64_t c = col0; c < cols; c += STEP) {
+    const chunk v = R::load(s, (int)c, cols);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = c + e < cols ? (float)v[e] - mean : 0.f;
+      square[0] = __builtin_fmaf(d, d, square[0]);
+    }
+  }
+  norm_sums<WPR>(square, slots, turn);
+  const float rstd = rsqrtf(square[0] * p.inv_cols + p.eps);
+  if (p.mean && threadIdx.x == 0) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+  for (int64_t c = col0; c < cols; c += STEP) {
+    const chunk v = R::load(s, (int)c, cols);
+    float w[VEC], b[VEC];
+    R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
+    R::load_weight(b, p.bias, p.weight_f32, (int)c, cols, 0.f);
+    chunk y;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) y[e] = (E)__builtin_fmaf(((float)v[e] - mean) * rstd, w[e], b[e]);
+    R::store((E*)p.y + row * p.ldy, (int)c, cols, y);
+  }
+}
+
+// Backward: dx with a workgroup a row ...
+template <int IODT>
+__global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_backward_wide_kernel(const NormParams p) {
+  typedef NormRow<IODT> R;
+  typedef typename R::E E;
+  typedef typename R::chunk chunk;
+  constexpr int VEC = R::VEC, WPR = kNormWide / 64, STEP = kNormWide * VEC;
+  __shared__ float slots[4 * WPR];
+  const int64_t row = blockIdx.x;
+  const int cols = p.cols, col0 = threadIdx.x * VEC;
+  const E *x = (const E*)p.x + row * p.ldx, *dy = (const E*)p.dy + row * p.lddy, *ds = p.ds ? (const E*)p.ds + row * p.ldds : nullptr;
+  const float mean = p.mean[row], rstd = p.rstd[row];
+  int turn = 0;
+  float sums[2] = {0.f, 0.f};
+  for (int64_t c = col0; c < cols; c += STEP) {
+    const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
+    float w[VEC];
+    R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float g = (float)d[e] * w[e];
+      sums[0] += g;
+      sums[1] = __builtin_fmaf(g, ((float)v[e] - mean) * rstd, sums[1]);
+    }
+  }
+  norm_sums<WPR>(sums, slots, turn);
+  const float c1 = sums[0] * p.inv_cols, c2 = sums[1] * p.inv_cols;
+  for (int64_t c = col0; c < cols; c += STEP) {
+    const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
+    float w[VEC];
+    R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
+    chunk z, out;
+    if (ds) z = R::load(ds, (int)c, cols);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float o = rstd * ((float)d[e] * w[e] - c1 - ((float)v[e] - mean) * rstd * c2);
+      if (ds) o += (float)z[e];
+      out[e] = (E)o;
+    }
+    R::store((E*)p.y + row * p.ldy, (int)c, cols, out);
+  }
+}
+// ... and the sums with a thread a column over every gridDim.y-th row
+template <int IODT>
+__global__ __launch_bounds__(256) void cascmm_layer_norm_sums_kernel(const NormParams p) {
+  typedef typename IoType<IODT>::T E;
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (col >= p.cols) return;
+  float dw = 0.f, db = 0.f;
+  for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
+    const float d = (float)((const E*)p.dy)[row * p.lddy + col];
+    dw = __builtin_fmaf(d, ((float)((const E*)p.x)[row * p.ldx + col] - p.mean[row]) * p.rstd[row], dw);
+    db += d;
+  }
+  float* part = p.partials + (int64_t)blockIdx.y * 2 * p.cols;
+  part[col] = dw;
+  part[p.cols + col] = db;
+}
+
+// out[col] (and out2[col], the second half of a partial row) = sum over `parts` rows of partials, [parts][halves][cols].  Thirty-two columns a
+// workgroup, its 32 rows of threads a share of the parts each; they meet in LDS in order.
+constexpr int kFinishCols = 32;
+template <int ODT>
+__global__ __launch_bounds__(1024) void cascmm_column_finish_kernel(const float* __restrict__ partials, int parts, int halves, int64_t cols, void* out, void* out2) {
+  typedef typename IoType<ODT>::T E;
+  __shared__ float meet[32][kFinishCols + 1];
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, half = blockIdx.y;
+  const int64_t col = (int64_t)blockIdx.x * kFinishCols + c;
+  float s = 0.f;
+  if (col < cols) {
+    const float* src = partials + (int64_t)half * cols + col;
+    const int64_t step = (int64_t)halves * cols;
+    int i = r;
+    for (; i + 96 < parts; i += 128) {   // (four loads in flight)
+      const float a0 = src[i * step], a1 = src[(i + 32) * step], a2 = src[(i + 64) * step], a3 = src[(i + 96) * step];
+      s += a0; s += a1; s += a2; s += a3;
+    }
+    for (; i < parts; i += 32) s += src[i * step];
+  }
+  meet[r][c] = s;
+  __syncthreads();
+  if (r == 0 && col < cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += meet[i][c];
+    E* dst = (E*)(half ? out2 : out);
+    if (dst) IoType<ODT>::store(dst + col, t);
+  }
+}
+
+}  // namespace cascmm

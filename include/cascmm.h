@@ -323,6 +323,30 @@ int cascmm_gemm_fp8_autoscale(const void* A, const void* B, int b_prepared, void
                               int terms, int products, const int32_t* b_exp, int32_t* exps_out,
                               int32_t* scratch, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Layer norm over the last axis of x [rows, cols] (leading dimension ldx; all leading dimensions in elements), what stands in front of
+ * every projection of a transformer block (diffusers' BasicTransformerBlock, part of the model that the reference wraps at
+ * basedxl/unet.py:65-87, runs it in torch):
+ *     s = x + residual, rounded to `dtype` (residual NULL: s = x);   y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias
+ * weight, bias: [cols] of weight_dtype (`dtype` or fp32), NULL: ones, zeros.  With a residual s is written to `sum` (both or neither).
+ * mean, rstd: fp32 [rows] for the backward pass, both or neither.  Statistics and everything between a load and a store are fp32, each
+ * result is rounded once.  Rows of any alignment of whole elements; y and sum overlap no operand.
+ */
+int cascmm_layer_norm(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* sum,
+                      float* mean, float* rstd, int64_t rows, int64_t cols, int64_t ldx, int64_t ldr, int64_t ldy,
+                      int64_t lds, float eps, int dtype, int weight_dtype, void* stream);
+/* Its gradients, from the gradient dy of y and, optionally (NULL), the gradient ds that reaches s past the norm; x is what was normed (the
+ * sum, with a residual):  with xhat = (x - mean) rstd and g = dy * weight
+ *     dx = rstd (g - mean(g) - xhat mean(g xhat)) + ds;   dweight = sum over rows of dy xhat;   dbias = sum over rows of dy
+ * dx (of `dtype`; it is the residual's gradient too), dweight and dbias (of weight_dtype) may each be NULL.  For dweight or dbias the
+ * workspace holds cascmm_layer_norm_workspace_bytes(rows, cols) bytes (16-byte aligned, contents need no initialisation).  Sums over rows
+ * are fp32 in a fixed order, without atomics. */
+size_t cascmm_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
+int cascmm_layer_norm_backward(const void* dy, const void* ds, const void* x, const void* weight, const float* mean,
+                               const float* rstd, void* dx, void* dweight, void* dbias, int64_t rows, int64_t cols,
+                               int64_t lddy, int64_t ldds, int64_t ldx, int64_t lddx, int dtype, int weight_dtype,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
 /* The operand split alone (a test hook for parity of the split with the CPU oracle):
  * out is fp32 [terms][n]; term i holds lowp(r_i * 2^(tensor_exp + shift*i)) upcast to fp32
  * with r_0 = x, r_{i+1} = r_i - t_i / 2^(tensor_exp + shift*i); shift = 0 / 11 / 4 for
