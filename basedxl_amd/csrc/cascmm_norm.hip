@@ -12,8 +12,26 @@ static size_t norm_size(int dtype) { return dtype == CASCMM_DT_F32 ? 4 : 2; }
 static bool norm_dtype(int dtype) { return dtype == CASCMM_DT_F32 || dtype == CASCMM_DT_F16 || dtype == CASCMM_DT_BF16; }
 constexpr int64_t kNormMostCols = 1 << 30;   // (column numbers and a step beyond the last are 32-bit)
 
-// workgroups (rows of partial sums) of the backward pass
-static int64_t norm_parts(int64_t rows, int64_t) { return std::max<int64_t>(1, std::min<int64_t>((rows + 15) / 16, 512)); }
+// The waves of a row and the elements of a lane: a wave takes rows of up to 2048 columns (in the backward pass, which holds the sums beside a
+// row, 1536), four of them up to 8192; none: longer rows
+struct NormShape { int waves, values; };
+static NormShape norm_shape(int64_t cols, bool backward) {
+  const int most = backward ? 24 : 32;
+  const int one = (int)std::min<int64_t>((cols + 511) / 512 * 8, 1 << 20), four = (int)std::min<int64_t>((cols + 2047) / 2048 * 8, 1 << 20);
+  if (one <= most) return {1, one};
+  if (four <= 32) return {4, four};
+  return {0, 0};
+}
+// workgroups that walk over the rows
+constexpr int kNormForwardGroups = 1024, kNormBackwardGroups = 512;
+static int64_t norm_groups(int64_t rows, int waves, int64_t most) {
+  return std::max<int64_t>(1, std::min<int64_t>(waves == 1 ? (rows + 3) / 4 : rows, most));
+}
+// rows of partial sums of the backward pass
+static int64_t norm_parts(int64_t rows, int64_t cols) {
+  const NormShape f = norm_shape(cols, true);
+  return f.waves ? norm_groups(rows, f.waves, kNormBackwardGroups) : std::max<int64_t>(1, std::min<int64_t>((rows + 15) / 16, 512));
+}
 
 static int norm_check(int64_t rows, int64_t cols, int dtype, int weight_dtype) {
   if (!norm_dtype(dtype) || (weight_dtype != dtype && weight_dtype != CASCMM_DT_F32)) return CASCMM_ERR_BAD_DTYPE;
@@ -22,19 +40,57 @@ static int norm_check(int64_t rows, int64_t cols, int dtype, int weight_dtype) {
   return CASCMM_OK;
 }
 
-template <int IODT> static hipError_t norm_forward(const NormParams& p, hipStream_t s) {
+template <int IODT, bool ADD> static hipError_t norm_forward(const NormParams& p, hipStream_t s) {
   hipError_t err = hipSuccess;
-  if (p.residual) CASCMM_LAUNCH(err, (cascmm_layer_norm_wide_kernel<IODT, true>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
-  else CASCMM_LAUNCH(err, (cascmm_layer_norm_wide_kernel<IODT, false>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
+  const NormShape f = norm_shape(p.cols, false);
+  const dim3 grid((unsigned)norm_groups(p.rows, f.waves, kNormForwardGroups));
+#define NORM_CASE(W, NV) \
+  case (W) * 100 + (NV): CASCMM_LAUNCH(err, (cascmm_layer_norm_kernel<IODT, NV, W, ADD>), grid, dim3(256), 0, s, p); break
+  switch (f.waves * 100 + f.values) {
+    NORM_CASE(1, 8);
+    NORM_CASE(1, 16);
+    NORM_CASE(1, 24);
+    NORM_CASE(1, 32);
+    NORM_CASE(4, 16);
+    NORM_CASE(4, 24);
+    NORM_CASE(4, 32);
+    default: CASCMM_LAUNCH(err, (cascmm_layer_norm_wide_kernel<IODT, ADD>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
+  }
+#undef NORM_CASE
+  return err;
+}
+
+template <int IODT, bool DS, bool SUMS> static hipError_t norm_backward_rows(const NormParams& p, hipStream_t s) {
+  hipError_t err = hipSuccess;
+  const NormShape f = norm_shape(p.cols, true);
+  const dim3 grid((unsigned)norm_groups(p.rows, f.waves, kNormBackwardGroups));
+#define NORM_CASE(W, NV) \
+  case (W) * 100 + (NV): CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_kernel<IODT, NV, W, DS, SUMS>), grid, dim3(256), 0, s, p); break
+  switch (f.waves * 100 + f.values) {
+    NORM_CASE(1, 8);
+    NORM_CASE(1, 16);
+    NORM_CASE(1, 24);
+    NORM_CASE(4, 8);
+    NORM_CASE(4, 16);
+    NORM_CASE(4, 24);
+    NORM_CASE(4, 32);
+    default: return hipErrorInvalidValue;
+  }
+#undef NORM_CASE
   return err;
 }
 
 template <int IODT> static hipError_t norm_backward(const NormParams& p, void* dweight, void* dbias, int weight_dtype, hipStream_t s) {
   hipError_t err = hipSuccess;
-  if (p.y && p.rows > 0) CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_wide_kernel<IODT>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
-  if (!p.partials) return err;
   const int parts = (int)norm_parts(p.rows, p.cols);
-  CASCMM_LAUNCH(err, (cascmm_layer_norm_sums_kernel<IODT>), dim3((unsigned)((p.cols + 255) / 256), (unsigned)parts), dim3(256), 0, s, p);
+  // (no dx wanted: nothing but the sums.  No rows: sums of zeros)
+  const bool rows = p.y && p.rows > 0, wide = norm_shape(p.cols, true).waves == 0;
+  if (rows && wide) CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_wide_kernel<IODT>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
+  else if (rows && p.partials) err = p.ds ? norm_backward_rows<IODT, true, true>(p, s) : norm_backward_rows<IODT, false, true>(p, s);
+  else if (rows) err = p.ds ? norm_backward_rows<IODT, true, false>(p, s) : norm_backward_rows<IODT, false, false>(p, s);
+  if (!p.partials) return err;
+  if (!rows || wide)
+    CASCMM_LAUNCH(err, (cascmm_layer_norm_sums_kernel<IODT>), dim3((unsigned)((p.cols + 255) / 256), (unsigned)parts), dim3(256), 0, s, p);
   const dim3 grid((unsigned)((p.cols + kFinishCols - 1) / kFinishCols), 2);
   if (weight_dtype == CASCMM_DT_F32)
     CASCMM_LAUNCH(err, (cascmm_column_finish_kernel<CASCMM_DT_F32>), grid, dim3(1024), 0, s, (const float*)p.partials, parts, 2, (int64_t)p.cols, dweight, dbias);
@@ -68,9 +124,9 @@ int cascmm_layer_norm(const void* x, const void* residual, const void* weight, c
   p.eps = eps;
   p.inv_cols = 1.0f / (float)cols;
   const hipStream_t s = (hipStream_t)stream;
-  const hipError_t err = dtype == CASCMM_DT_F32   ? norm_forward<CASCMM_DT_F32>(p, s)
-                         : dtype == CASCMM_DT_F16 ? norm_forward<CASCMM_DT_F16>(p, s)
-                                                  : norm_forward<CASCMM_DT_BF16>(p, s);
+  const hipError_t err = dtype == CASCMM_DT_F32   ? (residual ? norm_forward<CASCMM_DT_F32, true>(p, s) : norm_forward<CASCMM_DT_F32, false>(p, s))
+                         : dtype == CASCMM_DT_F16 ? (residual ? norm_forward<CASCMM_DT_F16, true>(p, s) : norm_forward<CASCMM_DT_F16, false>(p, s))
+                                                  : (residual ? norm_forward<CASCMM_DT_BF16, true>(p, s) : norm_forward<CASCMM_DT_BF16, false>(p, s));
   return err == hipSuccess ? CASCMM_OK : CASCMM_ERR_LAUNCH;
 }
 

@@ -7,8 +7,11 @@
 // store is fp32: statistics, xhat, the sums over rows; results are rounded once.  The variance is the mean of the squared differences from
 // the mean, in a second run over registers, so rows far from zero lose nothing.
 //
-// A workgroup takes a row and runs over it three times (the second and third mostly from the caches); the weight's and bias' gradients are
-// added up by a thread a column, in a fixed order and without atomics, so that the same call gives the same bits.
+// Bound by memory.  A row lies in the registers of one wave (of four where it is longer), so every element is read once: a lane holds
+// chunks of 16 bytes, 64 (256) of them side by side.  A wave keeps weight and bias in registers and walks over rows a grid apart, the
+// next row's loads in flight while this one is reduced.  The backward pass adds the weight's and bias' gradients up in registers on its
+// way, the waves of a workgroup meet in LDS, and a second kernel adds the workgroups' sums: in a fixed order, without atomics, so that
+// the same call gives the same bits.
 #pragma once
 #include "cascmm_common.h"
 
@@ -112,7 +115,83 @@ template <int IODT> struct NormRow {
   }
 };
 
-// A workgroup a row, three runs over it (the second and third mostly from the caches)
+// rows of up to 64 WPR NV columns, NV a multiple of 8: NV elements a lane
+template <int IODT, int NV, int WPR, bool ADD>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void cascmm_layer_norm_kernel(const NormParams p) {
+  typedef NormRow<IODT> R;
+  typedef typename R::E E;
+  typedef typename R::chunk chunk;
+  constexpr int VEC = R::VEC, CH = NV / VEC, STEP = 64 * WPR * VEC;
+  __shared__ float slots[4 * WPR];
+  const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const int cols = p.cols, col0 = lane * VEC;
+  const int64_t waves = (int64_t)gridDim.x * (WPR == 1 ? 4 : 1);
+  int64_t row = (int64_t)blockIdx.x * (WPR == 1 ? 4 : 1) + (WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  int turn = 0;
+  if (row >= p.rows) return;   // (a whole wave; of several, a whole workgroup)
+  chunk x[CH], r[ADD ? CH : 1];
+  auto fetch = [&](int64_t at) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      x[c] = R::load((const E*)p.x + at * p.ldx, col0 + c * STEP, cols);
+      if constexpr (ADD) r[c] = R::load((const E*)p.residual + at * p.ldr, col0 + c * STEP, cols);
+    }
+  };
+  fetch(row);
+  float w[CH][VEC], b[CH][VEC];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    R::load_weight(w[c], p.weight, p.weight_f32, col0 + c * STEP, cols, 1.f);
+    R::load_weight(b[c], p.bias, p.weight_f32, col0 + c * STEP, cols, 0.f);
+  }
+  for (;;) {
+    float v[CH][VEC], total[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if constexpr (ADD) {
+        chunk s;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] = (E)((float)x[c][e] + (float)r[c][e]);
+        R::store((E*)p.sum + row * p.lds, col0 + c * STEP, cols, s);
+        x[c] = s;
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[c][e] = (float)x[c][e];
+        total[0] += v[c][e];
+      }
+    }
+    const int64_t next = row + waves;
+    if (next < p.rows) fetch(next);
+    norm_sums<WPR>(total, slots, turn);
+    const float mean = total[0] / (float)p.cols;
+    float square[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[c][e] = col0 + c * STEP + e < cols ? v[c][e] - mean : 0.f;
+        square[0] = __builtin_fmaf(v[c][e], v[c][e], square[0]);
+      }
+    norm_sums<WPR>(square, slots, turn);
+    const float rstd = rsqrtf(square[0] * p.inv_cols + p.eps);
+    if (p.mean && lane == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      chunk y;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y[e] = (E)__builtin_fmaf(v[c][e] * rstd, w[c][e], b[c][e]);
+      R::store((E*)p.y + row * p.ldy, col0 + c * STEP, cols, y);
+    }
+    if (next >= p.rows) return;
+    row = next;
+  }
+}
+
+// longer rows: a workgroup a row, three runs over it (the second and third mostly from the caches)
 constexpr int kNormWide = 1024;
 template <int IODT, bool ADD>
 __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const NormParams p) {
@@ -140,7 +219,7 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
   // (a thread reads back what it has written itself)
   const E* s = ADD ? (const E*)p.sum + row * p.lds : x;
   norm_sums<WPR>(total, slots, turn);
-  const float mean = total[0] * p.inv_cols;
+  const float mean = total[0] / (float)p.cols;
   float square[1] = {0.f};
   for (int64_t c = col0; c < cols; c += STEP) {
     const chunk v = R::load(s, (int)c, cols);
@@ -168,7 +247,121 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
   }
 }
 
-// Backward: dx with a workgroup a row ...
+// Backward.  SUMS: the sums for dweight and dbias too, a workgroup's at partials[blockIdx.x].
+template <int IODT, int NV, int WPR, bool DS, bool SUMS>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void cascmm_layer_norm_backward_kernel(const NormParams p) {
+  typedef NormRow<IODT> R;
+  typedef typename R::E E;
+  typedef typename R::chunk chunk;
+  constexpr int VEC = R::VEC, CH = NV / VEC, STEP = 64 * WPR * VEC;
+  __shared__ float slots[4 * WPR];
+  const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const int wave = WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int cols = p.cols, col0 = lane * VEC;
+  const int64_t waves = (int64_t)gridDim.x * (WPR == 1 ? 4 : 1);
+  int64_t row = (int64_t)blockIdx.x * (WPR == 1 ? 4 : 1) + wave;
+  int turn = 0;
+  chunk x[CH], dy[CH], ds[DS ? CH : 1];
+  float mean = 0.f, rstd = 0.f;
+  auto fetch = [&](int64_t at) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      x[c] = R::load((const E*)p.x + at * p.ldx, col0 + c * STEP, cols);
+      dy[c] = R::load((const E*)p.dy + at * p.lddy, col0 + c * STEP, cols);
+      if constexpr (DS) ds[c] = R::load((const E*)p.ds + at * p.ldds, col0 + c * STEP, cols);
+    }
+    mean = p.mean[at];
+    rstd = p.rstd[at];
+  };
+  float w[CH][VEC], dw[SUMS ? CH : 1][VEC], db[SUMS ? CH : 1][VEC];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    R::load_weight(w[c], p.weight, p.weight_f32, col0 + c * STEP, cols, 1.f);
+    if constexpr (SUMS) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) dw[c][e] = db[c][e] = 0.f;
+    }
+  }
+  if (row < p.rows) fetch(row);
+  while (row < p.rows) {
+    float xhat[CH][VEC], g[CH][VEC], sums[2] = {0.f, 0.f};
+    chunk keep[DS ? CH : 1];
+    const float rs = rstd;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        // (behind the last column x, dy and with it g are zeros, and xhat, which the mean is taken from, meets nothing but them)
+        xhat[c][e] = ((float)x[c][e] - mean) * rs;
+        const float d = (float)dy[c][e];
+        g[c][e] = d * w[c][e];
+        sums[0] += g[c][e];
+        sums[1] = __builtin_fmaf(g[c][e], xhat[c][e], sums[1]);
+        if constexpr (SUMS) {
+          dw[c][e] = __builtin_fmaf(d, xhat[c][e], dw[c][e]);
+          db[c][e] += d;
+        }
+      }
+      if constexpr (DS) keep[c] = ds[c];
+    }
+    const int64_t at = row;
+    row += waves;
+    if (row < p.rows) fetch(row);
+    norm_sums<WPR>(sums, slots, turn);
+    const float c1 = sums[0] * p.inv_cols, c2 = sums[1] * p.inv_cols;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      chunk out;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float d = rs * (g[c][e] - c1 - xhat[c][e] * c2);
+        if constexpr (DS) d += (float)keep[c][e];
+        out[e] = (E)d;
+      }
+      R::store((E*)p.y + at * p.ldy, col0 + c * STEP, cols, out);
+    }
+  }
+  if constexpr (SUMS) {
+    float* part = p.partials + (int64_t)blockIdx.x * 2 * cols;
+    if constexpr (WPR == 1) {
+      // the four waves one after the other, in LDS
+      __shared__ float meet[2][64 * NV];
+      for (int turn_of = 0; turn_of < 4; ++turn_of) {
+        if (wave == turn_of) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const int at = c * STEP + e * 64 + lane;   // (side by side over the lanes)
+              meet[0][at] = turn_of == 0 ? dw[c][e] : meet[0][at] + dw[c][e];
+              meet[1][at] = turn_of == 0 ? db[c][e] : meet[1][at] + db[c][e];
+            }
+        }
+        __syncthreads();
+      }
+      for (int i = threadIdx.x; i < 64 * NV; i += 256) {
+        const int col = i / STEP * STEP + (i % STEP % 64) * VEC + i % STEP / 64;
+        if (col < cols) {
+          part[col] = meet[0][i];
+          part[cols + col] = meet[1][i];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int col = col0 + c * STEP + e;
+          if (col < cols) {
+            part[col] = dw[c][e];
+            part[cols + col] = db[c][e];
+          }
+        }
+    }
+  }
+}
+
+// longer rows: dx with a workgroup a row ...
 template <int IODT>
 __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_backward_wide_kernel(const NormParams p) {
   typedef NormRow<IODT> R;
