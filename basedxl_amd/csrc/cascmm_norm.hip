@@ -12,25 +12,28 @@ static size_t norm_size(int dtype) { return dtype == CASCMM_DT_F32 ? 4 : 2; }
 static bool norm_dtype(int dtype) { return dtype == CASCMM_DT_F32 || dtype == CASCMM_DT_F16 || dtype == CASCMM_DT_BF16; }
 constexpr int64_t kNormMostCols = 1 << 30;   // (column numbers and a step beyond the last are 32-bit)
 
-// The waves of a row and the elements of a lane: a wave takes rows of up to 2048 columns (in the backward pass, which holds the sums beside a
-// row, 1536), four of them up to 8192; none: longer rows
-struct NormShape { int waves, values; };
+// The lanes of a row and the elements of a lane: eight lanes take rows of up to 64 columns, sixteen up to 256, a wave up to 2048 (in the backward pass, which
+// holds the sums beside a row, 1536), four of them up to 8192; none: longer rows
+struct NormShape { int lanes, values; };
 static NormShape norm_shape(int64_t cols, bool backward) {
-  const int most = backward ? 24 : 32;
-  const int one = (int)std::min<int64_t>((cols + 511) / 512 * 8, 1 << 20), four = (int)std::min<int64_t>((cols + 2047) / 2048 * 8, 1 << 20);
-  if (one <= most) return {1, one};
-  if (four <= 32) return {4, four};
+  const auto fit = [&](int lanes) { return (int)std::min<int64_t>((cols + 8 * lanes - 1) / (8 * lanes) * 8, 1 << 20); };
+  if (cols <= 64) return {8, 8};
+  if (fit(16) <= 16) return {16, fit(16)};
+  if (fit(64) <= (backward ? 24 : 32)) return {64, fit(64)};
+  if (fit(256) <= 32) return {256, fit(256)};
   return {0, 0};
 }
-// workgroups that walk over the rows
-constexpr int kNormForwardGroups = 1024, kNormBackwardGroups = 512;
-static int64_t norm_groups(int64_t rows, int waves, int64_t most) {
-  return std::max<int64_t>(1, std::min<int64_t>(waves == 1 ? (rows + 3) / 4 : rows, most));
+// Workgroups that walk over the rows: four on a CU forward and for short rows, backward else two, one where four waves hold a row (as many as their
+// registers leave room for; 65536 x 1280 bf16 backward 111 us, 768 workgroups 141, 1024 119), and backward two rows at least for each of a
+// workgroup's, since what a workgroup sums is written and read again.
+static int64_t norm_groups(int64_t rows, int lanes, bool backward) {
+  const int64_t at_a_time = 256 / lanes * (backward ? 2 : 1), most = backward ? (lanes == 256 ? 256 : lanes == 64 ? 512 : 1024) : 1024;
+  return std::max<int64_t>(1, std::min<int64_t>((rows + at_a_time - 1) / at_a_time, most));
 }
 // rows of partial sums of the backward pass
 static int64_t norm_parts(int64_t rows, int64_t cols) {
   const NormShape f = norm_shape(cols, true);
-  return f.waves ? norm_groups(rows, f.waves, kNormBackwardGroups) : std::max<int64_t>(1, std::min<int64_t>((rows + 15) / 16, 512));
+  return f.lanes ? norm_groups(rows, f.lanes, true) : std::max<int64_t>(1, std::min<int64_t>((rows + 15) / 16, 512));
 }
 
 static int norm_check(int64_t rows, int64_t cols, int dtype, int weight_dtype) {
@@ -43,17 +46,20 @@ static int norm_check(int64_t rows, int64_t cols, int dtype, int weight_dtype) {
 template <int IODT, bool ADD> static hipError_t norm_forward(const NormParams& p, hipStream_t s) {
   hipError_t err = hipSuccess;
   const NormShape f = norm_shape(p.cols, false);
-  const dim3 grid((unsigned)norm_groups(p.rows, f.waves, kNormForwardGroups));
-#define NORM_CASE(W, NV) \
-  case (W) * 100 + (NV): CASCMM_LAUNCH(err, (cascmm_layer_norm_kernel<IODT, NV, W, ADD>), grid, dim3(256), 0, s, p); break
-  switch (f.waves * 100 + f.values) {
-    NORM_CASE(1, 8);
-    NORM_CASE(1, 16);
-    NORM_CASE(1, 24);
-    NORM_CASE(1, 32);
-    NORM_CASE(4, 16);
-    NORM_CASE(4, 24);
-    NORM_CASE(4, 32);
+  const dim3 grid(f.lanes ? (unsigned)norm_groups(p.rows, f.lanes, false) : 1u);
+#define NORM_CASE(LPR, NV) \
+  case (LPR) * 100 + (NV): CASCMM_LAUNCH(err, (cascmm_layer_norm_kernel<IODT, NV, LPR, ADD>), grid, dim3(256), 0, s, p); break
+  switch (f.lanes * 100 + f.values) {
+    NORM_CASE(8, 8);
+    NORM_CASE(16, 8);
+    NORM_CASE(16, 16);
+    NORM_CASE(64, 8);
+    NORM_CASE(64, 16);
+    NORM_CASE(64, 24);
+    NORM_CASE(64, 32);
+    NORM_CASE(256, 16);
+    NORM_CASE(256, 24);
+    NORM_CASE(256, 32);
     default: CASCMM_LAUNCH(err, (cascmm_layer_norm_wide_kernel<IODT, ADD>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
   }
 #undef NORM_CASE
@@ -63,17 +69,20 @@ template <int IODT, bool ADD> static hipError_t norm_forward(const NormParams& p
 template <int IODT, bool DS, bool SUMS> static hipError_t norm_backward_rows(const NormParams& p, hipStream_t s) {
   hipError_t err = hipSuccess;
   const NormShape f = norm_shape(p.cols, true);
-  const dim3 grid((unsigned)norm_groups(p.rows, f.waves, kNormBackwardGroups));
-#define NORM_CASE(W, NV) \
-  case (W) * 100 + (NV): CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_kernel<IODT, NV, W, DS, SUMS>), grid, dim3(256), 0, s, p); break
-  switch (f.waves * 100 + f.values) {
-    NORM_CASE(1, 8);
-    NORM_CASE(1, 16);
-    NORM_CASE(1, 24);
-    NORM_CASE(4, 8);
-    NORM_CASE(4, 16);
-    NORM_CASE(4, 24);
-    NORM_CASE(4, 32);
+  const dim3 grid((unsigned)norm_groups(p.rows, f.lanes, true));
+#define NORM_CASE(LPR, NV) \
+  case (LPR) * 100 + (NV): CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_kernel<IODT, NV, LPR, DS, SUMS>), grid, dim3(256), 0, s, p); break
+  switch (f.lanes * 100 + f.values) {
+    NORM_CASE(8, 8);
+    NORM_CASE(16, 8);
+    NORM_CASE(16, 16);
+    NORM_CASE(64, 8);
+    NORM_CASE(64, 16);
+    NORM_CASE(64, 24);
+    NORM_CASE(256, 8);
+    NORM_CASE(256, 16);
+    NORM_CASE(256, 24);
+    NORM_CASE(256, 32);
     default: return hipErrorInvalidValue;
   }
 #undef NORM_CASE
@@ -84,7 +93,7 @@ template <int IODT> static hipError_t norm_backward(const NormParams& p, void* d
   hipError_t err = hipSuccess;
   const int parts = (int)norm_parts(p.rows, p.cols);
   // (no dx wanted: nothing but the sums.  No rows: sums of zeros)
-  const bool rows = p.y && p.rows > 0, wide = norm_shape(p.cols, true).waves == 0;
+  const bool rows = p.y && p.rows > 0, wide = norm_shape(p.cols, true).lanes == 0;
   if (rows && wide) CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_wide_kernel<IODT>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
   else if (rows && p.partials) err = p.ds ? norm_backward_rows<IODT, true, true>(p, s) : norm_backward_rows<IODT, false, true>(p, s);
   else if (rows) err = p.ds ? norm_backward_rows<IODT, true, false>(p, s) : norm_backward_rows<IODT, false, false>(p, s);

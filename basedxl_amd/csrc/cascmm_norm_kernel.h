@@ -50,12 +50,23 @@ __device__ __forceinline__ float norm_wave_sum(float v) {
   s += __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48));
   return s;
 }
-// N sums over the WPR waves of a workgroup.  `turn` counts the reductions: two sets of slots take turns, so one barrier each is enough
+// sum over eight or the sixteen lanes of a DPP row
+template <int LANES> __device__ __forceinline__ float norm_few_sum(float v) {
+  v += norm_dpp<0xB1>(v);
+  v += norm_dpp<0x4E>(v);
+  v += norm_dpp<0x141>(v);
+  return LANES == 8 ? v : v + norm_dpp<0x140>(v);
+}
+// N sums over the LPR lanes of a row: eight, sixteen, a wave or the waves of a workgroup.  `turn` counts the reductions: two sets of slots take turns, so one barrier each is enough
 // (a wave writes a set again only behind the barrier that all readers of it have passed).
-template <int WPR, int N> __device__ __forceinline__ void norm_sums(float (&v)[N], float* slots, int& turn) {
+template <int LPR, int N> __device__ __forceinline__ void norm_sums(float (&v)[N], float* slots, int& turn) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = norm_wave_sum(v[i]);
-  if constexpr (WPR > 1) {
+  for (int i = 0; i < N; ++i) {
+    if constexpr (LPR < 64) v[i] = norm_few_sum<LPR>(v[i]);
+    else v[i] = norm_wave_sum(v[i]);
+  }
+  if constexpr (LPR > 64) {
+    constexpr int WPR = LPR / 64;
     float* set = slots + (turn & 1) * (2 * WPR);
     ++turn;
     if ((threadIdx.x & 63) == 0) {
@@ -115,20 +126,20 @@ template <int IODT> struct NormRow {
   }
 };
 
-// rows of up to 64 WPR NV columns, NV a multiple of 8: NV elements a lane
-template <int IODT, int NV, int WPR, bool ADD>
-__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void cascmm_layer_norm_kernel(const NormParams p) {
+// Rows of up to LPR NV columns, NV a multiple of 8: LPR lanes a row (eight, sixteen, a wave, or all four waves of a workgroup), NV elements a lane.
+template <int IODT, int NV, int LPR, bool ADD>
+__global__ __launch_bounds__(256) void cascmm_layer_norm_kernel(const NormParams p) {
   typedef NormRow<IODT> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
-  constexpr int VEC = R::VEC, CH = NV / VEC, STEP = 64 * WPR * VEC;
-  __shared__ float slots[4 * WPR];
-  const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+  constexpr int VEC = R::VEC, CH = NV / VEC, STEP = LPR * VEC, ROWS = 256 / LPR;   // ROWS: of a workgroup at a time
+  __shared__ float slots[16];
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const int cols = p.cols, col0 = lane * VEC;
-  const int64_t waves = (int64_t)gridDim.x * (WPR == 1 ? 4 : 1);
-  int64_t row = (int64_t)blockIdx.x * (WPR == 1 ? 4 : 1) + (WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + (LPR == 64 ? __builtin_amdgcn_readfirstlane(group) : group);
   int turn = 0;
-  if (row >= p.rows) return;   // (a whole wave; of several, a whole workgroup)
+  if (row >= p.rows) return;   // (of a row's lanes all or none, so every barrier has its waves)
   chunk x[CH], r[ADD ? CH : 1];
   auto fetch = [&](int64_t at) {
 #pragma unroll
@@ -161,9 +172,9 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void cascmm_layer_norm_k
         total[0] += v[c][e];
       }
     }
-    const int64_t next = row + waves;
+    const int64_t next = row + stride;
     if (next < p.rows) fetch(next);
-    norm_sums<WPR>(total, slots, turn);
+    norm_sums<LPR>(total, slots, turn);
     const float mean = total[0] / (float)p.cols;
     float square[1] = {0.f};
 #pragma unroll
@@ -173,7 +184,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void cascmm_layer_norm_k
         v[c][e] = col0 + c * STEP + e < cols ? v[c][e] - mean : 0.f;
         square[0] = __builtin_fmaf(v[c][e], v[c][e], square[0]);
       }
-    norm_sums<WPR>(square, slots, turn);
+    norm_sums<LPR>(square, slots, turn);
     const float rstd = rsqrtf(square[0] * p.inv_cols + p.eps);
     if (p.mean && lane == 0) {
       p.mean[row] = mean;
@@ -198,8 +209,8 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
   typedef NormRow<IODT> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
-  constexpr int VEC = R::VEC, WPR = kNormWide / 64, STEP = kNormWide * VEC;
-  __shared__ float slots[4 * WPR];
+  constexpr int VEC = R::VEC, STEP = kNormWide * VEC;
+  __shared__ float slots[kNormWide / 16];
   const int64_t row = blockIdx.x;
   const int cols = p.cols, col0 = threadIdx.x * VEC;
   const E* x = (const E*)p.x + row * p.ldx;
@@ -218,7 +229,7 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
   }
   // (a thread reads back what it has written itself)
   const E* s = ADD ? (const E*)p.sum + row * p.lds : x;
-  norm_sums<WPR>(total, slots, turn);
+  norm_sums<kNormWide>(total, slots, turn);
   const float mean = total[0] / (float)p.cols;
   float square[1] = {0.f};
   for (int64_t c = col0; c < cols; c += STEP) {
@@ -229,7 +240,7 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
       square[0] = __builtin_fmaf(d, d, square[0]);
     }
   }
-  norm_sums<WPR>(square, slots, turn);
+  norm_sums<kNormWide>(square, slots, turn);
   const float rstd = rsqrtf(square[0] * p.inv_cols + p.eps);
   if (p.mean && threadIdx.x == 0) {
     p.mean[row] = mean;
@@ -248,30 +259,31 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
 }
 
 // Backward.  SUMS: the sums for dweight and dbias too, a workgroup's at partials[blockIdx.x].
-template <int IODT, int NV, int WPR, bool DS, bool SUMS>
-__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void cascmm_layer_norm_backward_kernel(const NormParams p) {
+template <int IODT, int NV, int LPR, bool DS, bool SUMS>
+__global__ __launch_bounds__(256) void cascmm_layer_norm_backward_kernel(const NormParams p) {
   typedef NormRow<IODT> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
-  constexpr int VEC = R::VEC, CH = NV / VEC, STEP = 64 * WPR * VEC;
-  __shared__ float slots[4 * WPR];
-  const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int wave = WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  constexpr int VEC = R::VEC, CH = NV / VEC, STEP = LPR * VEC, ROWS = 256 / LPR;
+  __shared__ float slots[16];
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const int cols = p.cols, col0 = lane * VEC;
-  const int64_t waves = (int64_t)gridDim.x * (WPR == 1 ? 4 : 1);
-  int64_t row = (int64_t)blockIdx.x * (WPR == 1 ? 4 : 1) + wave;
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  int64_t row = (int64_t)blockIdx.x * ROWS + (LPR == 64 ? __builtin_amdgcn_readfirstlane(group) : group);
   int turn = 0;
-  chunk x[CH], dy[CH], ds[DS ? CH : 1];
-  float mean = 0.f, rstd = 0.f;
+  struct Row {
+    chunk x[CH], dy[CH], ds[DS ? CH : 1];
+    float mean, rstd;
+  } next;
   auto fetch = [&](int64_t at) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      x[c] = R::load((const E*)p.x + at * p.ldx, col0 + c * STEP, cols);
-      dy[c] = R::load((const E*)p.dy + at * p.lddy, col0 + c * STEP, cols);
-      if constexpr (DS) ds[c] = R::load((const E*)p.ds + at * p.ldds, col0 + c * STEP, cols);
+      next.x[c] = R::load((const E*)p.x + at * p.ldx, col0 + c * STEP, cols);
+      next.dy[c] = R::load((const E*)p.dy + at * p.lddy, col0 + c * STEP, cols);
+      if constexpr (DS) next.ds[c] = R::load((const E*)p.ds + at * p.ldds, col0 + c * STEP, cols);
     }
-    mean = p.mean[at];
-    rstd = p.rstd[at];
+    next.mean = p.mean[at];
+    next.rstd = p.rstd[at];
   };
   float w[CH][VEC], dw[SUMS ? CH : 1][VEC], db[SUMS ? CH : 1][VEC];
 #pragma unroll
@@ -284,38 +296,34 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void cascmm_layer_norm_b
   }
   if (row < p.rows) fetch(row);
   while (row < p.rows) {
-    float xhat[CH][VEC], g[CH][VEC], sums[2] = {0.f, 0.f};
-    chunk keep[DS ? CH : 1];
-    const float rs = rstd;
+    const Row cur = next;
+    const int64_t at = row;
+    row += stride;
+    if (row < p.rows) fetch(row);
+    float sums[2] = {0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         // (behind the last column x, dy and with it g are zeros, and xhat, which the mean is taken from, meets nothing but them)
-        xhat[c][e] = ((float)x[c][e] - mean) * rs;
-        const float d = (float)dy[c][e];
-        g[c][e] = d * w[c][e];
-        sums[0] += g[c][e];
-        sums[1] = __builtin_fmaf(g[c][e], xhat[c][e], sums[1]);
+        const float xhat = ((float)cur.x[c][e] - cur.mean) * cur.rstd, d = (float)cur.dy[c][e], g = d * w[c][e];
+        sums[0] += g;
+        sums[1] = __builtin_fmaf(g, xhat, sums[1]);
         if constexpr (SUMS) {
-          dw[c][e] = __builtin_fmaf(d, xhat[c][e], dw[c][e]);
+          dw[c][e] = __builtin_fmaf(d, xhat, dw[c][e]);
           db[c][e] += d;
         }
       }
-      if constexpr (DS) keep[c] = ds[c];
-    }
-    const int64_t at = row;
-    row += waves;
-    if (row < p.rows) fetch(row);
-    norm_sums<WPR>(sums, slots, turn);
+    norm_sums<LPR>(sums, slots, turn);
     const float c1 = sums[0] * p.inv_cols, c2 = sums[1] * p.inv_cols;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       chunk out;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float d = rs * (g[c][e] - c1 - xhat[c][e] * c2);
-        if constexpr (DS) d += (float)keep[c][e];
+        const float xhat = ((float)cur.x[c][e] - cur.mean) * cur.rstd;
+        float d = cur.rstd * ((float)cur.dy[c][e] * w[c][e] - c1 - xhat * c2);
+        if constexpr (DS) d += (float)cur.ds[c][e];
         out[e] = (E)d;
       }
       R::store((E*)p.y + at * p.ldy, col0 + c * STEP, cols, out);
@@ -323,27 +331,30 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void cascmm_layer_norm_b
   }
   if constexpr (SUMS) {
     float* part = p.partials + (int64_t)blockIdx.x * 2 * cols;
-    if constexpr (WPR == 1) {
-      // the four waves one after the other, in LDS
-      __shared__ float meet[2][64 * NV];
-      for (int turn_of = 0; turn_of < 4; ++turn_of) {
-        if (wave == turn_of) {
+    if constexpr (LPR <= 64) {
+      // a wave's rows of lanes, then the four waves in order, in LDS (a lane's elements LPR apart: side by side over the lanes)
+      __shared__ float meet[4][2][LPR * NV];
 #pragma unroll
-          for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const int at = c * STEP + e * 64 + lane;   // (side by side over the lanes)
-              meet[0][at] = turn_of == 0 ? dw[c][e] : meet[0][at] + dw[c][e];
-              meet[1][at] = turn_of == 0 ? db[c][e] : meet[1][at] + db[c][e];
-            }
+        for (int e = 0; e < VEC; ++e) {
+          float a = dw[c][e], b = db[c][e];
+#pragma unroll
+          for (int off = LPR; off < 64; off *= 2) {
+            a += __shfl_xor(a, off, 64);
+            b += __shfl_xor(b, off, 64);
+          }
+          if (LPR == 64 || (threadIdx.x & 63) < LPR) {
+            meet[threadIdx.x >> 6][0][(c * VEC + e) * LPR + lane] = a;
+            meet[threadIdx.x >> 6][1][(c * VEC + e) * LPR + lane] = b;
+          }
         }
-        __syncthreads();
-      }
-      for (int i = threadIdx.x; i < 64 * NV; i += 256) {
-        const int col = i / STEP * STEP + (i % STEP % 64) * VEC + i % STEP / 64;
+      __syncthreads();
+      for (int i = threadIdx.x; i < LPR * NV; i += 256) {
+        const int col = i / STEP * STEP + (i % LPR) * VEC + i % STEP / LPR;
         if (col < cols) {
-          part[col] = meet[0][i];
-          part[cols + col] = meet[1][i];
+          part[col] = ((meet[0][0][i] + meet[1][0][i]) + meet[2][0][i]) + meet[3][0][i];
+          part[cols + col] = ((meet[0][1][i] + meet[1][1][i]) + meet[2][1][i]) + meet[3][1][i];
         }
       }
     } else {
@@ -367,8 +378,8 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_backward_wide_ker
   typedef NormRow<IODT> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
-  constexpr int VEC = R::VEC, WPR = kNormWide / 64, STEP = kNormWide * VEC;
-  __shared__ float slots[4 * WPR];
+  constexpr int VEC = R::VEC, STEP = kNormWide * VEC;
+  __shared__ float slots[kNormWide / 16];
   const int64_t row = blockIdx.x;
   const int cols = p.cols, col0 = threadIdx.x * VEC;
   const E *x = (const E*)p.x + row * p.ldx, *dy = (const E*)p.dy + row * p.lddy, *ds = p.ds ? (const E*)p.ds + row * p.ldds : nullptr;
@@ -386,7 +397,7 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_backward_wide_ker
       sums[1] = __builtin_fmaf(g, ((float)v[e] - mean) * rstd, sums[1]);
     }
   }
-  norm_sums<WPR>(sums, slots, turn);
+  norm_sums<kNormWide>(sums, slots, turn);
   const float c1 = sums[0] * p.inv_cols, c2 = sums[1] * p.inv_cols;
   for (int64_t c = col0; c < cols; c += STEP) {
     const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
@@ -433,12 +444,13 @@ __global__ __launch_bounds__(1024) void cascmm_column_finish_kernel(const float*
   if (col < cols) {
     const float* src = partials + (int64_t)half * cols + col;
     const int64_t step = (int64_t)halves * cols;
-    int i = r;
-    for (; i + 96 < parts; i += 128) {   // (four loads in flight)
-      const float a0 = src[i * step], a1 = src[(i + 32) * step], a2 = src[(i + 64) * step], a3 = src[(i + 96) * step];
-      s += a0; s += a1; s += a2; s += a3;
+    for (int i = r; i < parts; i += 32 * 16) {   // (sixteen loads in flight: a workgroup runs through its partial sums once, bound by their latency)
+      float v[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) v[u] = i + 32 * u < parts ? src[(i + 32 * u) * step] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) s += v[u];
     }
-    for (; i < parts; i += 32) s += src[i * step];
   }
   meet[r][c] = s;
   __syncthreads();

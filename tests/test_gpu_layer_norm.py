@@ -18,7 +18,7 @@ TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2
 TYPES = [(torch.float32, torch.float32), (torch.float16, torch.float16), (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16),
          (torch.bfloat16, torch.float32)]
 SIZES = [(1, 1), (1, 2), (3, 7), (5, 64), (2, 1280), (9, 512), (77, 640), (333, 457), (260, 1024), (4, 1536), (5, 1537), (6, 2048), (3, 2049), (3, 3001), (2, 4096),
-         (2, 6144), (3, 8192), (3, 8193), (2, 20001), (5000, 8), (2049, 96)]
+         (2, 6144), (3, 8192), (3, 8193), (2, 20001), (5000, 8), (2049, 96), (130, 65), (1000, 128), (77, 130), (40, 256), (41, 257)]
 
 
 def rows_of(gen, rows, cols, dtype, device, spread=1.0, mean=0.5):
