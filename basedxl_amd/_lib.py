@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libcascmm.so")
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 FMT_BF16, FMT_FP16, FMT_FP8 = 0, 1, 2
 PROD_TRI, PROD_FULL = 0, 1
+ACT_BY_NAME = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 ERR_BAD_FORMAT = -4   # CASCMM_ERR_BAD_FORMAT: no kernel for this (dtype, format, terms, products, shape)
 
 FMT_BY_NAME = {"bf16": FMT_BF16, "fp16": FMT_FP16, "fp8": FMT_FP8}
@@ -70,6 +71,11 @@ SIGNATURES = {
     "cascmm_gate": (c_int, [c_void_p, c_void_p] + [c_int64] * 4 + [c_int, c_void_p]),
     "cascmm_gemm_fp8_autoscale": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p] + [c_int64] * 6 + [c_int, c_int]
                                   + [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cascmm_gemm_epilogue": (c_int, [c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_int64] * 8 + [c_int] * 5
+                             + [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cascmm_epilogue_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "cascmm_epilogue_backward": (c_int, [c_void_p] * 4 + [c_int64] * 5 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "cascmm_transpose": (c_int, [c_void_p, c_void_p] + [c_int64] * 4 + [c_int, c_void_p]),
     "cascmm_layer_norm": (c_int, [c_void_p] * 8 + [c_int64] * 6 + [c_float, c_int, c_int, c_void_p]),
     "cascmm_layer_norm_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "cascmm_layer_norm_backward": (c_int, [c_void_p] * 9 + [c_int64] * 6 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),

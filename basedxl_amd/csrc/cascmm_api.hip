@@ -8,6 +8,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "cascmm_epilogue.h"
 #include "cascmm_gate_kernel.h"
 #include "cascmm_variants.h"
 
@@ -1677,6 +1678,28 @@ int cascmm_gate(const void* h, void* out, int64_t rows, int64_t inner, int64_t l
                          : dtype == CASCMM_DT_F16 ? launch_gate<CASCMM_DT_F16>(h, ldh, out, ldo, rows, inner, s)
                                                   : launch_gate<CASCMM_DT_BF16>(h, ldh, out, ldo, rows, inner, s);
   return err == hipSuccess ? CASCMM_OK : CASCMM_ERR_LAUNCH;
+}
+
+int cascmm_gemm_epilogue(const void* A, const void* B, int b_prepared, void* C, const void* bias, const void* residual, void* preact, int64_t M, int64_t N, int64_t K,
+                         int64_t lda, int64_t ldb, int64_t ldc, int64_t ldr, int64_t ldp, int dtype, int fmt, int terms, int products, int activation,
+                         const int32_t* tensor_exps, void* workspace, size_t workspace_bytes, void* stream) {
+  Problem q{M, N, K, lda, b_prepared ? N : ldb, ldc, dtype, fmt, terms, products};
+  q.bpre = b_prepared != 0;
+  const int st = check_problem(q);
+  if (st != CASCMM_OK) return st;
+  if (activation < CASCMM_ACT_NONE || activation > CASCMM_ACT_SILU) return CASCMM_ERR_BAD_FORMAT;
+  if ((residual && ldr != 0 && ldr < N) || (preact && ldp < N)) return CASCMM_ERR_BAD_SHAPE;
+  if (M == 0 || N == 0) return CASCMM_OK;
+  const size_t es = dtype_size(dtype);
+  if (!C) return CASCMM_ERR_NULL_POINTER;
+  if (!aligned_to(C, es) || !aligned_to(residual, es) || !aligned_to(preact, es)) return CASCMM_ERR_ALIGNMENT;
+  // the product where its values before the activation are wanted, or in place of the result
+  void* z = preact ? preact : C;
+  const int64_t ldz = preact ? ldp : ldc;
+  q.ldc = ldz;
+  const int sg = gemm_impl(1, &A, &B, &z, bias ? &bias : nullptr, q, tensor_exps, workspace, workspace_bytes, (hipStream_t)stream, -1);
+  if (sg != CASCMM_OK || (z == C && !residual && activation == CASCMM_ACT_NONE)) return sg;
+  return launch_epilogue(z, ldz, residual, ldr, C, ldc, M, N, activation, dtype, (hipStream_t)stream);
 }
 
 int cascmm_gemm_fp8_autoscale(const void* A, const void* B, int b_prepared, void* C, const void* bias, int64_t M, int64_t N,

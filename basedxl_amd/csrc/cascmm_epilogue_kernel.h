@@ -1,0 +1,211 @@
+// What follows a product in a Linear layer:  y = act(z) + residual,  z = A . B + bias,  as a pass of its own behind kernels that store z, and
+// its backward pass:  dz = dy act'(z),  dbias = sum over rows of dz.  fp32 between a load and a store whatever the elements are.
+//
+//   relu       max(z, 0)                                    z > 0
+//   gelu       z Phi(z)                                     Phi(z) + z phi(z)
+//   gelu_tanh  z s(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3)   s + 2 z s (1 - s) u',  s = s(2 u)
+//   silu       z s(z)                                       s (1 + z (1 - s)),  s(x) = 1 / (1 + exp(-x))
+//
+// (z s(2 u) is z (1 + tanh u) / 2 without the cancellation for z < 0.)  Slopes are taken at z clamped to where they are 0 and 1 to fp32's
+// last bit, so that no intermediate value overflows; a NaN stays one.
+//
+// Bound by memory: 16 bytes a load, rows of any alignment.
+#pragma once
+#include "cascmm_norm_kernel.h"
+
+namespace cascmm {
+
+constexpr float kLog2e = 1.4426950408889634f;
+// 1 / (1 + exp(-x))
+__device__ __forceinline__ float sigmoid_value(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * x)); }
+__device__ __forceinline__ float gelu_tanh_twice_u(float z) { return 1.5957691216057308f * z * __builtin_fmaf(0.044715f * z, z, 1.f); }
+
+// act of several at a time (kinds are uniform: one branch)
+template <int N> __device__ __forceinline__ void activate(float (&v)[N], int act) {
+  if (act == CASCMM_ACT_GELU) {
+    gelu_values(v);
+  } else if (act == CASCMM_ACT_GELU_TANH) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] *= sigmoid_value(gelu_tanh_twice_u(v[e]));
+  } else if (act == CASCMM_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] *= sigmoid_value(v[e]);
+  } else if (act == CASCMM_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+  }
+}
+
+__device__ __forceinline__ float clamped(float z, float most) { return z > most ? most : z < -most ? -most : z; }
+// d[e] *= act'(z[e])
+template <int N> __device__ __forceinline__ void times_slope(float (&d)[N], const float (&z)[N], int act) {
+  if (act == CASCMM_ACT_GELU) {
+    // 2 Phi(-|z|) as in gelu_values; phi(z) = exp(-z^2 / 2) / sqrt(2 pi)
+    float t[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = clamped(z[e], 20.f), a = __builtin_fabsf(x);
+      t[e] = kGeluFit[0];
+#pragma unroll
+      for (int i = 1; i < 10; ++i) t[e] = __builtin_fmaf(t[e], a, kGeluFit[i]);
+      const float tail = 0.5f * __builtin_amdgcn_exp2f(t[e] * a), density = 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * x * x);
+      d[e] *= __builtin_fmaf(x, density, x > 0.f ? 1.f - tail : tail);
+    }
+  } else if (act == CASCMM_ACT_GELU_TANH) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = clamped(z[e], 10.f), q = __builtin_amdgcn_exp2f(-kLog2e * gelu_tanh_twice_u(x)), s = __builtin_amdgcn_rcpf(1.f + q);
+      // (1 - s = q s)
+      d[e] *= __builtin_fmaf(x * s * (q * s), 1.5957691216057308f * __builtin_fmaf(0.134145f * x, x, 1.f), s);
+    }
+  } else if (act == CASCMM_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = clamped(z[e], 80.f), q = __builtin_amdgcn_exp2f(-kLog2e * x), s = __builtin_amdgcn_rcpf(1.f + q);
+      d[e] *= s * __builtin_fmaf(x, q * s, 1.f);
+    }
+  } else if (act == CASCMM_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] = z[e] <= 0.f ? 0.f : d[e];
+  }
+}
+
+// dst [rows][cols] = act(src) + residual (NULL: nothing; ldr 0: one row for all).  src may be dst.  A thread takes a chunk of 16 bytes; chunks are
+// counted in 32 bits (checked by the host).
+template <int IODT>
+__global__ __launch_bounds__(256) void cascmm_epilogue_kernel(const void* src, int64_t lds, const void* residual, int64_t ldr, void* dst, int64_t ldd, int cols,
+                                                             unsigned per_row, unsigned total, int act) {
+  typedef NormRow<IODT> R;
+  typedef typename R::E E;
+  typedef typename R::chunk chunk;
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= total) return;
+  const unsigned row = i / per_row;
+  const int col = (int)(i - row * per_row) * R::VEC;
+  const chunk z = R::load((const E*)src + (int64_t)row * lds, col, cols);
+  chunk r;
+  if (residual) r = R::load((const E*)residual + (int64_t)row * ldr, col, cols);
+  float v[R::VEC];
+#pragma unroll
+  for (int e = 0; e < R::VEC; ++e) v[e] = (float)z[e];
+  activate(v, act);
+  if (residual) {
+#pragma unroll
+    for (int e = 0; e < R::VEC; ++e) v[e] += (float)r[e];
+  }
+  chunk y;
+#pragma unroll
+  for (int e = 0; e < R::VEC; ++e) y[e] = (E)v[e];
+  R::store((E*)dst + (int64_t)row * ldd, col, cols, y);
+}
+
+// dz = dy act'(z) (dz NULL: not wanted; act none: z is not read) and, with partials, the workgroup's sums over its rows of dz for its columns at
+// partials[blockIdx.y].  LANES lanes side by side on a row, rows gridDim.y workgroups apart; the sums are of dz as it is before it is rounded.
+template <int IODT, int LANES>
+__global__ __launch_bounds__(256) void cascmm_epilogue_backward_kernel(const void* dy, int64_t lddy, const void* z, int64_t ldz, void* dz, int64_t lddz,
+                                                                      float* partials, int64_t rows, int cols, int act) {
+  typedef NormRow<IODT> R;
+  typedef typename R::E E;
+  typedef typename R::chunk chunk;
+  constexpr int VEC = R::VEC, GROUPS = 256 / LANES, AHEAD = 4;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int col = ((int)blockIdx.x * LANES + lane) * VEC;
+  const int64_t stride = (int64_t)gridDim.y * GROUPS;
+  float sums[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sums[e] = 0.f;
+  if (col < cols) {
+    for (int64_t row = (int64_t)blockIdx.y * GROUPS + group; row < rows; row += AHEAD * stride) {
+      chunk d[AHEAD], x[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int64_t at = row + u * stride;
+        if (at >= rows) continue;
+        d[u] = R::load((const E*)dy + at * lddy, col, cols);
+        if (act) x[u] = R::load((const E*)z + at * ldz, col, cols);
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int64_t at = row + u * stride;
+        if (at >= rows) continue;
+        float g[VEC], v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          g[e] = (float)d[u][e];
+          v[e] = act ? (float)x[u][e] : 0.f;
+        }
+        times_slope(g, v, act);
+        chunk out;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          sums[e] += g[e];
+          out[e] = (E)g[e];
+        }
+        if (dz) R::store((E*)dz + at * lddz, col, cols, out);
+      }
+    }
+  }
+  if (!partials) return;
+  __shared__ float meet[GROUPS][LANES * VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) meet[group][e * LANES + lane] = sums[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < LANES * VEC; i += 256) {
+    const int64_t c = ((int64_t)blockIdx.x * LANES + i % LANES) * VEC + i / LANES;
+    if (c >= cols) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) s += meet[g][i];
+    partials[(int64_t)blockIdx.y * cols + c] = s;
+  }
+}
+
+// out [cols][rows] = x [rows][cols] transposed; E: an unsigned type of the elements' size.  64 x 64 elements a workgroup through LDS: 16 bytes a load
+// along the rows of x and a store along the rows of out.  Rows of the tile are an odd number of dwords apart in LDS, so that the eight (sixteen)
+// groups of rows that the lanes of a store read start on banks of their own.
+template <typename E>
+__global__ __launch_bounds__(256) void cascmm_transpose_kernel(const E* __restrict__ x, int64_t ldx, E* __restrict__ out, int64_t ldo, int rows, int cols, unsigned tiles_across) {
+  constexpr int VEC = 16 / (int)sizeof(E), PER = 64 / VEC, PITCH = sizeof(E) == 2 ? 66 : 65, DW = 4 / (int)sizeof(E);
+  typedef E chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
+  __shared__ __attribute__((aligned(16))) E tile[64 * PITCH];
+  const int r0 = (int)(blockIdx.x / tiles_across) * 64, c0 = (int)(blockIdx.x % tiles_across) * 64;
+#pragma unroll
+  for (int i = threadIdx.x; i < 64 * PER; i += 256) {
+    const int r = i / PER, c = i % PER * VEC;
+    chunk v;
+    if (r0 + r < rows && c0 + c + VEC <= cols) {
+      v = *(const chunk*)(x + (int64_t)(r0 + r) * ldx + c0 + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = r0 + r < rows && c0 + c + e < cols ? x[(int64_t)(r0 + r) * ldx + c0 + c + e] : (E)0;
+    }
+    // (dword by dword: the pitch leaves no rows on 16 bytes)
+    typedef E pair __attribute__((ext_vector_type(DW)));
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      pair w;
+#pragma unroll
+      for (int e = 0; e < DW; ++e) w[e] = v[d * DW + e];
+      *(pair*)(tile + r * PITCH + c + d * DW) = w;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = threadIdx.x; i < 64 * PER; i += 256) {
+    const int c = i / PER, r = i % PER * VEC;
+    if (c0 + c >= cols) continue;
+    chunk v;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = tile[(r + e) * PITCH + c];
+    E* to = out + (int64_t)(c0 + c) * ldo + r0 + r;
+    if (r0 + r + VEC <= rows) {
+      *(chunk*)to = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (r0 + r + e < rows) to[e] = v[e];
+    }
+  }
+}
+
+}  // namespace cascmm

@@ -30,6 +30,8 @@ static int64_t norm_groups(int64_t rows, int lanes, bool backward) {
   const int64_t at_a_time = 256 / lanes * (backward ? 2 : 1), most = backward ? (lanes == 256 ? 256 : lanes == 64 ? 512 : 1024) : 1024;
   return std::max<int64_t>(1, std::min<int64_t>((rows + at_a_time - 1) / at_a_time, most));
 }
+// (a launch has fewer than 2^32 threads)
+static unsigned norm_wide_groups(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 20); }
 // rows of partial sums of the backward pass
 static int64_t norm_parts(int64_t rows, int64_t cols) {
   const NormShape f = norm_shape(cols, true);
@@ -60,7 +62,7 @@ template <int IODT, bool ADD> static hipError_t norm_forward(const NormParams& p
     NORM_CASE(256, 16);
     NORM_CASE(256, 24);
     NORM_CASE(256, 32);
-    default: CASCMM_LAUNCH(err, (cascmm_layer_norm_wide_kernel<IODT, ADD>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
+    default: CASCMM_LAUNCH(err, (cascmm_layer_norm_wide_kernel<IODT, ADD>), dim3(norm_wide_groups(p.rows)), dim3(kNormWide), 0, s, p);
   }
 #undef NORM_CASE
   return err;
@@ -94,7 +96,7 @@ template <int IODT> static hipError_t norm_backward(const NormParams& p, void* d
   const int parts = (int)norm_parts(p.rows, p.cols);
   // (no dx wanted: nothing but the sums.  No rows: sums of zeros)
   const bool rows = p.y && p.rows > 0, wide = norm_shape(p.cols, true).lanes == 0;
-  if (rows && wide) CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_wide_kernel<IODT>), dim3((unsigned)p.rows), dim3(kNormWide), 0, s, p);
+  if (rows && wide) CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_wide_kernel<IODT>), dim3(norm_wide_groups(p.rows)), dim3(kNormWide), 0, s, p);
   else if (rows && p.partials) err = p.ds ? norm_backward_rows<IODT, true, true>(p, s) : norm_backward_rows<IODT, false, true>(p, s);
   else if (rows) err = p.ds ? norm_backward_rows<IODT, true, false>(p, s) : norm_backward_rows<IODT, false, false>(p, s);
   if (!p.partials) return err;

@@ -211,50 +211,51 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
   typedef typename R::chunk chunk;
   constexpr int VEC = R::VEC, STEP = kNormWide * VEC;
   __shared__ float slots[kNormWide / 16];
-  const int64_t row = blockIdx.x;
   const int cols = p.cols, col0 = threadIdx.x * VEC;
-  const E* x = (const E*)p.x + row * p.ldx;
   int turn = 0;
-  float total[1] = {0.f};
-  for (int64_t c = col0; c < cols; c += STEP) {
-    chunk v = R::load(x, (int)c, cols);
-    if constexpr (ADD) {
-      const chunk r = R::load((const E*)p.residual + row * p.ldr, (int)c, cols);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const E* x = (const E*)p.x + row * p.ldx;
+    float total[1] = {0.f};
+    for (int64_t c = col0; c < cols; c += STEP) {
+      chunk v = R::load(x, (int)c, cols);
+      if constexpr (ADD) {
+        const chunk r = R::load((const E*)p.residual + row * p.ldr, (int)c, cols);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = (E)((float)v[e] + (float)r[e]);
-      R::store((E*)p.sum + row * p.lds, (int)c, cols, v);
+        for (int e = 0; e < VEC; ++e) v[e] = (E)((float)v[e] + (float)r[e]);
+        R::store((E*)p.sum + row * p.lds, (int)c, cols, v);
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) total[0] += (float)v[e];
     }
+    // (a thread reads back what it has written itself)
+    const E* s = ADD ? (const E*)p.sum + row * p.lds : x;
+    norm_sums<kNormWide>(total, slots, turn);
+    const float mean = total[0] / (float)p.cols;
+    float square[1] = {0.f};
+    for (int64_t c = col0; c < cols; c += STEP) {
+      const chunk v = R::load(s, (int)c, cols);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) total[0] += (float)v[e];
-  }
-  // (a thread reads back what it has written itself)
-  const E* s = ADD ? (const E*)p.sum + row * p.lds : x;
-  norm_sums<kNormWide>(total, slots, turn);
-  const float mean = total[0] / (float)p.cols;
-  float square[1] = {0.f};
-  for (int64_t c = col0; c < cols; c += STEP) {
-    const chunk v = R::load(s, (int)c, cols);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float d = c + e < cols ? (float)v[e] - mean : 0.f;
-      square[0] = __builtin_fmaf(d, d, square[0]);
+      for (int e = 0; e < VEC; ++e) {
+        const float d = c + e < cols ? (float)v[e] - mean : 0.f;
+        square[0] = __builtin_fmaf(d, d, square[0]);
+      }
     }
-  }
-  norm_sums<kNormWide>(square, slots, turn);
-  const float rstd = rsqrtf(square[0] * p.inv_cols + p.eps);
-  if (p.mean && threadIdx.x == 0) {
-    p.mean[row] = mean;
-    p.rstd[row] = rstd;
-  }
-  for (int64_t c = col0; c < cols; c += STEP) {
-    const chunk v = R::load(s, (int)c, cols);
-    float w[VEC], b[VEC];
-    R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
-    R::load_weight(b, p.bias, p.weight_f32, (int)c, cols, 0.f);
-    chunk y;
+    norm_sums<kNormWide>(square, slots, turn);
+    const float rstd = rsqrtf(square[0] * p.inv_cols + p.eps);
+    if (p.mean && threadIdx.x == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+    for (int64_t c = col0; c < cols; c += STEP) {
+      const chunk v = R::load(s, (int)c, cols);
+      float w[VEC], b[VEC];
+      R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
+      R::load_weight(b, p.bias, p.weight_f32, (int)c, cols, 0.f);
+      chunk y;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) y[e] = (E)__builtin_fmaf(((float)v[e] - mean) * rstd, w[e], b[e]);
-    R::store((E*)p.y + row * p.ldy, (int)c, cols, y);
+      for (int e = 0; e < VEC; ++e) y[e] = (E)__builtin_fmaf(((float)v[e] - mean) * rstd, w[e], b[e]);
+      R::store((E*)p.y + row * p.ldy, (int)c, cols, y);
+    }
   }
 }
 
@@ -380,38 +381,39 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_backward_wide_ker
   typedef typename R::chunk chunk;
   constexpr int VEC = R::VEC, STEP = kNormWide * VEC;
   __shared__ float slots[kNormWide / 16];
-  const int64_t row = blockIdx.x;
   const int cols = p.cols, col0 = threadIdx.x * VEC;
-  const E *x = (const E*)p.x + row * p.ldx, *dy = (const E*)p.dy + row * p.lddy, *ds = p.ds ? (const E*)p.ds + row * p.ldds : nullptr;
-  const float mean = p.mean[row], rstd = p.rstd[row];
   int turn = 0;
-  float sums[2] = {0.f, 0.f};
-  for (int64_t c = col0; c < cols; c += STEP) {
-    const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
-    float w[VEC];
-    R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const E *x = (const E*)p.x + row * p.ldx, *dy = (const E*)p.dy + row * p.lddy, *ds = p.ds ? (const E*)p.ds + row * p.ldds : nullptr;
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float sums[2] = {0.f, 0.f};
+    for (int64_t c = col0; c < cols; c += STEP) {
+      const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
+      float w[VEC];
+      R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float g = (float)d[e] * w[e];
-      sums[0] += g;
-      sums[1] = __builtin_fmaf(g, ((float)v[e] - mean) * rstd, sums[1]);
+      for (int e = 0; e < VEC; ++e) {
+        const float g = (float)d[e] * w[e];
+        sums[0] += g;
+        sums[1] = __builtin_fmaf(g, ((float)v[e] - mean) * rstd, sums[1]);
+      }
     }
-  }
-  norm_sums<kNormWide>(sums, slots, turn);
-  const float c1 = sums[0] * p.inv_cols, c2 = sums[1] * p.inv_cols;
-  for (int64_t c = col0; c < cols; c += STEP) {
-    const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
-    float w[VEC];
-    R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
-    chunk z, out;
-    if (ds) z = R::load(ds, (int)c, cols);
+    norm_sums<kNormWide>(sums, slots, turn);
+    const float c1 = sums[0] * p.inv_cols, c2 = sums[1] * p.inv_cols;
+    for (int64_t c = col0; c < cols; c += STEP) {
+      const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
+      float w[VEC];
+      R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
+      chunk z, out;
+      if (ds) z = R::load(ds, (int)c, cols);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float o = rstd * ((float)d[e] * w[e] - c1 - ((float)v[e] - mean) * rstd * c2);
-      if (ds) o += (float)z[e];
-      out[e] = (E)o;
+      for (int e = 0; e < VEC; ++e) {
+        float o = rstd * ((float)d[e] * w[e] - c1 - ((float)v[e] - mean) * rstd * c2);
+        if (ds) o += (float)z[e];
+        out[e] = (E)o;
+      }
+      R::store((E*)p.y + row * p.ldy, (int)c, cols, out);
     }
-    R::store((E*)p.y + row * p.ldy, (int)c, cols, out);
   }
 }
 // ... and the sums with a thread a column over every gridDim.y-th row

@@ -44,7 +44,7 @@ def _check_residual(x: torch.Tensor, residual: torch.Tensor) -> None:
 
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """``t`` as rows of its last axis, a view where its strides allow one."""
-    return _rows(t.reshape(-1, t.shape[-1]))
+    return _rows(t.reshape(t.shape[:-1].numel(), t.shape[-1]))
 
 
 def _ld(t2: torch.Tensor) -> int:

@@ -46,6 +46,9 @@ enum cascmm_fmt { CASCMM_FMT_BF16 = 0, CASCMM_FMT_FP16 = 1, CASCMM_FMT_FP8 = 2 }
 /* which partial products A_i.B_j are summed: TRI keeps i + j <= terms - 1, FULL keeps all */
 enum cascmm_products { CASCMM_PROD_TRI = 0, CASCMM_PROD_FULL = 1 };
 
+/* what follows a product (cascmm_gemm_epilogue); gelu in its erf form and in its tanh form */
+enum cascmm_activation { CASCMM_ACT_NONE = 0, CASCMM_ACT_RELU = 1, CASCMM_ACT_GELU = 2, CASCMM_ACT_GELU_TANH = 3, CASCMM_ACT_SILU = 4 };
+
 enum cascmm_status {
   CASCMM_OK = 0,
   CASCMM_ERR_NULL_POINTER = -1,
@@ -322,6 +325,30 @@ int cascmm_gemm_fp8_autoscale(const void* A, const void* B, int b_prepared, void
                               int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
                               int terms, int products, const int32_t* b_exp, int32_t* exps_out,
                               int32_t* scratch, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A product with what follows it in a Linear layer:
+ *     z = A . B (+ bias);   C = activation(z) (+ residual)
+ * The reference runs the layer (basedxl/modules/lowp_linear.py:15-20) and what its model does with the result (the residual adds of a
+ * transformer block, an embedding's SiLU) as separate kernels.  Operands as cascmm_gemm (b_prepared == 0) or cascmm_gemm_prepared with one
+ * problem (b_prepared != 0, ldb ignored); residual [M, N] of `dtype` or NULL, its rows ldr >= N apart or all the same one (ldr == 0);
+ * preact: NULL or [M, N], receives z for the backward pass.  The activation is one of cascmm_activation, in fp32.
+ * C and preact overlap no operand and not each other.  tensor_exps, workspace: as cascmm_gemm.
+ */
+int cascmm_gemm_epilogue(const void* A, const void* B, int b_prepared, void* C, const void* bias, const void* residual,
+                         void* preact, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
+                         int64_t ldr, int64_t ldp, int dtype, int fmt, int terms, int products, int activation,
+                         const int32_t* tensor_exps, void* workspace, size_t workspace_bytes, void* stream);
+/* The way back: dz = dy * activation'(z) and dbias = sum over rows of dz (before dz is rounded), [rows, cols] with leading dimensions; dz or
+ * dbias may be NULL, and without an activation z too.  For dbias the workspace holds cascmm_epilogue_workspace_bytes(rows, cols, dtype) bytes
+ * (16-byte aligned, contents need no initialisation); the sums are fp32 in a fixed order, without atomics.  The gradients of A and B are
+ * products of dz with the transposed operands. */
+size_t cascmm_epilogue_workspace_bytes(int64_t rows, int64_t cols, int dtype);
+int cascmm_epilogue_backward(const void* dy, const void* z, void* dz, void* dbias, int64_t rows, int64_t cols,
+                             int64_t lddy, int64_t ldz, int64_t lddz, int activation, int dtype, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* out [cols, rows] (leading dimension ldo >= rows) = x [rows, cols] transposed: the operands of those products. */
+int cascmm_transpose(const void* x, void* out, int64_t rows, int64_t cols, int64_t ldx, int64_t ldo, int dtype, void* stream);
 
 /*
  * Layer norm over the last axis of x [rows, cols] (leading dimension ldx; all leading dimensions in elements), what stands in front of

@@ -1,0 +1,388 @@
+"""activation(a @ b + bias) + residual and its gradients against the formulas in 64 bits.
+
+Tolerances, element by element.  u = 2^-24, ``half`` the half step of the tensors' type, S = |a| @ |b|.  K products summed in fp32 are off by at
+most K u S whatever the order; splitting fp32 into terms leaves out ``lost`` S: two bf16 terms hold 2^-16 of an operand and leave out lo lo (three
+times 2^-16), three fp16 terms less than u.  Activations have slopes up to 1.13, curvatures up to 0.8 and are computed to 8 u (1 + |z|).  Where
+a kernel stores z first (no fused store, or z kept for the backward pass), z is off by half |z| more.
+"""
+import math
+
+import pytest
+import torch
+
+from basedxl_amd import _lib, PreparedWeight, add_layer_norm, cascaded_lowp_matmul, cascaded_lowp_matmul_epilogue, layer_norm
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}
+CASCADES = {"fp32": (torch.float32, {}, 3 * 2.0 ** -16), "fp32x3": (torch.float32, {"lowp": "fp16", "terms": 3}, 2.0 ** -24), "fp16": (torch.float16, {}, 0.0),
+            "bf16": (torch.bfloat16, {}, 0.0)}
+F = torch.nn.functional
+ACTIVATIONS = {None: lambda z: z, "relu": F.relu, "gelu": F.gelu, "gelu_tanh": lambda z: F.gelu(z, approximate="tanh"), "silu": F.silu}
+SIZES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (2, 320, 1280), (77, 50, 30), (154, 128, 320), (64, 64, 64), (333, 456, 211), (257, 136, 130), (513, 72, 1032),
+         (64, 5120, 640), (16, 2048, 66), (300, 1280, 1280), (1100, 640, 2560), (130, 33, 4100)]
+
+
+def slope_of(z, name):
+    z = z.detach().clone().requires_grad_()
+    return torch.autograd.grad(ACTIVATIONS[name](z).sum(), z)[0] if name else torch.ones_like(z)
+
+
+def within(got, want, tol, what, mean=True):
+    assert got.shape == want.shape, what
+    got = got.detach()
+    off = (got.double() - want).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} values off, the worst {float((off / tol).nan_to_num(nan=math.inf).max()):.2f} of the tolerance"
+    norm = float(want.norm())
+    if mean and want.numel() >= 1000 and norm > 0:
+        # (single errors are at most a few half steps, mostly of independent signs: twice a half step in the mean square is beyond what they add up to)
+        assert float((got.double() - want).norm()) <= 2 * max(HALF[got.dtype], 2.0 ** -16 if got.dtype == torch.float32 else 0) * norm, what
+
+
+def operands(M, K, N, dtype, device, seed=0, w_std=None):
+    gen = torch.Generator().manual_seed(seed + 7 * M + 13 * K + 17 * N)
+    r = lambda *s, std=1.0: (torch.randn(*s, generator=gen) * std).to(dtype).to(device)   # noqa: E731
+    return r(M, K), r(K, N, std=w_std or 1.0 / math.sqrt(K)), r(N), r(M, N), r(M, N)
+
+
+def z_of(a, b, bias, dtype, lost):
+    """(z, its error before any rounding, its error where it is stored), in 64 bits."""
+    A, B = a.double(), b.double()
+    z = A @ B + (0 if bias is None else bias.double())
+    S = A.abs() @ B.abs()
+    tol = (a.shape[1] + 4) * U * S + lost * S + 2 * U * z.abs() + (0 if bias is None else U * bias.double().abs())
+    return z, tol, tol + HALF[dtype] * z.abs() + TINY[dtype]
+
+
+def check_forward(y, a, b, bias, act, residual, dtype, lost, what, fused=False):
+    z, tol, stored = z_of(a, b, bias, dtype, lost)
+    want = ACTIVATIONS[act](z)
+    tol = 1.13 * (tol if fused else stored) + 8 * U * (1 + z.abs())
+    if residual is not None:
+        want = want + residual.double()
+        tol = tol + U * (want.abs() + residual.double().abs())
+    within(y, want, tol + HALF[dtype] * want.abs() + TINY[dtype], what)
+
+
+def check_backward(grads, dy, a, b, bias, act, residual, dtype, lost, what):
+    z, _, stored = z_of(a, b, bias, dtype, lost)
+    A, B, dy = a.double(), b.double(), dy.double()
+    slope = slope_of(z, act)
+    dz = dy * slope
+    if act == "relu":
+        off = (z.abs() <= stored).double()
+    else:
+        off = 0.8 * stored + 8 * U * (1 + z.abs()) if act else torch.zeros_like(z)
+    sum_tol = dy.abs() * off + 2 * U * dz.abs()
+    tol = sum_tol + (HALF[dtype] * dz.abs() + TINY[dtype] if act else 0)
+    # (relu's slope jumps: a z within its error of 0 changes dz by all of dy, and of 70000 values some are there (error 2^-15: two of them), which
+    # is (2 / 70000)^1/2 = 5e-3 in the mean square, far above the half steps of the others; the elements' own tolerances hold it)
+    mean = act != "relu"
+    got = iter(grads)
+    M, K = a.shape
+    N = b.shape[1]
+    want = dz @ B.t()
+    within(next(got), want, tol @ B.abs().t() + ((N + 4) * U + lost) * ((dz.abs() + tol) @ B.abs().t()) + HALF[dtype] * want.abs() + TINY[dtype], what + " da", mean)
+    want = A.t() @ dz
+    within(next(got), want, A.abs().t() @ tol + ((M + 4) * U + lost) * (A.abs().t() @ (dz.abs() + tol)) + HALF[dtype] * want.abs() + TINY[dtype], what + " db", mean)
+    if bias is not None:
+        want = dz.sum(0)
+        within(next(got), want, sum_tol.sum(0) + (64 + M // 8) * U * dz.abs().sum(0) + HALF[dtype] * want.abs() + TINY[dtype], what + " dbias", mean)
+    if residual is not None:
+        assert torch.equal(next(got).double(), dy), what
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+@pytest.mark.parametrize("M, K, N", SIZES)
+def test_forward_and_backward(gpu_device, M, K, N, cascade):
+    dtype, options, lost = CASCADES[cascade]
+    a, b, bias, residual, dy = operands(M, K, N, dtype, gpu_device)
+    for act in ACTIVATIONS:
+        for bi, r in ((bias, residual), (None, None), (None, residual), (bias, None)):
+            what = f"{act} bias={bi is not None} residual={r is not None}"
+            y = cascaded_lowp_matmul_epilogue(a, b, bias=bi, activation=act, residual=r, **options)
+            check_forward(y, a, b, bi, act, r, dtype, lost, what)
+            if (bi is None) != (r is None):
+                continue
+            leaves = [None if t is None else t.clone().requires_grad_() for t in (a, b, bi, r)]
+            y1 = cascaded_lowp_matmul_epilogue(leaves[0], leaves[1], bias=leaves[2], activation=act, residual=leaves[3], **options)
+            check_forward(y1, a, b, bi, act, r, dtype, lost, what + " differentiated")
+            check_backward(torch.autograd.grad(y1, [t for t in leaves if t is not None], dy), dy, a, b, bi, act, r, dtype, lost, what)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M, K, N", [(1, 64, 64), (2, 320, 1280), (154, 1280, 5120), (2048, 1280, 1280), (333, 456, 212), (70, 136, 33), (40, 5120, 640), (700, 1280, 100)])
+def test_prepared_weights(gpu_device, M, K, N, dtype):
+    a, b, bias, residual, _ = operands(M, K, N, dtype, gpu_device)
+    lost = CASCADES["fp32"][2] if dtype == torch.float32 else 0.0
+    pw = PreparedWeight(b)
+    for act in ACTIVATIONS:
+        y = cascaded_lowp_matmul_epilogue(a, pw, bias=bias, activation=act, residual=residual)
+        check_forward(y, a, b, bias, act, residual, dtype, lost, f"{act}")
+    y = cascaded_lowp_matmul_epilogue(a, pw)
+    check_forward(y, a, b, None, None, None, dtype, lost, "plain")
+    # rows off 16-byte boundaries
+    wide = torch.zeros(M, K + 11, dtype=dtype, device=gpu_device)
+    wide[:, 3:3 + K] = a
+    y = cascaded_lowp_matmul_epilogue(wide[:, 3:3 + K], pw, bias=bias, activation="silu", residual=residual)
+    check_forward(y, a, b, bias, "silu", residual, dtype, lost, "off the boundaries")
+
+
+def test_other_cascades_are_the_plain_product_with_the_epilogue_behind(gpu_device):
+    for lowp, terms in (("fp8", 3), ("fp8", 2), ("bf16", 3), ("fp16", 2)):
+        for M, K, N in ((130, 192, 320), (3, 77, 50)):
+            a, b, bias, residual, _ = operands(M, K, N, torch.float32, gpu_device)
+            z = cascaded_lowp_matmul(a, b, bias=bias, lowp=lowp, terms=terms).double()
+            y = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="gelu", residual=residual, lowp=lowp, terms=terms)
+            want = F.gelu(z) + residual.double()
+            within(y, want, 8 * U * (1 + z.abs()) + 2 * U * (want.abs() + residual.double().abs()), f"{lowp} x {terms}")
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+def test_no_inputs_rows_or_outputs(gpu_device, cascade):
+    dtype, options, _ = CASCADES[cascade]
+    for M, K, N in ((0, 8, 8), (4, 8, 0), (5, 0, 9), (0, 0, 0)):
+        a, b = torch.ones(M, K, dtype=dtype, device=gpu_device, requires_grad=True), torch.ones(K, N, dtype=dtype, device=gpu_device, requires_grad=True)
+        bias = torch.linspace(-1, 1, max(N, 1)).to(dtype).to(gpu_device)[:N].requires_grad_()
+        residual = torch.ones(M, N, dtype=dtype, device=gpu_device)
+        with torch.no_grad():
+            y = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="relu", residual=residual, **options)
+        assert torch.equal(y, (F.relu(bias.detach()) + 1).expand(M, N))
+        y = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="relu", residual=residual, **options)
+        da, db, dbias = torch.autograd.grad(y, (a, b, bias), torch.ones_like(y))
+        assert torch.equal(dbias, M * (bias > 0).to(dtype)) and bool((db == 0).all()) and da.shape == a.shape
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+def test_shapes_strides_and_results_in_place(gpu_device, cascade):
+    dtype, options, lost = CASCADES[cascade]
+    a, b, bias, residual, _ = operands(60, 136, 72, dtype, gpu_device)
+    want = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="gelu", residual=residual, **options)
+    how = dict(bias=bias, activation="gelu", **options)
+    y = cascaded_lowp_matmul_epilogue(a.view(3, 4, 5, 136), b, residual=residual.view(3, 4, 5, 72), **how)
+    assert y.shape == (3, 4, 5, 72) and torch.equal(y.view(60, 72), want)
+    assert torch.equal(cascaded_lowp_matmul_epilogue(a[7], b, residual=residual[7], **how), cascaded_lowp_matmul_epilogue(a[7:8], b, residual=residual[7:8], **how)[0])
+    # rows of larger tensors, for every operand and the result; what lies around the result stays
+    for pad in (8, 3):
+        big = [torch.full((62, w + 2 * pad), 5.0, dtype=dtype, device=gpu_device) for w in (136, 72, 72)]
+        va, vr, vo = big[0][1:61, pad:pad + 136], big[1][1:61, pad:pad + 72], big[2][1:61, pad:pad + 72]
+        va.copy_(a)
+        vr.copy_(residual)
+        got = cascaded_lowp_matmul_epilogue(va, b, residual=vr, out=vo, **how)
+        assert got.data_ptr() == vo.data_ptr()
+        check_forward(vo, a, b, bias, "gelu", residual, dtype, lost, f"strided {pad}")
+        vo.fill_(5.0)
+        assert bool((big[2] == 5.0).all())
+    # result and residual as columns of one tensor
+    both = torch.zeros(60, 144, dtype=dtype, device=gpu_device)
+    both[:, 72:] = residual
+    cascaded_lowp_matmul_epilogue(a, b, residual=both[:, 72:], out=both[:, :72], **how)
+    check_forward(both[:, :72], a, b, bias, "gelu", residual, dtype, lost, "side by side")
+    assert torch.equal(both[:, 72:], residual)
+    # transposed a
+    at = a.t().contiguous().t()
+    assert torch.equal(cascaded_lowp_matmul_epilogue(at, b, residual=residual, **how), want)
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+def test_broadcast_residuals(gpu_device, cascade):
+    dtype, options, lost = CASCADES[cascade]
+    a, b, bias, residual, dy = operands(60, 136, 72, dtype, gpu_device)
+    a3, dy3 = a.view(4, 15, 136), dy.view(4, 15, 72)
+    for r in (residual[0], residual[:1], residual[:15].view(1, 15, 72), residual[:4].view(4, 1, 72), residual[0, :1], residual[0, 0]):
+        full = r.expand(4, 15, 72).reshape(60, 72)
+        leaf = r.clone().requires_grad_()
+        y = cascaded_lowp_matmul_epilogue(a3, b, bias=bias, activation="silu", residual=r, **options)
+        check_forward(y.view(60, 72), a, b, bias, "silu", full, dtype, lost, f"{tuple(r.shape)}")
+        y = cascaded_lowp_matmul_epilogue(a3, b, bias=bias, activation="silu", residual=leaf, **options)
+        (g,) = torch.autograd.grad(y, leaf, dy3)
+        want = dy3.double().sum_to_size(r.shape)
+        within(g, want, HALF[dtype] * want.abs() + 72 * HALF[dtype] * dy3.double().abs().sum_to_size(r.shape), "its gradient")
+
+
+def test_gradients_of_some_operands(gpu_device):
+    a, b, bias, residual, dy = operands(90, 136, 72, torch.float16, gpu_device)
+    every = [t.clone().requires_grad_() for t in (a, b, bias, residual)]
+    want = torch.autograd.grad(cascaded_lowp_matmul_epilogue(every[0], every[1], bias=every[2], activation="gelu", residual=every[3]), every, dy)
+    for mask in range(1, 16):
+        leaves = [t.clone().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((a, b, bias, residual))]
+        y = cascaded_lowp_matmul_epilogue(leaves[0], leaves[1], bias=leaves[2], activation="gelu", residual=leaves[3])
+        y.backward(dy)
+        for leaf, grad in zip(leaves, want):
+            assert leaf.grad is None if not leaf.requires_grad else torch.equal(leaf.grad, grad)
+    # a gradient that is one value for every element, as a sum gives
+    y = cascaded_lowp_matmul_epilogue(every[0], every[1], bias=every[2], activation="gelu", residual=every[3])
+    ones = torch.autograd.grad(y.sum(), every, retain_graph=True)
+    again = torch.autograd.grad(y, every, torch.ones_like(y))
+    assert all(torch.equal(p, q) for p, q in zip(ones, again))
+
+
+def test_against_differences(gpu_device):
+    gen = torch.Generator().manual_seed(5)
+    a, b, bias, residual, dy = (torch.randn(*s, generator=gen) for s in ((20, 24), (24, 30), (30,), (20, 30), (20, 30)))
+    for act in ("gelu", "gelu_tanh", "silu", None):
+        def loss(a, b, bias, residual):
+            return ((ACTIVATIONS[act](a @ b / 5 + bias) + residual) * dy.double()).sum()
+
+        leaves = [t.to(gpu_device).requires_grad_() for t in (a, b / 5, bias, residual)]
+        y = cascaded_lowp_matmul_epilogue(leaves[0], leaves[1], bias=leaves[2], activation=act, residual=leaves[3], lowp="fp16", terms=3)
+        grads = list(torch.autograd.grad(y, leaves, dy.to(gpu_device)))
+        grads[1] = grads[1] / 5
+        at = [t.double() for t in (a, b, bias, residual)]
+        for i, grad in enumerate(grads):
+            direction = torch.randn(at[i].shape, generator=gen).double()
+            plus, minus = [t.clone() for t in at], [t.clone() for t in at]
+            plus[i] += 1e-5 * direction
+            minus[i] -= 1e-5 * direction
+            slope = (loss(*plus) - loss(*minus)) / 2e-5
+            scale = (grad.cpu().double() * direction).abs().sum()
+            assert abs(slope - (grad.cpu().double() * direction).sum()) <= 500 * U * scale + 1e-8 * scale
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_activations_over_the_whole_range(gpu_device, dtype):
+    """z as the bias of a product without inputs: single points, infinities and NaN."""
+    z = torch.cat([torch.linspace(-12, 12, 4801), torch.logspace(-30, 4, 400), -torch.logspace(-30, 4, 400), torch.zeros(1)]).to(dtype).to(gpu_device)
+    z = z[z.isfinite()]
+    none = torch.zeros(1, 0, dtype=dtype, device=gpu_device), torch.zeros(0, z.numel(), dtype=dtype, device=gpu_device)
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        leaf = z.clone().requires_grad_()
+        y = cascaded_lowp_matmul_epilogue(*none, bias=leaf, activation=act)[0]
+        want = ACTIVATIONS[act](z.double())
+        # (behind 12 relative only: an exponential's argument x log2(e), rounded, is off by u |x| log2(e), and the exponential by a relative u |x|: silu(-80)
+        # is off by 80 u of itself; a sigmoid below the normal numbers, 2^-126, counts as zero, and z times it, z from -88 to -104, is below 2^-119)
+        within(y, want, 8 * U * (1 + z.double().abs()) * (z.double().abs() < 12) + (4 + 2 * z.double().abs().clamp(max=150)) * U * want.abs() + HALF[dtype] * want.abs() + TINY[dtype] + 2.0 ** -119, act)
+        (g,) = torch.autograd.grad(y.sum(), leaf)
+        slope = slope_of(z.double(), act)
+        within(g, slope, 8 * U * (1 + z.double().abs()) * (z.double().abs() < 20) + (4 + 2 * z.double().abs().clamp(max=150)) * U * slope.abs() + HALF[dtype] * slope.abs() + TINY[dtype] + 2.0 ** -100, act + " slope")
+    ends = torch.tensor([math.inf, math.nan], dtype=dtype, device=gpu_device)
+    none = torch.zeros(1, 0, dtype=dtype, device=gpu_device), torch.zeros(0, 2, dtype=dtype, device=gpu_device)
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        y = cascaded_lowp_matmul_epilogue(*none, bias=ends, activation=act)[0]
+        assert float(y[0]) == math.inf and bool(y[1].isnan())
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+def test_nan_and_infinity_stay_in_their_rows(gpu_device, cascade):
+    dtype, options, _ = CASCADES[cascade]
+    if cascade == "fp32x3":
+        return      # (the scale of an operand is one for all its rows there)
+    a, b, bias, residual, _ = operands(140, 136, 72, dtype, gpu_device)
+    want = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="gelu", residual=residual, **options)
+    a[37, 5] = math.nan
+    residual[99, 3] = math.inf
+    y = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="gelu", residual=residual, **options)
+    assert bool(y[37].isnan().all()) and float(y[99, 3]) == math.inf
+    keep = torch.ones_like(y, dtype=torch.bool)
+    keep[37], keep[99, 3] = False, False
+    assert torch.equal(y[keep], want[keep])
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+def test_streams_graphs_and_repetition(gpu_device, cascade):
+    dtype, options, _ = CASCADES[cascade]
+    a, b, bias, residual, dy = operands(300, 640, 320, dtype, gpu_device)
+
+    def step(a, b, bias, residual, dy):
+        y = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="gelu", residual=residual, **options)
+        return (y, *torch.autograd.grad(y, (a, b, bias, residual), dy))
+
+    side, graphs = torch.cuda.Stream(), []
+    for seed in (1, 2):
+        ins = [t.clone().requires_grad_() for t in (a, b, bias, residual)] + [dy.clone()]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*ins)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(*ins)
+        graphs.append((graph, ins, outs, torch.Generator().manual_seed(seed)))
+    for _ in range(4):
+        for graph, ins, outs, gen in graphs:
+            with torch.no_grad():
+                for t in ins:
+                    t.copy_(torch.randn(t.shape, generator=gen) * 0.2)
+            graph.replay()
+            want = step(*[t.detach().clone().requires_grad_() for t in ins[:4]], ins[4])
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(outs, want))
+
+
+def test_a_block_of_them(gpu_device):
+    """A pre-norm feed-forward block and the norm of the next one, forward and backward: x1 = x + W2 gelu(W1 norm(x)), y = norm(x1)."""
+    gen = torch.Generator().manual_seed(77)
+    M, D, H = 700, 320, 1280
+    P = {"x": torch.randn(M, D, generator=gen), "g1": 1 + 0.1 * torch.randn(D, generator=gen), "c1": 0.1 * torch.randn(D, generator=gen),
+         "w1": torch.randn(D, H, generator=gen) / D ** 0.5, "b1": 0.1 * torch.randn(H, generator=gen), "w2": torch.randn(H, D, generator=gen) / H ** 0.5,
+         "b2": 0.1 * torch.randn(D, generator=gen), "g2": 1 + 0.1 * torch.randn(D, generator=gen), "c2": 0.1 * torch.randn(D, generator=gen)}
+    dy, ds = torch.randn(M, D, generator=gen), torch.randn(M, D, generator=gen)
+
+    def block(p, norm, add_norm, product, split):
+        h = product(norm(p["x"], p["g1"], p["c1"]), p["w1"], p["b1"], "gelu", None)
+        if split:
+            return add_norm(product(h, p["w2"], p["b2"], None, None), p["x"], p["g2"], p["c2"])
+        s = product(h, p["w2"], p["b2"], None, p["x"])
+        return norm(s, p["g2"], p["c2"]), s
+
+    def plain(p):
+        n = lambda x, g, c: F.layer_norm(x, (D,), g, c, 1e-5)   # noqa: E731
+        def pr(a, b, bias, act, r):
+            y = ACTIVATIONS[act](a @ b + bias)
+            return y if r is None else y + r
+        return block(p, n, None, pr, False)
+
+    for dtype, options, bound in ((torch.float32, {"lowp": "fp16", "terms": 3}, 2e-6), (torch.float16, {}, 4 * HALF[torch.float16]), (torch.bfloat16, {}, 4 * HALF[torch.bfloat16])):
+        own = lambda a, b, bias, act, r: cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation=act, residual=r, **options)   # noqa: E731
+        q = {k: v.to(dtype).to(gpu_device) for k, v in P.items()}
+        e = {k: v.double().requires_grad_() for k, v in q.items()}
+        d1, d2 = dy.to(dtype).to(gpu_device), ds.to(dtype).to(gpu_device)
+        want = plain(e)
+        wanted = [*want, *torch.autograd.grad(want, list(e.values()), (d1.double(), d2.double()))]
+        for split in (False, True):
+            leaves = {k: v.clone().requires_grad_() for k, v in q.items()}
+            got = block(leaves, layer_norm, add_layer_norm, own, split)
+            gots = [*got, *torch.autograd.grad(got, list(leaves.values()), (d1, d2))]
+            for name, p, w in zip(["y", "s", *P], gots, wanted):
+                # (a handful of roundings one behind the other, each of at most a half step and of independent signs: four in the mean square)
+                assert float((p.detach().double() - w.detach()).norm() / w.detach().norm()) <= bound, (dtype, split, name)
+
+
+def test_refusals(gpu_device):
+    a, b = torch.zeros(4, 16, device=gpu_device), torch.zeros(16, 8, device=gpu_device)
+    bad = [(dict(activation="tanh"), ValueError), (dict(products="all"), ValueError), (dict(lowp="fp4"), ValueError), (dict(bias=torch.zeros(7, device=gpu_device)), ValueError),
+           (dict(bias=torch.zeros(8, device=gpu_device, dtype=torch.float16)), ValueError), (dict(residual=torch.zeros(4, 8)), ValueError),
+           (dict(residual=torch.zeros(4, 8, device=gpu_device, dtype=torch.float16)), ValueError), (dict(residual=torch.zeros(3, 8, device=gpu_device)), ValueError),
+           (dict(residual=torch.zeros(2, 4, 8, device=gpu_device)), ValueError), (dict(out=torch.zeros(4, 9, device=gpu_device)), ValueError),
+           (dict(out=torch.zeros(4, 8, device=gpu_device, dtype=torch.float16)), ValueError), (dict(out=torch.zeros(8, 4, device=gpu_device).t()), ValueError),
+           (dict(out=torch.zeros(1, 8, device=gpu_device).expand(4, 8)), ValueError), (dict(out=a.view(8, 8)[:4]), ValueError)]
+    for change, error in bad:
+        with pytest.raises(error):
+            cascaded_lowp_matmul_epilogue(a, b, **change)
+    r = torch.zeros(4, 8, device=gpu_device)
+    with pytest.raises(ValueError, match="overlaps"):
+        cascaded_lowp_matmul_epilogue(a, b, residual=r, out=r)
+    for pair, error in (((a, b.t()), ValueError), ((a, b.half()), TypeError), ((a.double(), b.double()), TypeError), ((a, b.view(1, 16, 8)), ValueError),
+                        ((a[:, :8], b), ValueError), ((a, b.t().contiguous().t()), ValueError), ((a, b.cpu()), RuntimeError)):
+        with pytest.raises(error):
+            cascaded_lowp_matmul_epilogue(*pair)
+    pw = PreparedWeight(torch.zeros(64, 8, device=gpu_device))
+    x = torch.zeros(4, 64, device=gpu_device)
+    assert cascaded_lowp_matmul_epilogue(x, pw).shape == (4, 8)
+    for args, change in (((x.requires_grad_(), pw), {}), ((x.detach(), pw), dict(bias=torch.zeros(8, device=gpu_device, requires_grad=True))),
+                         ((a.clone().requires_grad_(), b), dict(out=torch.zeros(4, 8, device=gpu_device)))):
+        with pytest.raises(RuntimeError):
+            cascaded_lowp_matmul_epilogue(*args, **change)
+    with torch.no_grad():
+        assert cascaded_lowp_matmul_epilogue(x, pw).shape == (4, 8)
+    for change in (dict(lowp="fp16"), dict(terms=3)):
+        with pytest.raises(ValueError):
+            cascaded_lowp_matmul_epilogue(x.detach(), pw, **change)
+    with pytest.raises(ValueError):
+        cascaded_lowp_matmul_epilogue(x.detach(), PreparedWeight(torch.zeros(64, 128, device=gpu_device), glu=True))
+    leaf = a.clone().requires_grad_()
+    (g,) = torch.autograd.grad(cascaded_lowp_matmul_epilogue(leaf, b).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

@@ -1,0 +1,85 @@
+"""Products with an epilogue without a GPU: what the C entry points and the Python function refuse, before anything is launched."""
+import pytest
+import torch
+
+from basedxl_amd import _lib, cascaded_lowp_matmul_epilogue
+from basedxl_amd.matmul_epilogue import _overlap, _residual_rows
+
+F32, F16, BF16 = _lib.DT_F32, _lib.DT_F16, _lib.DT_BF16
+P = 1 << 20   # (stands for a device pointer: the checks come before any launch)
+
+
+def product(A=P, B=P, prepared=0, C=P, bias=None, residual=None, preact=None, M=4, N=8, K=16, lda=16, ldb=8, ldc=8, ldr=8, ldp=8, dtype=F32, fmt=0, terms=2,
+            products=0, activation=2, ws=None, nbytes=0):
+    return _lib.lib().cascmm_gemm_epilogue(A, B, prepared, C, bias, residual, preact, M, N, K, lda, ldb, ldc, ldr, ldp, dtype, fmt, terms, products, activation,
+                                           None, ws, nbytes, None)
+
+
+def backward(dy=P, z=P, dz=P, dbias=P, rows=4, cols=8, lddy=8, ldz=8, lddz=8, activation=2, dtype=F32, ws=P, nbytes=1 << 20):
+    return _lib.lib().cascmm_epilogue_backward(dy, z, dz, dbias, rows, cols, lddy, ldz, lddz, activation, dtype, ws, nbytes, None)
+
+
+def transpose(x=P, out=P, rows=4, cols=8, ldx=8, ldo=4, dtype=F32):
+    return _lib.lib().cascmm_transpose(x, out, rows, cols, ldx, ldo, dtype, None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(dtype=9), -3), (dict(fmt=9), -4), (dict(terms=4), -4), (dict(products=2), -4), (dict(activation=-1), -4), (dict(activation=5), -4), (dict(M=-1), -2),
+    (dict(lda=15), -2), (dict(ldb=7), -2), (dict(ldc=7), -2), (dict(residual=P, ldr=7), -2), (dict(residual=P, ldr=-8), -2), (dict(preact=P, ldp=7), -2),
+    (dict(C=None), -1), (dict(A=None), -1), (dict(B=None), -1), (dict(C=P + 2), -6), (dict(residual=P + 2), -6), (dict(preact=P + 1), -6), (dict(A=P + 2), -6),
+    (dict(bias=P + 2), -6), (dict(M=2 ** 31), -9), (dict(M=0, A=None), 0), (dict(N=0, ldb=0, ldc=0, B=None), 0)])
+def test_product_arguments(change, status):
+    assert product(**change) == status
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(dtype=9), -3), (dict(activation=5), -4), (dict(rows=-1), -2), (dict(lddy=7), -2), (dict(ldz=7), -2), (dict(lddz=7), -2), (dict(dy=None), -1),
+    (dict(z=None), -1), (dict(dy=P + 2), -6), (dict(dz=P + 2), -6), (dict(dbias=P + 2), -6), (dict(ws=None), -5), (dict(nbytes=4), -5), (dict(ws=P + 4), -6),
+    (dict(rows=2 ** 31), -9), (dict(dz=None, dbias=None), 0), (dict(rows=0, dbias=None, dy=None, z=None), 0), (dict(cols=0, lddy=0, ldz=0, lddz=0, dy=None), 0)])
+def test_backward_arguments(change, status):
+    assert backward(**change) == status
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(dtype=9), -3), (dict(rows=-1), -2), (dict(ldx=7), -2), (dict(ldo=3), -2), (dict(x=None), -1), (dict(out=None), -1), (dict(x=P + 2), -6), (dict(out=P + 2), -6),
+    (dict(rows=2 ** 30 + 1, ldo=2 ** 31), -9), (dict(rows=2 ** 20, cols=2 ** 20, ldx=2 ** 20, ldo=2 ** 20), -9), (dict(rows=0, x=None), 0),
+    (dict(cols=0, ldx=0, x=None), 0)])
+def test_transpose_arguments(change, status):
+    assert transpose(**change) == status
+
+
+def test_workspace_of_the_sums():
+    size = _lib.lib().cascmm_epilogue_workspace_bytes
+    assert size(-1, 8, F32) == size(8, -1, F32) == size(8, 8, 7) == size(4, 0, F32) == 0
+    for rows, cols in ((0, 5), (1, 1280), (65536, 1280), (3, 20000)):
+        for dtype in (F32, F16, BF16):
+            assert size(rows, cols, dtype) >= 4 * cols and size(rows, cols, dtype) % (4 * cols) == 0
+
+
+def test_tensors_off_the_gpu_are_refused():
+    with pytest.raises(RuntimeError, match="only runs on an AMD GPU"):
+        cascaded_lowp_matmul_epilogue(torch.zeros(2, 8), torch.zeros(8, 4))
+
+
+def test_which_tensors_overlap():
+    buf = torch.zeros(6, 32)
+    assert _overlap(buf, buf) and _overlap(buf[1:3], buf[2:4]) and not _overlap(buf[:3], buf[3:])
+    assert not _overlap(buf[:, :16], buf[:, 16:]) and not _overlap(buf[:, 16:], buf[:, :16]) and not _overlap(buf[1:, 16:], buf[:4, :16])
+    assert _overlap(buf[:, :17], buf[:, 16:]) and _overlap(buf[:, 16:], buf[:, :17]) and _overlap(buf[:, 8:16], buf[0])
+    assert not _overlap(buf[:0], buf) and not _overlap(buf, torch.zeros(6, 32))
+    assert _overlap(buf[:1, :8], buf[0, 4:12]) and not _overlap(buf[:1, :8], buf[0, 8:12])
+
+
+def test_rows_of_a_residual():
+    t = torch.arange(24.0).view(4, 6)
+    assert _residual_rows(t, 4, 6)[1] == 6 and _residual_rows(t[1:2], 1, 6)[1] == 6
+    for r in (t[0].expand(4, 6), t[:1].expand(4, 6), t[0].expand(2, 2, 6)):
+        row, ld = _residual_rows(r, 4, 6)
+        assert ld == 0 and torch.equal(row, t[0])
+    row, ld = _residual_rows(t[:, :1].expand(4, 6), 4, 6)
+    assert ld == 6 and torch.equal(row, t[:, :1].expand(4, 6))
+    row, ld = _residual_rows(t[0, 0].expand(4, 6), 4, 6)
+    assert ld == 0 and torch.equal(row, torch.zeros(6))
+    row, ld = _residual_rows(t.view(2, 2, 6)[:1].expand(2, 2, 6), 4, 6)
+    assert ld == 6 and torch.equal(row, t[[0, 1, 0, 1]])
+    assert _residual_rows(torch.zeros(4, 9)[:, 1:7], 4, 6)[1] == 9
