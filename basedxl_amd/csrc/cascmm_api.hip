@@ -72,6 +72,7 @@ struct Problem {
   // stages, of which the operands hold k_valid, and their rows need no alignment
   bool split_first = false;
   int64_t k_valid = 0;
+  const Epilogue* epi = nullptr;   // what follows the product (one problem)
   bool whole_k = false;   // no K split over workgroups (cascmm_ksplit.h)
 };
 
@@ -1172,7 +1173,26 @@ static int gemm_on_rows(int count, const void* const* A, const void* const* B, v
   for (int i = 0; i < count; ++i) {
     p.A[i] = A[i]; p.B[i] = B[i]; p.C[i] = C[i]; p.bias[i] = bias ? bias[i] : nullptr;
   }
-  return v.launch(p, stream);
+  if (!q.epi) return v.launch(p, stream);
+  // the epilogue: in the store where the kernel has one that holds it, else behind it, on z in preact or in the result's place (z is rounded to the
+  // elements' type then: 16-bit elements meet that in the bounds-checked kernels only)
+  const Epilogue& ep = *q.epi;
+  if (v.kind == KIND_H16 || v.kind == KIND_HWK) {
+    p.epi = 1;
+    p.act = ep.act;
+    p.residual = ep.residual;
+    p.preact = ep.preact;
+    p.ldr = ep.residual ? ep.ldr : 0;
+    p.ldp = ep.preact ? ep.ldp : 0;
+    return v.launch(p, stream);
+  }
+  if (ep.preact) {
+    p.C[0] = ep.preact;
+    p.ldc = ep.ldp;
+  }
+  const int st = v.launch(p, stream);
+  if (st != CASCMM_OK || (!ep.preact && !ep.residual && !ep.act)) return st;
+  return launch_epilogue(p.C[0], p.ldc, ep.residual, ep.ldr, C[0], q.ldc, q.M, q.N, ep.act, q.dtype, stream);
 }
 
 // whether the rows of A are whole 16-byte chunks by K alone
@@ -1693,7 +1713,12 @@ int cascmm_gemm_epilogue(const void* A, const void* B, int b_prepared, void* C, 
   const size_t es = dtype_size(dtype);
   if (!C) return CASCMM_ERR_NULL_POINTER;
   if (!aligned_to(C, es) || !aligned_to(residual, es) || !aligned_to(preact, es)) return CASCMM_ERR_ALIGNMENT;
-  // the product where its values before the activation are wanted, or in place of the result
+  const Epilogue ep{activation, residual, ldr, preact, ldp};
+  if (K > 0) {
+    q.epi = &ep;
+    return gemm_impl(1, &A, &B, &C, bias ? &bias : nullptr, q, tensor_exps, workspace, workspace_bytes, (hipStream_t)stream, -1);
+  }
+  // (no inputs: z is the bias or zero, which its kernel writes in preact or in the result's place)
   void* z = preact ? preact : C;
   const int64_t ldz = preact ? ldp : ldc;
   q.ldc = ldz;

@@ -378,6 +378,12 @@ struct GroupParams {
   // host side only: when set, the variant's launch function stores the handle of its GEMM kernel here
   // and returns without checking or launching anything (the library names its kernels this way)
   const void** kernel_out;
+  // Epilogue (one problem): C = act(z) + residual, z = A . B + bias, and z itself to preact where that is set (see cascmm_epilogue.h).  Set for
+  // the kernels whose store holds it only
+  int epi, act;
+  const void* residual;
+  void* preact;
+  int64_t ldr, ldp;
   // kernels that split their operands into slots first (three fp8 / fp16 terms): K is rounded up to whole stages, the
   // operands hold k_valid of it and the slots beyond are zeros
   int k_valid;

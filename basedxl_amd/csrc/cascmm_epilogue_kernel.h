@@ -11,30 +11,10 @@
 //
 // Bound by memory: 16 bytes a load, rows of any alignment.
 #pragma once
+#include "cascmm_activation.h"
 #include "cascmm_norm_kernel.h"
 
 namespace cascmm {
-
-constexpr float kLog2e = 1.4426950408889634f;
-// 1 / (1 + exp(-x))
-__device__ __forceinline__ float sigmoid_value(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * x)); }
-__device__ __forceinline__ float gelu_tanh_twice_u(float z) { return 1.5957691216057308f * z * __builtin_fmaf(0.044715f * z, z, 1.f); }
-
-// act of several at a time (kinds are uniform: one branch)
-template <int N> __device__ __forceinline__ void activate(float (&v)[N], int act) {
-  if (act == CASCMM_ACT_GELU) {
-    gelu_values(v);
-  } else if (act == CASCMM_ACT_GELU_TANH) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] *= sigmoid_value(gelu_tanh_twice_u(v[e]));
-  } else if (act == CASCMM_ACT_SILU) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] *= sigmoid_value(v[e]);
-  } else if (act == CASCMM_ACT_RELU) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
-  }
-}
 
 __device__ __forceinline__ float clamped(float z, float most) { return z > most ? most : z < -most ? -most : z; }
 // d[e] *= act'(z[e])

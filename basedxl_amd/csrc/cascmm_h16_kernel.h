@@ -26,6 +26,7 @@
 #pragma once
 #include <type_traits>
 
+#include "cascmm_activation.h"
 #include "cascmm_ksplit.h"
 
 namespace cascmm {
@@ -91,12 +92,13 @@ template <> struct H16Elem<CASCMM_FMT_FP16> { typedef _Float16 T; static constex
 // N % 2 == 0 and rows on dwords, K * ldb * 2 below 2 GiB.  Any M and N: rows and columns past the edge are loaded as zeros or as
 // some other column's values and not stored.  grid.y: the problem of a group.  k_splits > 1: K in splits of k_per (a
 // multiple of 64), fp32 sums to the workspace instead of a result, see cascmm_ksplit.h.
-// GLU: gated store (see GroupParams; RAWB = 0, NTL even: a wave owns whole value / gate pairs of blocks).
+// GLU = 1: gated store (see GroupParams; RAWB = 0, NTL even: a wave owns whole value / gate pairs of blocks); 2: the epilogue of GroupParams.
 template <class T, int FMT, int RAWB, int GLU>
 __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams p) {
   typedef typename H16Elem<FMT>::T E;
   typedef IoType<H16Elem<FMT>::DT> Io;
-  static_assert(!GLU || (!RAWB && T::NTL % 2 == 0), "the gated store pairs a wave's blocks");
+  constexpr bool GATED = GLU == 1;
+  static_assert(!GATED || (!RAWB && T::NTL % 2 == 0), "the gated store pairs a wave's blocks");
   extern __shared__ __attribute__((aligned(1024))) unsigned char h16_smem[];
   unsigned char* smem = h16_smem;
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, g = lane >> 5;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
   __syncthreads();
 
   // ---- two wave groups: each finishes its share of the blocks, the other one's sums come through LDS ----
-  constexpr int OB = GLU ? T::NTL / 2 : T::NTL;              // 32-column blocks of C per row block
+  constexpr int OB = GATED ? T::NTL / 2 : T::NTL;              // 32-column blocks of C per row block
   constexpr int HALF = T::WK == 2 ? (OB + 1) / 2 : OB;       // wave group 0: blocks 0 .. HALF - 1, group 1: the others
   unsigned char* area = smem + wave * T::OUT_WAVE;
   // (The store is straight-line code that every wave runs once, so its length is time: instructions come from L2 at
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
   auto finish = [&](auto first_tag, auto count_tag, auto bias_tag) {
     constexpr int B0 = decltype(first_tag)::value, NB = decltype(count_tag)::value;
     constexpr bool BIAS = decltype(bias_tag)::value != 0;
-    if constexpr (!BIAS && !GLU) {
+    if constexpr (!BIAS && !GATED) {
       if (p.k_splits > 1) {   // (a lane's four consecutive columns of its row; the wave's rows of a block, 32 bytes each)
         const int row = (p.N + 3) & ~3, col0 = n0 + wn0 + 32 * B0;
         float* part = (float*)p.workspace + ((int64_t)split * p.M + m0 + wm0) * row + col0;
@@ -357,15 +359,15 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
       }
     }
     // ---- store: of block (mi, ni) a lane holds row 32 mi + l31, columns 32 ni + 8 q + 4 g + e in register 4 q + e ----
-    const int no = GLU ? p.N >> 1 : p.N;
-    const int oc0 = (GLU ? (n0 + wn0) >> 1 : n0 + wn0) + 32 * B0;
+    const int no = GATED ? p.N >> 1 : p.N;
+    const int oc0 = (GATED ? (n0 + wn0) >> 1 : n0 + wn0) + 32 * B0;
     float* bl = (float*)(area + 32 * T::OUT_ROW);   // the wave's bias values, in the order of its columns
     if constexpr (BIAS) {
       const E* bias = (const E*)p.bias[prob];
-      for (int c = lane; c < NB * (GLU ? 64 : 32); c += 64) {
+      for (int c = lane; c < NB * (GATED ? 64 : 32); c += 64) {
         // (gated: blocks alternate value and gate columns)
-        const int col = GLU ? oc0 + (c >> 6) * 32 + (c & 31) : oc0 + c;
-        bl[c] = col < no ? Io::load(bias + (GLU && (c & 32) ? no : 0) + col) : 0.f;
+        const int col = GATED ? oc0 + (c >> 6) * 32 + (c & 31) : oc0 + c;
+        bl[c] = col < no ? Io::load(bias + (GATED && (c & 32) ? no : 0) + col) : 0.f;
       }
     }
     E* C = (E*)p.C[prob] + (int64_t)(m0 + wm0) * p.ldc + oc0;
@@ -408,14 +410,14 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
         // (The large tiles' sums stay in the accumulation registers up to here.  Left alone the compiler moves all of them to ordinary ones
         // behind the loop, through scratch memory what does not fit: 26 k cycles of store in place of 16 k on 256 x 320, 16 k in place of
         // 10 k on 256 x 256; gated, and of smaller tiles, its own order is the better one.)
-        if (!GLU && T::MT * T::NTL >= 16 && mi * T::NTL + B0 + b < 16) asm volatile("" : "+a"(acc[mi][B0 + b]));
+        if (!GATED && T::MT * T::NTL >= 16 && mi * T::NTL + B0 + b < 16) asm volatile("" : "+a"(acc[mi][B0 + b]));
         // (a block's bias values at once: quad by quad, every quad waits for its own)
         f32x4 bv[4], bg[4];
         if constexpr (BIAS) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            bv[q] = *(const f32x4*)(bl + (GLU ? 64 : 32) * b + 8 * q + 4 * g);
-            if constexpr (GLU) bg[q] = *(const f32x4*)(bl + 64 * b + 32 + 8 * q + 4 * g);
+            bv[q] = *(const f32x4*)(bl + (GATED ? 64 : 32) * b + 8 * q + 4 * g);
+            if constexpr (GATED) bg[q] = *(const f32x4*)(bl + 64 * b + 32 + 8 * q + 4 * g);
           }
         }
         auto sum = [&](int block, const f32x4* bias4, int q, int x) { return BIAS ? acc[mi][block][4 * q + x] + bias4[q][x] : acc[mi][block][4 * q + x]; };
@@ -423,7 +425,7 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
         for (int q = 0; q < 4; ++q) {
           typedef E e2 __attribute__((ext_vector_type(2)));
           float y[4];
-          if constexpr (GLU) {
+          if constexpr (GATED) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) y[x] = sum(2 * b + 1, bg, q, x);
             gelu_values(y);
@@ -469,12 +471,127 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
       }
     }
   };
+  // The epilogue's store: z = sums + bias as fp32 through the wave's LDS area, CB blocks of columns at a time, then 16 bytes of a row a lane.  The residual's
+  // chunks are asked for while the run before is at work (behind one of a few its loads were waited for); z to preact and the activation are a
+  // loop over LDS of their own, which keeps five activations out of the straight code (instructions come from L2 at some 10 KB per us).
+  auto epilogue = [&](auto first_tag, auto count_tag) {
+    constexpr int B0 = decltype(first_tag)::value, NB = decltype(count_tag)::value, CB = NB <= 5 ? NB : 5, GROUPS = NB / CB;
+    constexpr int ROW = CB * 128 + 16, CHUNKS = 4 * CB, ITS = 2 * CB;   // bytes of a row; 16-byte chunks of a row of C, a lane's of 32 rows
+    constexpr int AREA = T::LDS_BYTES / 4 / 16 * 16;
+    static_assert(NB % CB == 0 && 32 * ROW + NB * 128 <= AREA, "a wave's area");
+    unsigned char* own = smem + wave * AREA;
+    float* bl = (float*)(own + 32 * ROW);
+    const int N = p.N, oc0 = n0 + wn0 + 32 * B0, act = p.act;
+    const E *bias = (const E*)p.bias[prob], *res = (const E*)p.residual;
+    E *C = (E*)p.C[prob], *pre = (E*)p.preact;
+    const int64_t ldc = p.ldc, ldr = p.ldr, ldp = p.ldp, row0 = m0 + wm0;
+    for (int c = lane; c < NB * 32; c += 64) bl[c] = bias && oc0 + c < N ? Io::load(bias + oc0 + c) : 0.f;
+    const bool near_rows = (ldc > ldr ? (ldc > ldp ? ldc : ldp) : (ldr > ldp ? ldr : ldp)) * (2 * T::WTM) <= 0x7FFFFFFF;
+    const bool vec = near_rows && ((ldc | ldr | ldp | N) & 7) == 0 && (((uintptr_t)C | (uintptr_t)res | (uintptr_t)pre) & 15) == 0;
+    // (rows past M fall beyond the end of a buffer, columns past N are sent there; of one residual row for all, all rows are that one)
+    auto rows_of = [&](const E* base, int64_t ld) {
+      const int64_t bytes = ((p.M - 1 - row0) * ld + (N - oc0)) * 2;
+      return make_rsrc(base + row0 * ld + oc0, bytes < 0 ? 0 : bytes);
+    };
+    const i32x4 rc = rows_of(C, ldc), rr = rows_of(res, ldr), rp = rows_of(pre, ldp);
+    auto offset = [&](int mi, int gr, int it, int64_t ld) {
+      const int i = it * 64 + lane, c = gr * CB * 32 + i % CHUNKS * 8;
+      return oc0 + c < N ? (mi * 32 + i / CHUNKS) * (int)(ld * 2) + c * 2 : 0x7FFFFFFF;
+    };
+    u32x4 ahead[2][ITS];
+    auto ask = [&](int mi, int gr, u32x4 (&to)[ITS]) {
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) to[it] = __builtin_bit_cast(u32x4, llvm_raw_buffer_load_v4f32(rr, offset(mi, gr, it, ldr), 0, 0));
+    };
+    if (vec && res) ask(0, 0, ahead[0]);
+#pragma unroll
+    for (int mi = 0; mi < T::MT; ++mi)
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        constexpr int RUNS = T::MT * GROUPS;
+        const int run = mi * GROUPS + gr;
+#pragma unroll
+        for (int b = 0; b < CB; ++b) {
+          const int block = B0 + gr * CB + b;
+          if (T::MT * T::NTL >= 16 && mi * T::NTL + block < 16) asm volatile("" : "+a"(acc[mi][block]));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 bv = *(const f32x4*)(bl + (gr * CB + b) * 32 + 8 * q + 4 * g);
+            f32x4 z;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) z[x] = acc[mi][block][4 * q + x] + bv[x];
+            *(f32x4*)(own + l31 * ROW + (32 * b + 8 * q + 4 * g) * 4) = z;
+          }
+        }
+        if (vec) {
+          if (res && run + 1 < RUNS) ask((run + 1) / GROUPS, (run + 1) % GROUPS, ahead[(run + 1) & 1]);
+          if (act || pre) {
+#pragma unroll 1
+            for (int it = 0; it < ITS; ++it) {
+              const int i = it * 64 + lane;
+              f32x4* at = (f32x4*)(own + i / CHUNKS * ROW + i % CHUNKS * 32);
+              const f32x4 lo = at[0], hi = at[1];
+              float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+              if (pre) {
+                typedef E e8 __attribute__((ext_vector_type(8)));
+                e8 h;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[e] = (E)v[e];
+                llvm_raw_buffer_store_v4f32(__builtin_bit_cast(f32x4, h), rp, offset(mi, gr, it, ldp), 0, 0);
+              }
+              activate(v, act);
+              at[0] = (f32x4){v[0], v[1], v[2], v[3]};
+              at[1] = (f32x4){v[4], v[5], v[6], v[7]};
+            }
+          }
+#pragma unroll
+          for (int it = 0; it < ITS; ++it) {
+            typedef E e8 __attribute__((ext_vector_type(8)));
+            const int i = it * 64 + lane;
+            const f32x4* at = (const f32x4*)(own + i / CHUNKS * ROW + i % CHUNKS * 32);
+            const f32x4 lo = at[0], hi = at[1];
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if (res) {
+              const e8 r = __builtin_bit_cast(e8, ahead[run & 1][it]);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] += (float)r[e];
+            }
+            e8 y;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = (E)v[e];
+            llvm_raw_buffer_store_v4f32(__builtin_bit_cast(f32x4, y), rc, offset(mi, gr, it, ldc), 0, 0);
+          }
+        } else {
+          // rows off 16-byte chunks, or too far apart for 32-bit offsets: an element a lane, eight of them at a time
+#pragma unroll 1
+          for (int i0 = lane; i0 < 32 * CB * 32; i0 += 8 * 64) {
+            float v[8], r[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int i = i0 + 64 * u, row = i / (32 * CB), c = i % (32 * CB), col = oc0 + gr * CB * 32 + c;
+              const int64_t at = row0 + mi * 32 + row;
+              v[u] = *(const float*)(own + row * ROW + c * 4);
+              r[u] = res && at < p.M && col < N ? Io::load(res + at * ldr + col) : 0.f;
+              if (pre && at < p.M && col < N) Io::store(pre + at * ldp + col, v[u]);
+            }
+            activate(v, act);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int i = i0 + 64 * u, row = i / (32 * CB), c = i % (32 * CB), col = oc0 + gr * CB * 32 + c;
+              const int64_t at = row0 + mi * 32 + row;
+              if (at < p.M && col < N) Io::store(C + at * ldc + col, v[u] + r[u]);
+            }
+          }
+        }
+      }
+  };
   auto with_bias = [&](auto first, auto count) {
-    if (p.bias[prob]) finish(first, count, std::integral_constant<int, 1>{});
+    if constexpr (GLU == 2) epilogue(first, count);
+    else if (p.bias[prob]) finish(first, count, std::integral_constant<int, 1>{});
     else finish(first, count, std::integral_constant<int, 0>{});
   };
   if constexpr (T::WK == 2) {
-    static_assert(T::MT == 1 && !GLU, "one row block per wave");
+    static_assert(T::MT == 1 && !GATED, "one row block per wave");
     unsigned char* other = smem + (wave ^ (T::WM * T::WN)) * T::OUT_WAVE;
 #pragma unroll
     for (int b = 0; b < T::NTL; ++b)
@@ -494,6 +611,7 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[0][b][4 * q + e] += o[e];
         }
+    if (GLU == 2) __syncthreads();   // (its areas lie elsewhere)
     if (wk == 0) with_bias(std::integral_constant<int, 0>{}, std::integral_constant<int, HALF>{});
     else with_bias(std::integral_constant<int, HALF>{}, std::integral_constant<int, OB - HALF>{});
   } else {

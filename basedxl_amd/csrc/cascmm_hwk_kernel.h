@@ -37,15 +37,16 @@ struct HWK {
 // Host-checked, as for cascmm_h16_kernel: the rows of A start on dwords and are whole 16-byte chunks, zeros past K (K % 8 == 0, or
 // padded); RAWB = 0: B prepared (prepared_kgroups(K) x N slots, zeros beyond K), 2 GiB not reached with K rounded up to 64; RAWB = 1:
 // B [K][ldb] with N % 2 == 0 and rows on dwords, (K + 64) * ldb * 2 below 2 GiB.  Any M and N: rows past M read as zero, columns past the
-// edge as some other column's, neither is stored.  GLU (RAWB = 0, NB = 4): the gated store, C has N / 2 columns, B alternates 32
-// value and 32 gate columns.
+// edge as some other column's, neither is stored.  GLU = 1 (RAWB = 0, NB = 4): the gated store, C has N / 2 columns, B alternates 32
+// value and 32 gate columns.  GLU = 2: the epilogue of GroupParams.
 template <int MB, int NB, int FMT, int RAWB, int GLU>
 __global__ __launch_bounds__(512) void cascmm_hwk_kernel(const GroupParams p) {
   typedef HWK<MB, NB, RAWB> T;
   typedef Lowp<FMT> L;
   typedef typename H16Elem<FMT>::T E;
   typedef IoType<H16Elem<FMT>::DT> Io;
-  static_assert(!GLU || (!RAWB && NB == 4), "a value block and its gate block in one tile");
+  constexpr bool GATED = GLU == 1;   // (2: the epilogue of GroupParams)
+  static_assert(!GATED || (!RAWB && NB == 4), "a value block and its gate block in one tile");
   static_assert(!RAWB || NB == 2 || NB == 4, "whole dwords of a row of B");
   extern __shared__ __attribute__((aligned(1024))) unsigned char hwk_smem[];
   const int tid = threadIdx.x, lane = tid & 63, lw = lane & 15, kg = lane >> 4;
@@ -203,24 +204,25 @@ __global__ __launch_bounds__(512) void cascmm_hwk_kernel(const GroupParams p) {
       part[((wave * MB + mb) * NB + i) * 64 + lane] = v;
     }
   __syncthreads();
-  const int no = GLU ? N >> 1 : N;
+  const int no = GATED ? N >> 1 : N;
   E* C = (E*)p.C[prob];
   const E* bias = (const E*)p.bias[prob];
   typedef E e4 __attribute__((ext_vector_type(4)));
-  const bool vec = (p.ldc & 3) == 0 && (no & 3) == 0 && ((uintptr_t)C & 7) == 0;
-  constexpr int OB = GLU ? NB / 2 : NB, QUADS = MB * OB * 64;
+  bool vec = (p.ldc & 3) == 0 && (no & 3) == 0 && ((uintptr_t)C & 7) == 0;
+  if constexpr (GLU == 2) vec = vec && ((p.ldr | p.ldp) & 3) == 0 && (((uintptr_t)p.residual | (uintptr_t)p.preact) & 7) == 0;
+  constexpr int OB = GATED ? NB / 2 : NB, QUADS = MB * OB * 64;
 #pragma unroll
   for (int q = 0; q < (QUADS + T::NT - 1) / T::NT; ++q) {
     const int pos = q * T::NT + tid;
     if (QUADS % T::NT != 0 && pos >= QUADS) break;
     const int blk = pos >> 6, ln = pos & 63, mb = blk / OB, i = blk % OB;
     const int row = m0 + 16 * mb + (ln & 15);
-    const int col = (GLU ? n0 >> 1 : n0) + (RAWB ? 4 * NB * (ln >> 4) + 4 * i : 16 * i + 4 * (ln >> 4));
+    const int col = (GATED ? n0 >> 1 : n0) + (RAWB ? 4 * NB * (ln >> 4) + 4 * i : 16 * i + 4 * (ln >> 4));
     f32x4 s = {0.f, 0.f, 0.f, 0.f}, g = s;
 #pragma unroll
     for (int w = 0; w < T::NW; ++w) {
       s += part[((w * MB + mb) * NB + i) * 64 + ln];
-      if constexpr (GLU) g += part[((w * MB + mb) * NB + i + 2) * 64 + ln];
+      if constexpr (GATED) g += part[((w * MB + mb) * NB + i + 2) * 64 + ln];
     }
     if (row >= M || col >= no) continue;
     if (bias) {
@@ -228,15 +230,16 @@ __global__ __launch_bounds__(512) void cascmm_hwk_kernel(const GroupParams p) {
       for (int e = 0; e < 4; ++e)
         if (col + e < no) {
           s[e] += Io::load(bias + col + e);
-          if constexpr (GLU) g[e] += Io::load(bias + no + col + e);
+          if constexpr (GATED) g[e] += Io::load(bias + no + col + e);
         }
     }
-    if constexpr (GLU) {
+    if constexpr (GATED) {
       float gate[4] = {g[0], g[1], g[2], g[3]};
       gelu_values(gate);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[e] *= gate[e];
     }
+    if constexpr (GLU == 2) quad_epilogue<H16Elem<FMT>::DT>(s, p.residual, p.ldr, p.preact, p.ldp, p.act, row, col, no, vec);
     E* c = C + (int64_t)row * p.ldc + col;
     if (vec) *(e4*)c = __builtin_convertvector(s, e4);
     else

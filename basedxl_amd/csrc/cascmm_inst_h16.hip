@@ -25,15 +25,17 @@ static int launch_h16(const GroupParams& p, hipStream_t stream) {
   if constexpr (GLU) {
     if (p.glu) return launch_h16_kernel<T, FMT, 0, 1>(p, stream);
   }
+  if (p.epi && (p.count != 1 || p.glu)) return CASCMM_ERR_BAD_VARIANT;
   if (p.k_splits > 1) {
     const int st = ksplit_check(p);
     if (st != CASCMM_OK) return st;
     GroupParams q = p;
     q.bias[0] = nullptr;
+    q.epi = 0;
     const int sg = launch_h16_kernel<T, FMT, RAWB, 0>(q, stream);
     return sg == CASCMM_OK ? launch_ksplit_reduce<H16Elem<FMT>::DT>(p, stream) : sg;
   }
-  return launch_h16_kernel<T, FMT, RAWB, 0>(p, stream);
+  return p.epi ? launch_h16_kernel<T, FMT, RAWB, 2>(p, stream) : launch_h16_kernel<T, FMT, RAWB, 0>(p, stream);
 }
 
 // WM, WN, WK, MT, NTL, BK, NS: see H16.  An even NTL has the gated store.

@@ -28,6 +28,7 @@ static int launch_hwk(const GroupParams& p, hipStream_t stream) {
   if constexpr (kGlu) {
     if (p.glu) return launch_hwk_kernel<MB, NB, FMT, 0, 1>(p, stream);
   }
+  if (p.epi) return p.count == 1 && !p.glu ? launch_hwk_kernel<MB, NB, FMT, RAWB, 2>(p, stream) : (int)CASCMM_ERR_BAD_VARIANT;
   return launch_hwk_kernel<MB, NB, FMT, RAWB, 0>(p, stream);
 }
 

@@ -2,6 +2,7 @@
 // split's share of K and writes its fp32 sums to the workspace, [split][M][ksplit_row(N)]; a second launch adds the
 // splits in order, the bias, and writes C.
 #pragma once
+#include "cascmm_activation.h"
 #include "cascmm_tile_kernel.h"
 
 namespace cascmm {
@@ -29,9 +30,16 @@ inline size_t ksplit_bytes(int64_t M, int64_t N, int splits) { return splits > 1
 // A thread adds four consecutive columns of one row; the loads of up to eight splits are in flight.  Bound by its
 // latency, not by bytes: 2.5 - 4.2 us (kernel trace, medians) for 0.3 to 10 MB of partial results alike
 // (profiles/cascmm_ksplit_kernels.txt).
-template <int IODT>
+// EPI: the epilogue of GroupParams behind the bias (vec_out: residual and preact on whole quads too).
+struct KsplitEpilogue {
+  const void* residual;
+  void* preact;
+  int64_t ldr, ldp;
+  int act;
+};
+template <int IODT, int EPI>
 __global__ __launch_bounds__(256) void ksplit_reduce_kernel(const float* __restrict__ parts, int splits, int M, int N, const void* __restrict__ bias,
-                                                           void* __restrict__ C, int64_t ldc, int vec_out) {
+                                                           void* __restrict__ C, int64_t ldc, int vec_out, KsplitEpilogue ep) {
   typedef IoType<IODT> Io;
   typedef typename Io::T E;
   const int quads = (N + 3) >> 2;
@@ -54,6 +62,7 @@ __global__ __launch_bounds__(256) void ksplit_reduce_kernel(const float* __restr
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += n + e < N ? Io::load((const E*)bias + n + e) : 0.f;
   }
+  if constexpr (EPI) quad_epilogue<IODT>(s, ep.residual, ep.ldr, ep.preact, ep.ldp, ep.act, m, n, N, vec_out != 0);
   if (vec_out) {   // N % 4 == 0, rows of C on whole quads
     *(e4*)c = __builtin_convertvector(s, e4);
   } else {
@@ -72,9 +81,12 @@ inline int ksplit_check(const GroupParams& p) {
 template <int IODT> int launch_ksplit_reduce(const GroupParams& p, hipStream_t stream) {
   typedef typename IoType<IODT>::T E;
   const int64_t total = (int64_t)p.M * ((p.N + 3) / 4);
-  const int vec_out = p.N % 4 == 0 && p.ldc % 4 == 0 && (uintptr_t)p.C[0] % (4 * sizeof(E)) == 0;
-  return launch_kernel(ksplit_reduce_kernel<IODT>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, (const float*)p.workspace, p.k_splits,
-                       p.M, p.N, p.bias[0], p.C[0], p.ldc, vec_out) == hipSuccess
+  const int vec_out = p.N % 4 == 0 && p.ldc % 4 == 0 && p.ldr % 4 == 0 && p.ldp % 4 == 0 &&
+                      ((uintptr_t)p.C[0] | (uintptr_t)p.residual | (uintptr_t)p.preact) % (4 * sizeof(E)) == 0;
+  const KsplitEpilogue ep{p.residual, p.preact, p.ldr, p.ldp, p.act};
+  auto kfn = p.epi ? ksplit_reduce_kernel<IODT, 1> : ksplit_reduce_kernel<IODT, 0>;
+  return launch_kernel(kfn, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, (const float*)p.workspace, p.k_splits,
+                       p.M, p.N, p.bias[0], p.C[0], p.ldc, vec_out, ep) == hipSuccess
              ? CASCMM_OK
              : CASCMM_ERR_LAUNCH;
 }
