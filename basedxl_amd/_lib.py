@@ -133,7 +133,7 @@ def native():
             module = importlib.import_module("._native", __package__)
             module.init(workspaces)
             module.init_scales(scale_scratch)
-            if any(not hasattr(module, name) for name in ("matmul", "prepared", "fp8")):
+            if any(not hasattr(module, name) for name in ("matmul", "prepared", "fp8", "layer_norm", "add_layer_norm", "epilogue", "epilogue_prepared")):
                 raise AttributeError("a function is missing")
         except (ImportError, AttributeError) as e:      # (AttributeError: the extension of an earlier build)
             raise ImportError(f"the host extension {os.path.join(_HERE, '_native.so')} is not built or does not load: {e}. "
@@ -149,7 +149,7 @@ class _NoShortCut:
     def matmul(*_args):
         return None
 
-    prepared = fp8 = matmul
+    prepared = fp8 = layer_norm = add_layer_norm = epilogue = epilogue_prepared = matmul
 
 
 _short_cut = None

@@ -44,29 +44,32 @@ def _compile(src: str) -> str:
     return obj
 
 
-def _compile_native() -> str:
-    """The host extension's object (in a folder of its own: what lies beside it is the library's)."""
+HOST_SOURCES = ("native.cpp", "native_operators.cpp")
+
+
+def _compile_native(src: str) -> str:
+    """An object of the host extension (in a folder of its own: what lies beside it is the library's)."""
     import sysconfig
 
     import torch
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
-    obj = os.path.join(OBJ, "host", "native.o")
+    obj = os.path.join(OBJ, "host", src[:-4] + ".o")
     os.makedirs(os.path.dirname(obj), exist_ok=True)
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
-           "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"], "-c", os.path.join(CSRC, "host", "native.cpp"), "-o", obj]
+           "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"], "-c", os.path.join(CSRC, "host", src), "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("g++ failed on native.cpp:\n" + r.stderr[-4000:])
+        raise RuntimeError(f"g++ failed on {src}:\n" + r.stderr[-4000:])
     if r.stderr.strip():
         sys.stderr.write(r.stderr)
     return obj
 
 
-def _link_native(obj: str) -> None:
+def _link_native(objs) -> None:
     import torch
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", NATIVE, obj, "-L", libs, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", NATIVE, *objs, "-L", libs, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
            "-L", HERE, "-l:libcascmm.so", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
@@ -76,8 +79,8 @@ def _link_native(obj: str) -> None:
 def build(verbose: bool = True, jobs: int = 8) -> str:
     os.makedirs(OBJ, exist_ok=True)
     srcs = sources()
-    with ThreadPoolExecutor(max_workers=min(jobs, len(srcs) + 1)) as ex:
-        native = ex.submit(_compile_native)
+    with ThreadPoolExecutor(max_workers=min(jobs, len(srcs) + len(HOST_SOURCES))) as ex:
+        native = [ex.submit(_compile_native, src) for src in HOST_SOURCES]
         objs = list(ex.map(_compile, srcs))
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -89,7 +92,7 @@ def build(verbose: bool = True, jobs: int = 8) -> str:
         ctypes.CDLL(LIB)
     except OSError as e:
         raise RuntimeError(f"{LIB} was linked but does not load: {e}") from None
-    _link_native(native.result())   # (behind the library, which also works without it)
+    _link_native([f.result() for f in native])   # (behind the library, which also works without it)
     if verbose:
         print(f"built {LIB} from {len(srcs)} translation units, and {NATIVE}")
     return LIB

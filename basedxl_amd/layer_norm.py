@@ -145,6 +145,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     dimensions, ``weight`` / ``bias`` 1-D of the dtype of ``x`` or fp32 (None: ones, zeros).  Statistics and arithmetic are fp32, the
     result is rounded once.  Differentiable once in ``x``, ``weight`` and ``bias``; the sums over rows behind the last two are
     added in a fixed order, so the same call gives the same bits."""
+    y = _lib.short_cut().layer_norm(x, weight, bias, eps)   # the ordinary eager call in one native function; None: it is decided below
+    if y is not None:
+        return y
     _check(x, weight, bias, eps)
     if _differentiated(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
@@ -156,6 +159,9 @@ def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[tor
     """``s = x + residual; return layer_norm(s, weight, bias), s`` in one kernel: ``s`` is written but not read back.  The norm is of ``s``
     as it is returned, rounded to the tensors' dtype.  Differentiable like :func:`layer_norm`, through both results; ``x`` and
     ``residual`` get the same tensor as their gradient."""
+    both = _lib.short_cut().add_layer_norm(x, residual, weight, bias, eps)
+    if both is not None:
+        return both
     _check(x, weight, bias, eps)
     _check_residual(x, residual)
     if _differentiated(x, residual, weight, bias):

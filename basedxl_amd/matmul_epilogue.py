@@ -141,13 +141,24 @@ def cascaded_lowp_matmul_epilogue(a: torch.Tensor, b, *, bias: Optional[torch.Te
 
     Differentiable once in ``a``, ``b`` (a tensor: a prepared weight is a constant that no gradient passes through), ``bias`` and
     ``residual``; the gradients' products run with the cascade of the product itself, and sums over rows in a fixed order."""
+    act = _lib.ACT_BY_NAME.get(activation) if activation is None or type(activation) is str else None
+    if out is None and act is not None and b_exp is None:
+        # the ordinary eager call in one native function; None: whatever is not ordinary about it is decided below
+        if type(b) is not PreparedWeight:
+            y = _lib.short_cut().epilogue(a, b, bias, residual, act, lowp, terms, products)
+        elif not b.glu and (lowp is None or lowp == b.lowp) and (terms is None or terms == b.terms):
+            y = _lib.short_cut().epilogue_prepared(a, b.slots, bias, residual, act, b.K, b.N, b.fmt, b.terms, products, b.dt)
+        else:
+            y = None
+        if y is not None:
+            return y
     prepared = isinstance(b, PreparedWeight)
     _check_device_tensor(a, "a")
     if a.dtype not in _DTYPES:
         raise TypeError(f"cascaded_lowp_matmul_epilogue: unsupported dtype {a.dtype}")
     if a.dim() < 1:
         raise ValueError("cascaded_lowp_matmul_epilogue: a needs at least one dimension")
-    if activation not in _lib.ACT_BY_NAME:
+    if act is None:
         raise ValueError(f"activation must be one of {list(_lib.ACT_BY_NAME)}, got {activation!r}")
     if products not in _lib.PROD_BY_NAME:
         raise ValueError(f"products must be 'tri' or 'full', got {products!r}")

@@ -12,6 +12,18 @@ import torch
 from basedxl_amd import _lib, add_layer_norm, layer_norm
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["native", "python"])
+def path(request, monkeypatch):
+    """Ordinary eager calls by the host extension, and everything by the Python code."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_short_cut", _lib._NoShortCut)
+    else:
+        assert _lib.short_cut() is _lib.native()
+    return request.param
+
+
 U = 2.0 ** -24
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}   # (results below the normal numbers: half a step there)
@@ -78,7 +90,7 @@ def check_backward(dx, dw, db, dy, ds, s, weight, bias, eps, what):
 
 @pytest.mark.parametrize("dtype, wdtype", TYPES)
 @pytest.mark.parametrize("rows, cols", SIZES)
-def test_forward_and_backward(gpu_device, rows, cols, dtype, wdtype):
+def test_forward_and_backward(gpu_device, path, rows, cols, dtype, wdtype):
     gen = torch.Generator().manual_seed(rows * 131 + cols)
     x, r, dy, ds = (rows_of(gen, rows, cols, dtype, gpu_device) for _ in range(4))
     w = (1 + 0.2 * torch.randn(cols, generator=gen)).to(wdtype).to(gpu_device)
@@ -100,7 +112,7 @@ def test_forward_and_backward(gpu_device, rows, cols, dtype, wdtype):
 
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("cols", [640, 457, 2500, 9000])
-def test_strided_rows_leave_their_surroundings_alone(gpu_device, cols, dtype):
+def test_strided_rows_leave_their_surroundings_alone(gpu_device, path, cols, dtype):
     gen = torch.Generator().manual_seed(cols)
     wide = rows_of(gen, 23, cols + 37, dtype, gpu_device)
     for first in (0, 1, 3, 8):
@@ -131,7 +143,7 @@ def test_strided_rows_leave_their_surroundings_alone(gpu_device, cols, dtype):
     assert bool((out == 7.0).all())
 
 
-def test_optional_weight_and_bias(gpu_device):
+def test_optional_weight_and_bias(gpu_device, path):
     gen = torch.Generator().manual_seed(3)
     x, dy = rows_of(gen, 50, 320, torch.float32, gpu_device), rows_of(gen, 50, 320, torch.float32, gpu_device)
     w, b = torch.randn(320, generator=gen).to(gpu_device), torch.randn(320, generator=gen).to(gpu_device)
@@ -151,7 +163,7 @@ def test_optional_weight_and_bias(gpu_device):
         assert [t.grad is not None for t in leaves] == list(keep)
 
 
-def test_one_result_of_the_sum_only(gpu_device):
+def test_one_result_of_the_sum_only(gpu_device, path):
     gen = torch.Generator().manual_seed(4)
     x, r, d = (rows_of(gen, 30, 200, torch.float32, gpu_device).requires_grad_() for _ in range(3))
     d = d.detach()
@@ -198,7 +210,7 @@ def test_infinities_and_nan_stay_in_their_rows(gpu_device):
             assert torch.equal(y[:4], clean[:4]) and torch.equal(y[5:], clean[5:])
 
 
-def test_empty_tensors(gpu_device):
+def test_empty_tensors(gpu_device, path):
     for shape in ((0, 64), (4, 0), (2, 0, 8)):
         x = torch.empty(shape, device=gpu_device, requires_grad=True)
         w = torch.ones(shape[-1], device=gpu_device, requires_grad=True)
@@ -247,7 +259,7 @@ def test_against_differences(gpu_device):
         assert abs(slope - (grad.cpu().double() * direction).sum()) <= 500 * U * scale + 1e-8 * scale
 
 
-def test_other_streams_and_recorded_calls(gpu_device):
+def test_other_streams_and_recorded_calls(gpu_device, path):
     gen = torch.Generator().manual_seed(30)
     x, dy = rows_of(gen, 700, 640, torch.float16, gpu_device), rows_of(gen, 700, 640, torch.float16, gpu_device)
     w = torch.ones(640, device=gpu_device, dtype=torch.float16)
@@ -295,7 +307,7 @@ def test_offsets_beyond_32_bits(gpu_device):
     assert torch.equal(layer_norm(x), layer_norm(x.contiguous()))
 
 
-def test_refusals(gpu_device):
+def test_refusals(gpu_device, path):
     x = torch.zeros(4, 8, device=gpu_device)
     ok = torch.zeros(8, device=gpu_device)
     for bad, error in ((dict(weight=ok[:7]), ValueError), (dict(bias=torch.zeros(8, 1, device=gpu_device)), ValueError), (dict(weight=ok.cpu()), ValueError),
@@ -315,3 +327,18 @@ def test_refusals(gpu_device):
     (g,) = torch.autograd.grad(layer_norm(leaf).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_the_host_extension_takes_ordinary_calls(gpu_device):
+    native = _lib.native()
+    x, w = torch.randn(3, 5, 64, device=gpu_device), torch.ones(64, device=gpu_device)
+    y = native.layer_norm(x, w, None, 1e-5)
+    assert torch.equal(y, layer_norm(x, w))
+    assert native.layer_norm(x.clone().requires_grad_(), w, None, 1e-5).requires_grad
+    y, s = native.add_layer_norm(x, x, w, w, 1e-5)
+    assert torch.equal(s, 2 * x) and torch.equal(y, add_layer_norm(x, x, w, w)[0])
+    # what is left to the Python code, which refuses or copies
+    for args in ((x.cpu(), w, None, 1e-5), (x, w[:7], None, 1e-5), (x, w.half(), None, 1e-5), (x, w, w.half(), 1e-5), (x, w, None, -1.0), (x, w, None, math.nan),
+                 (x, w, None, "a"), (x.double(), None, None, 1e-5), (x[:0], w, None, 1e-5), (x.transpose(0, 1), w, None, 1e-5), (x, w, None), (x, 3, None, 1e-5)):
+        assert native.layer_norm(*args) is None
+    assert native.add_layer_norm(x, x[:2], w, None, 1e-5) is None and native.add_layer_norm(x, x.half(), w, None, 1e-5) is None

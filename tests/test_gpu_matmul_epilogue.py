@@ -13,6 +13,18 @@ import torch
 from basedxl_amd import _lib, PreparedWeight, add_layer_norm, cascaded_lowp_matmul, cascaded_lowp_matmul_epilogue, layer_norm
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["native", "python"])
+def path(request, monkeypatch):
+    """Ordinary eager calls by the host extension, and everything by the Python code."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_short_cut", _lib._NoShortCut)
+    else:
+        assert _lib.short_cut() is _lib.native()
+    return request.param
+
+
 U = 2.0 ** -24
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}
@@ -96,7 +108,7 @@ def check_backward(grads, dy, a, b, bias, act, residual, dtype, lost, what):
 
 @pytest.mark.parametrize("cascade", CASCADES)
 @pytest.mark.parametrize("M, K, N", SIZES)
-def test_forward_and_backward(gpu_device, M, K, N, cascade):
+def test_forward_and_backward(gpu_device, path, M, K, N, cascade):
     dtype, options, lost = CASCADES[cascade]
     a, b, bias, residual, dy = operands(M, K, N, dtype, gpu_device)
     for act in ACTIVATIONS:
@@ -115,7 +127,7 @@ def test_forward_and_backward(gpu_device, M, K, N, cascade):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("M, K, N", [(1, 64, 64), (2, 320, 1280), (154, 1280, 5120), (2048, 1280, 1280), (333, 456, 212), (70, 136, 33), (40, 5120, 640), (700, 1280, 100)])
-def test_prepared_weights(gpu_device, M, K, N, dtype):
+def test_prepared_weights(gpu_device, path, M, K, N, dtype):
     a, b, bias, residual, _ = operands(M, K, N, dtype, gpu_device)
     lost = CASCADES["fp32"][2] if dtype == torch.float32 else 0.0
     pw = PreparedWeight(b)
@@ -142,7 +154,7 @@ def test_other_cascades_are_the_plain_product_with_the_epilogue_behind(gpu_devic
 
 
 @pytest.mark.parametrize("cascade", CASCADES)
-def test_no_inputs_rows_or_outputs(gpu_device, cascade):
+def test_no_inputs_rows_or_outputs(gpu_device, path, cascade):
     dtype, options, _ = CASCADES[cascade]
     for M, K, N in ((0, 8, 8), (4, 8, 0), (5, 0, 9), (0, 0, 0)):
         a, b = torch.ones(M, K, dtype=dtype, device=gpu_device, requires_grad=True), torch.ones(K, N, dtype=dtype, device=gpu_device, requires_grad=True)
@@ -157,7 +169,7 @@ def test_no_inputs_rows_or_outputs(gpu_device, cascade):
 
 
 @pytest.mark.parametrize("cascade", CASCADES)
-def test_shapes_strides_and_results_in_place(gpu_device, cascade):
+def test_shapes_strides_and_results_in_place(gpu_device, path, cascade):
     dtype, options, lost = CASCADES[cascade]
     a, b, bias, residual, _ = operands(60, 136, 72, dtype, gpu_device)
     want = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="gelu", residual=residual, **options)
@@ -188,7 +200,7 @@ def test_shapes_strides_and_results_in_place(gpu_device, cascade):
 
 
 @pytest.mark.parametrize("cascade", CASCADES)
-def test_broadcast_residuals(gpu_device, cascade):
+def test_broadcast_residuals(gpu_device, path, cascade):
     dtype, options, lost = CASCADES[cascade]
     a, b, bias, residual, dy = operands(60, 136, 72, dtype, gpu_device)
     a3, dy3 = a.view(4, 15, 136), dy.view(4, 15, 72)
@@ -203,7 +215,7 @@ def test_broadcast_residuals(gpu_device, cascade):
         within(g, want, HALF[dtype] * want.abs() + 72 * HALF[dtype] * dy3.double().abs().sum_to_size(r.shape), "its gradient")
 
 
-def test_gradients_of_some_operands(gpu_device):
+def test_gradients_of_some_operands(gpu_device, path):
     a, b, bias, residual, dy = operands(90, 136, 72, torch.float16, gpu_device)
     every = [t.clone().requires_grad_() for t in (a, b, bias, residual)]
     want = torch.autograd.grad(cascaded_lowp_matmul_epilogue(every[0], every[1], bias=every[2], activation="gelu", residual=every[3]), every, dy)
@@ -282,7 +294,7 @@ def test_nan_and_infinity_stay_in_their_rows(gpu_device, cascade):
 
 
 @pytest.mark.parametrize("cascade", CASCADES)
-def test_streams_graphs_and_repetition(gpu_device, cascade):
+def test_streams_graphs_and_repetition(gpu_device, path, cascade):
     dtype, options, _ = CASCADES[cascade]
     a, b, bias, residual, dy = operands(300, 640, 320, dtype, gpu_device)
 
@@ -312,7 +324,7 @@ def test_streams_graphs_and_repetition(gpu_device, cascade):
             assert all(torch.equal(p, q) for p, q in zip(outs, want))
 
 
-def test_a_block_of_them(gpu_device):
+def test_a_block_of_them(gpu_device, path):
     """A pre-norm feed-forward block and the norm of the next one, forward and backward: x1 = x + W2 gelu(W1 norm(x)), y = norm(x1)."""
     gen = torch.Generator().manual_seed(77)
     M, D, H = 700, 320, 1280
@@ -351,7 +363,7 @@ def test_a_block_of_them(gpu_device):
                 assert float((p.detach().double() - w.detach()).norm() / w.detach().norm()) <= bound, (dtype, split, name)
 
 
-def test_refusals(gpu_device):
+def test_refusals(gpu_device, path):
     a, b = torch.zeros(4, 16, device=gpu_device), torch.zeros(16, 8, device=gpu_device)
     bad = [(dict(activation="tanh"), ValueError), (dict(products="all"), ValueError), (dict(lowp="fp4"), ValueError), (dict(bias=torch.zeros(7, device=gpu_device)), ValueError),
            (dict(bias=torch.zeros(8, device=gpu_device, dtype=torch.float16)), ValueError), (dict(residual=torch.zeros(4, 8)), ValueError),
@@ -387,3 +399,23 @@ def test_refusals(gpu_device):
     (g,) = torch.autograd.grad(cascaded_lowp_matmul_epilogue(leaf, b).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_the_host_extension_takes_ordinary_calls(gpu_device):
+    native = _lib.native()
+    a, b, bias, residual, _ = operands(24, 64, 32, torch.float16, gpu_device)
+    cascaded_lowp_matmul_epilogue(a, b)     # (the stream's workspace exists)
+    want = cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="gelu", residual=residual)
+    assert torch.equal(native.epilogue(a, b, bias, residual, 2, None, None, "tri"), want)
+    assert native.epilogue(a.clone().requires_grad_(), b, bias, residual, 2, None, None, "tri").requires_grad
+    pw = PreparedWeight(b)
+    args = (pw.K, pw.N, pw.fmt, pw.terms, "tri", pw.dt)
+    assert torch.equal(native.epilogue_prepared(a, pw.slots, bias, residual, 2, *args), cascaded_lowp_matmul_epilogue(a, pw, bias=bias, activation="gelu", residual=residual))
+    assert native.epilogue_prepared(a.clone().requires_grad_(), pw.slots, bias, residual, 2, *args) is None
+    assert native.epilogue_prepared(a, pw.slots[:-1].clone(), bias, residual, 2, *args) is None
+    for change in ({0: a.cpu()}, {1: b.t()}, {1: b[:60]}, {2: bias[:3]}, {2: bias.float()}, {3: residual[:3]}, {3: residual.float()}, {3: residual[0]}, {4: 5}, {4: -1}, {4: None},
+                   {5: "fp8"}, {5: 3}, {6: "a"}, {7: "all"}, {0: a[:0]}, {0: a.double()}):
+        call = [a, b, bias, residual, 2, None, None, "tri"]
+        for k, v in change.items():
+            call[k] = v
+        assert native.epilogue(*call) is None, change
