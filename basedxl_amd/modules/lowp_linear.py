@@ -8,16 +8,27 @@ from typing import Optional
 
 from .. import _lib
 from ..cascaded_lowp_matmul import PreparedWeight, cascaded_lowp_matmul, default_cascade, raw_is_faster, tensor_scale_exp
+from ..matmul_epilogue import cascaded_lowp_matmul_epilogue
 
 
 class BasedXLLowPLinear(nn.Module):
     """Wraps an ``nn.Linear``: the weight is stored transposed as ``[in, out]``
     (lowp_linear.py:12) and the forward pass is one cascade GEMM with the bias add fused
-    into its store (the reference adds it in a second kernel, lowp_linear.py:17-19)."""
+    into its store (the reference adds it in a second kernel, lowp_linear.py:17-19).
+    ``activation`` ("relu", "gelu", "gelu_tanh", "silu") and ``forward(x, residual)`` put what follows the layer
+    in its epilogue: ``activation(x @ weight + bias) + residual``.  The weight is a constant; with an epilogue gradients
+    pass through to ``x`` and ``residual`` (by the raw weight, where they are asked for), without one they do not."""
+
+    #: what follows the product (an attribute: a patcher may set it on a layer that it knows the use of)
+    activation: Optional[str] = None
 
     def __init__(self, submodule: nn.Linear, *, lowp: Optional[str] = None, terms: Optional[int] = None,
-                 products: str = "tri", prepared: Optional[bool] = None):
+                 products: str = "tri", prepared: Optional[bool] = None, activation: Optional[str] = None):
         super().__init__()
+        if activation not in _lib.ACT_BY_NAME:
+            raise ValueError(f"activation must be one of {list(_lib.ACT_BY_NAME)}, got {activation!r}")
+        if activation is not None:
+            self.activation = activation
         self.in_features = submodule.in_features
         self.out_features = submodule.out_features
         self.weight = submodule.weight.detach().T.contiguous().clone()
@@ -44,7 +55,27 @@ class BasedXLLowPLinear(nn.Module):
         if self.lowp == "fp8" and self.weight.is_cuda and (self._weight_exp is None or self._weight_exp.device != self.weight.device):
             self._weight_exp = tensor_scale_exp(self.weight)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def _with_epilogue(self, x: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
+        pw, how = self._prepared_weight, dict(bias=self.bias, activation=self.activation, residual=residual, products=self.products)
+        if torch.compiler.is_compiling():
+            from ..compiled import cascade_linear_epilogue
+            return cascade_linear_epilogue(x, self.weight, None if pw is None else pw.slots, self.bias, residual, self.activation, self.lowp, self.terms,
+                                           self.products, self._weight_exp if pw is None else pw.exp)
+        differentiated = torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))
+        if self.prepared and x.is_cuda and x.dtype == self.weight.dtype and not differentiated and not raw_is_faster(
+                x.numel() // max(self.in_features, 1), self.in_features, self.out_features, x.dtype, self.lowp, self.terms, self.products):
+            if pw is None or pw.device != self.weight.device:
+                pw = self._prepared_weight = PreparedWeight(self.weight, lowp=self.lowp, terms=self.terms)
+            x2 = x.reshape(-1, self.in_features)
+            if pw.usable_with(x2 if x2.stride(-1) == 1 else x2.contiguous(), self.products):
+                return cascaded_lowp_matmul_epilogue(x, pw, **how)
+        if self.lowp == "fp8" and x.is_cuda and (self._weight_exp is None or self._weight_exp.device != self.weight.device):
+            self._weight_exp = tensor_scale_exp(self.weight)
+        return cascaded_lowp_matmul_epilogue(x, self.weight, lowp=self.lowp, terms=self.terms, b_exp=self._weight_exp, **how)
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if residual is not None or self.activation is not None:
+            return self._with_epilogue(x, residual)
         if torch.compiler.is_compiling():
             # traced by torch.compile: one opaque op (whatever was prepared before tracing is used)
             from ..compiled import cascade_linear

@@ -11,15 +11,15 @@ from __future__ import annotations
 
 import torch.nn as nn
 
-from .modules import chain_feed_forward_layers, patch_linear_layers, patch_pointwise_convs
-from .unet_skeleton import fuse_geglu_layers, fuse_kv_projections
+from .modules import chain_feed_forward_layers, patch_layer_norms, patch_linear_layers, patch_pointwise_convs
+from .unet_skeleton import fuse_epilogues, fuse_geglu_layers, fuse_kv_projections
 from .utils import BasedXLConfig
 
 
 def patch_unet(model: nn.Module, cfg: BasedXLConfig) -> nn.Module:
     """Applies ``cfg`` to ``model`` in place: the fusions first (they take plain ``nn.Linear``
     children), then the reference's walk over the remaining ``nn.Linear`` layers (unet.py:81-87) and,
-    if asked, the same walk over the 1x1 convolutions.  Does nothing unless ``cfg.fp16_acc_matmul``."""
+    if asked, the same walk over the 1x1 convolutions, the epilogues of the routed layers and the layer norms.  Does nothing unless ``cfg.fp16_acc_matmul``."""
     if not cfg.fp16_acc_matmul:
         return model
     kw = cfg.cascade_kwargs()
@@ -33,6 +33,10 @@ def patch_unet(model: nn.Module, cfg: BasedXLConfig) -> nn.Module:
     patch_linear_layers(model, **lin_kw)
     if cfg.route_pointwise_convs:
         patch_pointwise_convs(model, **kw)
+    if cfg.fuse_epilogues:
+        fuse_epilogues(model)
+    if cfg.fuse_norms:
+        patch_layer_norms(model)
     return model
 
 

@@ -27,6 +27,8 @@ import torch.nn.functional as F
 
 from .modules.fused_kv import BasedXLFusedKV, BasedXLFusedQKV
 from .modules.geglu import BasedXLLowPGEGLU
+from .modules.layer_norm import BasedXLLayerNorm
+from .modules.lowp_linear import BasedXLLowPLinear
 
 W_STD = 0.02   # every weight ~ N(0, 0.02); biases zero-mean with the same spread
 
@@ -41,15 +43,22 @@ class GEGLU(nn.Module):
         return value * F.gelu(gate)
 
 
+def last_layer(layer: nn.Module, x: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
+    """``layer(x) + residual``, in the layer's epilogue where it has one."""
+    if residual is None:
+        return layer(x)
+    return layer(x, residual) if isinstance(layer, BasedXLLowPLinear) else residual + layer(x)
+
+
 class FeedForward(nn.Module):
     def __init__(self, dim: int, mult: int = 4):
         super().__init__()
         self.net = nn.ModuleList([GEGLU(dim, dim * mult), nn.Dropout(0.0), nn.Linear(dim * mult, dim)])
 
-    def forward(self, x):
-        for m in self.net:
+    def forward(self, x, residual=None):
+        for m in self.net[:-1]:
             x = m(x)
-        return x
+        return last_layer(self.net[-1], x, residual)
 
 
 class Attention(nn.Module):
@@ -70,7 +79,7 @@ class Attention(nn.Module):
         self.to_v = nn.Linear(kv_dim, query_dim, bias=False)
         self.to_out = nn.ModuleList([nn.Linear(query_dim, query_dim), nn.Dropout(0.0)])
 
-    def forward(self, x, context=None):
+    def forward(self, x, context=None, residual=None):
         src = x if context is None else context
         if hasattr(self, "to_qkv"):
             q, k, v = self.to_qkv(x)
@@ -88,10 +97,17 @@ class Attention(nn.Module):
 
         o = F.scaled_dot_product_attention(heads(q), heads(k), heads(v))
         o = o.transpose(1, 2).reshape(B, T, C)
-        return self.to_out[1](self.to_out[0](o))
+        drop = self.to_out[1]
+        if residual is not None and (not drop.training or getattr(drop, "p", 1.0) == 0):
+            return last_layer(self.to_out[0], o, residual)
+        o = drop(self.to_out[0](o))
+        return o if residual is None else residual + o
 
 
 class BasicTransformerBlock(nn.Module):
+    #: the residual adds go in the epilogues of the layers in front of them (:func:`fuse_epilogues`)
+    fused_epilogues = False
+
     def __init__(self, dim: int, heads: int, cross_dim: int):
         super().__init__()
         self.norm1 = nn.LayerNorm(dim)
@@ -102,6 +118,14 @@ class BasicTransformerBlock(nn.Module):
         self.ff = FeedForward(dim)
 
     def forward(self, x, context):
+        if self.fused_epilogues:
+            x = self.attn1(self.norm1(x), residual=x)
+            x = self.attn2(self.norm2(x), context, residual=x)
+            return self.ff(self.norm3(x), residual=x)
+        if isinstance(self.norm2, BasedXLLayerNorm) and isinstance(self.norm3, BasedXLLayerNorm):
+            h, x = self.norm2(self.attn1(self.norm1(x)), x)       # (the add and the norm behind it in one kernel)
+            h, x = self.norm3(self.attn2(h, context), x)
+            return x + self.ff(h)
         x = x + self.attn1(self.norm1(x))
         x = x + self.attn2(self.norm2(x), context)
         return x + self.ff(self.norm3(x))
@@ -182,13 +206,17 @@ class _Block(nn.Module):
 
 
 class TimestepEmbedding(nn.Module):
+    #: the SiLU goes in the epilogue of ``linear_1`` (:func:`fuse_epilogues`)
+    fused_epilogues = False
+
     def __init__(self, cin: int, dim: int):
         super().__init__()
         self.linear_1 = nn.Linear(cin, dim)
         self.linear_2 = nn.Linear(dim, dim)
 
     def forward(self, x):
-        return self.linear_2(F.silu(self.linear_1(x)))
+        h = self.linear_1(x)
+        return self.linear_2(h if self.fused_epilogues else F.silu(h))
 
 
 def sinusoidal(t: torch.Tensor, dim: int) -> torch.Tensor:
@@ -346,6 +374,18 @@ def fuse_geglu_layers(model: nn.Module, **cascade_kwargs) -> nn.Module:
         for name, child in list(module.named_children()):
             if type(child).__name__ == "GEGLU" and isinstance(getattr(child, "proj", None), nn.Linear):
                 setattr(module, name, BasedXLLowPGEGLU(child.proj, **cascade_kwargs))
+    return model
+
+
+def fuse_epilogues(model: nn.Module) -> nn.Module:
+    """What follows a routed Linear layer goes in its epilogue, in the modules whose forward is known here: the residual adds of
+    :class:`BasicTransformerBlock` in the last layers of its attention and feed-forward modules, the SiLU of
+    :class:`TimestepEmbedding` in its first layer.  Call it BEHIND patch_linear_layers (it looks for routed layers)."""
+    for module in model.modules():
+        if isinstance(module, BasicTransformerBlock):
+            module.fused_epilogues = any(isinstance(layer, BasedXLLowPLinear) for layer in (module.attn1.to_out[0], module.attn2.to_out[0], module.ff.net[-1]))
+        elif isinstance(module, TimestepEmbedding) and isinstance(module.linear_1, BasedXLLowPLinear):
+            module.linear_1.activation, module.fused_epilogues = "silu", True
     return model
 
 

@@ -36,6 +36,11 @@ class BasedXLConfig:
     #: the two Linear layers of every feed-forward block as a chain: the gated store of the first GEMM
     #: writes the operand slots of the second (fp32, two bf16 terms; other layers fall back by themselves)
     chain_ffn: bool = False
+    #: what follows a Linear layer in its epilogue, where the module around it is known: the residual adds of a transformer
+    #: block in the output projections, an embedding's SiLU in its first layer
+    fuse_epilogues: bool = False
+    #: the layer norms on this package's kernels (with the residual add in front of them where no epilogue takes it)
+    fuse_norms: bool = False
     #: keep the weights of the Linear layers split (None: the module's default for its dtype)
     prepared: Optional[bool] = None
 
