@@ -17,7 +17,7 @@ static int launch_epilogue_of(const void* src, int64_t lds, const void* residual
   if (per_row > (int64_t)(UINT32_MAX - 256) / rows) return CASCMM_ERR_TOO_LARGE;
   const int64_t total = rows * per_row;
   hipError_t err = hipSuccess;
-  CASCMM_LAUNCH(err, (cascmm_epilogue_kernel<IODT>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, src, lds, residual, ldr, dst, ldd, (int)cols,
+  CASCMM_LAUNCH(err, (cols < NormRow<IODT>::VEC ? cascmm_epilogue_kernel<IODT, true> : cascmm_epilogue_kernel<IODT, false>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, src, lds, residual, ldr, dst, ldd, (int)cols,
                 (unsigned)per_row, (unsigned)total, act);
   return err == hipSuccess ? CASCMM_OK : CASCMM_ERR_LAUNCH;
 }
@@ -28,13 +28,13 @@ int launch_epilogue(const void* src, int64_t lds, const void* residual, int64_t 
                                   : launch_epilogue_of<CASCMM_DT_BF16>(src, lds, residual, ldr, dst, ldd, rows, cols, act, s);
 }
 
-// The lanes on a row, and the workgroups that share the rows of a band of columns: eight for a CU, eight rows at least for each of their groups of lanes
+// The lanes on a row, and the workgroups that share the rows of a band of columns: eight for a CU, four rows at least for each of their groups of lanes
 // (what they sum is written and read again)
 static int ep_lanes(int64_t cols, int dtype) { return cols <= 16 * (int64_t)(16 / ep_size(dtype)) ? 16 : 64; }
 static int64_t ep_parts(int64_t rows, int64_t cols, int dtype) {
   const int lanes = ep_lanes(cols, dtype);
   const int64_t bands = (cols + lanes * (16 / (int64_t)ep_size(dtype)) - 1) / (lanes * (16 / (int64_t)ep_size(dtype)));
-  return std::max<int64_t>(1, std::min<int64_t>((rows + 8 * (256 / lanes) - 1) / (8 * (256 / lanes)), (2048 + bands - 1) / bands));
+  return std::max<int64_t>(1, std::min<int64_t>((rows + 4 * (256 / lanes) - 1) / (4 * (256 / lanes)), (2048 + bands - 1) / bands));
 }
 
 template <int IODT, int LANES>
@@ -42,7 +42,7 @@ static hipError_t ep_backward_lanes(const void* dy, int64_t lddy, const void* z,
                                     int act, hipStream_t s) {
   hipError_t err = hipSuccess;
   constexpr int BAND = LANES * NormRow<IODT>::VEC;
-  CASCMM_LAUNCH(err, (cascmm_epilogue_backward_kernel<IODT, LANES>), dim3((unsigned)((cols + BAND - 1) / BAND), (unsigned)parts), dim3(256), 0, s, dy, lddy, z, ldz, dz,
+  CASCMM_LAUNCH(err, (LANES == 16 && cols < NormRow<IODT>::VEC ? cascmm_epilogue_backward_kernel<IODT, LANES, LANES == 16> : cascmm_epilogue_backward_kernel<IODT, LANES, false>), dim3((unsigned)((cols + BAND - 1) / BAND), (unsigned)parts), dim3(256), 0, s, dy, lddy, z, ldz, dz,
                 lddz, partials, rows, (int)cols, act);
   return err;
 }

@@ -52,19 +52,19 @@ template <int N> __device__ __forceinline__ void times_slope(float (&d)[N], cons
 
 // dst [rows][cols] = act(src) + residual (NULL: nothing; ldr 0: one row for all).  src may be dst.  A thread takes a chunk of 16 bytes; chunks are
 // counted in 32 bits (checked by the host).
-template <int IODT>
+template <int IODT, bool TINY>
 __global__ __launch_bounds__(256) void cascmm_epilogue_kernel(const void* src, int64_t lds, const void* residual, int64_t ldr, void* dst, int64_t ldd, int cols,
                                                              unsigned per_row, unsigned total, int act) {
-  typedef NormRow<IODT> R;
+  typedef NormRow<IODT, TINY> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
   const unsigned i = blockIdx.x * 256u + threadIdx.x;
   if (i >= total) return;
   const unsigned row = i / per_row;
   const int col = (int)(i - row * per_row) * R::VEC;
-  const chunk z = R::load((const E*)src + (int64_t)row * lds, col, cols);
+  const chunk z = R::load_settled((const E*)src + (int64_t)row * lds, col, cols);
   chunk r;
-  if (residual) r = R::load((const E*)residual + (int64_t)row * ldr, col, cols);
+  if (residual) r = R::load_settled((const E*)residual + (int64_t)row * ldr, col, cols);
   float v[R::VEC];
 #pragma unroll
   for (int e = 0; e < R::VEC; ++e) v[e] = (float)z[e];
@@ -81,10 +81,10 @@ __global__ __launch_bounds__(256) void cascmm_epilogue_kernel(const void* src, i
 
 // dz = dy act'(z) (dz NULL: not wanted; act none: z is not read) and, with partials, the workgroup's sums over its rows of dz for its columns at
 // partials[blockIdx.y].  LANES lanes side by side on a row, rows gridDim.y workgroups apart; the sums are of dz as it is before it is rounded.
-template <int IODT, int LANES>
+template <int IODT, int LANES, bool TINY>
 __global__ __launch_bounds__(256) void cascmm_epilogue_backward_kernel(const void* dy, int64_t lddy, const void* z, int64_t ldz, void* dz, int64_t lddz,
                                                                       float* partials, int64_t rows, int cols, int act) {
-  typedef NormRow<IODT> R;
+  typedef NormRow<IODT, TINY> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
   constexpr int VEC = R::VEC, GROUPS = 256 / LANES, AHEAD = 4;
@@ -109,6 +109,8 @@ __global__ __launch_bounds__(256) void cascmm_epilogue_backward_kernel(const voi
         const int64_t at = row + u * stride;
         if (at >= rows) continue;
         float g[VEC], v[VEC];
+        d[u] = R::settle(d[u], col, cols);
+        if (act) x[u] = R::settle(x[u], col, cols);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           g[e] = (float)d[u][e];

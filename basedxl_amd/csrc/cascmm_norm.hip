@@ -12,11 +12,12 @@ static size_t norm_size(int dtype) { return dtype == CASCMM_DT_F32 ? 4 : 2; }
 static bool norm_dtype(int dtype) { return dtype == CASCMM_DT_F32 || dtype == CASCMM_DT_F16 || dtype == CASCMM_DT_BF16; }
 constexpr int64_t kNormMostCols = 1 << 30;   // (column numbers and a step beyond the last are 32-bit)
 
-// The lanes of a row and the elements of a lane: eight lanes take rows of up to 64 columns, sixteen up to 256, a wave up to 2048 (in the backward pass, which
+// The lanes of a row and the elements of a lane: four lanes take rows shorter than a chunk of 16 bytes, eight rows of up to 64 columns, sixteen up to 256, a wave up to 2048 (in the backward pass, which
 // holds the sums beside a row, 1536), four of them up to 8192; none: longer rows
 struct NormShape { int lanes, values; };
-static NormShape norm_shape(int64_t cols, bool backward) {
+static NormShape norm_shape(int64_t cols, bool backward, int64_t chunk) {
   const auto fit = [&](int lanes) { return (int)std::min<int64_t>((cols + 8 * lanes - 1) / (8 * lanes) * 8, 1 << 20); };
+  if (cols < chunk) return {4, 8};
   if (cols <= 64) return {8, 8};
   if (fit(16) <= 16) return {16, fit(16)};
   if (fit(64) <= (backward ? 24 : 32)) return {64, fit(64)};
@@ -33,8 +34,8 @@ static int64_t norm_groups(int64_t rows, int lanes, bool backward) {
 // (a launch has fewer than 2^32 threads)
 static unsigned norm_wide_groups(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 20); }
 // rows of partial sums of the backward pass
-static int64_t norm_parts(int64_t rows, int64_t cols) {
-  const NormShape f = norm_shape(cols, true);
+static int64_t norm_parts(int64_t rows, int64_t cols, int dtype) {
+  const NormShape f = norm_shape(cols, true, 16 / (int64_t)norm_size(dtype));
   return f.lanes ? norm_groups(rows, f.lanes, true) : std::max<int64_t>(1, std::min<int64_t>((rows + 15) / 16, 512));
 }
 
@@ -47,11 +48,12 @@ static int norm_check(int64_t rows, int64_t cols, int dtype, int weight_dtype) {
 
 template <int IODT, bool ADD> static hipError_t norm_forward(const NormParams& p, hipStream_t s) {
   hipError_t err = hipSuccess;
-  const NormShape f = norm_shape(p.cols, false);
+  const NormShape f = norm_shape(p.cols, false, NormRow<IODT>::VEC);
   const dim3 grid(f.lanes ? (unsigned)norm_groups(p.rows, f.lanes, false) : 1u);
 #define NORM_CASE(LPR, NV) \
   case (LPR) * 100 + (NV): CASCMM_LAUNCH(err, (cascmm_layer_norm_kernel<IODT, NV, LPR, ADD>), grid, dim3(256), 0, s, p); break
   switch (f.lanes * 100 + f.values) {
+    NORM_CASE(4, 8);
     NORM_CASE(8, 8);
     NORM_CASE(16, 8);
     NORM_CASE(16, 16);
@@ -70,11 +72,12 @@ template <int IODT, bool ADD> static hipError_t norm_forward(const NormParams& p
 
 template <int IODT, bool DS, bool SUMS> static hipError_t norm_backward_rows(const NormParams& p, hipStream_t s) {
   hipError_t err = hipSuccess;
-  const NormShape f = norm_shape(p.cols, true);
+  const NormShape f = norm_shape(p.cols, true, NormRow<IODT>::VEC);
   const dim3 grid((unsigned)norm_groups(p.rows, f.lanes, true));
 #define NORM_CASE(LPR, NV) \
   case (LPR) * 100 + (NV): CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_kernel<IODT, NV, LPR, DS, SUMS>), grid, dim3(256), 0, s, p); break
   switch (f.lanes * 100 + f.values) {
+    NORM_CASE(4, 8);
     NORM_CASE(8, 8);
     NORM_CASE(16, 8);
     NORM_CASE(16, 16);
@@ -93,9 +96,9 @@ template <int IODT, bool DS, bool SUMS> static hipError_t norm_backward_rows(con
 
 template <int IODT> static hipError_t norm_backward(const NormParams& p, void* dweight, void* dbias, int weight_dtype, hipStream_t s) {
   hipError_t err = hipSuccess;
-  const int parts = (int)norm_parts(p.rows, p.cols);
+  const int parts = (int)norm_parts(p.rows, p.cols, IODT);
   // (no dx wanted: nothing but the sums.  No rows: sums of zeros)
-  const bool rows = p.y && p.rows > 0, wide = norm_shape(p.cols, true).lanes == 0;
+  const bool rows = p.y && p.rows > 0, wide = norm_shape(p.cols, true, NormRow<IODT>::VEC).lanes == 0;
   if (rows && wide) CASCMM_LAUNCH(err, (cascmm_layer_norm_backward_wide_kernel<IODT>), dim3(norm_wide_groups(p.rows)), dim3(kNormWide), 0, s, p);
   else if (rows && p.partials) err = p.ds ? norm_backward_rows<IODT, true, true>(p, s) : norm_backward_rows<IODT, false, true>(p, s);
   else if (rows) err = p.ds ? norm_backward_rows<IODT, true, false>(p, s) : norm_backward_rows<IODT, false, false>(p, s);
@@ -141,9 +144,9 @@ int cascmm_layer_norm(const void* x, const void* residual, const void* weight, c
   return err == hipSuccess ? CASCMM_OK : CASCMM_ERR_LAUNCH;
 }
 
-size_t cascmm_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
-  if (rows < 0 || cols < 0 || rows > INT32_MAX || cols > kNormMostCols) return 0;
-  return (size_t)norm_parts(rows, cols) * 2 * (size_t)cols * sizeof(float);
+size_t cascmm_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
+  if (rows < 0 || cols < 0 || rows > INT32_MAX || cols > kNormMostCols || !norm_dtype(dtype)) return 0;
+  return (size_t)norm_parts(rows, cols, dtype) * 2 * (size_t)cols * sizeof(float);
 }
 
 int cascmm_layer_norm_backward(const void* dy, const void* ds, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
@@ -160,7 +163,7 @@ int cascmm_layer_norm_backward(const void* dy, const void* ds, const void* x, co
       !norm_aligned(dweight, ws) || !norm_aligned(dbias, ws) || !norm_aligned(mean, 4) || !norm_aligned(rstd, 4))
     return CASCMM_ERR_ALIGNMENT;
   if (sums) {
-    if (!workspace || workspace_bytes < cascmm_layer_norm_workspace_bytes(rows, cols)) return CASCMM_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < cascmm_layer_norm_workspace_bytes(rows, cols, dtype)) return CASCMM_ERR_WORKSPACE;
     if (!norm_aligned(workspace, 16)) return CASCMM_ERR_ALIGNMENT;
   }
   NormParams p;

@@ -50,14 +50,15 @@ __device__ __forceinline__ float norm_wave_sum(float v) {
   s += __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48));
   return s;
 }
-// sum over eight or the sixteen lanes of a DPP row
+// sum over four, eight or the sixteen lanes of a DPP row
 template <int LANES> __device__ __forceinline__ float norm_few_sum(float v) {
   v += norm_dpp<0xB1>(v);
   v += norm_dpp<0x4E>(v);
-  v += norm_dpp<0x141>(v);
-  return LANES == 8 ? v : v + norm_dpp<0x140>(v);
+  if (LANES > 4) v += norm_dpp<0x141>(v);
+  if (LANES > 8) v += norm_dpp<0x140>(v);
+  return v;
 }
-// N sums over the LPR lanes of a row: eight, sixteen, a wave or the waves of a workgroup.  `turn` counts the reductions: two sets of slots take turns, so one barrier each is enough
+// N sums over the LPR lanes of a row: four, eight, sixteen, a wave or the waves of a workgroup.  `turn` counts the reductions: two sets of slots take turns, so one barrier each is enough
 // (a wave writes a set again only behind the barrier that all readers of it have passed).
 template <int LPR, int N> __device__ __forceinline__ void norm_sums(float (&v)[N], float* slots, int& turn) {
 #pragma unroll
@@ -85,21 +86,46 @@ template <int LPR, int N> __device__ __forceinline__ void norm_sums(float (&v)[N
 }
 
 // 16 bytes of a row as fp32.  Rows start on element boundaries, not always on 16 bytes: the type says so to the compiler.
-template <int IODT> struct NormRow {
+// TINY: rows shorter than 16 bytes, element by element.
+template <int IODT, bool TINY = false> struct NormRow {
   typedef typename IoType<IODT>::T E;
   static constexpr int VEC = 16 / (int)sizeof(E);
   typedef E chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
-  // chunk at column c of a row of `cols` (past the end: zeros)
+  // The chunk at column c of a row of `cols` (past the end: zeros), in two steps, the load and what settle() does to it where it is used.  A chunk that hangs over
+  // the end is loaded as the row's last whole one and shifted: element by element its parts would be put together behind the load, and every load in
+  // front of it waited for there (8192 x 1001 bf16 backward 22.7 us, so 19.3; rows of whole chunks too, whose code it was: 65536 x 1280 110 us, so 96).
   static __device__ __forceinline__ chunk load(const E* row, int c, int cols) {
     chunk v;
-    if (c + VEC <= cols) {
-      v = *(const chunk*)(row + c);
-    } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = c + e < cols ? row[c + e] : (E)0.f;
+    for (int e = 0; e < VEC; ++e) v[e] = (E)0.f;
+    if constexpr (TINY) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (c + e < cols) v[e] = row[c + e];
+    } else if (c < cols) {
+      v = *(const chunk*)(row + (c < cols - VEC ? c : cols - VEC));
     }
     return v;
   }
+  static __device__ __forceinline__ bool ragged(int cols) { return !TINY && cols % VEC != 0; }
+  static __device__ __forceinline__ chunk settle(chunk v, int c, int cols) {
+    if (!ragged(cols)) return v;
+    const int s = c > cols - VEC && c < cols ? c - (cols - VEC) : 0;   // elements in front of the lane's own
+    const int dwords = sizeof(E) == 2 ? s >> 1 : s;
+    u32x4 w = __builtin_bit_cast(u32x4, v);
+    if (dwords & 1) w = (u32x4){w[1], w[2], w[3], 0u};
+    if (dwords & 2) w = (u32x4){w[2], w[3], 0u, 0u};
+    if (sizeof(E) == 2 && (s & 1))
+      w = (u32x4){__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16), __builtin_amdgcn_alignbit(w[3], w[2], 16), w[3] >> 16};
+    return __builtin_bit_cast(chunk, w);
+  }
+  // ... of a chunk that no row of this kernel ends in (whole: known at compile time)
+  static __device__ __forceinline__ chunk load(const E* row, int c, int cols, bool whole) { return whole ? *(const chunk*)(row + c) : load(row, c, cols); }
+  static __device__ __forceinline__ void store(E* row, int c, int cols, chunk v, bool whole) {
+    if (whole) *(chunk*)(row + c) = v;
+    else store(row, c, cols, v);
+  }
+  static __device__ __forceinline__ chunk load_settled(const E* row, int c, int cols) { return settle(load(row, c, cols), c, cols); }
   static __device__ __forceinline__ void store(E* row, int c, int cols, chunk v) {
     if (c + VEC <= cols) {
       *(chunk*)(row + c) = v;
@@ -109,61 +135,97 @@ template <int IODT> struct NormRow {
         if (c + e < cols) row[c + e] = v[e];
     }
   }
-  // a chunk of weight or bias
-  static __device__ __forceinline__ void load_weight(float (&w)[VEC], const void* p, int f32, int c, int cols, float otherwise) {
+  // CH chunks of weight or bias, `step` columns apart: all of them asked for before the first is looked at
+  template <int FULL, int CH> static __device__ __forceinline__ void load_weight(float (&w)[CH][VEC], const void* p, int f32, int c0, int step, int cols, float otherwise) {
+    if (!p) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) w[e] = otherwise;
-    if (!p) return;
-    if (f32 && sizeof(E) == 2) {
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[c][e] = otherwise;
+    } else if (f32 && sizeof(E) == 2) {
       const float* q = (const float*)p;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) w[e] = c + e < cols ? q[c + e] : 0.f;
-    } else {
-      const chunk v = load((const E*)p, c, cols);
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) w[e] = (float)v[e];
+        for (int e = 0; e < VEC; ++e) {
+          const int col = c0 + c * step + e;
+          w[c][e] = col < cols ? q[col] : 0.f;
+        }
+    } else if constexpr (TINY) {
+      static_assert(CH <= 2, "a row of one chunk");
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int col = c0 + c * step + e;
+          w[c][e] = col < cols ? (float)((const E*)p)[col] : 0.f;
+        }
+    } else {
+      chunk v[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) v[c] = load((const E*)p, c0 + c * step, cols, c < FULL);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (c >= FULL) v[c] = settle(v[c], c0 + c * step, cols);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[c][e] = (float)v[c][e];
+      }
     }
   }
 };
 
-// Rows of up to LPR NV columns, NV a multiple of 8: LPR lanes a row (eight, sixteen, a wave, or all four waves of a workgroup), NV elements a lane.
+// Rows of up to LPR NV columns, NV a multiple of 8: LPR lanes a row (eight, sixteen, a wave, or all four waves of a workgroup; four: rows
+// shorter than 16 bytes), NV elements a lane.
 template <int IODT, int NV, int LPR, bool ADD>
 __global__ __launch_bounds__(256) void cascmm_layer_norm_kernel(const NormParams p) {
-  typedef NormRow<IODT> R;
+  typedef NormRow<IODT, LPR == 4> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
   constexpr int VEC = R::VEC, CH = NV / VEC, STEP = LPR * VEC, ROWS = 256 / LPR;   // ROWS: of a workgroup at a time
+  constexpr int FULL = CH - 8 / VEC;   // chunks that lie inside every row: a shorter one has a kernel of fewer values
   __shared__ float slots[16];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const int cols = p.cols, col0 = lane * VEC;
+  int cols = p.cols;
+  const E *x_at = (const E*)p.x, *r_at = (const E*)p.residual;
+  E *y_at = (E*)p.y, *s_at = (E*)p.sum;
+  const void *weight = p.weight, *bias = p.bias;
+  int64_t rows = p.rows, ldx = p.ldx, ldr = p.ldr;
+  // (the arguments are requested together: left to themselves the reads sink to their uses and wait one behind the other, 1.2 us of 2 x 1280's 5.0 with a residual)
+  asm volatile("" : "+s"(cols), "+s"(x_at), "+s"(weight), "+s"(bias), "+s"(rows), "+s"(ldx));
+  if constexpr (ADD) asm volatile("" : "+s"(r_at), "+s"(ldr));
+  const int col0 = lane * VEC;
   const int64_t stride = (int64_t)gridDim.x * ROWS;
   int64_t row = (int64_t)blockIdx.x * ROWS + (LPR == 64 ? __builtin_amdgcn_readfirstlane(group) : group);
   int turn = 0;
-  if (row >= p.rows) return;   // (of a row's lanes all or none, so every barrier has its waves)
+  if (row >= rows) return;   // (of a row's lanes all or none, so every barrier has its waves)
   chunk x[CH], r[ADD ? CH : 1];
   auto fetch = [&](int64_t at) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      x[c] = R::load((const E*)p.x + at * p.ldx, col0 + c * STEP, cols);
-      if constexpr (ADD) r[c] = R::load((const E*)p.residual + at * p.ldr, col0 + c * STEP, cols);
+      x[c] = R::load(x_at + at * ldx, col0 + c * STEP, cols, c < FULL);
+      if constexpr (ADD) r[c] = R::load(r_at + at * ldr, col0 + c * STEP, cols, c < FULL);
     }
   };
   fetch(row);
   float w[CH][VEC], b[CH][VEC];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    R::load_weight(w[c], p.weight, p.weight_f32, col0 + c * STEP, cols, 1.f);
-    R::load_weight(b[c], p.bias, p.weight_f32, col0 + c * STEP, cols, 0.f);
-  }
+  R::template load_weight<FULL>(w, weight, p.weight_f32, col0, STEP, cols, 1.f);
+  R::template load_weight<FULL>(b, bias, p.weight_f32, col0, STEP, cols, 0.f);
   for (;;) {
     float v[CH][VEC], total[1] = {0.f};
+    if (R::ragged(cols)) {
+#pragma unroll
+      for (int c = FULL; c < CH; ++c) {
+        x[c] = R::settle(x[c], col0 + c * STEP, cols);
+        if constexpr (ADD) r[c] = R::settle(r[c], col0 + c * STEP, cols);
+      }
+    }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if constexpr (ADD) {
         chunk s;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s[e] = (E)((float)x[c][e] + (float)r[c][e]);
-        R::store((E*)p.sum + row * p.lds, col0 + c * STEP, cols, s);
+        R::store(s_at + row * p.lds, col0 + c * STEP, cols, s, c < FULL);
         x[c] = s;
       }
 #pragma unroll
@@ -173,15 +235,15 @@ __global__ __launch_bounds__(256) void cascmm_layer_norm_kernel(const NormParams
       }
     }
     const int64_t next = row + stride;
-    if (next < p.rows) fetch(next);
+    if (next < rows) fetch(next);
     norm_sums<LPR>(total, slots, turn);
-    const float mean = total[0] / (float)p.cols;
+    const float mean = total[0] / (float)cols;
     float square[1] = {0.f};
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        v[c][e] = col0 + c * STEP + e < cols ? v[c][e] - mean : 0.f;
+        v[c][e] = c < FULL || col0 + c * STEP + e < cols ? v[c][e] - mean : 0.f;
         square[0] = __builtin_fmaf(v[c][e], v[c][e], square[0]);
       }
     norm_sums<LPR>(square, slots, turn);
@@ -195,9 +257,9 @@ __global__ __launch_bounds__(256) void cascmm_layer_norm_kernel(const NormParams
       chunk y;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) y[e] = (E)__builtin_fmaf(v[c][e] * rstd, w[c][e], b[c][e]);
-      R::store((E*)p.y + row * p.ldy, col0 + c * STEP, cols, y);
+      R::store(y_at + row * p.ldy, col0 + c * STEP, cols, y, c < FULL);
     }
-    if (next >= p.rows) return;
+    if (next >= rows) return;
     row = next;
   }
 }
@@ -217,9 +279,9 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
     const E* x = (const E*)p.x + row * p.ldx;
     float total[1] = {0.f};
     for (int64_t c = col0; c < cols; c += STEP) {
-      chunk v = R::load(x, (int)c, cols);
+      chunk v = R::load_settled(x, (int)c, cols);
       if constexpr (ADD) {
-        const chunk r = R::load((const E*)p.residual + row * p.ldr, (int)c, cols);
+        const chunk r = R::load_settled((const E*)p.residual + row * p.ldr, (int)c, cols);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = (E)((float)v[e] + (float)r[e]);
         R::store((E*)p.sum + row * p.lds, (int)c, cols, v);
@@ -233,7 +295,7 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
     const float mean = total[0] / (float)p.cols;
     float square[1] = {0.f};
     for (int64_t c = col0; c < cols; c += STEP) {
-      const chunk v = R::load(s, (int)c, cols);
+      const chunk v = R::load_settled(s, (int)c, cols);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float d = c + e < cols ? (float)v[e] - mean : 0.f;
@@ -247,13 +309,13 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
       p.rstd[row] = rstd;
     }
     for (int64_t c = col0; c < cols; c += STEP) {
-      const chunk v = R::load(s, (int)c, cols);
-      float w[VEC], b[VEC];
-      R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
-      R::load_weight(b, p.bias, p.weight_f32, (int)c, cols, 0.f);
+      const chunk v = R::load_settled(s, (int)c, cols);
+      float w[1][VEC], b[1][VEC];
+      R::template load_weight<0>(w, p.weight, p.weight_f32, (int)c, 0, cols, 1.f);
+      R::template load_weight<0>(b, p.bias, p.weight_f32, (int)c, 0, cols, 0.f);
       chunk y;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) y[e] = (E)__builtin_fmaf(((float)v[e] - mean) * rstd, w[e], b[e]);
+      for (int e = 0; e < VEC; ++e) y[e] = (E)__builtin_fmaf(((float)v[e] - mean) * rstd, w[0][e], b[0][e]);
       R::store((E*)p.y + row * p.ldy, (int)c, cols, y);
     }
   }
@@ -262,13 +324,22 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_wide_kernel(const
 // Backward.  SUMS: the sums for dweight and dbias too, a workgroup's at partials[blockIdx.x].
 template <int IODT, int NV, int LPR, bool DS, bool SUMS>
 __global__ __launch_bounds__(256) void cascmm_layer_norm_backward_kernel(const NormParams p) {
-  typedef NormRow<IODT> R;
+  typedef NormRow<IODT, LPR == 4> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
   constexpr int VEC = R::VEC, CH = NV / VEC, STEP = LPR * VEC, ROWS = 256 / LPR;
+  constexpr int FULL = CH - 8 / VEC;   // (as above)
   __shared__ float slots[16];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const int cols = p.cols, col0 = lane * VEC;
+  int cols = p.cols;
+  const E *x_at = (const E*)p.x, *dy_at = (const E*)p.dy, *ds_at = (const E*)p.ds;
+  E* dx_at = (E*)p.y;
+  const void* weight = p.weight;
+  const float *mean_at = p.mean, *rstd_at = p.rstd;
+  int64_t rows = p.rows, ldx = p.ldx, lddy = p.lddy, ldds = p.ldds;
+  asm volatile("" : "+s"(cols), "+s"(x_at), "+s"(dy_at), "+s"(weight), "+s"(mean_at), "+s"(rstd_at), "+s"(rows), "+s"(ldx), "+s"(lddy));
+  if constexpr (DS) asm volatile("" : "+s"(ds_at), "+s"(ldds));
+  const int col0 = lane * VEC;
   const int64_t stride = (int64_t)gridDim.x * ROWS;
   int64_t row = (int64_t)blockIdx.x * ROWS + (LPR == 64 ? __builtin_amdgcn_readfirstlane(group) : group);
   int turn = 0;
@@ -279,28 +350,36 @@ __global__ __launch_bounds__(256) void cascmm_layer_norm_backward_kernel(const N
   auto fetch = [&](int64_t at) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      next.x[c] = R::load((const E*)p.x + at * p.ldx, col0 + c * STEP, cols);
-      next.dy[c] = R::load((const E*)p.dy + at * p.lddy, col0 + c * STEP, cols);
-      if constexpr (DS) next.ds[c] = R::load((const E*)p.ds + at * p.ldds, col0 + c * STEP, cols);
+      next.x[c] = R::load(x_at + at * ldx, col0 + c * STEP, cols, c < FULL);
+      next.dy[c] = R::load(dy_at + at * lddy, col0 + c * STEP, cols, c < FULL);
+      if constexpr (DS) next.ds[c] = R::load(ds_at + at * ldds, col0 + c * STEP, cols, c < FULL);
     }
-    next.mean = p.mean[at];
-    next.rstd = p.rstd[at];
+    next.mean = mean_at[at];
+    next.rstd = rstd_at[at];
   };
   float w[CH][VEC], dw[SUMS ? CH : 1][VEC], db[SUMS ? CH : 1][VEC];
+  R::template load_weight<FULL>(w, weight, p.weight_f32, col0, STEP, cols, 1.f);
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    R::load_weight(w[c], p.weight, p.weight_f32, col0 + c * STEP, cols, 1.f);
     if constexpr (SUMS) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) dw[c][e] = db[c][e] = 0.f;
     }
   }
-  if (row < p.rows) fetch(row);
-  while (row < p.rows) {
-    const Row cur = next;
+  if (row < rows) fetch(row);
+  while (row < rows) {
+    Row cur = next;
+    if (R::ragged(cols)) {
+#pragma unroll
+      for (int c = FULL; c < CH; ++c) {
+        cur.x[c] = R::settle(cur.x[c], col0 + c * STEP, cols);
+        cur.dy[c] = R::settle(cur.dy[c], col0 + c * STEP, cols);
+        if constexpr (DS) cur.ds[c] = R::settle(cur.ds[c], col0 + c * STEP, cols);
+      }
+    }
     const int64_t at = row;
     row += stride;
-    if (row < p.rows) fetch(row);
+    if (row < rows) fetch(row);
     float sums[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -327,7 +406,7 @@ __global__ __launch_bounds__(256) void cascmm_layer_norm_backward_kernel(const N
         if constexpr (DS) d += (float)cur.ds[c][e];
         out[e] = (E)d;
       }
-      R::store((E*)p.y + at * p.ldy, col0 + c * STEP, cols, out);
+      R::store(dx_at + at * p.ldy, col0 + c * STEP, cols, out, c < FULL);
     }
   }
   if constexpr (SUMS) {
@@ -388,12 +467,12 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_backward_wide_ker
     const float mean = p.mean[row], rstd = p.rstd[row];
     float sums[2] = {0.f, 0.f};
     for (int64_t c = col0; c < cols; c += STEP) {
-      const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
-      float w[VEC];
-      R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
+      const chunk v = R::load_settled(x, (int)c, cols), d = R::load_settled(dy, (int)c, cols);
+      float w[1][VEC];
+      R::template load_weight<0>(w, p.weight, p.weight_f32, (int)c, 0, cols, 1.f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float g = (float)d[e] * w[e];
+        const float g = (float)d[e] * w[0][e];
         sums[0] += g;
         sums[1] = __builtin_fmaf(g, ((float)v[e] - mean) * rstd, sums[1]);
       }
@@ -401,14 +480,14 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_backward_wide_ker
     norm_sums<kNormWide>(sums, slots, turn);
     const float c1 = sums[0] * p.inv_cols, c2 = sums[1] * p.inv_cols;
     for (int64_t c = col0; c < cols; c += STEP) {
-      const chunk v = R::load(x, (int)c, cols), d = R::load(dy, (int)c, cols);
-      float w[VEC];
-      R::load_weight(w, p.weight, p.weight_f32, (int)c, cols, 1.f);
+      const chunk v = R::load_settled(x, (int)c, cols), d = R::load_settled(dy, (int)c, cols);
+      float w[1][VEC];
+      R::template load_weight<0>(w, p.weight, p.weight_f32, (int)c, 0, cols, 1.f);
       chunk z, out;
-      if (ds) z = R::load(ds, (int)c, cols);
+      if (ds) z = R::load_settled(ds, (int)c, cols);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float o = rstd * ((float)d[e] * w[e] - c1 - ((float)v[e] - mean) * rstd * c2);
+        float o = rstd * ((float)d[e] * w[0][e] - c1 - ((float)v[e] - mean) * rstd * c2);
         if (ds) o += (float)z[e];
         out[e] = (E)o;
       }

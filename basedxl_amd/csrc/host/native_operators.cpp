@@ -112,7 +112,7 @@ variable_list norm_backward(const at::Tensor& dy, const at::Tensor& ds, const at
   if (want_x) out[0] = fresh(s.sizes(), s);
   if (want_weight) out[1] = fresh({cols}, weight);
   if (want_bias) out[2] = fresh({cols}, bias);
-  if (want_weight || want_bias) ws = scratch(cascmm_layer_norm_workspace_bytes(rows, cols), s);
+  if (want_weight || want_bias) ws = scratch(cascmm_layer_norm_workspace_bytes(rows, cols, dtype_code(s)), s);
   auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
   check(cascmm_layer_norm_backward(dy2.const_data_ptr(), data_of(ds2), s2.const_data_ptr(), data_of(weight), (const float*)mean.const_data_ptr(),
                                    (const float*)rstd.const_data_ptr(), ptr(out[0]), ptr(out[1]), ptr(out[2]), rows, cols, lddy, ldds, lds, cols, dtype_code(s),

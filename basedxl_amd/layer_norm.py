@@ -93,7 +93,7 @@ def _backward(dy, ds, s, weight, bias, mean, rstd, want_x, want_weight, want_bia
     with torch.cuda.device(s.device):
         ws = None
         if want_weight or want_bias:   # (a temporary of the call, as any operator's: of a recorded call in the graph's own memory)
-            ws = torch.empty(l.cascmm_layer_norm_workspace_bytes(rows, cols), dtype=torch.uint8, device=s.device)
+            ws = torch.empty(l.cascmm_layer_norm_workspace_bytes(rows, cols, _DTYPES[s.dtype]), dtype=torch.uint8, device=s.device)
         _lib.check(l.cascmm_layer_norm_backward(
             dy2.data_ptr(), _ptr(ds2), s2.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dweight), _ptr(dbias),
             rows, cols, _ld(dy2), 0 if ds2 is None else _ld(ds2), _ld(s2), cols, _DTYPES[s.dtype], _DTYPES[like.dtype],

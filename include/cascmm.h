@@ -366,9 +366,9 @@ int cascmm_layer_norm(const void* x, const void* residual, const void* weight, c
  * sum, with a residual):  with xhat = (x - mean) rstd and g = dy * weight
  *     dx = rstd (g - mean(g) - xhat mean(g xhat)) + ds;   dweight = sum over rows of dy xhat;   dbias = sum over rows of dy
  * dx (of `dtype`; it is the residual's gradient too), dweight and dbias (of weight_dtype) may each be NULL.  For dweight or dbias the
- * workspace holds cascmm_layer_norm_workspace_bytes(rows, cols) bytes (16-byte aligned, contents need no initialisation).  Sums over rows
+ * workspace holds cascmm_layer_norm_workspace_bytes(rows, cols, dtype) bytes (16-byte aligned, contents need no initialisation).  Sums over rows
  * are fp32 in a fixed order, without atomics. */
-size_t cascmm_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
+size_t cascmm_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int dtype);
 int cascmm_layer_norm_backward(const void* dy, const void* ds, const void* x, const void* weight, const float* mean,
                                const float* rstd, void* dx, void* dweight, void* dbias, int64_t rows, int64_t cols,
                                int64_t lddy, int64_t ldds, int64_t ldx, int64_t lddx, int dtype, int weight_dtype,

@@ -40,9 +40,10 @@ def test_backward_arguments(change, status):
 
 def test_workspace_of_the_sums():
     size = _lib.lib().cascmm_layer_norm_workspace_bytes
-    assert size(-1, 8) == size(8, -1) == size(8, 2 ** 31) == 0
+    assert size(-1, 8, F32) == size(8, -1, F32) == size(8, 2 ** 31, F32) == size(8, 8, 7) == 0
     for rows, cols in ((0, 5), (1, 1280), (65536, 1280), (3, 20000)):
-        assert size(rows, cols) >= 8 * cols and size(rows, cols) % (8 * cols) == 0
+        for dtype in (F32, F16, BF16):
+            assert size(rows, cols, dtype) >= 8 * cols and size(rows, cols, dtype) % (8 * cols) == 0
 
 
 def test_tensors_off_the_gpu_are_refused():
