@@ -28,13 +28,13 @@ int launch_epilogue(const void* src, int64_t lds, const void* residual, int64_t 
                                   : launch_epilogue_of<CASCMM_DT_BF16>(src, lds, residual, ldr, dst, ldd, rows, cols, act, s);
 }
 
-// The lanes on a row, and the workgroups that share the rows of a band of columns: eight for a CU, four rows at least for each of their groups of lanes
-// (what they sum is written and read again)
+// The lanes on a row, and the workgroups that share the rows of a band of columns: four for a CU, as their registers allow, four rows at least for each of
+// their groups of lanes (what a workgroup sums is written and read again)
 static int ep_lanes(int64_t cols, int dtype) { return cols <= 16 * (int64_t)(16 / ep_size(dtype)) ? 16 : 64; }
 static int64_t ep_parts(int64_t rows, int64_t cols, int dtype) {
   const int lanes = ep_lanes(cols, dtype);
   const int64_t bands = (cols + lanes * (16 / (int64_t)ep_size(dtype)) - 1) / (lanes * (16 / (int64_t)ep_size(dtype)));
-  return std::max<int64_t>(1, std::min<int64_t>((rows + 4 * (256 / lanes) - 1) / (4 * (256 / lanes)), (2048 + bands - 1) / bands));
+  return std::max<int64_t>(1, std::min<int64_t>((rows + 4 * (256 / lanes) - 1) / (4 * (256 / lanes)), (1024 + bands - 1) / bands));
 }
 
 template <int IODT, int LANES>

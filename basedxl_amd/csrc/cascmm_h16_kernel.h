@@ -527,21 +527,33 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
           if (res && run + 1 < RUNS) ask((run + 1) / GROUPS, (run + 1) % GROUPS, ahead[(run + 1) & 1]);
           if (act || pre) {
 #pragma unroll 1
-            for (int it = 0; it < ITS; ++it) {
-              const int i = it * 64 + lane;
-              f32x4* at = (f32x4*)(own + i / CHUNKS * ROW + i % CHUNKS * 32);
-              const f32x4 lo = at[0], hi = at[1];
-              float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-              if (pre) {
-                typedef E e8 __attribute__((ext_vector_type(8)));
-                e8 h;
+            for (int it = 0; it < ITS; it += 2) {   // (two chunks at a time: one alone waits for LDS and for its own instructions)
+              f32x4* at[2];
+              float v[16];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) h[e] = (E)v[e];
-                llvm_raw_buffer_store_v4f32(__builtin_bit_cast(f32x4, h), rp, offset(mi, gr, it, ldp), 0, 0);
+              for (int u = 0; u < 2; ++u) {
+                const int i = (it + u) * 64 + lane;
+                at[u] = (f32x4*)(own + i / CHUNKS * ROW + i % CHUNKS * 32);
+                const f32x4 lo = at[u][0], hi = at[u][1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[8 * u + e] = lo[e]; v[8 * u + 4 + e] = hi[e]; }
+              }
+              if (pre) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  typedef E e8 __attribute__((ext_vector_type(8)));
+                  e8 h;
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) h[e] = (E)v[8 * u + e];
+                  llvm_raw_buffer_store_v4f32(__builtin_bit_cast(f32x4, h), rp, offset(mi, gr, it + u, ldp), 0, 0);
+                }
               }
               activate(v, act);
-              at[0] = (f32x4){v[0], v[1], v[2], v[3]};
-              at[1] = (f32x4){v[4], v[5], v[6], v[7]};
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                at[u][0] = (f32x4){v[8 * u], v[8 * u + 1], v[8 * u + 2], v[8 * u + 3]};
+                at[u][1] = (f32x4){v[8 * u + 4], v[8 * u + 5], v[8 * u + 6], v[8 * u + 7]};
+              }
             }
           }
 #pragma unroll
