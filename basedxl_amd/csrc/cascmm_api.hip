@@ -1177,7 +1177,10 @@ static int gemm_on_rows(int count, const void* const* A, const void* const* B, v
   // the epilogue: in the store where the kernel has one that holds it, else behind it, on z in preact or in the result's place (z is rounded to the
   // elements' type then: 16-bit elements meet that in the bounds-checked kernels only)
   const Epilogue& ep = *q.epi;
-  if (v.kind == KIND_H16 || v.kind == KIND_HWK) {
+  // (the fp32 kernels' stores have 32-bit offsets over the rows of a tile)
+  const bool near_rows = std::max(ep.residual ? ep.ldr : 0, ep.preact ? ep.ldp : 0) * (2 * 256 * 4) <= INT32_MAX;
+  if (v.kind == KIND_H16 || v.kind == KIND_HWK ||
+      (near_rows && (v.kind == KIND_F16K || v.kind == KIND_WAVEK || v.kind == KIND_SLOTK || v.kind == KIND_W512 || v.kind == KIND_W512E))) {
     p.epi = 1;
     p.act = ep.act;
     p.residual = ep.residual;

@@ -207,7 +207,8 @@ __device__ __forceinline__ f16x8 f16k_half(const i32x8& v, int s) {
 // Host-checked: K % 32 == 0, 32 <= K <= MAX_K, the slot buffers below 2 GiB, C rows addressable with 32-bit byte
 // offsets inside a tile; p.k_splits is not used.
 // ---------------------------------------------------------------------------------------------------
-template <int UNUSED>
+// EPI: the epilogue of GroupParams in the store.
+template <int EPI>
 __global__ __launch_bounds__(F16K::NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void cascmm_f16k_kernel(const F8K64Params p) {
   typedef F16K T;
   extern __shared__ __attribute__((aligned(1024))) unsigned char f16k_smem[];
@@ -406,6 +407,22 @@ __global__ __launch_bounds__(F16K::NT) __attribute__((amdgpu_waves_per_eu(1, 1))
 
   // ---- epilogue: undo the scales, add the bias; a lane holds column l31, rows 8 q + 4 h + e ----
   const float out_scale = __builtin_ldexpf(1.f, -(p.tensor_exps[0] + p.tensor_exps[1]) - kF16KResultExp);
+  if constexpr (EPI) {
+    const ColumnEpilogue ep(p.ep, p.C, p.ldc, p.M, p.N, m0 + wm0, n0);
+    float r[2][16];
+    ep.ask(r[0], 0, 4 * h, l31, n0 + l31 < p.N);
+#pragma unroll
+    for (int b = 0; b < T::MT * T::NTL; ++b) {
+      const int ni = b / T::MT, mi = b % T::MT, nx = (b + 1) / T::MT, mx = (b + 1) % T::MT, col = ni * 32 + l31;
+      if (b + 1 < T::MT * T::NTL) ep.ask(r[(b + 1) & 1], mx * 32, 4 * h, nx * 32 + l31, n0 + nx * 32 + l31 < p.N);
+      const float bv = p.bias && n0 + col < p.N ? p.bias[n0 + col] : 0.f;
+      float z[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z[e] = acc[mi][ni][e] * out_scale + bv;
+      ep.store<kLargeTileStoreAux>(z, r[b & 1], mi * 32, 4 * h, col, n0 + col < p.N);
+    }
+    return;
+  }
   const int row_base = m0 + wm0 + 4 * h;
   if (m0 + T::BM <= p.M && n0 + T::BN <= p.N && p.ldc * (int64_t)(T::BM * 4) < 0x7FFFFFFF) {
     // whole tile inside C: buffer stores, the row as a scalar offset, nothing to mask
@@ -450,7 +467,7 @@ __global__ __launch_bounds__(F16K::NT) __attribute__((amdgpu_waves_per_eu(1, 1))
 // Host-checked: K % 32 == 0, K >= 32, the slot buffers 16-byte aligned and below 2 GiB, C rows addressable with
 // 32-bit byte offsets inside a tile.
 // ---------------------------------------------------------------------------------------------------
-template <int UNUSED>
+template <int EPI>
 __global__ __launch_bounds__(F16WK::NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void cascmm_f16wk_kernel(const F8K64Params p) {
   typedef F16WK T;
   extern __shared__ __attribute__((aligned(1024))) unsigned char f16wk_smem[];
@@ -594,6 +611,32 @@ __global__ __launch_bounds__(F16WK::NT) __attribute__((amdgpu_waves_per_eu(1, 1)
   __syncthreads();
   auto reduce_and_store = [&](auto owner_tag) {
     constexpr int W = decltype(owner_tag)::value;
+    if constexpr (EPI) {
+      const ColumnEpilogue ep(p.ep, p.C, p.ldc, p.M, p.N, m0, n0);
+#pragma unroll
+      for (int bk = W; bk < T::BLOCKS; bk += T::NW) {
+        const int mi = bk / T::NTL, ni = bk % T::NTL, col = ni * 32 + l31;
+        if (n0 + ni * 32 >= p.N) continue;
+        const bool inside = n0 + col < p.N;
+        float r[16], z[16];
+        ep.ask(r, mi * 32, 4 * h, col, inside);
+#pragma unroll
+        for (int w = 0; w < T::NW; ++w) {
+          const unsigned char* src = f16wk_smem + w * T::WAVE_BYTES + bk * T::BLOCK_BYTES + lane * 16;
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 x = *(const f32x4*)(src + r4 * 1024);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[4 * r4 + e] = w == 0 ? x[e] : z[4 * r4 + e] + x[e];
+          }
+        }
+        const float bv = p.bias && inside ? p.bias[n0 + col] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = z[e] * out_scale + bv;
+        ep.store<kResultStoreAux>(z, r, mi * 32, 4 * h, col, inside);
+      }
+      return;
+    }
     const int ldc_bytes = (int)p.ldc * 4;
     // rows past M fall beyond the end of the buffer and are dropped
     const int64_t c_bytes = ((int64_t)(p.M - 1 - m0) * p.ldc + (p.N - n0)) * 4;

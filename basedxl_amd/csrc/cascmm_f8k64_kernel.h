@@ -33,7 +33,7 @@
 #pragma once
 #include <type_traits>
 
-#include "cascmm_tile_kernel.h"
+#include "cascmm_column_epilogue.h"
 
 namespace cascmm {
 
@@ -221,6 +221,7 @@ struct F8K64Params {
   int tiles_m, tiles_n;
   int k_splits;           // > 1: workgroup (split, tile) multiplies K range split and writes partials[split][M][N]
   float* partials;
+  EpilogueArgs ep;        // the fp16 kernels' forms with an epilogue
 };
 
 typedef __attribute__((address_space(3))) void* f8k64_lds_ptr;

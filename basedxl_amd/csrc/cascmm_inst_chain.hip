@@ -76,8 +76,11 @@ static int slot_params(const GroupParams& p, SlotKParams& q) {
     q.ldc = ksplit_row(p.N);
     q.bias = nullptr;
   }
+  q.ep = epilogue_args(p);
   return CASCMM_OK;
 }
+// the epilogue goes in the store, or, where K is split over workgroups, in the reduction
+static bool slot_epilogue(const GroupParams& p) { return p.epi && p.k_splits <= 1; }
 static int slot_finish(const GroupParams& p, int st, hipStream_t stream) {
   return st == CASCMM_OK && p.k_splits > 1 ? launch_ksplit_reduce<CASCMM_DT_F32>(p, stream) : st;
 }
@@ -93,19 +96,21 @@ static int launch_slotk_variant(const GroupParams& p, hipStream_t stream) {
   SlotKParams q;
   const int st = slot_params(p, q);
   if (st != CASCMM_OK) return st;
+  if (slot_epilogue(p)) return tail ? launch_slotk_t<1, 3>(q, stream) : launch_slotk_t<1, 2>(q, stream);
   return slot_finish(p, tail ? launch_slotk_t<1, 1>(q, stream, p.k_splits) : launch_slotk_t<1, 0>(q, stream, p.k_splits), stream);
 }
 
 // the 64 x 80 tile of the same design, for problems that make too few 64 x 160 tiles to occupy the chip
 static int launch_slotn_variant(const GroupParams& p, hipStream_t stream) {
   typedef SlotN T;
-  auto kfn = p.K % T::BK == 0 ? cascmm_slotn_kernel<0> : cascmm_slotn_kernel<1>;
+  const bool tail = p.K % T::BK != 0, epi = slot_epilogue(p);
+  auto kfn = epi ? (tail ? cascmm_slotn_kernel<3> : cascmm_slotn_kernel<2>) : (tail ? cascmm_slotn_kernel<1> : cascmm_slotn_kernel<0>);
   if (p.kernel_out) { *p.kernel_out = (const void*)kfn; return CASCMM_OK; }
   if (p.count != 1 || p.glu) return CASCMM_ERR_BAD_VARIANT;
   if ((int64_t)p.M * p.lda * 4 > 0x7FFFFFFF || prepared_kgroups(p.K) * p.N * 32 > 0x7FFFFFFF || p.ldc * (int64_t)(T::BM * 4) > 0x7FFFFFFF)
     return CASCMM_ERR_TOO_LARGE;
-  static LdsFlags lds_set[2];
-  if (!ensure_lds((const void*)kfn, T::LDS_BYTES, lds_set[p.K % T::BK == 0 ? 0 : 1])) return CASCMM_ERR_LAUNCH;
+  static LdsFlags lds_set[4];
+  if (!ensure_lds((const void*)kfn, T::LDS_BYTES, lds_set[(tail ? 1 : 0) + (epi ? 2 : 0)])) return CASCMM_ERR_LAUNCH;
   SlotKParams q;
   const int st = slot_params(p, q);
   if (st != CASCMM_OK) return st;
@@ -121,14 +126,15 @@ static int launch_slotn_variant(const GroupParams& p, hipStream_t stream) {
 static int launch_rawk_variant(const GroupParams& p, hipStream_t stream) {
   typedef SlotK T;
   const bool tail = p.K % (2 * T::BK) != 0;   // raw A comes in pairs of stages
-  auto kfn = tail ? cascmm_rawk_kernel<1> : cascmm_rawk_kernel<0>;
+  const bool epi = slot_epilogue(p);
+  auto kfn = epi ? (tail ? cascmm_rawk_kernel<3> : cascmm_rawk_kernel<2>) : (tail ? cascmm_rawk_kernel<1> : cascmm_rawk_kernel<0>);
   if (p.kernel_out) { *p.kernel_out = (const void*)kfn; return CASCMM_OK; }
   if (p.count != 1 || p.glu) return CASCMM_ERR_BAD_VARIANT;
   if (p.lda < 2 * T::BK) return CASCMM_ERR_BAD_VARIANT;
   if ((int64_t)p.M * p.lda * 4 > 0x7FFFFFFF || (int64_t)p.K * p.ldb * 4 > 0x7FFFFFFF || p.ldc * (int64_t)(T::BM * 4) > 0x7FFFFFFF)
     return CASCMM_ERR_TOO_LARGE;
-  static LdsFlags lds_set[2];
-  if (!ensure_lds((const void*)kfn, T::LDS_BYTES, lds_set[tail ? 1 : 0])) return CASCMM_ERR_LAUNCH;
+  static LdsFlags lds_set[4];
+  if (!ensure_lds((const void*)kfn, T::LDS_BYTES, lds_set[(tail ? 1 : 0) + (epi ? 2 : 0)])) return CASCMM_ERR_LAUNCH;
   SlotKParams q;
   const int st = slot_params(p, q);
   if (st != CASCMM_OK) return st;

@@ -2,8 +2,7 @@
 // split's share of K and writes its fp32 sums to the workspace, [split][M][ksplit_row(N)]; a second launch adds the
 // splits in order, the bias, and writes C.
 #pragma once
-#include "cascmm_activation.h"
-#include "cascmm_tile_kernel.h"
+#include "cascmm_column_epilogue.h"
 
 namespace cascmm {
 
@@ -31,15 +30,9 @@ inline size_t ksplit_bytes(int64_t M, int64_t N, int splits) { return splits > 1
 // latency, not by bytes: 2.5 - 4.2 us (kernel trace, medians) for 0.3 to 10 MB of partial results alike
 // (profiles/cascmm_ksplit_kernels.txt).
 // EPI: the epilogue of GroupParams behind the bias (vec_out: residual and preact on whole quads too).
-struct KsplitEpilogue {
-  const void* residual;
-  void* preact;
-  int64_t ldr, ldp;
-  int act;
-};
 template <int IODT, int EPI>
 __global__ __launch_bounds__(256) void ksplit_reduce_kernel(const float* __restrict__ parts, int splits, int M, int N, const void* __restrict__ bias,
-                                                           void* __restrict__ C, int64_t ldc, int vec_out, KsplitEpilogue ep) {
+                                                           void* __restrict__ C, int64_t ldc, int vec_out, EpilogueArgs ep) {
   typedef IoType<IODT> Io;
   typedef typename Io::T E;
   const int quads = (N + 3) >> 2;
@@ -83,7 +76,7 @@ template <int IODT> int launch_ksplit_reduce(const GroupParams& p, hipStream_t s
   const int64_t total = (int64_t)p.M * ((p.N + 3) / 4);
   const int vec_out = p.N % 4 == 0 && p.ldc % 4 == 0 && p.ldr % 4 == 0 && p.ldp % 4 == 0 &&
                       ((uintptr_t)p.C[0] | (uintptr_t)p.residual | (uintptr_t)p.preact) % (4 * sizeof(E)) == 0;
-  const KsplitEpilogue ep{p.residual, p.preact, p.ldr, p.ldp, p.act};
+  const EpilogueArgs ep = epilogue_args(p);
   auto kfn = p.epi ? ksplit_reduce_kernel<IODT, 1> : ksplit_reduce_kernel<IODT, 0>;
   return launch_kernel(kfn, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, (const float*)p.workspace, p.k_splits,
                        p.M, p.N, p.bias[0], p.C[0], p.ldc, vec_out, ep) == hipSuccess

@@ -36,8 +36,10 @@ namespace cascmm {
 // no alignment: see cascmm_wavek_kernel), C rows addressable with 32-bit byte offsets inside a tile.  TAIL = 0:
 // K % 16 == 0, K >= 16 (raw A: K % 32 == 0).  TAIL = 1 (raw A only): any K whose rows of A are whole 16-byte chunks,
 // zeros past K; the chunks past K are fetched from beyond the buffer, as zeros (the slots of B past K are zeros).
-template <int ARAW, int TAIL>
+// FORM: 1 is TAIL, 2 the epilogue of GroupParams in the store.
+template <int ARAW, int FORM>
 __global__ __launch_bounds__(SlotK::NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void cascmm_slotk_kernel(const SlotKParams p) {
+  constexpr int TAIL = FORM & 1;
   typedef SlotK T;
   extern __shared__ __attribute__((aligned(1024))) unsigned char slotk_smem[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, g = lane >> 5;
@@ -268,10 +270,13 @@ __global__ __launch_bounds__(SlotK::NT) __attribute__((amdgpu_waves_per_eu(1, 1)
     // rows past M fall beyond the end of the buffer and are dropped
     const int64_t c_bytes = ((int64_t)(p.M - 1 - m0) * p.ldc + (p.N - n0)) * 4;
     const i32x4 rc = make_rsrc(C + (int64_t)m0 * p.ldc + n0, c_bytes);
+    const ColumnEpilogue ep(p.ep, C, p.ldc, p.M, p.N, m0, n0);
 #pragma unroll
     for (int b = W; b < T::BLOCKS; b += T::NW) {
       const int mi = b / T::NTL, ni = b % T::NTL;
       if (n0 + ni * 32 >= p.N) continue;
+      float residual[16];
+      if constexpr ((FORM & 2) != 0) ep.ask(residual, mi * 32, 4 * g, ni * 32 + l31, n0 + ni * 32 + l31 < p.N);
       f32x16 sum;
       // partial sums in wave order 0, 1, 2, 3: the own one at its place
 #pragma unroll
@@ -294,6 +299,14 @@ __global__ __launch_bounds__(SlotK::NT) __attribute__((amdgpu_waves_per_eu(1, 1)
       }
       // columns past N (a ragged last tile; their slots were some other column's) are sent beyond the end too
       const bool inside = n0 + ni * 32 + l31 < p.N;
+      if constexpr ((FORM & 2) != 0) {
+        const float bias = (p.bias && inside) ? p.bias[n0 + ni * 32 + l31] : 0.f;
+        float z[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[e] = sum[e] + bias;
+        ep.store<kResultStoreAux>(z, residual, mi * 32, 4 * g, ni * 32 + l31, inside);
+        continue;
+      }
       const float bv = (p.bias && inside) ? p.bias[n0 + ni * 32 + l31] : 0.f;
       const int voff = inside ? (g * 4 * ldc_bytes) + (ni * 32 + l31) * 4 : (int)(c_bytes > 0x7FFFFFFF ? 0x7FFFFFFF : c_bytes);
 #pragma unroll
@@ -331,8 +344,9 @@ struct RawK {
 // Host-checked: fp32 operands, lda >= 32, M * lda * 4 and K * ldb * 4 below 2 GiB, C rows addressable with 32-bit byte
 // offsets inside a tile; any N and any alignment of rows.  TAIL as above (0: K % 32 == 0; the rows of B past K lie
 // beyond its buffer).  c_vec: N % 4 == 0, ldc % 4 == 0 and C 16-byte aligned (16-byte stores).
-template <int TAIL>
+template <int FORM>
 __global__ __launch_bounds__(SlotK::NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void cascmm_rawk_kernel(const SlotKParams p, int c_vec) {
+  constexpr int TAIL = FORM & 1;
   typedef SlotK T;
   constexpr int D = RawK::D, AHEAD = RawK::AHEAD;
   extern __shared__ __attribute__((aligned(1024))) unsigned char slotk_smem[];
@@ -558,6 +572,49 @@ __global__ __launch_bounds__(SlotK::NT) __attribute__((amdgpu_waves_per_eu(1, 1)
       for (int j = 0; j < 4; ++j) bq[j] = n0 + colq + j < p.N ? p.bias[n0 + colq + j] : 0.f;
     }
     if (p.bias && ins) bs = p.bias[n0 + cols];
+    if constexpr ((FORM & 2) != 0) {
+      // register e is row 8 W + 4 g + e: its four adjacent columns (16 bytes where the rows of all tensors allow it) and the one behind the first 128
+      const ColumnEpilogue ep(p.ep, C, p.ldc, p.M, p.N, m0, n0);
+      const bool vec = c_vec && ((p.ep.ldr | p.ep.ldp) & 3) == 0 && (((uintptr_t)p.ep.residual | (uintptr_t)p.ep.preact) & 15) == 0;
+      auto place = [&](int mi, int e, int ld, int col, bool inside) {
+        return (int)((inside ? (unsigned)(4 * g * ld + col * 4) : 0x7FFFFFFFu) + (unsigned)((mi * 32 + W * 8 + e) * ld));
+      };
+      f32x4 rq[T::MT][4];
+      float rs[T::MT][4];
+#pragma unroll
+      for (int mi = 0; mi < T::MT; ++mi)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          rq[mi][e] = (f32x4){0.f, 0.f, 0.f, 0.f};
+          rs[mi][e] = 0.f;
+          if (!ep.res) continue;
+          if (vec) rq[mi][e] = llvm_raw_buffer_load_v4f32(ep.rr, place(mi, e, ep.ldr, colq, inq), 0, 0);
+          else
+#pragma unroll
+            for (int j = 0; j < 4; ++j) rq[mi][e][j] = llvm_raw_buffer_load_f32(ep.rr, place(mi, e, ep.ldr, colq + j, n0 + colq + j < p.N), 0, 0);
+          rs[mi][e] = llvm_raw_buffer_load_f32(ep.rr, place(mi, e, ep.ldr, cols, ins), 0, 0);
+        }
+      auto out = [&](const i32x4& to, int ld, int mi, int e, const float (&z)[5]) {
+        if (vec) llvm_raw_buffer_store_v4f32((f32x4){z[0], z[1], z[2], z[3]}, to, place(mi, e, ld, colq, inq), 0, kResultStoreAux);
+        else
+#pragma unroll
+          for (int j = 0; j < 4; ++j) llvm_raw_buffer_store_f32(z[j], to, place(mi, e, ld, colq + j, n0 + colq + j < p.N), 0, kResultStoreAux);
+        llvm_raw_buffer_store_f32(z[4], to, place(mi, e, ld, cols, ins), 0, kResultStoreAux);
+      };
+#pragma unroll
+      for (int mi = 0; mi < T::MT; ++mi)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float z[5] = {sum[mi][0][e] + bq[0], sum[mi][1][e] + bq[1], sum[mi][2][e] + bq[2], sum[mi][3][e] + bq[3], sum[mi][4][e] + bs};
+          if (ep.pre) out(ep.rp, ep.ldp, mi, e, z);
+          activate(z, ep.act);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[j] += rq[mi][e][j];
+          z[4] += rs[mi][e];
+          out(ep.rc, ep.ldc, mi, e, z);
+        }
+      return;
+    }
     const int voq = inq ? (g * 4 * ldc_bytes) + colq * 4 : c_bytes;
     const int vos = ins ? (g * 4 * ldc_bytes) + cols * 4 : c_bytes;
 #pragma unroll

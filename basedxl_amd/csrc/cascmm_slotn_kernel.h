@@ -36,8 +36,10 @@ struct SlotN {
 // Host-checked: the slot buffer 16-byte aligned and below 2 GiB, M * lda * 4 below 2 GiB, C rows addressable with 32-bit
 // byte offsets inside a tile.  TAIL as in cascmm_slotk_kernel (0: K % 32 == 0, K >= 32).
 // (SlotKParams: a = fp32 [M][lda], b_slots = [2][4 ceil(K/32)][N] x 16 bytes.)
-template <int TAIL>
+// FORM: 1 is TAIL, 2 the epilogue of GroupParams in the store.
+template <int FORM>
 __global__ __launch_bounds__(SlotN::NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void cascmm_slotn_kernel(const SlotKParams p) {
+  constexpr int TAIL = FORM & 1;
   typedef SlotN T;
   extern __shared__ __attribute__((aligned(1024))) unsigned char slotn_smem[];
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, kg = lane >> 4;
@@ -247,10 +249,13 @@ __global__ __launch_bounds__(SlotN::NT) __attribute__((amdgpu_waves_per_eu(1, 1)
   const int64_t c_bytes64 = ((int64_t)(p.M - 1 - m0) * p.ldc + (p.N - n0)) * 4;
   const int c_bytes = (int)(c_bytes64 > 0x7FFFFFFF ? 0x7FFFFFFF : c_bytes64);
   const i32x4 rc = make_rsrc(C + (int64_t)m0 * p.ldc + n0, c_bytes);
+  const ColumnEpilogue ep(p.ep, C, p.ldc, p.M, p.N, m0, n0);
 #pragma unroll
   for (int x = 0; x < T::BLOCKS / T::NW; ++x) {
     const int b = wave + T::NW * x;          // (wave-uniform)
     const int mb = b / T::NB, nb = b % T::NB;
+    float residual[4];
+    if constexpr ((FORM & 2) != 0) ep.ask(residual, mb * 16, 4 * kg, nb * 16 + l15, n0 + nb * 16 + l15 < p.N);
     f32x4 sum = *(const f32x4*)(slotn_smem + b * T::BLOCK_BYTES + lane * 16);
 #pragma unroll
     for (int w = 1; w < T::NW; ++w) sum += *(const f32x4*)(slotn_smem + (w * T::BLOCKS + b) * T::BLOCK_BYTES + lane * 16);
@@ -259,6 +264,11 @@ __global__ __launch_bounds__(SlotN::NT) __attribute__((amdgpu_waves_per_eu(1, 1)
     const int col = nb * 16 + l15;
     const bool inside = n0 + col < p.N;
     const float bv = (p.bias && inside) ? p.bias[n0 + col] : 0.f;
+    if constexpr ((FORM & 2) != 0) {
+      float z[4] = {sum[0] + bv, sum[1] + bv, sum[2] + bv, sum[3] + bv};
+      ep.store<kResultStoreAux>(z, residual, mb * 16, 4 * kg, col, inside);
+      continue;
+    }
     const int voff = inside ? kg * 4 * ldc_bytes + col * 4 : c_bytes;
 #pragma unroll
     for (int e = 0; e < 4; ++e) llvm_raw_buffer_store_f32(sum[e] + bv, rc, voff, (mb * 16 + e) * ldc_bytes, kResultStoreAux);

@@ -219,6 +219,7 @@ int launch_w512(const GroupParams& p, hipStream_t stream) {
     return CASCMM_ERR_TOO_LARGE;
   // (the gated stores are instantiations of their own; glu == 2: the result leaves as operand slots)
   if (p.glu == 2) return launch_w512_kernel<BPRE, 2>(p, stream);
+  if (p.epi) return p.glu ? (int)CASCMM_ERR_BAD_VARIANT : launch_w512_kernel<BPRE, 3>(p, stream);
   return p.glu ? launch_w512_kernel<BPRE, 1>(p, stream) : launch_w512_kernel<BPRE, 0>(p, stream);
 }
 
@@ -236,7 +237,7 @@ int launch_w512_edge(const GroupParams& p, hipStream_t stream) {
   if constexpr (BPRE && NTL != 3) {
     if (p.glu) return launch_w512_kernel<BPRE, 1, NTL, 1>(p, stream);
   }
-  return launch_w512_kernel<BPRE, 0, NTL, 1>(p, stream);
+  return p.epi ? launch_w512_kernel<BPRE, 3, NTL, 1>(p, stream) : launch_w512_kernel<BPRE, 0, NTL, 1>(p, stream);
 }
 
 // the tiles of KIND_WAVEK that the selection functions know
@@ -245,7 +246,7 @@ constexpr bool wavek_for_shapes(int bm, int bn) { return bm == 32 && bn >= 32; }
 template <int W, int MB, int NB, int FMT, int TERMS, int BPRE, int GLU>
 int launch_wavek_kernel(const GroupParams& p, hipStream_t stream) {
   constexpr int ALL = W * MB / 8, FEW = W * MB == 16 ? 1 : ALL;
-  const bool tail = (!GLU && p.N % (W * NB) != 0) || p.K % 32 != 0, few = FEW != ALL && p.M <= 8;
+  const bool tail = (GLU != 1 && p.N % (W * NB) != 0) || p.K % 32 != 0, few = FEW != ALL && p.M <= 8;
   void (*kfn)(const GroupParams) = few ? (tail ? cascmm_wavek_kernel<W, MB, NB, FEW, 1, FMT, TERMS, BPRE, GLU> : cascmm_wavek_kernel<W, MB, NB, FEW, 0, FMT, TERMS, BPRE, GLU>)
                                        : (tail ? cascmm_wavek_kernel<W, MB, NB, ALL, 1, FMT, TERMS, BPRE, GLU> : cascmm_wavek_kernel<W, MB, NB, ALL, 0, FMT, TERMS, BPRE, GLU>);
   if (p.kernel_out) { *p.kernel_out = (const void*)kfn; return CASCMM_OK; }
@@ -262,13 +263,14 @@ int launch_wavek_kernel(const GroupParams& p, hipStream_t stream) {
 // (SCALED: the bounds-checked form only, and eight words more of LDS)
 template <int W, int MB, int NB>
 int launch_wavek_scaled(const GroupParams& p, hipStream_t stream) {
-  auto kfn = cascmm_wavek_kernel<W, MB, NB, W * MB / 8, 1, CASCMM_FMT_FP16, 3, 0, 0, 1>;
+  auto kfn = p.epi ? cascmm_wavek_kernel<W, MB, NB, W * MB / 8, 1, CASCMM_FMT_FP16, 3, 0, 2, 1> : cascmm_wavek_kernel<W, MB, NB, W * MB / 8, 1, CASCMM_FMT_FP16, 3, 0, 0, 1>;
   if (p.kernel_out) { *p.kernel_out = (const void*)kfn; return CASCMM_OK; }
+  if (p.epi && p.count != 1) return CASCMM_ERR_BAD_VARIANT;
   if (p.glu || p.k_splits > 1 || p.count < 1 || p.K <= 0) return CASCMM_ERR_BAD_VARIANT;
   if ((int64_t)p.M * p.lda * 4 > 0x7FFFFFFF || (int64_t)p.K * p.ldb * 4 > 0x7FFFFFFF) return CASCMM_ERR_TOO_LARGE;
   constexpr int lds = WaveKOf<W, MB, NB, W * MB / 8, CASCMM_FMT_FP16, 3, 0>::LDS_BYTES + 32;
-  static LdsFlags lds_set;
-  if (!ensure_lds((const void*)kfn, lds, lds_set)) return CASCMM_ERR_LAUNCH;
+  static LdsFlags lds_set[2];
+  if (!ensure_lds((const void*)kfn, lds, lds_set[p.epi ? 1 : 0])) return CASCMM_ERR_LAUNCH;
   const int64_t grid = (int64_t)p.count * p.tiles_m * p.tiles_n;
   if (grid <= 0 || grid > 0x7FFFFFFF) return CASCMM_ERR_TOO_LARGE;
   return launch_kernel(kfn, dim3((unsigned)grid), dim3(512), (size_t)lds, stream, p) == hipSuccess ? CASCMM_OK : CASCMM_ERR_LAUNCH;
@@ -283,6 +285,7 @@ int launch_wavek(const GroupParams& p, hipStream_t stream) {
   if constexpr (kGlu) {
     if (p.glu) return launch_wavek_kernel<W, MB, NB, FMT, TERMS, BPRE, 1>(p, stream);
   }
+  if (p.epi) return p.count == 1 && !p.glu ? launch_wavek_kernel<W, MB, NB, FMT, TERMS, BPRE, 2>(p, stream) : (int)CASCMM_ERR_BAD_VARIANT;
   return launch_wavek_kernel<W, MB, NB, FMT, TERMS, BPRE, 0>(p, stream);
 }
 
@@ -402,15 +405,15 @@ inline size_t f16k_workspace_bytes(int64_t M, int64_t N, int64_t K) {
 template <bool WK>
 int launch_f16k(const GroupParams& p, hipStream_t stream) {
   typedef typename std::conditional<WK, F16WK, F16K>::type T;
-  void (*kfn)(const F8K64Params) = WK ? cascmm_f16wk_kernel<0> : cascmm_f16k_kernel<0>;
+  void (*kfn)(const F8K64Params) = p.epi ? (WK ? cascmm_f16wk_kernel<1> : cascmm_f16k_kernel<1>) : (WK ? cascmm_f16wk_kernel<0> : cascmm_f16k_kernel<0>);
   if (p.kernel_out) { *p.kernel_out = (const void*)kfn; return CASCMM_OK; }
   if (p.count != 1 || p.glu || p.k_splits > 1 || p.K % T::BK != 0 || p.K == 0 || (!WK && p.K > F16K::MAX_K)) return CASCMM_ERR_BAD_VARIANT;
   const size_t need = f16k_workspace_bytes(p.M, p.N, p.K);
   if (!p.workspace || p.workspace_bytes < need) return CASCMM_ERR_WORKSPACE;
   if ((uintptr_t)p.workspace % 16 != 0) return CASCMM_ERR_ALIGNMENT;
   if (f16k_slot_bytes(p.M, p.K) > 0x7FFFFFFF || f16k_slot_bytes(p.N, p.K) > 0x7FFFFFFF) return CASCMM_ERR_TOO_LARGE;
-  static LdsFlags lds_set;
-  if (!ensure_lds((const void*)kfn, T::LDS_BYTES, lds_set)) return CASCMM_ERR_LAUNCH;
+  static LdsFlags lds_set[2];
+  if (!ensure_lds((const void*)kfn, T::LDS_BYTES, lds_set[p.epi ? 1 : 0])) return CASCMM_ERR_LAUNCH;
   char* ws = (char*)p.workspace;
   u32x4* a_slots = (u32x4*)ws;
   ws += f8k64_up(f16k_slot_bytes(p.M, p.K));
@@ -439,6 +442,7 @@ int launch_f16k(const GroupParams& p, hipStream_t stream) {
   q.tiles_m = (p.M + T::BM - 1) / T::BM; q.tiles_n = (p.N + T::BN - 1) / T::BN;
   q.k_splits = 1;
   q.partials = nullptr;
+  q.ep = epilogue_args(p);
   const unsigned grid = (unsigned)(q.tiles_m * q.tiles_n);
   if (launch_kernel(kfn, dim3(grid), dim3(T::NT), (size_t)T::LDS_BYTES, stream, q) != hipSuccess) return CASCMM_ERR_LAUNCH;
   return CASCMM_OK;
@@ -518,6 +522,7 @@ struct SlotKParams {
   int tiles_m, tiles_n;
   int group_m;             // tile rows an XCD's range of tiles walks down before moving one tile to the right
   int stack_m, k_per;      // tiles_m x splits; k of a split (fewer than K: C is the partial results): see cascmm_ksplit.h
+  EpilogueArgs ep;         // the forms with an epilogue
 };
 
 int launch_slotk(const SlotKParams& q, int araw, hipStream_t stream);

@@ -31,7 +31,7 @@
 // in vector registers use the MFMA through inline assembly, because the compiler gives every MFMA it
 // selects an accumulator in the accumulation registers (of which there are sixteen blocks' worth).
 #pragma once
-#include "cascmm_tile_kernel.h"
+#include "cascmm_column_epilogue.h"
 
 namespace cascmm {
 
@@ -115,8 +115,10 @@ __device__ __forceinline__ void w512_in_vec(f32x16& c) { asm volatile("" : "+v"(
 // 16-byte reads instead of eight 4-byte ones, and the split of B, 55 % of the kernel's VALU work,
 // is gone.  Same terms, same order of products: the results equal the raw kernel's bit for bit.
 // (a template, so that only the translation unit that lists the variant compiles it)
-template <int BPRE, int GLU = 0, int NTL = 5, int EDGE = 0>
+// FORM = 1, 2: GLU; 3: the epilogue of GroupParams in the store.
+template <int BPRE, int FORM = 0, int NTL = 5, int EDGE = 0>
 __global__ __launch_bounds__(W512Tile<NTL>::NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void cascmm_w512_kernel(const GroupParams p) {
+  constexpr int GLU = FORM == 3 ? 0 : FORM;
   typedef W512Tile<NTL> T;
   static_assert(NTL >= 2 && NTL <= 5, "");
   static_assert(!GLU || NTL == 5 || (GLU == 1 && BPRE && EDGE && NTL != 3), "");
@@ -593,6 +595,23 @@ __global__ __launch_bounds__(W512Tile<NTL>::NT) __attribute__((amdgpu_waves_per_
       out_pair(2, 0, 2, [&](int mi, int r) { return xbuf[(mi * 16 + r) * 64 + elane]; }, [&](int mi, int r) { return acc[mi][0][r] + b2; });
       own_pair(3, 1, 2);
       own_pair(4, 3, 4);
+    }
+    return;
+  }
+  if constexpr (FORM == 3) {
+    const ColumnEpilogue ep(epilogue_args(p), (float*)p.C[0], p.ldc, p.M, p.N, m0 + wm0, n0 + wn0);
+    float r[2][16];
+    ep.ask(r[0], 0, 4 * eg, el31, n0 + wn0 + el31 < p.N);
+#pragma unroll
+    for (int b = 0; b < T::MT * T::NTL; ++b) {
+      const int ni = b / T::MT, mi = b % T::MT, nx = (b + 1) / T::MT, mx = (b + 1) % T::MT, col = ni * 32 + el31;
+      const bool inside = n0 + wn0 + col < p.N;
+      if (b + 1 < T::MT * T::NTL) ep.ask(r[(b + 1) & 1], mx * 32, 4 * eg, nx * 32 + el31, n0 + wn0 + nx * 32 + el31 < p.N);
+      const float bv = bias && inside ? bias[n0 + wn0 + col] : 0.f;
+      float z[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z[e] = acc[mi][ni][e] + bv;
+      ep.store<kLargeTileStoreAux>(z, r[b & 1], mi * 32, 4 * eg, col, inside);
     }
     return;
   }

@@ -165,8 +165,10 @@ using WaveKOf = WaveK<W, MB, NB, AL, BPRE ? Lowp<FMT>::planes(TERMS) * NB * (W /
 // 14.9, 21.5; 71 x 3801 x 3520 96.4, 54.8, 66.1.  A second pass is dearer: with one element of A beyond the range 33.3, 29.7, 33.0, 86.6, with A's
 // first 512 k 2^30 below the others 37.9, 37.1, 39.2, 128.9.  Errors against 64 bits: 1.1 to 7.2 1e-9 (rms, of the sum of magnitudes), 6.1e-9
 // to 1.2e-8 in slots.
-template <int W, int MB, int NB, int AL, int TAIL, int FMT, int TERMS, int BPRE = 0, int GLU = 0, int SCALED = 0>
+// FORM: 1 is GLU, 2 the epilogue of GroupParams in the store.
+template <int W, int MB, int NB, int AL, int TAIL, int FMT, int TERMS, int BPRE = 0, int FORM = 0, int SCALED = 0>
 __global__ __launch_bounds__(512) void cascmm_wavek_kernel(const GroupParams p) {
+  constexpr int GLU = FORM == 1;
   static_assert(!GLU || (BPRE && W == 16 && NB == 4), "a value block and its gate block in one tile");
   static_assert(!SCALED || (FMT == CASCMM_FMT_FP16 && TERMS == 3 && !BPRE && TAIL), "for the calls of the slot kernels");
   typedef WaveKOf<W, MB, NB, AL, FMT, TERMS, BPRE> T;
@@ -599,10 +601,24 @@ __global__ __launch_bounds__(512) void cascmm_wavek_kernel(const GroupParams p) 
     const int blk = pos / (W * W), e = (pos / 64) % REGS, ln = pos % 64;
     const int row = m0 + W * (blk / NB) + 8 * (e >> 2) + 4 * (ln / W) + (e & 3);
     const int col = n0 + (BPRE ? W * (blk % NB) + (ln & (W - 1)) : NB * (ln & (W - 1)) + blk % NB);
+    float residual = 0.f;
+    if constexpr (FORM == 2) {
+      if (p.residual && row < p.M && (!TAIL || col < p.N)) residual = ((const float*)p.residual)[(int64_t)row * p.ldr + col];
+    }
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < T::NW; ++w) sum += part[((w * MB * NB + blk) * REGS + e) * 64 + ln];
     if constexpr (kScaled8 || SCALED) sum *= scale_out;
+    if constexpr (FORM == 2) {
+      // (a thread's residual is asked for before its sums are added)
+      if (row < p.M && (!TAIL || col < p.N)) {
+        float z[1] = {sum + (bias ? bias[col] : 0.f)};
+        if (p.preact) ((float*)p.preact)[(int64_t)row * p.ldp + col] = z[0];
+        activate(z, p.act);
+        C[(int64_t)row * p.ldc + col] = z[0] + residual;
+      }
+      continue;
+    }
     if (row < p.M && (!TAIL || col < p.N)) C[(int64_t)row * p.ldc + col] = sum + (bias ? bias[col] : 0.f);
   }
 }
