@@ -1173,14 +1173,18 @@ static int gemm_on_rows(int count, const void* const* A, const void* const* B, v
   for (int i = 0; i < count; ++i) {
     p.A[i] = A[i]; p.B[i] = B[i]; p.C[i] = C[i]; p.bias[i] = bias ? bias[i] : nullptr;
   }
-  if (!q.epi) return v.launch(p, stream);
+  if (!q.epi || (!q.epi->act && !q.epi->residual && !q.epi->preact)) return v.launch(p, stream);
   // the epilogue: in the store where the kernel has one that holds it, else behind it, on z in preact or in the result's place (z is rounded to the
   // elements' type then: 16-bit elements meet that in the bounds-checked kernels only)
   const Epilogue& ep = *q.epi;
   // (the fp32 kernels' stores have 32-bit offsets over the rows of a tile)
   const bool near_rows = std::max(ep.residual ? ep.ldr : 0, ep.preact ? ep.ldp : 0) * (2 * 256 * 4) <= INT32_MAX;
+  // An LDS-tiled kernel of twelve waves has 168 registers a wave: with z kept as well its store spills (8192 x 640 x 640, two bf16 terms, us: residual 36.6 here,
+  // 38.5 as a pass behind it; gelu 35.4, 36.1; gelu and z 36.9, 36.1; silu, residual and z 43.3, 39.1)
+  const bool tile = v.kind == KIND_TILE && !variant_info()[variant].bdirect && p.k_splits <= 1 && q.ldc * (2 * 256 * 4) <= INT32_MAX &&
+                    tile_has_epilogue(v.iodt, v.fmt, v.terms, v.full != 0, v.fast) && !(ep.preact && v.threads >= 768);
   if (v.kind == KIND_H16 || v.kind == KIND_HWK ||
-      (near_rows && (v.kind == KIND_F16K || v.kind == KIND_WAVEK || v.kind == KIND_SLOTK || v.kind == KIND_W512 || v.kind == KIND_W512E))) {
+      (near_rows && (tile || v.kind == KIND_F16K || v.kind == KIND_WAVEK || v.kind == KIND_SLOTK || v.kind == KIND_W512 || v.kind == KIND_W512E))) {
     p.epi = 1;
     p.act = ep.act;
     p.residual = ep.residual;
@@ -1194,7 +1198,7 @@ static int gemm_on_rows(int count, const void* const* A, const void* const* B, v
     p.ldc = ep.ldp;
   }
   const int st = v.launch(p, stream);
-  if (st != CASCMM_OK || (!ep.preact && !ep.residual && !ep.act)) return st;
+  if (st != CASCMM_OK) return st;
   return launch_epilogue(p.C[0], p.ldc, ep.residual, ep.ldr, C[0], q.ldc, q.M, q.N, ep.act, q.dtype, stream);
 }
 

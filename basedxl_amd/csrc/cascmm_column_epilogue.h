@@ -64,4 +64,94 @@ struct ColumnEpilogue {
   }
 };
 
+// The store of the LDS-tiled kernels: blocks of permuted columns come in runs of RUN, block b of the tile and lane l31 <-> column 128 (b / 4) + 4 l31 + b % 4, so a
+// lane holds RUN adjacent columns of a row; the others are as above.  A quad of rows at a time, the next one's residual asked for before.
+template <class TL>
+__device__ __forceinline__ void tile_epilogue(const GroupParams& p, float* C, const float* bias, int m0, int n0, int wm0, int wn0, int l31, int g,
+                                              f32x16 (&res)[TL::MT][TL::NTL]) {
+  constexpr int NQ = (TL::BNQ == 0) ? 0 : (TL::WN == 1 ? TL::BNQ / 32 : TL::NTL), RUN = (NQ % 4 == 0) ? 4 : 2;
+  const EpilogueArgs args = epilogue_args(p);
+  const ColumnEpilogue ep(args, C, p.ldc, p.M, p.N, m0 + wm0, n0);
+  const bool vec = ((p.N | p.ldc | p.ldr | p.ldp) & 3) == 0 && (((uintptr_t)C | (uintptr_t)p.residual | (uintptr_t)p.preact) & 15) == 0;
+  typedef float run_t __attribute__((ext_vector_type(RUN)));
+#pragma unroll
+  for (int r0 = 0; r0 < NQ; r0 += RUN) {
+    const int b = (wn0 >> 5) + r0, col = (b >> 2) * 128 + 4 * l31 + (b & 3);   // (col + i exists or not together with the run where vec)
+    float bv[RUN];
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) bv[i] = bias && n0 + col + i < p.N ? bias[n0 + col + i] : 0.f;
+    auto place = [&](int row, int ld, int i) {
+      return (int)((n0 + col + i < p.N ? (unsigned)(4 * g * ld + (col + i) * 4) : 0x7FFFFFFFu) + (unsigned)(row * ld));
+    };
+    auto ask = [&](int k, run_t (&to)[4]) {
+      if (!ep.res) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = (k >> 2) * 32 + (k & 3) * 8 + e;
+        if (vec) {
+          if constexpr (RUN == 4) to[e] = llvm_raw_buffer_load_v4f32(ep.rr, place(row, ep.ldr, 0), 0, 0);
+          else to[e] = llvm_raw_buffer_load_v2f32(ep.rr, place(row, ep.ldr, 0), 0, 0);
+        } else {
+#pragma unroll
+          for (int i = 0; i < RUN; ++i) to[e][i] = llvm_raw_buffer_load_f32(ep.rr, place(row, ep.ldr, i), 0, 0);
+        }
+      }
+    };
+    auto out = [&](const i32x4& to, int ld, int row, const run_t& z) {
+      if (vec) {
+        if constexpr (RUN == 4) llvm_raw_buffer_store_v4f32(z, to, place(row, ld, 0), 0, kResultStoreAux);
+        else llvm_raw_buffer_store_v2f32(z, to, place(row, ld, 0), 0, kResultStoreAux);
+      } else {
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) llvm_raw_buffer_store_f32(z[i], to, place(row, ld, i), 0, kResultStoreAux);
+      }
+    };
+    run_t r[2][4];
+    ask(0, r[0]);
+#pragma unroll
+    for (int k = 0; k < 4 * TL::MT; ++k) {
+      const int mi = k >> 2, q = k & 3;
+      if (k + 1 < 4 * TL::MT) ask(k + 1, r[(k + 1) & 1]);
+      float z[4 * RUN];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) z[e * RUN + i] = res[mi][r0 + i][4 * q + e] + bv[i];
+      if (ep.pre) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          run_t v;
+#pragma unroll
+          for (int i = 0; i < RUN; ++i) v[i] = z[e * RUN + i];
+          out(ep.rp, ep.ldp, mi * 32 + q * 8 + e, v);
+        }
+      }
+      activate(z, ep.act);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        run_t v;
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) v[i] = z[e * RUN + i];
+        if (ep.res) v += r[k & 1][e];
+        out(ep.rc, ep.ldc, mi * 32 + q * 8 + e, v);
+      }
+    }
+  }
+  if constexpr (NQ < TL::NTL) {
+    constexpr int BLOCKS = TL::MT * (TL::NTL - NQ);
+    float r[2][16];
+    ep.ask(r[0], 0, 4 * g, wn0 + NQ * 32 + l31, n0 + wn0 + NQ * 32 + l31 < p.N);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      const int ni = NQ + b / TL::MT, mi = b % TL::MT, nx = NQ + (b + 1) / TL::MT, mx = (b + 1) % TL::MT, col = wn0 + ni * 32 + l31;
+      if (b + 1 < BLOCKS) ep.ask(r[(b + 1) & 1], mx * 32, 4 * g, wn0 + nx * 32 + l31, n0 + wn0 + nx * 32 + l31 < p.N);
+      const float bv = bias && n0 + col < p.N ? bias[n0 + col] : 0.f;
+      float z[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z[e] = res[mi][ni][e] + bv;
+      ep.store<kResultStoreAux>(z, r[b & 1], mi * 32, 4 * g, col, n0 + col < p.N);
+    }
+  }
+}
+
 }  // namespace cascmm

@@ -151,10 +151,16 @@ __device__ __forceinline__ i32x4 make_rsrc(const void* base, int64_t bytes) {
   return r;
 }
 
+// (cascmm_column_epilogue.h)
+template <class TL>
+__device__ __forceinline__ void tile_epilogue(const GroupParams& p, float* C, const float* bias, int m0, int n0, int wm0, int wn0, int l31, int g,
+                                              f32x16 (&res)[TL::MT][TL::NTL]);
+
 // BPRE: the right operand comes already split ("prepared", see prepare_weight_kernel in
 // cascmm_api.hip): B[i] points to 16-byte operand slots [plane][K/8][N], the producers copy
 // slots to LDS without touching the VALU.  Fast path only, every column staged singly.
-template <class TL, int IODT, int FMT, int TERMS, bool FULL, bool BPRE = false>
+// EPI: the epilogue of GroupParams in the store (fp32 elements, one problem, no K split).
+template <class TL, int IODT, int FMT, int TERMS, bool FULL, bool BPRE = false, bool EPI = false>
 struct TileGemm {
   typedef Lowp<FMT> LP;
   typedef typename LP::Vec Vec;
@@ -759,6 +765,10 @@ struct TileGemm {
       ldc = p.N;
     }
     const bool interior = (m0 + TL::BM <= p.M) && (n0 + TL::BN <= p.N) && ldc * (int64_t)(TL::BM * ES) < 0x7FFFFFFF;
+    if constexpr (EPI) {
+      tile_epilogue<TL>(p, (float*)C, (const float*)bias, m0, n0, wm0, wn0, l31, g, res);
+      return;
+    }
     // Column blocks of this wave that hold permuted columns come in runs of RUN blocks of one
     // 128-column group: block b of the tile (b = wn0/32 + ni), lane l31 <-> column
     // 128*(b/4) + 4*l31 + b%4.
@@ -923,6 +933,12 @@ struct TileGemm {
     }
   }
 };
+
+template <class TL, int FMT, int TERMS, bool BPRE>
+__global__ __launch_bounds__(TL::NT) void cascmm_tile_epilogue_kernel(const GroupParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char cascmm_smem[];
+  TileGemm<TL, CASCMM_DT_F32, FMT, TERMS, false, BPRE, true>::template run<true>(p, (u32x4*)cascmm_smem);
+}
 
 template <class TL, int IODT, int FMT, int TERMS, bool FULL, bool FAST, bool BPRE = false>
 __global__ __launch_bounds__(TL::NT) void cascmm_tile_kernel(const GroupParams p) {

@@ -77,25 +77,34 @@ struct VariantDesc {
   bool scaled = false;      // takes the calls of the slot kernels (cascmm_wavek_kernel.h, SCALED)
 };
 
+// the LDS-tiled kernels that have a form with the epilogue in the store: the cascades of fp32 elements that calls choose, whole stages
+constexpr bool tile_has_epilogue(int iodt, int fmt, int terms, bool full, bool fast) {
+  return iodt == CASCMM_DT_F32 && fast && !full && ((fmt == CASCMM_FMT_BF16 && terms == 2) || (fmt == CASCMM_FMT_FP16 && terms == 3));
+}
 template <class TL, int IODT, int FMT, int TERMS, bool FULL, bool FAST, bool BPRE = false>
 int launch_tile(const GroupParams& p, hipStream_t stream) {
-  auto kfn = cascmm_tile_kernel<TL, IODT, FMT, TERMS, FULL, FAST, BPRE>;
+  void (*kfn)(const GroupParams) = cascmm_tile_kernel<TL, IODT, FMT, TERMS, FULL, FAST, BPRE>;
+  if (p.epi) {
+    if constexpr (tile_has_epilogue(IODT, FMT, TERMS, FULL, FAST)) kfn = cascmm_tile_epilogue_kernel<TL, FMT, TERMS, BPRE>;
+    else return CASCMM_ERR_BAD_VARIANT;
+    if (p.count != 1 || p.glu || p.k_splits > 1) return CASCMM_ERR_BAD_VARIANT;
+  }
   if (p.kernel_out) { *p.kernel_out = (const void*)kfn; return CASCMM_OK; }
   constexpr int lds = LdsLayout<TL, Lowp<FMT>::planes(TERMS)>::kBytes;
   static_assert(lds <= 160 * 1024, "tile does not fit the 160 KB LDS");
   if (lds > 64 * 1024) {
-    static LdsFlags lds_set;
-    if (!ensure_lds((const void*)kfn, lds, lds_set)) return CASCMM_ERR_LAUNCH;
+    static LdsFlags lds_set[2];
+    if (!ensure_lds((const void*)kfn, lds, lds_set[p.epi ? 1 : 0])) return CASCMM_ERR_LAUNCH;
   }
   // persistent grid: at most as many workgroups as can be resident at once on this device
-  static std::atomic<int> occupancy[kMaxDevices];
+  static std::atomic<int> occupancy[2][kMaxDevices];
   const int dev = device_index();
   if (dev < 0) return CASCMM_ERR_LAUNCH;
-  int per_cu = occupancy[dev].load(std::memory_order_relaxed);
+  int per_cu = occupancy[p.epi ? 1 : 0][dev].load(std::memory_order_relaxed);
   if (per_cu == 0) {
     int n = 0;
     per_cu = (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, (const void*)kfn, TL::NT, lds) == hipSuccess && n > 0) ? n : 1;
-    occupancy[dev].store(per_cu, std::memory_order_relaxed);
+    occupancy[p.epi ? 1 : 0][dev].store(per_cu, std::memory_order_relaxed);
   }
   const int splits = p.k_splits > 1 ? p.k_splits : 1;
   if (splits > 1) {
@@ -160,7 +169,7 @@ inline size_t skinny_workspace_bytes(int64_t M, int64_t N, int64_t K, int bm, in
 template <class TL, int FMT, int TERMS, bool FULL, bool SPLITK>
 int launch_bdirect(const GroupParams& gp, hipStream_t stream) {
   if (gp.kernel_out) { *gp.kernel_out = (const void*)cascmm_bdirect_kernel<TL, FMT, TERMS, FULL, SPLITK>; return CASCMM_OK; }
-  if (gp.count != 1) return CASCMM_ERR_BAD_VARIANT;
+  if (gp.count != 1 || gp.epi) return CASCMM_ERR_BAD_VARIANT;
   GemmParams p;
   memset(&p, 0, sizeof(p));
   p.A = gp.A[0]; p.B = gp.B[0]; p.C = gp.C[0]; p.bias = gp.bias[0];
@@ -331,7 +340,7 @@ int launch_f8k64(const GroupParams& p, hipStream_t stream) {
   typedef typename F8Tile<MT>::T T;
   void (*kfn)(const F8K64Params) = MT == 0 ? cascmm_f8wk_kernel<0> : cascmm_f8k64_kernel<(MT == 0 ? 1 : MT)>;
   if (p.kernel_out) { *p.kernel_out = (const void*)kfn; return CASCMM_OK; }
-  if (p.count != 1 || p.glu || p.k_splits > 1 || p.K % T::BK != 0 || p.K == 0) return CASCMM_ERR_BAD_VARIANT;
+  if (p.count != 1 || p.glu || p.epi || p.k_splits > 1 || p.K % T::BK != 0 || p.K == 0) return CASCMM_ERR_BAD_VARIANT;
   const size_t need = f8k64_workspace_bytes(p.M, p.N, p.K, BPRE, T::BM);
   if (!p.workspace || p.workspace_bytes < need) return CASCMM_ERR_WORKSPACE;
   if ((uintptr_t)p.workspace % 16 != 0) return CASCMM_ERR_ALIGNMENT;
