@@ -12,7 +12,8 @@ from ..layer_norm import add_layer_norm, layer_norm
 
 class BasedXLLayerNorm(nn.Module):
     """Wraps an ``nn.LayerNorm`` over the last axis, whose parameters it keeps (the same objects: they train as before).
-    ``forward(x)`` is the norm; ``forward(x, residual)`` returns the norm of ``x + residual`` and the sum itself, in one kernel."""
+    ``forward(x)`` is the norm; ``forward(x, residual)`` returns the norm of ``x + residual`` and the sum itself, in one kernel.
+    Traced by torch.compile it is one opaque op without gradients."""
 
     def __init__(self, submodule: nn.LayerNorm):
         super().__init__()
@@ -36,9 +37,9 @@ class BasedXLLayerNorm(nn.Module):
 
 
 def patch_layer_norms(model: nn.Module) -> nn.Module:
-    """Replace every ``nn.LayerNorm`` child over the last axis with :class:`BasedXLLayerNorm`."""
+    """Replace every ``nn.LayerNorm`` child over the last axis with :class:`BasedXLLayerNorm` (subclasses, which may compute something else, stay)."""
     for module in list(model.modules()):
         for name, child in list(module.named_children()):
-            if isinstance(child, nn.LayerNorm) and len(child.normalized_shape) == 1:
+            if type(child) is nn.LayerNorm and len(child.normalized_shape) == 1:
                 setattr(module, name, BasedXLLayerNorm(child))
     return model

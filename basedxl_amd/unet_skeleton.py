@@ -56,9 +56,10 @@ class FeedForward(nn.Module):
         self.net = nn.ModuleList([GEGLU(dim, dim * mult), nn.Dropout(0.0), nn.Linear(dim * mult, dim)])
 
     def forward(self, x, residual=None):
-        for m in self.net[:-1]:
+        *inner, last = self.net
+        for m in inner:
             x = m(x)
-        return last_layer(self.net[-1], x, residual)
+        return last_layer(last, x, residual)
 
 
 class Attention(nn.Module):

@@ -30,6 +30,16 @@ def test_norm_patcher_keeps_parameters_and_leaves_other_norms_alone():
         model["a"](torch.zeros(2, 7))
 
 
+def test_norm_patcher_leaves_subclasses_alone():
+    class Scaled(nn.LayerNorm):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    model = nn.Sequential(Scaled(8), nn.LayerNorm(8))
+    patch_layer_norms(model)
+    assert type(model[0]) is Scaled and isinstance(model[1], BasedXLLayerNorm)
+
+
 def test_linear_wrapper_checks_its_activation():
     with pytest.raises(ValueError, match="activation"):
         BasedXLLowPLinear(nn.Linear(4, 4), activation="tanh")
