@@ -147,10 +147,10 @@ static bool variant_matches(const VariantDesc& v, const Problem& q, RowFit fit) 
   if (v.fast && !any_rows && v.kind != KIND_H16 && v.kind != KIND_HWK && (v.kind != KIND_W512E || q.glu) && q.K % v.BK != 0) return false;
   if (v.kind == KIND_SPLITK && (q.M > 5 * v.BM || q.K < 4 * v.BK)) return false;  // skinny: few row tiles, deep K
   if (v.kind == KIND_F8K64 && (q.products != CASCMM_PROD_TRI || q.K % v.BK != 0 || q.K == 0 || q.glu ||
-                               f8k64_slot_bytes(q.M, q.K) > INT32_MAX || f8k64_slot_bytes(q.N, q.K) > INT32_MAX))
+                               (v.BM == F8WK::BM && beyond_i32(q.ldc, F8WK::BM, 4)) || f8k64_slot_bytes(q.M, q.K) > INT32_MAX || f8k64_slot_bytes(q.N, q.K) > INT32_MAX))
     return false;
   if (v.kind == KIND_F16K && (q.products != CASCMM_PROD_TRI || q.K % v.BK != 0 || q.K == 0 || q.glu || q.bpre ||
-                              (v.BM == F16K::BM && q.K > F16K::MAX_K) || q.K * q.ldb * 4 > INT32_MAX ||
+                              (v.BM == F16K::BM && q.K > F16K::MAX_K) || (v.BM == F16WK::BM && beyond_i32(q.ldc, F16WK::BM, 4)) || q.K * q.ldb * 4 > INT32_MAX ||
                               f16k_slot_bytes(q.M, q.K) > INT32_MAX || f16k_slot_bytes(q.N, q.K) > INT32_MAX))
     return false;
   if (v.bpre && v.kind != KIND_F8K64 && prepared_as_k16_slots(q.K, q.fmt, q.terms, q.glu)) return false;   // other layout
@@ -1178,10 +1178,10 @@ static int gemm_on_rows(int count, const void* const* A, const void* const* B, v
   // elements' type then: 16-bit elements meet that in the bounds-checked kernels only)
   const Epilogue& ep = *q.epi;
   // (the fp32 kernels' stores have 32-bit offsets over the rows of a tile)
-  const bool near_rows = std::max(ep.residual ? ep.ldr : 0, ep.preact ? ep.ldp : 0) * (2 * 256 * 4) <= INT32_MAX;
+  const bool near_rows = std::max({ep.residual ? ep.ldr : 0, ep.preact ? ep.ldp : 0, q.ldc}) <= INT32_MAX / (2 * 256 * 4);
   // An LDS-tiled kernel of twelve waves has 168 registers a wave: with z kept as well its store spills (8192 x 640 x 640, two bf16 terms, us: residual 36.6 here,
   // 38.5 as a pass behind it; gelu 35.4, 36.1; gelu and z 36.9, 36.1; silu, residual and z 43.3, 39.1)
-  const bool tile = v.kind == KIND_TILE && !variant_info()[variant].bdirect && p.k_splits <= 1 && q.ldc * (2 * 256 * 4) <= INT32_MAX &&
+  const bool tile = v.kind == KIND_TILE && !variant_info()[variant].bdirect && p.k_splits <= 1 &&
                     tile_has_epilogue(v.iodt, v.fmt, v.terms, v.full != 0, v.fast) && !(ep.preact && v.threads >= 768);
   if (v.kind == KIND_H16 || v.kind == KIND_HWK ||
       (near_rows && (tile || v.kind == KIND_F16K || v.kind == KIND_WAVEK || v.kind == KIND_SLOTK || v.kind == KIND_W512 || v.kind == KIND_W512E))) {

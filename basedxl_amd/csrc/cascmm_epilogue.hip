@@ -65,7 +65,7 @@ using namespace cascmm;
 extern "C" {
 
 size_t cascmm_epilogue_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
-  if (rows < 0 || cols <= 0 || rows > INT32_MAX || cols > (1 << 30) || !ep_dtype(dtype)) return 0;
+  if (rows < 0 || cols <= 0 || rows > INT32_MAX || cols > kFinishMostCols || !ep_dtype(dtype)) return 0;
   return (size_t)ep_parts(rows, cols, dtype) * (size_t)cols * sizeof(float);
 }
 
@@ -74,7 +74,7 @@ int cascmm_epilogue_backward(const void* dy, const void* z, void* dz, void* dbia
   if (!ep_dtype(dtype)) return CASCMM_ERR_BAD_DTYPE;
   if (activation < CASCMM_ACT_NONE || activation > CASCMM_ACT_SILU) return CASCMM_ERR_BAD_FORMAT;
   if (rows < 0 || cols < 0 || lddy < cols || (activation && ldz < cols) || (dz && lddz < cols)) return CASCMM_ERR_BAD_SHAPE;
-  if (rows > INT32_MAX || cols > (1 << 30)) return CASCMM_ERR_TOO_LARGE;
+  if (rows > INT32_MAX || cols > kFinishMostCols) return CASCMM_ERR_TOO_LARGE;
   if (cols == 0 || (!dz && !dbias) || (rows == 0 && !dbias)) return CASCMM_OK;
   if (rows > 0 && (!dy || (activation && !z))) return CASCMM_ERR_NULL_POINTER;
   const size_t es = ep_size(dtype);

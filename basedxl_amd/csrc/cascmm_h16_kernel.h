@@ -486,7 +486,7 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
     E *C = (E*)p.C[prob], *pre = (E*)p.preact;
     const int64_t ldc = p.ldc, ldr = p.ldr, ldp = p.ldp, row0 = m0 + wm0;
     for (int c = lane; c < NB * 32; c += 64) bl[c] = bias && oc0 + c < N ? Io::load(bias + oc0 + c) : 0.f;
-    const bool near_rows = (ldc > ldr ? (ldc > ldp ? ldc : ldp) : (ldr > ldp ? ldr : ldp)) * (2 * T::WTM) <= 0x7FFFFFFF;
+    const bool near_rows = (ldc > ldr ? (ldc > ldp ? ldc : ldp) : (ldr > ldp ? ldr : ldp)) <= 0x7FFFFFFF / (2 * T::WTM);
     const bool vec = near_rows && ((ldc | ldr | ldp | N) & 7) == 0 && (((uintptr_t)C | (uintptr_t)res | (uintptr_t)pre) & 15) == 0;
     // (rows past M fall beyond the end of a buffer, columns past N are sent there; of one residual row for all, all rows are that one)
     auto rows_of = [&](const E* base, int64_t ld) {

@@ -10,7 +10,6 @@ namespace cascmm {
 static bool norm_aligned(const void* p, size_t a) { return (uintptr_t)p % a == 0; }
 static size_t norm_size(int dtype) { return dtype == CASCMM_DT_F32 ? 4 : 2; }
 static bool norm_dtype(int dtype) { return dtype == CASCMM_DT_F32 || dtype == CASCMM_DT_F16 || dtype == CASCMM_DT_BF16; }
-constexpr int64_t kNormMostCols = 1 << 30;   // (column numbers and a step beyond the last are 32-bit)
 
 // The lanes of a row and the elements of a lane: four lanes take rows shorter than a chunk of 16 bytes, eight rows of up to 64 columns, sixteen up to 256, a wave up to 2048 (in the backward pass, which
 // holds the sums beside a row, 1536), four of them up to 8192; none: longer rows
@@ -42,7 +41,7 @@ static int64_t norm_parts(int64_t rows, int64_t cols, int dtype) {
 static int norm_check(int64_t rows, int64_t cols, int dtype, int weight_dtype) {
   if (!norm_dtype(dtype) || (weight_dtype != dtype && weight_dtype != CASCMM_DT_F32)) return CASCMM_ERR_BAD_DTYPE;
   if (rows < 0 || cols < 0) return CASCMM_ERR_BAD_SHAPE;
-  if (rows > INT32_MAX || cols > kNormMostCols) return CASCMM_ERR_TOO_LARGE;
+  if (rows > INT32_MAX || cols > kFinishMostCols) return CASCMM_ERR_TOO_LARGE;
   return CASCMM_OK;
 }
 
@@ -145,7 +144,7 @@ int cascmm_layer_norm(const void* x, const void* residual, const void* weight, c
 }
 
 size_t cascmm_layer_norm_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
-  if (rows < 0 || cols < 0 || rows > INT32_MAX || cols > kNormMostCols || !norm_dtype(dtype)) return 0;
+  if (rows < 0 || cols < 0 || rows > INT32_MAX || cols > kFinishMostCols || !norm_dtype(dtype)) return 0;
   return (size_t)norm_parts(rows, cols, dtype) * 2 * (size_t)cols * sizeof(float);
 }
 

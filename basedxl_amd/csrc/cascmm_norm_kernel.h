@@ -515,6 +515,7 @@ __global__ __launch_bounds__(256) void cascmm_layer_norm_sums_kernel(const NormP
 // out[col] (and out2[col], the second half of a partial row) = sum over `parts` rows of partials, [parts][halves][cols].  Thirty-two columns a
 // workgroup, its 32 rows of threads a share of the parts each; they meet in LDS in order.
 constexpr int kFinishCols = 32;
+constexpr int64_t kFinishMostCols = 1 << 26;   // (a launch has fewer than 2^32 threads; column numbers and a step beyond the last stay in 32 bits)
 template <int ODT>
 __global__ __launch_bounds__(1024) void cascmm_column_finish_kernel(const float* __restrict__ partials, int parts, int halves, int64_t cols, void* out, void* out2) {
   typedef typename IoType<ODT>::T E;

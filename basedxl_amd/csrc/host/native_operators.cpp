@@ -61,6 +61,13 @@ struct Wanted {
   bool next(bool there = true) { return there && ctx->needs_input_grad(edge++); }
 };
 
+// a tensor whose forward-mode tangent would be lost here (the wrapper raises)
+bool dual(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
+  return false;
+}
+
 // a tensor or None (undefined); false: not the ordinary case
 bool optional_tensor(PyObject* o, int device, at::Tensor& t) {
   if (o == Py_None) return true;
@@ -169,7 +176,7 @@ bool norm_arguments(PyObject* const* args, int device, const at::Tensor*& x, at:
   eps = PyFloat_AsDouble(eps_arg);
   if (PyErr_Occurred()) { PyErr_Clear(); return false; }
   if (!(eps >= 0) || !(eps < 1e30)) return false;
-  if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type()) return false;
+  if ((weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type()) || dual({x, &weight, &bias})) return false;
   for (const at::Tensor* t : {&weight, &bias})
     if (t->defined() && (t->dim() != 1 || t->size(0) != cols || !t->is_contiguous() || (t->scalar_type() != x->scalar_type() && t->scalar_type() != at::kFloat))) return false;
   return true;
@@ -283,6 +290,7 @@ bool result_arguments(Product& p, int64_t N) {
   const at::Tensor& a = *p.a;
   if (p.bias.defined() && (p.bias.dim() != 1 || p.bias.size(0) != N || p.bias.scalar_type() != a.scalar_type() || !p.bias.is_contiguous())) return false;
   p.ldr = 0;
+  if (dual({&a, &p.bias, &p.residual})) return false;
   if (!p.residual.defined()) return true;
   int64_t rows, cols;
   if (p.residual.scalar_type() != a.scalar_type() || p.residual.dim() != a.dim() || !rows_of(p.residual, rows, cols, p.ldr) || cols != N) return false;
@@ -337,7 +345,7 @@ PyObject* add_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int64_t rows, cols, ld;
     if (!residual || !optional_tensor(args[2], device, weight) || !optional_tensor(args[3], device, bias) || !norm_arguments(args, device, x, weight, bias, args[4], eps))
       Py_RETURN_NONE;
-    if (residual->scalar_type() != x->scalar_type() || residual->sizes() != x->sizes() || !rows_of(*residual, rows, cols, ld)) Py_RETURN_NONE;
+    if (residual->scalar_type() != x->scalar_type() || residual->sizes() != x->sizes() || dual({residual}) || !rows_of(*residual, rows, cols, ld)) Py_RETURN_NONE;
     at::Tensor y, s;
     if (differentiated({x, residual, &weight, &bias})) {
       variable_list both = AddLayerNormNode::apply(*x, *residual, optional_of(weight), optional_of(bias), eps);
@@ -374,7 +382,7 @@ PyObject* epilogue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int products = products_code(args[7]);
     if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
     const int64_t N = b->size(1);
-    if (fmt < 0 || terms < 1 || products < 0 || !result_arguments(p, N)) Py_RETURN_NONE;
+    if (fmt < 0 || terms < 1 || products < 0 || !result_arguments(p, N) || dual({b})) Py_RETURN_NONE;
     if (differentiated({p.a, b, &p.bias, &p.residual}))
       return THPVariable_Wrap(EpilogueNode::apply(*p.a, *b, optional_of(p.bias), optional_of(p.residual), (int64_t)p.act, (int64_t)fmt, (int64_t)terms, (int64_t)products));
     return run_product(p, b->const_data_ptr(), 0, N, fmt, terms, products, device);

@@ -7,10 +7,17 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .cascaded_lowp_matmul import _DTYPES, _rows
+
+
+def refuse_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode differentiation (dual tensors) would lose its tangents here."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} is differentiable in reverse mode only")
 
 
 def _check(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float) -> None:
@@ -149,6 +156,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if y is not None:
         return y
     _check(x, weight, bias, eps)
+    refuse_tangents("layer_norm", x, weight, bias)
     if _differentiated(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _forward(x, None, weight, bias, float(eps), False)[0]
@@ -164,6 +172,7 @@ def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[tor
         return both
     _check(x, weight, bias, eps)
     _check_residual(x, residual)
+    refuse_tangents("add_layer_norm", x, residual, weight, bias)
     if _differentiated(x, residual, weight, bias):
         return _AddLayerNorm.apply(x, residual, weight, bias, float(eps))
     y, s, _, _ = _forward(x, residual, weight, bias, float(eps), False)

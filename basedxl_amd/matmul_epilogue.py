@@ -13,6 +13,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .cascaded_lowp_matmul import (_DTYPES, PreparedWeight, _activation_exps, _check_bias, _check_device_tensor, _rows, _workspace, _workspace_bytes,
                                    cascaded_lowp_matmul, default_cascade)
+from .layer_norm import refuse_tangents
 
 
 def _ld(t2: torch.Tensor) -> int:
@@ -203,6 +204,7 @@ def cascaded_lowp_matmul_epilogue(a: torch.Tensor, b, *, bias: Optional[torch.Te
         except RuntimeError:
             raise ValueError(f"residual of shape {tuple(residual.shape)} does not broadcast to the result's {shape}") from None
     operands = [t for t in (a, None if prepared else b, bias, residual) if t is not None]
+    refuse_tangents("cascaded_lowp_matmul_epilogue", *operands)
     if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
         if prepared and a.requires_grad:
             raise RuntimeError("cascaded_lowp_matmul_epilogue: a gradient with respect to a needs the weight itself, not a PreparedWeight")

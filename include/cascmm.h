@@ -341,8 +341,8 @@ int cascmm_gemm_epilogue(const void* A, const void* B, int b_prepared, void* C, 
                          const int32_t* tensor_exps, void* workspace, size_t workspace_bytes, void* stream);
 /* The way back: dz = dy * activation'(z) and dbias = sum over rows of dz (before dz is rounded), [rows, cols] with leading dimensions; dz or
  * dbias may be NULL, and without an activation z too.  For dbias the workspace holds cascmm_epilogue_workspace_bytes(rows, cols, dtype) bytes
- * (16-byte aligned, contents need no initialisation); the sums are fp32 in a fixed order, without atomics.  The gradients of A and B are
- * products of dz with the transposed operands. */
+ * (16-byte aligned, contents need no initialisation); the sums are fp32 in a fixed order, without atomics.  Up to 2^26 columns.  The gradients
+ * of A and B are products of dz with the transposed operands. */
 size_t cascmm_epilogue_workspace_bytes(int64_t rows, int64_t cols, int dtype);
 int cascmm_epilogue_backward(const void* dy, const void* z, void* dz, void* dbias, int64_t rows, int64_t cols,
                              int64_t lddy, int64_t ldz, int64_t lddz, int activation, int dtype, void* workspace,
@@ -357,7 +357,7 @@ int cascmm_transpose(const void* x, void* out, int64_t rows, int64_t cols, int64
  *     s = x + residual, rounded to `dtype` (residual NULL: s = x);   y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias
  * weight, bias: [cols] of weight_dtype (`dtype` or fp32), NULL: ones, zeros.  With a residual s is written to `sum` (both or neither).
  * mean, rstd: fp32 [rows] for the backward pass, both or neither.  Statistics and everything between a load and a store are fp32, each
- * result is rounded once.  Rows of any alignment of whole elements; y and sum overlap no operand.
+ * result is rounded once.  Rows of any alignment of whole elements, up to 2^26 columns; y and sum overlap no operand.
  */
 int cascmm_layer_norm(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* sum,
                       float* mean, float* rstd, int64_t rows, int64_t cols, int64_t ldx, int64_t ldr, int64_t ldy,

@@ -342,3 +342,15 @@ def test_the_host_extension_takes_ordinary_calls(gpu_device):
                  (x, w, None, "a"), (x.double(), None, None, 1e-5), (x[:0], w, None, 1e-5), (x.transpose(0, 1), w, None, 1e-5), (x, w, None), (x, 3, None, 1e-5)):
         assert native.layer_norm(*args) is None
     assert native.add_layer_norm(x, x[:2], w, None, 1e-5) is None and native.add_layer_norm(x, x.half(), w, None, 1e-5) is None
+
+
+def test_forward_mode_tangents_are_refused(gpu_device, path):
+    from torch.autograd import forward_ad
+    x, w = torch.randn(4, 8, device=gpu_device), torch.ones(8, device=gpu_device)
+    with forward_ad.dual_level():
+        for call in ((forward_ad.make_dual(x, x), w, w), (x, forward_ad.make_dual(w, w), w), (x, w, forward_ad.make_dual(w, w))):
+            with pytest.raises(NotImplementedError):
+                layer_norm(*call)
+        with pytest.raises(NotImplementedError):
+            add_layer_norm(x, forward_ad.make_dual(x, x), w, w)
+        assert torch.equal(layer_norm(x, w, w), layer_norm(x, w, w))

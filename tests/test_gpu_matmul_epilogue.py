@@ -419,3 +419,75 @@ def test_the_host_extension_takes_ordinary_calls(gpu_device):
         for k, v in change.items():
             call[k] = v
         assert native.epilogue(*call) is None, change
+
+
+@pytest.mark.parametrize("cascade", [*CASCADES, "fp8x3"])
+def test_rows_far_apart(gpu_device, cascade):
+    """Results and residuals whose rows are 2.2 GB apart, beyond what a store's offsets span, and a single row whose distance to the next is beyond all numbers."""
+    dtype, options, lost = CASCADES[cascade] if cascade in CASCADES else (torch.float32, {"lowp": "fp8", "terms": 3}, None)
+
+    def check(y, a, b, bias, act, residual):
+        if lost is not None:
+            return check_forward(y, a, b, bias, act, residual, dtype, lost, cascade)
+        # (three fp8 terms leave out 2^-12 of an operand and products of 2^-12 twice: below 2^-9 S, and S is some 0.8 K^1/2 of z: 0.06 z; a lost row is 0.7 of it)
+        z = ACTIVATIONS[act](z_of(a, b, bias, dtype, 0)[0]) + (0 if residual is None else residual.double())
+        assert float((y.double() - z).norm()) <= 0.1 * float(z.norm())
+
+    for M, K, N in ((1, 64, 64), (2, 640, 320), (2, 1280, 2560)):
+        a, b, bias, residual, _ = operands(M, K, N, dtype, gpu_device)
+        far = 2_200_000_000 // a.element_size()
+        store = torch.empty(far * (M - 1) + N, dtype=dtype, device=gpu_device)
+        rows = store.as_strided((M, N), (far if M > 1 else 2 ** 59, 1))
+        for act, r in (("silu", residual), (None, None)):
+            rows.fill_(math.nan)
+            check(cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation=act, residual=r, out=rows, **options), a, b, bias, act, r)
+        rows.copy_(residual)
+        check(cascaded_lowp_matmul_epilogue(a, b, bias=bias, activation="silu", residual=rows, **options), a, b, bias, "silu", residual)
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_gradients_that_arrive_strided(gpu_device, path, cascade, act):
+    """dy as columns of wider rows, at a distance and an offset of their own."""
+    dtype, options, lost = CASCADES[cascade]
+    for M, K, N in ((70, 33, 45), (64, 128, 96), (5, 640, 1283)):
+        a, b, bias, residual, dy = operands(M, K, N, dtype, gpu_device)
+        wide = torch.full((M, N + 13), math.nan, dtype=dtype, device=gpu_device)
+        wide[:, 5:5 + N] = dy
+        leaves = [t.clone().requires_grad_() for t in (a, b, bias, residual)]
+        y = cascaded_lowp_matmul_epilogue(leaves[0], leaves[1], bias=leaves[2], activation=act, residual=leaves[3], **options)
+        grads = torch.autograd.grad(y, leaves, wide[:, 5:5 + N])
+        check_backward(grads, dy, a, b, bias, act, residual, dtype, lost, f"{M} {K} {N}")
+
+
+def test_two_threads_on_one_stream(gpu_device):
+    """Calls whose launches meet in the stream's workspace, from two threads at once."""
+    import threading
+    stream, wrong = torch.cuda.current_stream(gpu_device), []
+    sets = [operands(154, 1280, 640, torch.float32, gpu_device, seed=s) for s in (1, 2)]
+    options = {"lowp": "fp16", "terms": 3}
+    wants = [cascaded_lowp_matmul_epilogue(s[0], s[1], bias=s[2], activation="gelu", residual=s[3], **options) for s in sets]
+
+    def work(ops, want):
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                got = cascaded_lowp_matmul_epilogue(ops[0], ops[1], bias=ops[2], activation="gelu", residual=ops[3], **options)
+                if not torch.equal(got, want):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=work, args=pair) for pair in zip(sets, wants)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_forward_mode_tangents_are_refused(gpu_device, path):
+    from torch.autograd import forward_ad
+    a, b, bias, residual, _ = operands(24, 64, 32, torch.float16, gpu_device)
+    with forward_ad.dual_level():
+        for k in range(4):
+            ops = [forward_ad.make_dual(t, t) if i == k else t for i, t in enumerate((a, b, bias, residual))]
+            with pytest.raises(NotImplementedError):
+                cascaded_lowp_matmul_epilogue(ops[0], ops[1], bias=ops[2], residual=ops[3])

@@ -52,3 +52,9 @@ def test_tensors_off_the_gpu_are_refused():
         layer_norm(x)
     with pytest.raises(RuntimeError, match="only runs on an AMD GPU"):
         add_layer_norm(x, x)
+
+
+def test_rows_longer_than_a_launch_can_sum():
+    long = 2 ** 26 + 1
+    assert forward(cols=long, ldx=long, ldy=long) == -9 and backward(cols=long, lddy=long, ldx=long, lddx=long, nbytes=2 ** 62) == -9
+    assert _lib.lib().cascmm_layer_norm_workspace_bytes(4, long, F32) == 0

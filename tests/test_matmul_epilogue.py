@@ -83,3 +83,9 @@ def test_rows_of_a_residual():
     row, ld = _residual_rows(t.view(2, 2, 6)[:1].expand(2, 2, 6), 4, 6)
     assert ld == 6 and torch.equal(row, t[[0, 1, 0, 1]])
     assert _residual_rows(torch.zeros(4, 9)[:, 1:7], 4, 6)[1] == 9
+
+
+def test_rows_longer_than_a_launch_can_sum():
+    long = 2 ** 26 + 1
+    assert backward(cols=long, lddy=long, ldz=long, lddz=long, nbytes=2 ** 62) == -9
+    assert _lib.lib().cascmm_epilogue_workspace_bytes(4, long, F32) == 0
