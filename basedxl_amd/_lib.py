@@ -75,6 +75,7 @@ SIGNATURES = {
                              + [c_void_p, c_void_p, c_size_t, c_void_p]),
     "cascmm_epilogue_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
     "cascmm_epilogue_backward": (c_int, [c_void_p] * 4 + [c_int64] * 5 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "cascmm_epilogue_backward_operands": (c_int, [c_void_p] * 8 + [c_int64] * 10 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "cascmm_transpose": (c_int, [c_void_p, c_void_p] + [c_int64] * 4 + [c_int, c_void_p]),
     "cascmm_layer_norm": (c_int, [c_void_p] * 8 + [c_int64] * 6 + [c_float, c_int, c_int, c_void_p]),
     "cascmm_layer_norm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),

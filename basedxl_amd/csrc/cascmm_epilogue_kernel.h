@@ -11,6 +11,8 @@
 //
 // Bound by memory: 16 bytes a load, rows of any alignment.
 #pragma once
+#include <type_traits>
+
 #include "cascmm_activation.h"
 #include "cascmm_norm_kernel.h"
 
@@ -91,17 +93,30 @@ __global__ __launch_bounds__(256) void cascmm_epilogue_kernel(const void* src, i
 // looked at; the sums are of dz as it is before it is rounded.
 // Measured (graph replay): 8192 x 2560 bf16, gelu, dz 29.5 us (4.3 TB/s; the slope is some 30 instructions an element, 18 us of every SIMD), with dbias, whose
 // sums are a second kernel, 34.0; 8192 x 640 fp32 12.9 (4.9 TB/s) and 16.8.
+struct SlopeParams {
+  const void *dy, *z;
+  void* dz;
+  float* partials;
+  int64_t lddy, ldz, lddz, rows;
+  int cols, act;
+};
+// Workgroup `band` (of columns), `part` (of `parts` that share the rows); lds: kSlopeLds bytes.
+constexpr int kSlopeLds = 256 * 16 * 2;
 template <int IODT, int LANES, bool TINY>
-__global__ __launch_bounds__(256) void cascmm_epilogue_backward_kernel(const void* dy, int64_t lddy, const void* z, int64_t ldz, void* dz, int64_t lddz,
-                                                                      float* partials, int64_t rows, int cols, int act) {
+__device__ __forceinline__ void slope_rows(const SlopeParams& p, int band, int part, int parts, unsigned char* lds) {
   typedef NormRow<IODT, TINY> R;
   typedef typename R::E E;
   typedef typename R::chunk chunk;
   constexpr int VEC = R::VEC, GROUPS = 256 / LANES, AHEAD = 4;
+  const void *dy = p.dy, *z = p.z;
+  void* dz = p.dz;
+  float* partials = p.partials;
+  int64_t lddy = p.lddy, ldz = p.ldz, lddz = p.lddz, rows = p.rows;
+  int cols = p.cols, act = p.act;
   asm volatile("" : "+s"(dy), "+s"(lddy), "+s"(z), "+s"(ldz), "+s"(dz), "+s"(lddz), "+s"(rows), "+s"(cols), "+s"(act));   // (requested together)
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int col = ((int)blockIdx.x * LANES + lane) * VEC;
-  const int64_t stride = (int64_t)gridDim.y * GROUPS;
+  const int col = (band * LANES + lane) * VEC;
+  const int64_t stride = (int64_t)parts * GROUPS;
   float sums[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) sums[e] = 0.f;
@@ -117,7 +132,7 @@ __global__ __launch_bounds__(256) void cascmm_epilogue_backward_kernel(const voi
   };
   if (col < cols) {
     Rows next;
-    int64_t row = (int64_t)blockIdx.y * GROUPS + (LANES == 64 ? __builtin_amdgcn_readfirstlane(group) : group);
+    int64_t row = (int64_t)part * GROUPS + (LANES == 64 ? __builtin_amdgcn_readfirstlane(group) : group);
     if (row < rows) fetch(next, row);
     while (row < rows) {
       Rows cur = next;
@@ -148,30 +163,49 @@ __global__ __launch_bounds__(256) void cascmm_epilogue_backward_kernel(const voi
     }
   }
   if (!partials) return;
-  __shared__ float meet[GROUPS][LANES * VEC];
+  static_assert(GROUPS * LANES * VEC * (int)sizeof(float) <= kSlopeLds, "");
+  float(*meet)[LANES * VEC] = (float(*)[LANES * VEC])lds;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) meet[group][e * LANES + lane] = sums[e];
   __syncthreads();
   for (int i = threadIdx.x; i < LANES * VEC; i += 256) {
-    const int64_t c = ((int64_t)blockIdx.x * LANES + i % LANES) * VEC + i / LANES;
+    const int64_t c = ((int64_t)band * LANES + i % LANES) * VEC + i / LANES;
     if (c >= cols) continue;
     float s = 0.f;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) s += meet[g][i];
-    partials[(int64_t)blockIdx.y * cols + c] = s;
+    partials[(int64_t)part * cols + c] = s;
   }
+}
+
+template <int IODT, int LANES, bool TINY>
+__global__ __launch_bounds__(256) void cascmm_epilogue_backward_kernel(const SlopeParams p) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kSlopeLds];
+  slope_rows<IODT, LANES, TINY>(p, (int)blockIdx.x, (int)blockIdx.y, (int)gridDim.y, lds);
 }
 
 // out [cols][rows] = x [rows][cols] transposed; E: an unsigned type of the elements' size.  64 x 64 elements a workgroup through LDS: 16 bytes a load
 // along the rows of x and a store along the rows of out.  Rows of the tile are an odd number of dwords apart in LDS, so that the eight (sixteen)
 // groups of rows that the lanes of a store read start on banks of their own.
 // Measured (graph replay): 8192 x 2560 bf16 13.6 us (6.2 TB/s, part of it from the Infinity Cache), 8192 x 640 fp32 8.1 (5.2 TB/s), 333 x 211 fp16 3.0.
-template <typename E>
-__global__ __launch_bounds__(256) void cascmm_transpose_kernel(const E* __restrict__ x, int64_t ldx, E* __restrict__ out, int64_t ldo, int rows, int cols, unsigned tiles_across) {
+struct TransposeParams {
+  const void* x;
+  void* out;
+  int64_t ldx, ldo;
+  int rows, cols;
+  unsigned across, tiles;   // tiles side by side over the columns, all of them (0: nothing to do)
+};
+constexpr int kTransposeLds = 64 * 65 * 4;
+template <typename E> __device__ __forceinline__ void transpose_tile(const TransposeParams& p, unsigned at, unsigned char* lds) {
+  const E* __restrict__ x = (const E*)p.x;
+  E* __restrict__ out = (E*)p.out;
+  const int64_t ldx = p.ldx, ldo = p.ldo;
+  const int rows = p.rows, cols = p.cols;
   constexpr int VEC = 16 / (int)sizeof(E), PER = 64 / VEC, PITCH = sizeof(E) == 2 ? 66 : 65, DW = 4 / (int)sizeof(E);
   typedef E chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
-  __shared__ __attribute__((aligned(16))) E tile[64 * PITCH];
-  const int r0 = (int)(blockIdx.x / tiles_across) * 64, c0 = (int)(blockIdx.x % tiles_across) * 64;
+  static_assert(64 * PITCH * (int)sizeof(E) <= kTransposeLds, "");
+  E* tile = (E*)lds;
+  const int r0 = (int)(at / p.across) * 64, c0 = (int)(at % p.across) * 64;
 #pragma unroll
   for (int i = threadIdx.x; i < 64 * PER; i += 256) {
     const int r = i / PER, c = i % PER * VEC;
@@ -209,6 +243,18 @@ __global__ __launch_bounds__(256) void cascmm_transpose_kernel(const E* __restri
         if (r0 + r + e < rows) to[e] = v[e];
     }
   }
+}
+// Both passes and two transpositions side by side in one launch: what the gradients of a product want before its two products run.  The first `slopes`
+// workgroups are the slopes' (bands x parts of them), then the tiles of the one operand, then the other's.
+template <int IODT, int LANES, bool TINY>
+__global__ __launch_bounds__(256) void cascmm_epilogue_operands_kernel(const SlopeParams p, unsigned bands, unsigned parts, const TransposeParams a, const TransposeParams b) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kSlopeLds > kTransposeLds ? kSlopeLds : kTransposeLds];
+  typedef typename std::conditional<sizeof(typename IoType<IODT>::T) == 4, unsigned, unsigned short>::type E;
+  unsigned at = blockIdx.x;
+  if (at < bands * parts) return slope_rows<IODT, LANES, TINY>(p, (int)(at % bands), (int)(at / bands), (int)parts, lds);
+  at -= bands * parts;
+  if (at < a.tiles) return transpose_tile<E>(a, at, lds);
+  transpose_tile<E>(b, at - a.tiles, lds);
 }
 
 }  // namespace cascmm

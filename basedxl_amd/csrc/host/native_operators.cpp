@@ -239,30 +239,29 @@ struct EpilogueNode : torch::autograd::Function<EpilogueNode> {
       const at::Tensor a = as_rows(v[0], M, K, lda), dy = as_rows(grads[0], M, N, lddz);
       const int dt = dtype_code(a);
       const hipStream_t stream = stream_of(a);
-      at::Tensor dz = dy, ws;
-      if (want_bias || (act && (want_a || want_b))) {
-        const int64_t lddy = lddz;
-        if (act && (want_a || want_b)) {
-          dz = fresh({M, N}, a);
-          lddz = N;
-        }
-        if (want_bias) {
-          out[2] = fresh({N}, a);
-          ws = scratch(cascmm_epilogue_workspace_bytes(M, N, dt), a);
-        }
-        check(cascmm_epilogue_backward(dy.const_data_ptr(), data_of(v[2]), dz.is_same(dy) ? nullptr : dz.data_ptr(), want_bias ? out[2].data_ptr() : nullptr, M, N, lddy, N, N,
-                                       act, dt, want_bias ? ws.data_ptr() : nullptr, want_bias ? ws.nbytes() : 0, stream),
-              "cascmm_epilogue_backward");
+      // dz, dbias and the products' other operands in one launch
+      const bool slope = act && (want_a || want_b);
+      at::Tensor dz = dy, ws, at, bt;
+      const int64_t lddy = lddz;
+      if (slope) {
+        dz = fresh({M, N}, a);
+        lddz = N;
       }
+      if (want_bias) {
+        out[2] = fresh({N}, a);
+        ws = scratch(cascmm_epilogue_workspace_bytes(M, N, dt), a);
+      }
+      if (want_b) at = fresh({K, M}, a);
+      if (want_a) bt = fresh({N, K}, b);
+      auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+      check(cascmm_epilogue_backward_operands(dy.const_data_ptr(), data_of(v[2]), slope ? dz.data_ptr() : nullptr, ptr(out[2]), a.const_data_ptr(), ptr(at), b.const_data_ptr(),
+                                              ptr(bt), M, N, K, lddy, N, N, lda, M, N, K, act, dt, ptr(ws), ws.defined() ? ws.nbytes() : 0, stream),
+            "cascmm_epilogue_backward_operands");
       if (want_a) {
-        const at::Tensor bt = fresh({N, K}, b);
-        check(cascmm_transpose(b.const_data_ptr(), bt.data_ptr(), K, N, N, K, dt, stream), "cascmm_transpose");
         out[0] = fresh(v[0].sizes(), a);
         product(dz.const_data_ptr(), lddz, bt.const_data_ptr(), K, out[0], M, K, N, fmt, terms, products);
       }
       if (want_b) {
-        const at::Tensor at = fresh({K, M}, a);
-        check(cascmm_transpose(a.const_data_ptr(), at.data_ptr(), M, K, lda, M, dt, stream), "cascmm_transpose");
         out[1] = fresh({K, N}, b);
         product(at.const_data_ptr(), M, dz.const_data_ptr(), lddz, out[1], K, N, M, fmt, terms, products);
       }

@@ -79,15 +79,6 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
     return _rows(t.reshape(t.shape[:-1].numel(), t.shape[-1]))
 
 
-def _transposed(x2: torch.Tensor) -> torch.Tensor:
-    rows, cols = x2.shape
-    out = torch.empty(cols, rows, dtype=x2.dtype, device=x2.device)
-    if out.numel():
-        _lib.check(_lib.lib().cascmm_transpose(x2.data_ptr(), out.data_ptr(), rows, cols, _ld(x2), rows, _DTYPES[x2.dtype],
-                                               torch.cuda.current_stream(x2.device).cuda_stream), "cascmm_transpose")
-    return out
-
-
 class _EpilogueProduct(torch.autograd.Function):
     """Tensors only: ``a`` [..., K], ``b`` [K, N], ``residual`` of the result's shape."""
 
@@ -110,25 +101,26 @@ class _EpilogueProduct(torch.autograd.Function):
         want_a, want_b, want_bias, want_residual = ctx.needs_input_grad[:4]
         K, N = b.shape
         dev, dt = a.device, _DTYPES[a.dtype]
-        da = db = dbias = None
+        da = db = None
         with torch.cuda.device(dev):
             dy2 = _flat(dy)
             M = dy2.shape[0]
-            dz = dy2
-            if want_bias or (activation is not None and (want_a or want_b)):
-                l, stream = _lib.lib(), torch.cuda.current_stream(dev).cuda_stream
-                if activation is not None and (want_a or want_b):
-                    dz = torch.empty(M, N, dtype=a.dtype, device=dev)
-                ws = None
-                if want_bias:
-                    dbias = torch.empty(N, dtype=a.dtype, device=dev)
-                    ws = torch.empty(l.cascmm_epilogue_workspace_bytes(M, N, dt), dtype=torch.uint8, device=dev)
-                _lib.check(l.cascmm_epilogue_backward(dy2.data_ptr(), _ptr(preact), None if dz is dy2 else dz.data_ptr(), _ptr(dbias), M, N, _ld(dy2), N, N,
-                                                      _lib.ACT_BY_NAME[activation], dt, _ptr(ws), 0 if ws is None else ws.numel(), stream), "cascmm_epilogue_backward")
+            # dz, dbias and the products' other operands in one launch
+            a2, slope = _flat(a), activation is not None and (want_a or want_b)
+            new = lambda *shape: torch.empty(shape, dtype=a.dtype, device=dev)   # noqa: E731
+            dz, dbias = new(M, N) if slope else dy2, new(N) if want_bias else None
+            at, bt = new(K, M) if want_b else None, new(N, K) if want_a else None
+            l, ws = _lib.lib(), None
+            if want_bias:
+                ws = torch.empty(l.cascmm_epilogue_workspace_bytes(M, N, dt), dtype=torch.uint8, device=dev)
+            _lib.check(l.cascmm_epilogue_backward_operands(
+                dy2.data_ptr(), _ptr(preact), dz.data_ptr() if slope else None, _ptr(dbias), a2.data_ptr(), _ptr(at), b.data_ptr(), _ptr(bt), M, N, K, _ld(dy2), N, N,
+                _ld(a2), M, N, K, _lib.ACT_BY_NAME[activation], dt, _ptr(ws), 0 if ws is None else ws.numel(), torch.cuda.current_stream(dev).cuda_stream),
+                "cascmm_epilogue_backward_operands")
             if want_a:
-                da = cascaded_lowp_matmul(dz, _transposed(b), lowp=lowp, terms=terms, products=products).reshape(a.shape)
+                da = cascaded_lowp_matmul(dz, bt, lowp=lowp, terms=terms, products=products).reshape(a.shape)
             if want_b:
-                db = cascaded_lowp_matmul(_transposed(_flat(a)), dz.contiguous(), lowp=lowp, terms=terms, products=products)
+                db = cascaded_lowp_matmul(at, dz.contiguous(), lowp=lowp, terms=terms, products=products)
         return da, db, dbias, dy if want_residual else None, None, None, None, None, None
 
 

@@ -347,6 +347,12 @@ size_t cascmm_epilogue_workspace_bytes(int64_t rows, int64_t cols, int dtype);
 int cascmm_epilogue_backward(const void* dy, const void* z, void* dz, void* dbias, int64_t rows, int64_t cols,
                              int64_t lddy, int64_t ldz, int64_t lddz, int activation, int dtype, void* workspace,
                              size_t workspace_bytes, void* stream);
+/* The same with what the gradients' products want beside dz, in one launch: At [K, M] = A [M, K] transposed and Bt [N, K] = B [K, N] transposed (each NULL: not
+ * wanted), dA = dz . Bt and dB = At . dz.  rows, cols of the above are M, N; dz and dbias may both be NULL. */
+int cascmm_epilogue_backward_operands(const void* dy, const void* z, void* dz, void* dbias, const void* A, void* At,
+                                      const void* B, void* Bt, int64_t M, int64_t N, int64_t K, int64_t lddy,
+                                      int64_t ldz, int64_t lddz, int64_t lda, int64_t ldat, int64_t ldb, int64_t ldbt,
+                                      int activation, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 /* out [cols, rows] (leading dimension ldo >= rows) = x [rows, cols] transposed: the operands of those products. */
 int cascmm_transpose(const void* x, void* out, int64_t rows, int64_t cols, int64_t ldx, int64_t ldo, int dtype, void* stream);
 

@@ -89,3 +89,16 @@ def test_rows_longer_than_a_launch_can_sum():
     long = 2 ** 26 + 1
     assert backward(cols=long, lddy=long, ldz=long, lddz=long, nbytes=2 ** 62) == -9
     assert _lib.lib().cascmm_epilogue_workspace_bytes(4, long, F32) == 0
+
+
+def operands(dy=P, z=P, dz=P, dbias=None, A=P, At=P, B=P, Bt=P, M=4, N=8, K=16, lddy=8, ldz=8, lddz=8, lda=16, ldat=4, ldb=8, ldbt=16, activation=2, dtype=F32, ws=None, nbytes=0):
+    return _lib.lib().cascmm_epilogue_backward_operands(dy, z, dz, dbias, A, At, B, Bt, M, N, K, lddy, ldz, lddz, lda, ldat, ldb, ldbt, activation, dtype, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(dtype=9), -3), (dict(activation=5), -4), (dict(M=-1), -2), (dict(K=-1), -2), (dict(lddy=7), -2), (dict(lda=15), -2), (dict(ldat=3), -2), (dict(ldb=7), -2),
+    (dict(ldbt=15), -2), (dict(A=None), -1), (dict(B=None), -1), (dict(dy=None), -1), (dict(z=None), -1), (dict(At=P + 2), -6), (dict(B=P + 1), -6), (dict(dz=P + 2), -6),
+    (dict(dbias=P), -5), (dict(dbias=P, ws=P + 4, nbytes=1 << 20), -6), (dict(M=2 ** 31, ldat=2 ** 31), -9),
+    (dict(dz=None, At=None, Bt=None), 0), (dict(M=0, Bt=None), 0), (dict(N=0, ldb=0, At=None), 0), (dict(M=0, N=0, K=0, ldb=0), 0)])
+def test_backward_with_operands_arguments(change, status):
+    assert operands(**change) == status
