@@ -51,11 +51,17 @@ static hipError_t ep_backward_launch(const SlopeParams& p, unsigned bands, unsig
 // (slopes: dz or the sums are wanted; else the transpositions alone)
 template <int IODT> static hipError_t ep_backward(const SlopeParams& p, bool slopes, void* dbias, const TransposeParams& a, const TransposeParams& b, hipStream_t s) {
   typedef NormRow<IODT> R;
-  const int parts = slopes ? (int)ep_parts(p.rows, p.cols, IODT) : 1, lanes = ep_lanes(p.cols, IODT);
-  const unsigned bands = slopes ? (unsigned)((p.cols + lanes * R::VEC - 1) / (lanes * R::VEC)) : 0;
-  hipError_t err = lanes == 64          ? ep_backward_launch<IODT, 64, false>(p, bands, (unsigned)parts, a, b, s)
-                   : p.cols < R::VEC ? ep_backward_launch<IODT, 16, true>(p, bands, (unsigned)parts, a, b, s)
-                                        : ep_backward_launch<IODT, 16, false>(p, bands, (unsigned)parts, a, b, s);
+  hipError_t err = hipSuccess;
+  if (!slopes) {
+    typedef typename std::conditional<sizeof(typename IoType<IODT>::T) == 4, unsigned, unsigned short>::type E;
+    CASCMM_LAUNCH(err, (cascmm_transpose_kernel<E>), dim3(a.tiles + b.tiles), dim3(256), 0, s, a, b);
+    return err;
+  }
+  const int parts = (int)ep_parts(p.rows, p.cols, IODT), lanes = ep_lanes(p.cols, IODT);
+  const unsigned bands = (unsigned)((p.cols + lanes * R::VEC - 1) / (lanes * R::VEC));
+  err = lanes == 64         ? ep_backward_launch<IODT, 64, false>(p, bands, (unsigned)parts, a, b, s)
+        : p.cols < R::VEC ? ep_backward_launch<IODT, 16, true>(p, bands, (unsigned)parts, a, b, s)
+                            : ep_backward_launch<IODT, 16, false>(p, bands, (unsigned)parts, a, b, s);
   if (p.partials)
     CASCMM_LAUNCH(err, (cascmm_column_finish_kernel<IODT>), dim3((unsigned)((p.cols + kFinishCols - 1) / kFinishCols), 1), dim3(1024), 0, s, (const float*)p.partials, parts, 1,
                   (int64_t)p.cols, dbias, (void*)nullptr);

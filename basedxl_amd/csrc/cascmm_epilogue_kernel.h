@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256) void cascmm_epilogue_backward_kernel(const Slo
 // out [cols][rows] = x [rows][cols] transposed; E: an unsigned type of the elements' size.  64 x 64 elements a workgroup through LDS: 16 bytes a load
 // along the rows of x and a store along the rows of out.  Rows of the tile are an odd number of dwords apart in LDS, so that the eight (sixteen)
 // groups of rows that the lanes of a store read start on banks of their own.
-// Measured (graph replay): 8192 x 2560 bf16 13.6 us (6.2 TB/s, part of it from the Infinity Cache), 8192 x 640 fp32 8.1 (5.2 TB/s), 333 x 211 fp16 3.0.
+// Measured (graph replay): 8192 x 2560 bf16 13.6 - 16.4 us (5.1 - 6.2 TB/s, part of it from the Infinity Cache), 8192 x 640 fp32 8.1 (5.2 TB/s), 333 x 211 fp16 3.0.
 struct TransposeParams {
   const void* x;
   void* out;
@@ -244,8 +244,16 @@ template <typename E> __device__ __forceinline__ void transpose_tile(const Trans
     }
   }
 }
-// Both passes and two transpositions side by side in one launch: what the gradients of a product want before its two products run.  The first `slopes`
-// workgroups are the slopes' (bands x parts of them), then the tiles of the one operand, then the other's.
+// two of them in one launch
+template <typename E> __global__ __launch_bounds__(256) void cascmm_transpose_kernel(const TransposeParams a, const TransposeParams b) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kTransposeLds];
+  if (blockIdx.x < a.tiles) return transpose_tile<E>(a, blockIdx.x, lds);
+  transpose_tile<E>(b, blockIdx.x - a.tiles, lds);
+}
+
+// Slopes and two transpositions side by side in one launch: what the gradients of a product want before its two products run.  The first workgroups are
+// the slopes' (bands x parts of them), then the tiles of the one operand, then the other's.  8192 x 640 x 2560 bf16, gelu, with the finishing kernel: 38 us,
+// one launch each 45; without slopes the kernel above, which more of fit on a CU (8192 x 2560 16.4 us, in this one 18.2).
 template <int IODT, int LANES, bool TINY>
 __global__ __launch_bounds__(256) void cascmm_epilogue_operands_kernel(const SlopeParams p, unsigned bands, unsigned parts, const TransposeParams a, const TransposeParams b) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[kSlopeLds > kTransposeLds ? kSlopeLds : kTransposeLds];
