@@ -946,7 +946,7 @@ static Problem relayed(const Problem& q0, const Relay& r) {
   Problem q = q0;
   if (r.a) q.lda = r.a_chunks * (16 / (int64_t)dtype_size(q.dtype));
   q.chunked = true;
-  q.bpre = r.b;
+  q.bpre = q0.bpre || r.b;
   if (r.b) q.ldb = q.N;
   return q;
 }
@@ -955,15 +955,16 @@ static Relay relay_of(const Problem& q0, int count, const void* const* A, const 
   Problem q = q0;
   q.call = true;
   Relay r;
-  if (q.bpre || q.split_first || q.K == 0) return r;
   const bool f32 = q.dtype == CASCMM_DT_F32;
+  // (prepared 16-bit weights: the call with an epilogue takes rows of any length, the plain one refuses them)
+  if ((q.bpre && (f32 || !q.epi)) || q.split_first || q.K == 0) return r;
   if (f32 ? !(q.fmt == CASCMM_FMT_BF16 && q.terms == 2 && (q.products == CASCMM_PROD_TRI)) : !own_format16(q)) return r;
   const int64_t es = f32 ? 4 : 2, per = 16 / es;
   r.a = q.K % per != 0 || (!f32 && q.lda % 2 != 0);
-  r.b = !f32 && (q.N % 2 != 0 || q.ldb % 2 != 0);
+  r.b = !f32 && !q.bpre && (q.N % 2 != 0 || q.ldb % 2 != 0);
   for (int i = 0; i < count; ++i) {
     r.a = r.a || (!f32 && A && !aligned_to(A[i], 4));
-    r.b = r.b || (!f32 && B && !aligned_to(B[i], 4));
+    r.b = r.b || (!f32 && !q.bpre && B && !aligned_to(B[i], 4));
   }
   const int64_t lines = (q.K * es + 127) / 128;   // (rows of whole cache lines)
   int64_t a_bytes = 0, b_bytes = r.b ? prepared_bytes(q.K, q.N, q.fmt, 1) : 0;

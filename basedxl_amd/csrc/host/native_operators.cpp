@@ -406,10 +406,10 @@ PyObject* epilogue_prepared(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
     if (fmt == CASCMM_FMT_FP8 || products < 0 || N <= 0 || p.K != wk || p.dt != w_dt || !result_arguments(p, N) || differentiated({p.a, &p.bias, &p.residual})) Py_RETURN_NONE;
     const size_t slot_bytes = cascmm_prepared_bytes(wk, N, fmt, terms);
     if (slots->nbytes() != (slot_bytes > 16 ? slot_bytes : 16)) Py_RETURN_NONE;   // (not this layout: the wrapper raises)
-    if ((uintptr_t)p.a->const_data_ptr() % 16 != 0 || (size_t)p.lda * p.a->element_size() % 16 != 0) Py_RETURN_NONE;   // (the wrapper copies such rows)
     if (p.dt == CASCMM_DT_F32) {
+      if ((uintptr_t)p.a->const_data_ptr() % 16 != 0 || p.lda % 4 != 0) Py_RETURN_NONE;   // (the wrapper copies such rows)
       if (!(fmt == CASCMM_FMT_BF16 && terms == 2 && p.K % 8 == 0) && (p.K % 64 != 0 || N % 4 != 0)) Py_RETURN_NONE;
-    } else if (terms != 1 || p.K % 8 != 0) {
+    } else if (terms != 1 || fmt != (p.dt == CASCMM_DT_F16 ? CASCMM_FMT_FP16 : CASCMM_FMT_BF16)) {   // (rows of any alignment: the library copies what it has to)
       Py_RETURN_NONE;
     }
     return run_product(p, slots->const_data_ptr(), 1, N, fmt, terms, products, device);

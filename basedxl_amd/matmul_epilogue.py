@@ -128,7 +128,7 @@ def cascaded_lowp_matmul_epilogue(a: torch.Tensor, b, *, bias: Optional[torch.Te
                                   residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, lowp: Optional[str] = None,
                                   terms: Optional[int] = None, products: str = "tri", b_exp: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``activation(a @ b + bias) + residual``: :func:`cascaded_lowp_matmul` of ``a`` [..., K] and a 2-D ``b`` [K, N] (or a plain
-    :class:`PreparedWeight`) with what follows a Linear layer.  ``activation``: None, "relu", "gelu" (erf), "gelu_tanh" or "silu", in fp32.
+    :class:`PreparedWeight`; of fp32 one whose K and N its kernels take, see ``usable_with``) with what follows a Linear layer.  ``activation``: None, "relu", "gelu" (erf), "gelu_tanh" or "silu", in fp32.
     ``residual``: of the result's dtype and of a shape that broadcasts to the result's.  ``lowp`` / ``terms`` / ``products`` / ``b_exp`` as there.
     ``out``: [M, N] rows or the result's shape; it overlaps no operand.
 
@@ -206,7 +206,7 @@ def cascaded_lowp_matmul_epilogue(a: torch.Tensor, b, *, bias: Optional[torch.Te
             raise RuntimeError("cascaded_lowp_matmul_epilogue: a PreparedWeight is for calls without gradients")
         return _EpilogueProduct.apply(a, b, bias, residual, activation, lowp, terms, products, b_exp)
     a2 = _flat(a)
-    if prepared and not b.usable_with(a2, products):
+    if prepared and not b.usable_with(a2, products) and (a.dtype == torch.float32 or K % 8 == 0):     # (16-bit rows of other lengths are copied by the library)
         a2 = a2.contiguous().clone() if a2.is_contiguous() else a2.contiguous()     # (rows off the boundaries that the prepared kernels want)
     if out is None:
         out = torch.empty(shape, dtype=a.dtype, device=a.device)

@@ -491,3 +491,16 @@ def test_forward_mode_tangents_are_refused(gpu_device, path):
             ops = [forward_ad.make_dual(t, t) if i == k else t for i, t in enumerate((a, b, bias, residual))]
             with pytest.raises(NotImplementedError):
                 cascaded_lowp_matmul_epilogue(ops[0], ops[1], bias=ops[2], residual=ops[3])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M, K, N", [(131, 881, 512), (1, 9, 7), (5, 1, 64), (300, 1283, 130), (40, 50, 640), (2000, 333, 1280), (64, 5119, 64), (513, 4001, 96)])
+def test_prepared_weights_of_any_depth(gpu_device, path, M, K, N, dtype):
+    a, b, bias, residual, _ = operands(M, K, N, dtype, gpu_device)
+    wide = torch.full((M, K + 3), math.nan, dtype=dtype, device=gpu_device)
+    wide[:, 1:1 + K] = a
+    pw = PreparedWeight(b)
+    for rows in (a, wide[:, 1:1 + K]):
+        for act, r in ((None, None), (None, residual), ("gelu", residual), ("silu", None)):
+            y = cascaded_lowp_matmul_epilogue(rows, pw, bias=bias, activation=act, residual=r)
+            check_forward(y, a, b, bias, act, r, dtype, 0.0, f"{act} {r is not None} {rows.stride(0)}", fused=True)
