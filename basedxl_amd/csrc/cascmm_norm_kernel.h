@@ -112,15 +112,17 @@ template <int IODT, bool TINY = false> struct NormRow {
     return v;
   }
   static __device__ __forceinline__ bool ragged(int cols) { return !TINY && cols % VEC != 0; }
-  static __device__ __forceinline__ chunk settle(chunk v, int c, int cols) {
+  // TURN: what lies behind the end are elements from in front of the lane's own, not zeros.
+  template <bool TURN = false> static __device__ __forceinline__ chunk settle(chunk v, int c, int cols) {
     if (!ragged(cols)) return v;
     const int s = c > cols - VEC && c < cols ? c - (cols - VEC) : 0;   // elements in front of the lane's own
     const int dwords = sizeof(E) == 2 ? s >> 1 : s;
     u32x4 w = __builtin_bit_cast(u32x4, v);
-    if (dwords & 1) w = (u32x4){w[1], w[2], w[3], 0u};
-    if (dwords & 2) w = (u32x4){w[2], w[3], 0u, 0u};
+    if (dwords & 1) w = (u32x4){w[1], w[2], w[3], TURN ? w[0] : 0u};
+    if (dwords & 2) w = (u32x4){w[2], w[3], TURN ? w[0] : 0u, TURN ? w[1] : 0u};
     if (sizeof(E) == 2 && (s & 1))
-      w = (u32x4){__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16), __builtin_amdgcn_alignbit(w[3], w[2], 16), w[3] >> 16};
+      w = (u32x4){__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16), __builtin_amdgcn_alignbit(w[3], w[2], 16),
+                  TURN ? __builtin_amdgcn_alignbit(w[0], w[3], 16) : w[3] >> 16};
     return __builtin_bit_cast(chunk, w);
   }
   // ... of a chunk that no row of this kernel ends in (whole: known at compile time)
@@ -130,6 +132,7 @@ template <int IODT, bool TINY = false> struct NormRow {
     else store(row, c, cols, v);
   }
   static __device__ __forceinline__ chunk load_settled(const E* row, int c, int cols) { return settle(load(row, c, cols), c, cols); }
+  static __device__ __forceinline__ chunk load_turned(const E* row, int c, int cols) { return settle<true>(load(row, c, cols), c, cols); }
   static __device__ __forceinline__ void store(E* row, int c, int cols, chunk v) {
     if (c + VEC <= cols) {
       *(chunk*)(row + c) = v;
@@ -389,10 +392,11 @@ __global__ __launch_bounds__(256) void cascmm_layer_norm_backward_kernel(const N
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        // (behind the last column x, dy and with it g are zeros, and xhat, which the mean is taken from, meets nothing but them)
+        // (behind the last column x, dy and with it g are zeros; xhat, which the mean is taken from, is held to zero too: of a row far from zero the
+        // mean times rstd may be infinite there, and zero times that is no zero)
         const float xhat = ((float)cur.x[c][e] - cur.mean) * cur.rstd, d = (float)cur.dy[c][e], g = d * w[c][e];
         sums[0] += g;
-        sums[1] = __builtin_fmaf(g, xhat, sums[1]);
+        sums[1] = __builtin_fmaf(g, c < FULL || col0 + c * STEP + e < cols ? xhat : 0.f, sums[1]);
         if constexpr (SUMS) {
           dw[c][e] = __builtin_fmaf(d, xhat, dw[c][e]);
           db[c][e] += d;
@@ -471,7 +475,8 @@ __global__ __launch_bounds__(kNormWide) void cascmm_layer_norm_backward_wide_ker
     const float mean = p.mean[row], rstd = p.rstd[row];
     float sums[2] = {0.f, 0.f};
     for (int64_t c = col0; c < cols; c += STEP) {
-      const chunk v = R::load_settled(x, (int)c, cols), d = R::load_settled(dy, (int)c, cols);
+      // (behind the last column xhat meets a zero of dy; of turned chunks it is some other column's there, and finite where the row's are)
+      const chunk v = R::load_turned(x, (int)c, cols), d = R::load_settled(dy, (int)c, cols);
       float w[1][VEC];
       R::template load_weight<0>(w, p.weight, p.weight_f32, (int)c, 0, cols, 1.f);
 #pragma unroll

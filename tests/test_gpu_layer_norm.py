@@ -354,3 +354,25 @@ def test_forward_mode_tangents_are_refused(gpu_device, path):
         with pytest.raises(NotImplementedError):
             add_layer_norm(x, forward_ad.make_dual(x, x), w, w)
         assert torch.equal(layer_norm(x, w, w), layer_norm(x, w, w))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [2, 5, 40, 200, 457, 640, 1281, 2049, 8200, 8201, 9003])
+def test_gradients_of_rows_of_one_large_value(gpu_device, path, cols, dtype):
+    """Rows of 2^112 with eps = 1e-12: the mean is exact and xhat zero, while mean times rstd is beyond fp32."""
+    gen = torch.Generator().manual_seed(cols)
+    x = torch.full((70, cols), 2.0 ** 112, dtype=dtype, device=gpu_device)
+    dy, w, b = rows_of(gen, 70, cols, dtype, gpu_device), rows_of(gen, 1, cols, dtype, gpu_device)[0], rows_of(gen, 1, cols, dtype, gpu_device)[0]
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = layer_norm(*leaves, eps=1e-12)
+    assert torch.equal(y, b.expand(70, cols))
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    g = dy.double() * w.double()
+    c1 = g.mean(-1, keepdim=True)
+    want = 1e6 * (g - c1)
+    # (g and its difference are rounded, the mean is a sum of cols / 64 + 16 numbers and two roundings, rstd and the product with it some more)
+    tol = 1e6 * U * (4 * (g.abs() + c1.abs()) + (cols / 64 + 18) * g.abs().mean(-1, keepdim=True)) + 8 * U * want.abs()
+    within(dx, want, tol + HALF[dtype] * want.abs() + TINY[dtype], "dx")
+    assert bool((dw == 0).all())
+    want = dy.double().sum(0)
+    within(db, want, HALF[dtype] * want.abs() + 70 * U * dy.double().abs().sum(0) + TINY[dtype], "dbias")
