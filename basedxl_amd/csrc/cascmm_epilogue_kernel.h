@@ -91,6 +91,9 @@ __global__ __launch_bounds__(256) void cascmm_epilogue_kernel(const void* src, i
 // dz = dy act'(z) (dz NULL: not wanted; act none: z is not read) and, with partials, the workgroup's sums over its rows of dz for its columns at
 // partials[blockIdx.y].  LANES lanes side by side on a row, rows gridDim.y workgroups apart, AHEAD of them at a time and the next ones asked for before these are
 // looked at; the sums are of dz as it is before it is rounded.
+// z and dz are of the elements' type: in 16 bits both are rounded on their way between kernels.  Of the gradients' mean error, 1.45 times that of fp32 z and dz (8192 x
+// 640 x 2560 bf16 2.43e-3 for 1.66e-3), dz's rounding makes nearly all, the slope at a rounded z 6e-4.  fp32 dz would want products of two terms, twice their matrix
+// work (some 70 us more there); fp32 z 42 MB more written and read, 16 us.
 // Measured (graph replay): 8192 x 2560 bf16, gelu, dz 29.5 us (4.3 TB/s; the slope is some 30 instructions an element, 18 us of every SIMD), with dbias, whose
 // sums are a second kernel, 34.0; 8192 x 640 fp32 12.9 (4.9 TB/s) and 16.8.
 struct SlopeParams {

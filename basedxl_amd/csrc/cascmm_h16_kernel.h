@@ -472,7 +472,7 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
     }
   };
   // The epilogue's store: z = sums + bias as fp32 through the wave's LDS area, CB blocks of columns at a time, then 16 bytes of a row a lane.  The residual's
-  // chunks are asked for while the run before is at work (behind one of a few its loads were waited for); z to preact and the activation are a
+  // chunks are asked for while the run before is at work (behind one of a few its loads were waited for); z to preact (rounded: cascmm_epilogue_kernel.h) and the activation are a
   // loop over LDS of their own, which keeps five activations out of the straight code (instructions come from L2 at some 10 KB per us).  It
   // stores the result too where no residual follows (written back and read again by the straight code: gelu 2 us slower below).
   // What it adds to 8192 x 640 x 2560 bf16 (31 us plain, one round of tiles, so nothing hides it): residual 9.5 us, its 42 MB; gelu 12, some 20 instructions

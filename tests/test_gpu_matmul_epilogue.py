@@ -504,3 +504,24 @@ def test_prepared_weights_of_any_depth(gpu_device, path, M, K, N, dtype):
         for act, r in ((None, None), (None, residual), ("gelu", residual), ("silu", None)):
             y = cascaded_lowp_matmul_epilogue(rows, pw, bias=bias, activation=act, residual=r)
             check_forward(y, a, b, bias, act, r, dtype, 0.0, f"{act} {r is not None} {rows.stride(0)}", fused=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_what_a_backward_pass_in_16_bits_rounds(gpu_device, path, dtype):
+    """z and dz are held in the tensors' type between the kernels, dbias is summed before dz is rounded: bit by bit what the separate steps give."""
+    M, K, N = 333, 456, 640
+    a, b, bias, _, dy = operands(M, K, N, dtype, gpu_device)
+    z = cascaded_lowp_matmul_epilogue(a, b, bias=bias)
+    l, code, act = _lib.lib(), {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}[dtype], _lib.ACT_BY_NAME["gelu"]
+    dz, dbias = torch.empty_like(dy), torch.empty_like(bias)
+    ws = torch.empty(l.cascmm_epilogue_workspace_bytes(M, N, code), dtype=torch.uint8, device=gpu_device)
+    assert l.cascmm_epilogue_backward(dy.data_ptr(), z.data_ptr(), dz.data_ptr(), dbias.data_ptr(), M, N, N, N, N, act, code, ws.data_ptr(), ws.numel(),
+                                      torch.cuda.current_stream().cuda_stream) == 0
+    want = dy.double() * slope_of(z.double(), "gelu")
+    off = dy.double().abs() * 8 * U * (1 + z.double().abs()) + 2 * U * want.abs()
+    within(dz, want, off + HALF[dtype] * want.abs() + TINY[dtype], "dz")
+    within(dbias, want.sum(0), off.sum(0) + (64 + M // 8) * U * want.abs().sum(0) + HALF[dtype] * want.sum(0).abs() + TINY[dtype], "dbias")
+    leaves = [t.clone().requires_grad_() for t in (a, b, bias)]
+    da, db, got = torch.autograd.grad(cascaded_lowp_matmul_epilogue(*leaves[:2], bias=leaves[2], activation="gelu"), leaves, dy)
+    assert torch.equal(got, dbias)
+    assert torch.equal(da, cascaded_lowp_matmul(dz, b.t().contiguous())) and torch.equal(db, cascaded_lowp_matmul(a.t().contiguous(), dz))
