@@ -1149,7 +1149,7 @@ static int gemm_on_rows(int count, const void* const* A, const void* const* B, v
   memset(&p, 0, sizeof(p));
   p.M = (int)q.M; p.N = (int)q.N; p.K = (int)q.K;
   p.k_valid = (int)(q.split_first ? q.k_valid : q.K);
-  p.lda = q.lda; p.ldb = q.ldb; p.ldc = q.ldc;
+  p.lda = q.lda; p.ldb = q.ldb; p.ldc = q.epi ? q.epi->ldc : q.ldc;
   const int64_t tm = (q.M + v.BM - 1) / v.BM, tn = (q.N + v.BN - 1) / v.BN;
   if (tm * tn * count > INT32_MAX) return CASCMM_ERR_TOO_LARGE;
   p.tiles_m = (int)tm; p.tiles_n = (int)tn;
@@ -1200,7 +1200,7 @@ static int gemm_on_rows(int count, const void* const* A, const void* const* B, v
   }
   const int st = v.launch(p, stream);
   if (st != CASCMM_OK) return st;
-  return launch_epilogue(p.C[0], p.ldc, ep.residual, ep.ldr, C[0], q.ldc, q.M, q.N, ep.act, q.dtype, stream);
+  return launch_epilogue(p.C[0], p.ldc, ep.residual, ep.ldr, C[0], ep.ldc, q.M, q.N, ep.act, q.dtype, stream);
 }
 
 // whether the rows of A are whole 16-byte chunks by K alone
@@ -1721,9 +1721,10 @@ int cascmm_gemm_epilogue(const void* A, const void* B, int b_prepared, void* C, 
   const size_t es = dtype_size(dtype);
   if (!C) return CASCMM_ERR_NULL_POINTER;
   if (!aligned_to(C, es) || !aligned_to(residual, es) || !aligned_to(preact, es)) return CASCMM_ERR_ALIGNMENT;
-  const Epilogue ep{activation, residual, ldr, preact, ldp};
+  const Epilogue ep{activation, residual, ldr, preact, ldp, ldc};
   if (K > 0) {
     q.epi = &ep;
+    if (preact) q.ldc = std::max(ldc, ldp);   // (whichever of them the product stores, its kernel reaches the rows of both)
     return gemm_impl(1, &A, &B, &C, bias ? &bias : nullptr, q, tensor_exps, workspace, workspace_bytes, (hipStream_t)stream, -1);
   }
   // (no inputs: z is the bias or zero, which its kernel writes in preact or in the result's place)

@@ -12,6 +12,7 @@ struct Epilogue {
   int64_t ldr;
   void* preact;   // z too (or NULL)
   int64_t ldp;
+  int64_t ldc;    // of the result (a Problem's own is what its kernel is chosen for: the product may store z instead)
 };
 // dst = act(src) + residual as a pass of its own (src may be dst)
 int launch_epilogue(const void* src, int64_t lds, const void* residual, int64_t ldr, void* dst, int64_t ldd, int64_t rows, int64_t cols, int act, int dtype,

@@ -525,3 +525,24 @@ def test_what_a_backward_pass_in_16_bits_rounds(gpu_device, path, dtype):
     da, db, got = torch.autograd.grad(cascaded_lowp_matmul_epilogue(*leaves[:2], bias=leaves[2], activation="gelu"), leaves, dy)
     assert torch.equal(got, dbias)
     assert torch.equal(da, cascaded_lowp_matmul(dz, b.t().contiguous())) and torch.equal(db, cascaded_lowp_matmul(a.t().contiguous(), dz))
+
+
+@pytest.mark.parametrize("cascade, M, K, N, far", [("fp32", 2, 320, 1280, 1 << 29), ("fp32", 256, 5120, 128, 8_600_000), ("fp32", 512, 64, 1280, 2_200_000),
+                                                   ("fp32", 2048, 64, 10240, 2_200_000), ("fp32x3", 400, 640, 5120, 8_600_000), ("fp32x3", 2, 320, 1280, 1 << 29),
+                                                   ("fp16", 70, 640, 320, 9_000_000), ("bf16", 300, 640, 2560, 9_000_000)])
+def test_z_with_rows_far_apart(gpu_device, cascade, M, K, N, far):
+    """z kept in rows further apart than the offsets of a tile's stores, beside results that are not, through the C entry."""
+    dtype, options, lost = CASCADES[cascade]
+    a, b, bias, residual, _ = operands(M, K, N, dtype, gpu_device)
+    code, fmt, terms = {"fp32": (0, 0, 2), "fp32x3": (0, 1, 3), "fp16": (1, 1, 1), "bf16": (2, 0, 1)}[cascade]
+    l = _lib.lib()
+    need = l.cascmm_workspace_bytes(M, N, K, code, fmt, terms, 0)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=gpu_device)
+    z = torch.empty((M - 1) * far + N, dtype=dtype, device=gpu_device).as_strided((M, N), (far, 1))
+    z.fill_(math.nan)
+    y = torch.full((M, N), math.nan, dtype=dtype, device=gpu_device)
+    assert l.cascmm_gemm_epilogue(a.data_ptr(), b.data_ptr(), 0, y.data_ptr(), bias.data_ptr(), residual.data_ptr(), z.data_ptr(), M, N, K, K, N, N, N, far, code, fmt, terms, 0,
+                                  _lib.ACT_BY_NAME["silu"], None, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+    check_forward(y, a, b, bias, "silu", residual, dtype, lost, "y")
+    want, _, stored = z_of(a, b, bias, dtype, lost)
+    within(z.contiguous(), want, stored, "z")

@@ -102,3 +102,49 @@ def operands(dy=P, z=P, dz=P, dbias=None, A=P, At=P, B=P, Bt=P, M=4, N=8, K=16, 
     (dict(dz=None, At=None, Bt=None), 0), (dict(M=0, Bt=None), 0), (dict(N=0, ldb=0, At=None), 0), (dict(M=0, N=0, K=0, ldb=0), 0)])
 def test_backward_with_operands_arguments(change, status):
     assert operands(**change) == status
+
+
+# Calls in a child process that sees no GPU, on addresses that are never read: they have to reach the launch, which fails for want of a device
+CHILD = """
+import json, sys
+from basedxl_amd import _lib
+l = _lib.lib()
+if l.cascmm_init() == 0:
+    raise SystemExit("a GPU is visible")
+A, B, C, Z, R, WS = (i << 44 for i in range(1, 7))
+out = []
+for c in json.load(sys.stdin):
+    M, K, N, (dt, fmt, terms) = c["M"], c["K"], c["N"], c["cascade"]
+    need = l.cascmm_workspace_bytes(M, N, K, dt, fmt, terms, 0)
+    out.append(l.cascmm_gemm_epilogue(A + c.get("a_offset", 0), B, c.get("prepared", 0), C, None, R if c.get("residual") else None, Z if c.get("ldp") else None, M, N, K,
+                                      c.get("lda", K), N, c.get("ldc", N), c.get("ldr", N), c.get("ldp", N), dt, fmt, terms, 0, c.get("act", 2), None,
+                                      WS if need else None, need, None))
+json.dump(out, sys.stdout)
+"""
+LAUNCH = -7
+CASCADES = {"bf16x2": (0, 0, 2), "fp16x3": (0, 1, 3), "bf16x3": (0, 0, 3), "fp8x3": (0, 2, 3), "fp16": (1, 1, 1), "bf16": (2, 0, 1)}
+
+
+def refused(cases):
+    """The cases that do not reach the launch, with their statuses."""
+    import json
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=root, HIP_VISIBLE_DEVICES="-1", ROCR_VISIBLE_DEVICES="")
+    r = subprocess.run([sys.executable, "-c", CHILD], input=json.dumps(cases), cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return [(c, st) for c, st in zip(cases, json.loads(r.stdout)) if st != LAUNCH]
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+def test_rows_far_apart_reach_the_launch(cascade):
+    """Results, residuals and z whose rows are further apart than the offsets of some kernel's stores."""
+    cases = []
+    for M, K, N in ((2, 320, 1280), (70, 640, 640), (300, 1280, 1280), (1024, 1280, 1280), (2048, 5120, 1280), (2048, 1280, 5120), (8192, 640, 640), (333, 456, 211), (4096, 640, 2560)):
+        for prepared in (0, 1) if cascade in ("bf16x2", "fp16", "bf16") and K % 64 == 0 else (0,):
+            for far in (1 << 20, 1 << 22, 1 << 24, 1 << 30):
+                for at in ({"ldp": far}, {"ldc": far, "ldp": N}, {"ldc": far}, {"residual": 1, "ldr": far, "ldp": N}):
+                    cases.append(dict(M=M, K=K, N=N, cascade=CASCADES[cascade], prepared=prepared, **at))
+    assert not refused(cases)
