@@ -991,6 +991,19 @@ static Relay relay_of(const Problem& q0, int count, const void* const* A, const 
   }
   return r;
 }
+// Calls with an epilogue on a prepared 16-bit weight have no kernel but for copied rows where K is no multiple of 8 or rows lie off dwords, whatever their number:
+// the rows whose copies a workspace holds go at a time (copies stay below 2 GiB too), whole tiles of them where it holds as many.  What a
+// workspace of cascmm_workspace_bytes holds of rows that are more than that: 1048576 x 1025 x 64 fp16 in nine blocks 1.2 ms (the raw
+// weight, element by element, 3.4), x 1280 3.6 (52).
+constexpr int64_t kCopiedRowBytes = 256 << 20;
+static int64_t copied_row(const Problem& q) { return (q.K * 2 + 127) / 128 * 128; }
+static int64_t rows_at_a_time(const Problem& q, const void* A, size_t room) {
+  if (!q.bpre || !own_format16(q) || (q.K % 8 == 0 && q.lda % 2 == 0 && aligned_to(A, 4))) return q.M;
+  const int64_t row = copied_row(q);
+  if (!beyond_i32(q.M, row, 1) && f8k64_up(q.M * row) <= room) return q.M;
+  const int64_t fit = ((int64_t)std::min<size_t>(room, kCopiedRowBytes) - 256) / row;   // (a copy's bytes are rounded up to whole 256)
+  return fit < 1 ? q.M : fit < 256 ? fit : fit / 256 * 256;
+}
 static size_t relay_bytes(const Relay& r, int count) { return (size_t)count * (r.a_bytes + r.b_bytes); }
 // what the partial results of the chosen kernel's K split take, at most `room`
 static size_t ksplit_need(const Problem& q, RowFit fit, size_t room) {
@@ -1541,6 +1554,8 @@ size_t cascmm_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int fm
     }
   }
   need += parts;
+  // (copies of all rows would be too large: see rows_at_a_time)
+  if (own_format16(q) && K % 8 != 0 && beyond_i32(M, copied_row(q), 1)) need = std::max(need, (size_t)kCopiedRowBytes);
   for (const auto& v : table()) {
     if (v.kind != KIND_SPLITK || !variant_matches(v, q, fit)) continue;
     const size_t n = skinny_workspace_bytes(M, N, K, v.BM, v.BN, v.BK);
@@ -1721,11 +1736,19 @@ int cascmm_gemm_epilogue(const void* A, const void* B, int b_prepared, void* C, 
   const size_t es = dtype_size(dtype);
   if (!C) return CASCMM_ERR_NULL_POINTER;
   if (!aligned_to(C, es) || !aligned_to(residual, es) || !aligned_to(preact, es)) return CASCMM_ERR_ALIGNMENT;
-  const Epilogue ep{activation, residual, ldr, preact, ldp, ldc};
   if (K > 0) {
-    q.epi = &ep;
     if (preact) q.ldc = std::max(ldc, ldp);   // (whichever of them the product stores, its kernel reaches the rows of both)
-    return gemm_impl(1, &A, &B, &C, bias ? &bias : nullptr, q, tensor_exps, workspace, workspace_bytes, (hipStream_t)stream, -1);
+    const int64_t rows = rows_at_a_time(q, A, workspace ? workspace_bytes : 0);
+    for (int64_t m = 0; m < M; m += rows) {
+      q.M = std::min(rows, M - m);
+      const Epilogue part{activation, residual ? (const char*)residual + m * ldr * es : nullptr, ldr, preact ? (char*)preact + m * ldp * es : nullptr, ldp, ldc};
+      q.epi = &part;
+      const void* a = A ? (const char*)A + m * lda * es : nullptr;
+      void* c = (char*)C + m * ldc * es;
+      const int sg = gemm_impl(1, &a, &B, &c, bias ? &bias : nullptr, q, tensor_exps, workspace, workspace_bytes, (hipStream_t)stream, -1);
+      if (sg != CASCMM_OK) return sg;
+    }
+    return CASCMM_OK;
   }
   // (no inputs: z is the bias or zero, which its kernel writes in preact or in the result's place)
   void* z = preact ? preact : C;

@@ -331,7 +331,9 @@ int cascmm_gemm_fp8_autoscale(const void* A, const void* B, int b_prepared, void
  *     z = A . B (+ bias);   C = activation(z) (+ residual)
  * The reference runs the layer (basedxl/modules/lowp_linear.py:15-20) and what its model does with the result (the residual adds of a
  * transformer block, an embedding's SiLU) as separate kernels.  Operands as cascmm_gemm (b_prepared == 0) or cascmm_gemm_prepared with one
- * problem (b_prepared != 0, ldb ignored; 16-bit weights of one term with a workspace for any K and any rows of A); residual [M, N] of `dtype` or NULL, its rows ldr >= N apart or all the same one (ldr == 0);
+ * problem (b_prepared != 0, ldb ignored; 16-bit weights of one term for any K and any rows of A, which are copied to the workspace first, as many at a time as it holds,
+ * where K is no multiple of 8 or they lie off dwords: cascmm_workspace_bytes counts them for such K, and rows off dwords need some room, 2 K bytes rounded up to whole 128 a row);
+ * residual [M, N] of `dtype` or NULL, its rows ldr >= N apart or all the same one (ldr == 0);
  * preact: NULL or [M, N], receives z for the backward pass.  The activation is one of cascmm_activation, in fp32.
  * C and preact overlap no operand and not each other.  tensor_exps, workspace: as cascmm_gemm.
  */

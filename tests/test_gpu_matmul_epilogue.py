@@ -546,3 +546,44 @@ def test_z_with_rows_far_apart(gpu_device, cascade, M, K, N, far):
     check_forward(y, a, b, bias, "silu", residual, dtype, lost, "y")
     want, _, stored = z_of(a, b, bias, dtype, lost)
     within(z.contiguous(), want, stored, "z")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act, broadcast", [(None, False), ("gelu", True), ("silu", False)])
+def test_copied_rows_a_block_at_a_time(gpu_device, dtype, act, broadcast):
+    """Prepared 16-bit weights on rows that are copied first, in workspaces that hold some of the copies."""
+    l, (code, fmt) = _lib.lib(), {torch.float16: (1, 1), torch.bfloat16: (2, 0)}[dtype]
+    for M, K, N, shift in ((1000, 283, 64, 0), (777, 129, 211, 1), (300, 128, 320, 1), (65, 1, 8, 0)):
+        a, b, bias, residual, _ = operands(M, K, N, dtype, gpu_device)
+        pw = PreparedWeight(b)
+        wide = torch.full((M, K + 3), math.nan, dtype=dtype, device=gpu_device)
+        wide[:, shift:shift + K] = a
+        r = residual[0] if broadcast else residual
+        row = (2 * K + 127) // 128 * 128
+        for held in (1, 40, 256, 300, 600, M):
+            room = held * row + 256
+            ws = torch.empty(room + 1, dtype=torch.uint8, device=gpu_device)
+            ws[room] = 77
+            z, y = (torch.full((M + 1, N + 5), math.inf, dtype=dtype, device=gpu_device) for _ in range(2))
+            assert l.cascmm_gemm_epilogue(wide[:, shift:].data_ptr(), pw.slots.data_ptr(), 1, y.data_ptr(), bias.data_ptr(), r.data_ptr(), z.data_ptr(), M, N, K, K + 3, N,
+                                          N + 5, 0 if broadcast else N, N + 5, code, fmt, 1, 0, _lib.ACT_BY_NAME[act], None, ws.data_ptr(), room,
+                                          torch.cuda.current_stream().cuda_stream) == 0
+            check_forward(y[:M, :N], a, b, bias, act, r.expand(M, N), dtype, 0.0, f"{M} {K} {N} {held}", fused=True)
+            want, _, stored = z_of(a, b, bias, dtype, 0.0)
+            within(z[:M, :N], want, stored, "z")
+            assert int(ws[room]) == 77
+            assert all(bool((t[M] == math.inf).all()) and bool((t[:, N:] == math.inf).all()) for t in (y, z))
+
+
+def test_prepared_weights_of_any_depth_on_more_rows_than_one_copy_holds(gpu_device, path):
+    """Copies of A beyond 2 GiB as a whole: every row is its weights' row, at the ends of blocks too."""
+    M, K, N = 1 << 20, 1025, 16
+    b = torch.randn(K, N, device=gpu_device).half()
+    a = (torch.arange(M, device=gpu_device, dtype=torch.int32) % 7 - 3).half()[:, None].expand(M, K).contiguous()
+    y = cascaded_lowp_matmul_epilogue(a, PreparedWeight(b), activation="relu")
+    one = cascaded_lowp_matmul_epilogue(a[:7].contiguous(), PreparedWeight(b), activation="relu")
+    want = F.relu(a[:7].double() @ b.double())
+    for m in range(7):     # (rows of one kind are alike whichever block they are in, up to the order of K products)
+        S = a[m].double().abs() @ b.double().abs()
+        tol = K * U * S + HALF[torch.float16] * want[m] + TINY[torch.float16]
+        assert bool(((y[m::7].double() - want[m]).abs() <= tol).all()) and bool(((one[m].double() - want[m]).abs() <= tol).all())

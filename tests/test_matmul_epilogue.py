@@ -148,3 +148,12 @@ def test_rows_far_apart_reach_the_launch(cascade):
                 for at in ({"ldp": far}, {"ldc": far, "ldp": N}, {"ldc": far}, {"residual": 1, "ldr": far, "ldp": N}):
                     cases.append(dict(M=M, K=K, N=N, cascade=CASCADES[cascade], prepared=prepared, **at))
     assert not refused(cases)
+
+
+@pytest.mark.parametrize("cascade", ["fp16", "bf16"])
+def test_prepared_16_bit_weights_on_any_number_of_rows_reach_the_launch(cascade):
+    """K off 8 and rows off dwords, whose copies are beyond 2 GiB as a whole."""
+    cases = [dict(M=M, K=K, N=N, cascade=CASCADES[cascade], prepared=1, **more) for M, K in ((1 << 20, 1025), (1 << 21, 1283), (1 << 30, 9), (2 ** 31 - 1, 1), (3000, 500_001))
+             for N in (1, 64, 211) for more in ({}, {"lda": K + 4}, {"residual": 1, "ldp": N, "a_offset": 2})]
+    cases += [dict(M=1 << 20, K=1032, N=64, cascade=CASCADES[cascade], prepared=1, **more) for more in ({}, {"lda": 1040})]
+    assert not refused(cases)
