@@ -17,6 +17,7 @@ import torch.nn as nn
 from ..cascaded_lowp_matmul import (ChainedWeight, PreparedWeight, cascaded_lowp_matmul_chained, cascaded_lowp_matmul_glu_chained,
                                     chained_supported, glu_chained_worthwhile)
 from .geglu import BasedXLLowPGEGLU
+from .gradients import differentiated, gradient_of, with_gradient
 from .lowp_linear import BasedXLLowPLinear
 
 
@@ -28,7 +29,10 @@ class BasedXLChainedFeedForward(nn.Module):
     in % 32 == 0, and where the library's estimates favour the large-tile kernel with the gate in its store
     over a plain kernel plus a gate pass (few rows on many CUs: they do not); anything else goes through :class:`BasedXLLowPGEGLU` and :class:`BasedXLLowPLinear`,
     which this module also holds (same weights).  ``prepared=True`` keeps the first weight split as
-    well (the second one always is: the chained GEMM has no other form)."""
+    well (the second one always is: the chained GEMM has no other form).  The weights are constants; a gradient passes through to ``x``
+    (by the two layers, computed once more)."""
+
+    gradient_reads_input = True
 
     def __init__(self, proj: nn.Linear, out: nn.Linear, *, lowp: Optional[str] = None, terms: Optional[int] = None,
                  products: str = "tri", prepared: Optional[bool] = None):
@@ -48,9 +52,17 @@ class BasedXLChainedFeedForward(nn.Module):
         M = x.numel() // self.in_features
         return glu_chained_worthwhile(x, 2 * self.inner) and chained_supported(M, self.out_features, self.inner)
 
+    def constants(self):
+        return (*self.geglu.constants(), *self.linear.constants())
+
+    def input_gradient(self, dy: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+        return gradient_of(lambda t: self.linear(self.geglu(t)), x, dy)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not self._chain_ok(x):
             return self.linear(self.geglu(x))
+        if differentiated(x):
+            return with_gradient(self, x)
         dev = self.linear.weight.device
         if self._chained_weight is None or self._chained_weight.device != dev:
             self._chained_weight = ChainedWeight(self.linear.weight)

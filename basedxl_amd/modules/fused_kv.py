@@ -19,7 +19,8 @@ class BasedXLFusedKV(nn.Module):
     result (attn.py:79).  With ``cache=True`` the result is kept and returned again until
     ``forward(..., recompute=True)`` or :meth:`reset`: the reference recomputes the
     cross-attention K/V only on the first denoising step (attn.py:57, 74-78), since the text
-    conditioning is the same on every step.
+    conditioning is the same on every step.  What is kept is a constant: a gradient reaches ``states``
+    through the result of the call that computed it, not through later ones.
     """
 
     def __init__(self, to_k: nn.Linear, to_v: nn.Linear, *, cache: bool = False, **cascade_kwargs):
@@ -45,9 +46,10 @@ class BasedXLFusedKV(nn.Module):
         if not self.cache:
             kv = self.to_kv(states)
         else:
-            if recompute or self.kv_cache is None:
-                self.kv_cache = self.to_kv(states)
             kv = self.kv_cache
+            if recompute or kv is None:
+                kv = self.to_kv(states)
+                self.kv_cache = kv.detach() if kv.requires_grad else kv
         return kv.narrow(-1, 0, self.out_features), kv.narrow(-1, self.out_features, self.out_features)
 
 

@@ -16,6 +16,8 @@ import torch.nn.functional as F
 
 from .. import _lib
 from ..cascaded_lowp_matmul import PreparedWeight, cascaded_lowp_matmul, cascaded_lowp_matmul_glu, default_cascade, gate_product, gated_variant
+from ..matmul_epilogue import cascaded_lowp_matmul_epilogue
+from .gradients import differentiated, gradient_of, with_gradient
 
 
 class BasedXLLowPGEGLU(nn.Module):
@@ -27,7 +29,10 @@ class BasedXLLowPGEGLU(nn.Module):
     (pre-split, column-interleaved) copy of the weight, made on first use.  ``prepared=False`` keeps
     no such copy: the large-tile kernel applies the gate on the raw weight where it takes the problem
     (fp32, two bf16 terms, rows % 256 == 0, inner % 160 == 0).  Anything else runs the cascade GEMM on the
-    raw weight followed by a kernel that applies the gate (the same arithmetic in two kernels)."""
+    raw weight followed by a kernel that applies the gate (the same arithmetic in two kernels).
+    Weight and bias are constants; a gradient passes through to ``x`` (``h`` is computed once more for it, by the raw weight)."""
+
+    gradient_reads_input = True
 
     def __init__(self, proj: nn.Linear, *, lowp: Optional[str] = None, terms: Optional[int] = None,
                  products: str = "tri", prepared: Optional[bool] = None):
@@ -60,6 +65,17 @@ class BasedXLLowPGEGLU(nn.Module):
                 self._prepared is None or self._prepared.device != self.weight.device):
             self._prepared = PreparedWeight(self.weight, lowp=self.lowp, terms=self.terms, glu=True)
 
+    def constants(self):
+        return (self.weight,) if self.bias is None else (self.weight, self.bias)
+
+    def input_gradient(self, dy: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+        def gated(t):
+            h = cascaded_lowp_matmul_epilogue(t, self.weight, bias=self.bias, lowp=self.lowp, terms=self.terms, products=self.products)
+            value, gate = h.float().chunk(2, dim=-1)
+            return value * F.gelu(gate)
+
+        return gradient_of(gated, x, dy)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if torch.compiler.is_compiling() and self._prepared is not None and x.dtype == self.weight.dtype:
             from ..compiled import cascade_linear
@@ -70,6 +86,8 @@ class BasedXLLowPGEGLU(nn.Module):
             h = cascade_linear(x, self.weight, None, self.bias, self.lowp, self.terms, self.products, False, None)
             value, gate = h.chunk(2, dim=-1)
             return value * F.gelu(gate)
+        if differentiated(x):
+            return with_gradient(self, x)
         pw = self._prepared
         if self.prepared and pw is not None and pw.device == self.weight.device and x.dtype == self.weight.dtype:
             # the ordinary eager call in one native function; None: whatever is not ordinary about it is decided below

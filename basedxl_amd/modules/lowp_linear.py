@@ -9,6 +9,7 @@ from typing import Optional
 from .. import _lib
 from ..cascaded_lowp_matmul import PreparedWeight, cascaded_lowp_matmul, default_cascade, raw_is_faster, tensor_scale_exp
 from ..matmul_epilogue import cascaded_lowp_matmul_epilogue
+from .gradients import differentiated, with_gradient
 
 
 class BasedXLLowPLinear(nn.Module):
@@ -16,8 +17,10 @@ class BasedXLLowPLinear(nn.Module):
     (lowp_linear.py:12) and the forward pass is one cascade GEMM with the bias add fused
     into its store (the reference adds it in a second kernel, lowp_linear.py:17-19).
     ``activation`` ("relu", "gelu", "gelu_tanh", "silu") and ``forward(x, residual)`` put what follows the layer
-    in its epilogue: ``activation(x @ weight + bias) + residual``.  The weight is a constant; with an epilogue gradients
-    pass through to ``x`` and ``residual`` (by the raw weight, where they are asked for), without one they do not."""
+    in its epilogue: ``activation(x @ weight + bias) + residual``.  Weight and bias are constants; gradients pass through to ``x`` and
+    ``residual``, once differentiable (with an epilogue both ways go by the raw weight, without one the way back)."""
+
+    gradient_reads_input = False
 
     #: what follows the product (an attribute: a patcher may set it on a layer that it knows the use of)
     activation: Optional[str] = None
@@ -61,8 +64,8 @@ class BasedXLLowPLinear(nn.Module):
             from ..compiled import cascade_linear_epilogue
             return cascade_linear_epilogue(x, self.weight, None if pw is None else pw.slots, self.bias, residual, self.activation, self.lowp, self.terms,
                                            self.products, self._weight_exp if pw is None else pw.exp)
-        differentiated = torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))
-        if self.prepared and x.is_cuda and x.dtype == self.weight.dtype and not differentiated and not raw_is_faster(
+        constant = not differentiated(x) and (residual is None or not differentiated(residual))
+        if self.prepared and x.is_cuda and x.dtype == self.weight.dtype and constant and not raw_is_faster(
                 x.numel() // max(self.in_features, 1), self.in_features, self.out_features, x.dtype, self.lowp, self.terms, self.products):
             if pw is None or pw.device != self.weight.device:
                 pw = self._prepared_weight = PreparedWeight(self.weight, lowp=self.lowp, terms=self.terms)
@@ -73,6 +76,13 @@ class BasedXLLowPLinear(nn.Module):
             self._weight_exp = tensor_scale_exp(self.weight)
         return cascaded_lowp_matmul_epilogue(x, self.weight, lowp=self.lowp, terms=self.terms, b_exp=self._weight_exp, **how)
 
+    def constants(self):
+        return (self.weight,)
+
+    def input_gradient(self, dy: torch.Tensor, _x) -> torch.Tensor:
+        """``dy @ weight.T`` by the layer's own cascade."""
+        return cascaded_lowp_matmul(dy, self.weight.t().contiguous(), lowp=self.lowp, terms=self.terms, products=self.products)
+
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if residual is not None or self.activation is not None:
             return self._with_epilogue(x, residual)
@@ -82,6 +92,8 @@ class BasedXLLowPLinear(nn.Module):
             pw = self._prepared_weight
             return cascade_linear(x, self.weight, None if pw is None else pw.slots, self.bias, self.lowp, self.terms,
                                   self.products, False, self._weight_exp if pw is None else pw.exp)
+        if differentiated(x):
+            return with_gradient(self, x)
         # the ordinary eager call in one native function; None: whatever is not ordinary about it is decided below
         pw, raw = self._prepared_weight, not self.prepared
         if not raw and pw is not None and (pw.dt or not (pw.fmt or pw.terms != 2 or pw.K & 7 or self.products != "tri")):

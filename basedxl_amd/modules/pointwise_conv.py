@@ -12,6 +12,7 @@ import torch
 import torch.nn as nn
 
 from ..cascaded_lowp_matmul import cascaded_lowp_matmul, cascaded_lowp_matmul_grouped, default_cascade, tensor_scale_exp
+from .gradients import differentiated, with_gradient
 
 MAX_GROUP = 8   # problems one grouped launch takes
 
@@ -31,7 +32,11 @@ class BasedXLLowPConv1x1(nn.Module):
     * NCHW-contiguous input: per image ``[C_out, C_in] x [C_in, H*W]`` (the image is already the
       row-major right-hand operand), all images of the batch in one grouped launch; the bias
       runs along rows there and is added afterwards.
+
+    Weight and bias are constants; a gradient passes through to the input.
     """
+
+    gradient_reads_input = False
 
     def __init__(self, conv: nn.Conv2d, *, lowp: Optional[str] = None, terms: Optional[int] = None,
                  products: str = "tri"):
@@ -40,13 +45,20 @@ class BasedXLLowPConv1x1(nn.Module):
             raise ValueError("BasedXLLowPConv1x1 takes 1x1 convolutions with stride 1 and no padding, dilation or groups")
         self.in_channels, self.out_channels = conv.in_channels, conv.out_channels
         w = conv.weight.detach().reshape(conv.out_channels, conv.in_channels)
-        # buffers, so that .to() / .cuda() move them; not parameters: the path has no backward
+        # buffers, so that .to() / .cuda() move them; not parameters: they get no gradient
         self.register_buffer("weight", w.contiguous().clone())       # [C_out, C_in]: left operand for NCHW input
         self.register_buffer("weight_t", w.T.contiguous().clone())   # [C_in, C_out]: right operand for channels-last input
         self.register_buffer("bias", conv.bias.detach().clone() if conv.bias is not None else None)
         d_lowp, d_terms = default_cascade(self.weight.dtype)
         self.lowp, self.terms, self.products = d_lowp if lowp is None else lowp, d_terms if terms is None else terms, products
         self._weight_exp = None
+
+    def constants(self):
+        return (self.weight,)
+
+    def input_gradient(self, dy: torch.Tensor, _x) -> torch.Tensor:
+        """The product with the weight as it lies, [C_out, C_in], over the pixels' channels."""
+        return cascaded_lowp_matmul(dy.permute(0, 2, 3, 1).contiguous(), self.weight, lowp=self.lowp, terms=self.terms, products=self.products).permute(0, 3, 1, 2)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() != 4 or x.shape[1] != self.in_channels:
@@ -64,6 +76,8 @@ class BasedXLLowPConv1x1(nn.Module):
                                  self.products, False, None) for b in range(B)]
             out = torch.stack(ys).reshape(B, self.out_channels, H, W)
             return out if self.bias is None else out + self.bias.view(1, -1, 1, 1)
+        if differentiated(x):
+            return with_gradient(self, x)
         rows = x.permute(0, 2, 3, 1)
         if rows.is_contiguous() and not x.is_contiguous():
             if self.lowp == "fp8" and (self._weight_exp is None or self._weight_exp.device != x.device):

@@ -7,10 +7,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from basedxl_amd import (BasedXLLayerNorm, BasedXLLowPLinear, add_layer_norm, cascaded_lowp_matmul, cascaded_lowp_matmul_epilogue, layer_norm, patch_layer_norms,
-                         patch_linear_layers)
+from basedxl_amd import (BasedXLChainedFeedForward, BasedXLFusedKV, BasedXLLayerNorm, BasedXLLowPConv1x1, BasedXLLowPGEGLU, BasedXLLowPLinear, add_layer_norm,
+                         cascaded_lowp_matmul, cascaded_lowp_matmul_epilogue, chain_feed_forward_layers, layer_norm, patch_layer_norms, patch_linear_layers)
 from basedxl_amd.unet import BasedXLUnet, patch_unet
-from basedxl_amd.unet_skeleton import BasicTransformerBlock, SDXLUNetSkeleton, TimestepEmbedding, fuse_epilogues, synthetic_inputs
+from basedxl_amd.unet_skeleton import BasicTransformerBlock, SDXLUNetSkeleton, TimestepEmbedding, fuse_epilogues, fuse_geglu_layers, fuse_kv_projections, synthetic_inputs
 from basedxl_amd.utils import BasedXLConfig
 
 SMALL = dict(channels=(64, 128, 256), head_dim=32, depths=(1, 2), cross_dim=96, add_time_dim=32)
@@ -204,3 +204,163 @@ def test_small_unet_with_and_without(gpu_device, dtype, bound):
         for flags in (dict(fuse_epilogues=True), dict(fuse_norms=True), dict(fuse_epilogues=True, fuse_norms=True, fuse_geglu=True), dict(fuse_epilogues=True, chain_ffn=True)):
             got = BasedXLUnet(copy.deepcopy(base), BasedXLConfig(dtype=dtype, fp16_acc_matmul=True, **flags))(*inputs).double()
             assert float((got - want).norm() / want.norm()) <= bound, flags
+
+
+# ---- gradients through module trees ----
+# Products of fp32 operands by two bf16 terms leave out 3 2^-16 of |a| @ |b|, by three fp16 terms 2^-24, by three fp8 terms 2^-9 of it (tests/test_gpu_matmul_epilogue.py)
+LOST = {(torch.float32, "bf16"): 3 * 2.0 ** -16, (torch.float32, "fp16"): 2.0 ** -24, (torch.float32, "fp8"): 2.0 ** -9, (torch.float16, "fp16"): 0.0, (torch.bfloat16, "bf16"): 0.0}
+LAYERS = [(torch.float32, {}), (torch.float32, dict(prepared=True)), (torch.float32, dict(lowp="fp16", terms=3)), (torch.float32, dict(lowp="fp8", terms=3)),
+          (torch.float32, dict(lowp="fp8", terms=3, prepared=True)), (torch.float16, {}), (torch.bfloat16, dict(prepared=False)), (torch.bfloat16, {})]
+
+
+def product_tolerance(dy, w, dtype, lowp):
+    """(dy @ w.T in 64 bits, how far a product of one cascade may be off)."""
+    want, S = dy.double() @ w.double().t(), dy.double().abs() @ w.double().abs().t()
+    u = torch.finfo(dtype).eps / 2
+    return want, ((w.shape[1] + 4) * 2.0 ** -24 + LOST[dtype, lowp]) * S + u * want.abs() + torch.finfo(dtype).smallest_normal
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, kw", LAYERS)
+@pytest.mark.parametrize("rows, i, o", [(2, 64, 96), (300, 128, 320), (77, 50, 30), (1, 1, 1)])
+def test_gradients_pass_a_linear_wrapper(gpu_device, dtype, kw, rows, i, o):
+    torch.manual_seed(7)
+    layer = linear(gpu_device, i, o, dtype, **kw)
+    x, dy = torch.randn(2, rows, i, device=gpu_device, dtype=dtype), torch.randn(2, rows, o, device=gpu_device, dtype=dtype)
+    with torch.no_grad():
+        want = layer(x)
+    leaf = x.clone().requires_grad_()
+    y = layer(leaf)
+    assert torch.equal(y, want)          # (the same kernels, prepared weights among them)
+    (g,) = torch.autograd.grad(y, leaf, dy, create_graph=True)
+    dx, tol = product_tolerance(dy, layer.weight, dtype, layer.lowp)
+    assert bool(((g.detach().double() - dx).abs() <= tol).all())
+    with pytest.raises(RuntimeError):    # (once differentiable)
+        g.sum().backward()
+    # a gradient that is one value for all, and no graph where none is wanted
+    (g,) = torch.autograd.grad(layer(leaf).sum(), leaf)
+    assert torch.equal(g, torch.autograd.grad(layer(leaf), leaf, torch.ones_like(dy))[0])
+    with torch.no_grad():
+        assert layer(leaf).grad_fn is None
+    assert layer(x).grad_fn is None
+    # weights written to between the two ways are noticed
+    y = layer(leaf)
+    layer.weight.mul_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, kw", LAYERS)
+@pytest.mark.parametrize("rows, i, inner", [(130, 128, 64), (20, 50, 30)])
+def test_gradients_pass_a_gated_wrapper(gpu_device, dtype, kw, rows, i, inner):
+    torch.manual_seed(8)
+    layer = BasedXLLowPGEGLU(nn.Linear(i, 2 * inner).to(device=gpu_device, dtype=dtype), **kw)
+    x, dy = torch.randn(rows, i, device=gpu_device, dtype=dtype), torch.randn(rows, inner, device=gpu_device, dtype=dtype)
+    with torch.no_grad():
+        want = layer(x)
+    leaf = x.clone().requires_grad_()
+    y = layer(leaf)
+    assert torch.equal(y, want)
+    (g,) = torch.autograd.grad(y, leaf, dy)
+    e = x.double().requires_grad_()
+    value, gate = (e @ layer.weight.double() + layer.bias.double()).chunk(2, dim=-1)
+    (dx,) = torch.autograd.grad(value * F.gelu(gate), e, dy.double())
+    # In the mean square: h, dh and the result are rounded once each (half a step at most), dh follows h with slopes up to 1.13 in the value and 0.8 of the value
+    # in the gate; the products leave out `lost` of |a| @ |b|, which adds up over K as they do, twice: four of the larger
+    assert float((g.double() - dx).norm() / dx.norm()) <= 4 * max(torch.finfo(dtype).eps / 2, LOST[dtype, layer.lowp], 2.0 ** -22)
+
+
+@pytest.mark.gpu
+def test_gradients_pass_a_chained_feed_forward(gpu_device):
+    torch.manual_seed(9)
+    proj, out = nn.Linear(320, 2560).to(gpu_device), nn.Linear(1280, 320).to(gpu_device)
+    for prepared in (False, True):
+        ff = BasedXLChainedFeedForward(proj, out, prepared=prepared)
+        for rows in (8192, 100):    # (with the chain, and layer by layer)
+            x, dy = torch.randn(rows, 320, device=gpu_device), torch.randn(rows, 320, device=gpu_device)
+            with torch.no_grad():
+                want = ff(x)
+            chained, leaf = ff.chained_calls, x.clone().requires_grad_()
+            y = ff(leaf)
+            assert torch.equal(y, want) and (ff.chained_calls > chained) == (rows == 8192)
+            (g,) = torch.autograd.grad(y, leaf, dy)
+            (wg,) = torch.autograd.grad(ff.linear(ff.geglu(leaf)), leaf, dy)
+            assert torch.equal(g, wg)
+            e = x.double().requires_grad_()
+            value, gate = F.linear(e, proj.weight.double(), proj.bias.double()).chunk(2, dim=-1)
+            (dx,) = torch.autograd.grad(F.linear(value * F.gelu(gate), out.weight.double()), e, dy.double())
+            assert float((g.double() - dx).norm() / dx.norm()) <= 6 * 3 * 2.0 ** -16   # (three products of the cascade, the first one's error with slopes up to 1.13)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_gradients_pass_a_pointwise_convolution(gpu_device, dtype):
+    torch.manual_seed(10)
+    conv = BasedXLLowPConv1x1(nn.Conv2d(64, 96, 1).to(device=gpu_device, dtype=dtype))
+    for layout in (torch.contiguous_format, torch.channels_last):
+        x = torch.randn(3, 64, 9, 7, device=gpu_device, dtype=dtype).contiguous(memory_format=layout)
+        dy = torch.randn(3, 96, 9, 7, device=gpu_device, dtype=dtype)
+        with torch.no_grad():
+            want = conv(x)
+        leaf = x.clone().requires_grad_()
+        y = conv(leaf)
+        assert torch.equal(y, want)
+        for d in (dy, dy.contiguous(memory_format=torch.channels_last)):
+            (g,) = torch.autograd.grad(conv(leaf), leaf, d)
+            dx, tol = product_tolerance(dy.permute(0, 2, 3, 1), conv.weight.t(), dtype, conv.lowp)
+            assert g.shape == x.shape and bool(((g.permute(0, 2, 3, 1).double() - dx).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+def test_a_kept_key_and_value_are_constants(gpu_device):
+    torch.manual_seed(11)
+    kv = BasedXLFusedKV(nn.Linear(64, 32).to(gpu_device), nn.Linear(64, 32).to(gpu_device), cache=True)
+    s = torch.randn(10, 64, device=gpu_device, requires_grad=True)
+    k, v = kv(s)
+    (g,) = torch.autograd.grad((k.sum() + 2 * v.sum()), s)
+    dx, tol = product_tolerance(torch.cat([torch.ones(10, 32), 2 * torch.ones(10, 32)], 1).to(gpu_device), kv.to_kv.weight, torch.float32, "bf16")
+    assert bool(((g.double() - dx).abs() <= tol).all())
+    k2, v2 = kv(s)
+    assert torch.equal(k2, k) and torch.equal(v2, v) and not k2.requires_grad
+    k3, _ = kv(s, recompute=True)
+    assert torch.equal(k3, k) and k3.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw, bound", [({}, 2e-3), (dict(lowp="fp16", terms=3), 2e-5)])
+@pytest.mark.parametrize("what", ["linear", "epilogues", "norms", "both", "fused", "chained"])
+def test_gradients_of_a_whole_block(gpu_device, what, kw, bound):
+    """dx, the context's gradient and the norms' of a transformer block in fp32, against torch in 64 bits.  In the mean square a product by two bf16
+    terms leaves out at most 3 2^-16 = 4.6e-5 of itself, some ten of them follow each other either way, and norms and softmax at most quadruple an error: 2e-3;
+    three fp16 terms hold fp32's own accuracy, some thirty sums of 128 and more numbers in fp32, 2^-24 (128)^1/2 each: 2e-5."""
+    torch.manual_seed(12)
+    base = BasicTransformerBlock(128, 4, 96).to(gpu_device)
+    for p in base.parameters():
+        p.data.normal_(0, 0.1)
+    for n in (base.norm1, base.norm2, base.norm3):
+        n.weight.data += 1
+    block = copy.deepcopy(base)
+    if what == "chained":
+        chain_feed_forward_layers(block, **kw)
+    if what == "fused":
+        fuse_kv_projections(block, fuse_q=True, **kw)
+        fuse_geglu_layers(block, **kw)
+    patch_linear_layers(block, **kw)
+    if what in ("epilogues", "both", "fused", "chained"):
+        fuse_epilogues(block)
+    if what in ("norms", "both", "fused", "chained"):
+        patch_layer_norms(block)
+    x, ctx, dy = torch.randn(2, 70, 128, device=gpu_device), torch.randn(2, 11, 96, device=gpu_device), torch.randn(2, 70, 128, device=gpu_device)
+    norms = ["norm1", "norm2", "norm3"]
+
+    def grads(b, x, ctx, dy):
+        leaves = [x.detach().clone().requires_grad_(), ctx.detach().clone().requires_grad_()]
+        params = [p for n in norms for p in (getattr(b, n).weight, getattr(b, n).bias)]
+        y = b(leaves[0], leaves[1])
+        return [y.detach(), *torch.autograd.grad(y, leaves + params, dy)]
+
+    got = grads(block, x, ctx, dy)
+    want = grads(base.double().cpu(), x.double().cpu(), ctx.double().cpu(), dy.double().cpu())
+    for name, g, w in zip(["y", "x", "context", *[n + "." + p for n in norms for p in ("weight", "bias")]], got, want):
+        assert float((g.cpu().double() - w).norm() / w.norm()) <= bound, name
