@@ -36,10 +36,15 @@ class BasedXLLayerNorm(nn.Module):
         return add_layer_norm(x, residual, self.weight, self.bias, eps=self.eps)
 
 
+def _hooked(module: nn.Module) -> bool:
+    return any(getattr(module, hooks, None) for hooks in ("_forward_pre_hooks", "_forward_hooks", "_backward_pre_hooks", "_backward_hooks"))
+
+
 def patch_layer_norms(model: nn.Module) -> nn.Module:
-    """Replace every ``nn.LayerNorm`` child over the last axis with :class:`BasedXLLayerNorm` (subclasses, which may compute something else, stay)."""
+    """Replace every ``nn.LayerNorm`` child over the last axis with :class:`BasedXLLayerNorm`.  Subclasses, which may compute something else, stay, and so
+    do norms with hooks, which would see other calls (a block may hand a norm the residual add in front of it)."""
     for module in list(model.modules()):
         for name, child in list(module.named_children()):
-            if type(child) is nn.LayerNorm and len(child.normalized_shape) == 1:
+            if type(child) is nn.LayerNorm and len(child.normalized_shape) == 1 and not _hooked(child):
                 setattr(module, name, BasedXLLayerNorm(child))
     return model

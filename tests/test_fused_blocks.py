@@ -40,6 +40,22 @@ def test_norm_patcher_leaves_subclasses_alone():
     assert type(model[0]) is Scaled and isinstance(model[1], BasedXLLayerNorm)
 
 
+def test_norm_patcher_leaves_norms_with_hooks_alone():
+    block, seen = BasicTransformerBlock(32, 2, 24), []
+    block.norm2.register_forward_hook(lambda m, args, y: seen.append(m))
+    block.norm3.register_forward_pre_hook(lambda m, args: seen.append(m))
+    norm2, norm3 = block.norm2, block.norm3
+    patch_layer_norms(block)
+    assert isinstance(block.norm1, BasedXLLayerNorm) and block.norm2 is norm2 and block.norm3 is norm3
+    block.norm1 = nn.Identity()
+    block(torch.randn(2, 5, 32), torch.randn(2, 3, 24))
+    assert seen == [norm2, norm3]
+    model = nn.ModuleList([nn.LayerNorm(4), nn.LayerNorm(4)])
+    model[0].register_full_backward_hook(lambda m, gi, go: None)
+    patch_layer_norms(model)
+    assert type(model[0]) is nn.LayerNorm and isinstance(model[1], BasedXLLayerNorm)
+
+
 def test_linear_wrapper_checks_its_activation():
     with pytest.raises(ValueError, match="activation"):
         BasedXLLowPLinear(nn.Linear(4, 4), activation="tanh")
