@@ -44,10 +44,18 @@ class GEGLU(nn.Module):
 
 
 def last_layer(layer: nn.Module, x: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
-    """``layer(x) + residual``, in the layer's epilogue where it has one."""
+    """``layer(x) + residual``, in the layer's epilogue where it has one and both are of one dtype (torch's add promotes them)."""
     if residual is None:
         return layer(x)
-    return layer(x, residual) if isinstance(layer, BasedXLLowPLinear) else residual + layer(x)
+    return layer(x, residual) if isinstance(layer, BasedXLLowPLinear) and residual.dtype == x.dtype else residual + layer(x)
+
+
+def add_and_norm(norm: nn.Module, h: torch.Tensor, x: torch.Tensor):
+    """``norm(x + h), x + h``, in one kernel where the norm has one and both are of one dtype."""
+    if isinstance(norm, BasedXLLayerNorm) and h.dtype == x.dtype:
+        return norm(h, x)
+    x = x + h
+    return norm(x), x
 
 
 class FeedForward(nn.Module):
@@ -123,13 +131,9 @@ class BasicTransformerBlock(nn.Module):
             x = self.attn1(self.norm1(x), residual=x)
             x = self.attn2(self.norm2(x), context, residual=x)
             return self.ff(self.norm3(x), residual=x)
-        if isinstance(self.norm2, BasedXLLayerNorm) and isinstance(self.norm3, BasedXLLayerNorm):
-            h, x = self.norm2(self.attn1(self.norm1(x)), x)       # (the add and the norm behind it in one kernel)
-            h, x = self.norm3(self.attn2(h, context), x)
-            return x + self.ff(h)
-        x = x + self.attn1(self.norm1(x))
-        x = x + self.attn2(self.norm2(x), context)
-        return x + self.ff(self.norm3(x))
+        h, x = add_and_norm(self.norm2, self.attn1(self.norm1(x)), x)
+        h, x = add_and_norm(self.norm3, self.attn2(h, context), x)
+        return x + self.ff(h)
 
 
 class Transformer2DModel(nn.Module):

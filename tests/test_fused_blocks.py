@@ -10,7 +10,7 @@ import torch.nn.functional as F
 from basedxl_amd import (BasedXLChainedFeedForward, BasedXLFusedKV, BasedXLLayerNorm, BasedXLLowPConv1x1, BasedXLLowPGEGLU, BasedXLLowPLinear, add_layer_norm,
                          cascaded_lowp_matmul, cascaded_lowp_matmul_epilogue, chain_feed_forward_layers, layer_norm, patch_layer_norms, patch_linear_layers)
 from basedxl_amd.unet import BasedXLUnet, patch_unet
-from basedxl_amd.unet_skeleton import BasicTransformerBlock, SDXLUNetSkeleton, TimestepEmbedding, fuse_epilogues, fuse_geglu_layers, fuse_kv_projections, synthetic_inputs
+from basedxl_amd.unet_skeleton import BasicTransformerBlock, SDXLUNetSkeleton, TimestepEmbedding, fuse_epilogues, fuse_geglu_layers, fuse_kv_projections, last_layer, synthetic_inputs
 from basedxl_amd.utils import BasedXLConfig
 
 SMALL = dict(channels=(64, 128, 256), head_dim=32, depths=(1, 2), cross_dim=96, add_time_dim=32)
@@ -380,3 +380,21 @@ def test_gradients_of_a_whole_block(gpu_device, what, kw, bound):
     want = grads(base.double().cpu(), x.double().cpu(), ctx.double().cpu(), dy.double().cpu())
     for name, g, w in zip(["y", "x", "context", *[n + "." + p for n in norms for p in ("weight", "bias")]], got, want):
         assert float((g.cpu().double() - w).norm() / w.norm()) <= bound, name
+
+
+@pytest.mark.gpu
+def test_sums_of_two_dtypes_are_promoted_as_torch_does(gpu_device):
+    """Under autocast the Linear layers of a block whose norms alone are patched give fp16, the residual stream stays fp32."""
+    torch.manual_seed(13)
+    base = BasicTransformerBlock(128, 4, 96).to(gpu_device).requires_grad_(False)
+    block = patch_layer_norms(copy.deepcopy(base))
+    x, ctx = torch.randn(2, 70, 128, device=gpu_device), torch.randn(2, 11, 96, device=gpu_device)
+    with torch.no_grad(), torch.autocast("cuda", torch.float16):
+        want, got = base(x, ctx), block(x, ctx)
+    assert got.dtype == want.dtype == torch.float32
+    # (the norms differ by fp32's half steps, which now and then turn a rounding to fp16 around: single half steps of it, far less in the mean square)
+    assert float((got - want).norm() / want.norm()) <= 2.0 ** -11
+    # an epilogue with a residual of another dtype
+    layer = linear(gpu_device, 64, 96, torch.float16)
+    a, r = torch.randn(5, 64, device=gpu_device).half(), torch.randn(5, 96, device=gpu_device)
+    assert torch.equal(last_layer(layer, a, r), r + layer(a)) and last_layer(layer, a, r).dtype == torch.float32
