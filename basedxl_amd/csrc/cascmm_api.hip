@@ -1193,10 +1193,11 @@ static int gemm_on_rows(int count, const void* const* A, const void* const* B, v
   const Epilogue& ep = *q.epi;
   // (the fp32 kernels' stores have 32-bit offsets over the rows of a tile)
   const bool near_rows = std::max({ep.residual ? ep.ldr : 0, ep.preact ? ep.ldp : 0, q.ldc}) <= INT32_MAX / (2 * 256 * 4);
-  // An LDS-tiled kernel of twelve waves has 168 registers a wave: with z kept as well its store spills (8192 x 640 x 640, two bf16 terms, us: residual 36.6 here,
-  // 38.5 as a pass behind it; gelu 35.4, 36.1; gelu and z 36.9, 36.1; silu, residual and z 43.3, 39.1)
+  // An LDS-tiled kernel of twelve waves has 168 registers a wave: with z kept as well its store spilled (8192 x 640 x 640, two bf16 terms, us: gelu and z 36.9, 36.1 as
+  // a pass behind it; silu, residual and z 43.3, 39.1), so it is compiled without z.  Without z (another card): residual 39.8, 42.2 as a pass, gelu 37.1, 38.6;
+  // 2048 x 640 x 1920 23.5, 28.8 and 22.0, 26.9; three fp16 terms 333 x 640 x 10240 43.5, 48.3 and 41.0, 46.8
   const bool tile = v.kind == KIND_TILE && !variant_info()[variant].bdirect && p.k_splits <= 1 &&
-                    tile_has_epilogue(v.iodt, v.fmt, v.terms, v.full != 0, v.fast) && !(ep.preact && v.threads >= 768);
+                    tile_has_epilogue(v.iodt, v.fmt, v.terms, v.full != 0, v.fast) && !(ep.preact && !tile_keeps_z(v.threads));
   if (v.kind == KIND_H16 || v.kind == KIND_HWK ||
       (near_rows && (tile || v.kind == KIND_F16K || v.kind == KIND_WAVEK || v.kind == KIND_SLOTK || v.kind == KIND_W512 || v.kind == KIND_W512E))) {
     p.epi = 1;

@@ -50,8 +50,9 @@ struct ColumnEpilogue {
 #pragma unroll
     for (int e = 0; e < R; ++e) r[e] = llvm_raw_buffer_load_f32(rr, (int)(base + (unsigned)((row + at(e)) * ldr)), 0, 0);
   }
-  template <int AUX, int R> __device__ __forceinline__ void store(float (&z)[R], const float (&r)[R], int row, int up, int col, bool inside) const {
-    if (pre) {
+  // (PRE: z may be wanted)
+  template <int AUX, bool PRE = true, int R> __device__ __forceinline__ void store(float (&z)[R], const float (&r)[R], int row, int up, int col, bool inside) const {
+    if (PRE && pre) {
       const unsigned base = inside ? (unsigned)(up * ldp + col * 4) : 0x7FFFFFFFu;
 #pragma unroll
       for (int e = 0; e < R; ++e) llvm_raw_buffer_store_f32(z[e], rp, (int)(base + (unsigned)((row + at(e)) * ldp)), 0, AUX);
@@ -69,10 +70,12 @@ struct ColumnEpilogue {
 
 // The store of the LDS-tiled kernels: blocks of permuted columns come in runs of RUN, block b of the tile and lane l31 <-> column 128 (b / 4) + 4 l31 + b % 4, so a
 // lane holds RUN adjacent columns of a row; the others are as above.  A quad of rows at a time, the next one's residual asked for before.
+// Without z in the kernels of twelve waves, which are not launched for it (tile_keeps_z).
 template <class TL>
 __device__ __forceinline__ void tile_epilogue(const GroupParams& p, float* C, const float* bias, int m0, int n0, int wm0, int wn0, int l31, int g,
                                               f32x16 (&res)[TL::MT][TL::NTL]) {
   constexpr int NQ = (TL::BNQ == 0) ? 0 : (TL::WN == 1 ? TL::BNQ / 32 : TL::NTL), RUN = (NQ % 4 == 0) ? 4 : 2;
+  constexpr bool PRE = tile_keeps_z(TL::NT);
   const EpilogueArgs args = epilogue_args(p);
   const ColumnEpilogue ep(args, C, p.ldc, p.M, p.N, m0 + wm0, n0);
   const bool vec = ((p.N | p.ldc | p.ldr | p.ldp) & 3) == 0 && (((uintptr_t)C | (uintptr_t)p.residual | (uintptr_t)p.preact) & 15) == 0;
@@ -120,7 +123,7 @@ __device__ __forceinline__ void tile_epilogue(const GroupParams& p, float* C, co
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int i = 0; i < RUN; ++i) z[e * RUN + i] = res[mi][r0 + i][4 * q + e] + bv[i];
-      if (ep.pre) {
+      if (PRE && ep.pre) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           run_t v;
@@ -152,7 +155,7 @@ __device__ __forceinline__ void tile_epilogue(const GroupParams& p, float* C, co
       float z[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) z[e] = res[mi][ni][e] + bv;
-      ep.store<kResultStoreAux>(z, r[b & 1], mi * 32, 4 * g, col, n0 + col < p.N);
+      ep.template store<kResultStoreAux, PRE>(z, r[b & 1], mi * 32, 4 * g, col, n0 + col < p.N);
     }
   }
 }

@@ -151,6 +151,8 @@ __device__ __forceinline__ i32x4 make_rsrc(const void* base, int64_t bytes) {
   return r;
 }
 
+// whether the store with an epilogue of a kernel of so many threads writes z too
+constexpr bool tile_keeps_z(int threads) { return threads < 768; }
 // (cascmm_column_epilogue.h)
 template <class TL>
 __device__ __forceinline__ void tile_epilogue(const GroupParams& p, float* C, const float* bias, int m0, int n0, int wm0, int wn0, int l31, int g,
