@@ -376,3 +376,61 @@ def test_gradients_of_rows_of_one_large_value(gpu_device, path, cols, dtype):
     assert bool((dw == 0).all())
     want = dy.double().sum(0)
     within(db, want, HALF[dtype] * want.abs() + 70 * U * dy.double().abs().sum(0) + TINY[dtype], "dbias")
+
+
+@pytest.mark.parametrize("dtype, wdtype", TYPES)
+@pytest.mark.parametrize("rows, cols", [(70000, 96), (20000, 457), (3000, 2500), (777, 9001), (50000, 3)])
+def test_gradients_of_weight_and_bias_alone(gpu_device, path, rows, cols, dtype, wdtype):
+    """No gradient of x: a thread a column sums over many rows."""
+    gen = torch.Generator().manual_seed(rows + cols)
+    x, dy = rows_of(gen, rows, cols, dtype, gpu_device), rows_of(gen, rows, cols, dtype, gpu_device)
+    w, b = ((1 + 0.2 * torch.randn(cols, generator=gen)).to(wdtype).to(gpu_device).requires_grad_() for _ in range(2))
+    dw, db = torch.autograd.grad(layer_norm(x, w, b), (w, b), dy)
+    _, _, _, xhat, e, _ = parts_of(x, w.detach(), b.detach(), 1e-5)
+    d, deep = dy.double(), 64 + rows // 16
+    for got, want, off, what in ((dw, (d * xhat).sum(0), deep * U * (d * xhat).abs().sum(0) + (d.abs() * e).sum(0), "dweight"), (db, d.sum(0), deep * U * d.abs().sum(0), "dbias")):
+        tol = HALF[wdtype] * want.abs() + TINY[wdtype] + off
+        # (a sum that rounds beyond the type's largest number is infinite: a computed one is within tol of it, so where |want| + tol is larger than that number it may be)
+        beyond = (got == want.sign() * math.inf) & (want.abs() + tol > torch.finfo(wdtype).max)
+        within(got[~beyond], want[~beyond], tol[~beyond], what)
+    (dw1,) = torch.autograd.grad(layer_norm(x, w, b.detach()), w, dy)
+    (db1,) = torch.autograd.grad(layer_norm(x, w.detach(), b), b, dy)
+    assert torch.equal(dw1, dw) and torch.equal(db1, db)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("cols", [3, 40, 457, 1280, 2500, 9001])
+def test_gradients_of_rows_with_infinities_and_nan(gpu_device, path, cols, dtype):
+    """They reach dx of their own rows, dbias of their own columns, and dweight where xhat or dy is one."""
+    gen = torch.Generator().manual_seed(cols)
+    rows = 300
+    x, r, dy, ds = (rows_of(gen, rows, cols, dtype, gpu_device) for _ in range(4))
+    w, b = rows_of(gen, 1, cols, dtype, gpu_device)[0], rows_of(gen, 1, cols, dtype, gpu_device)[0]
+
+    def grads(x, r, dy, ds):
+        leaves = [t.clone().requires_grad_() for t in (x, r, w, b)]
+        return torch.autograd.grad(add_layer_norm(*leaves), leaves, (dy, ds))
+
+    clean = grads(x, r, dy, ds)
+    last = cols - 1
+    for value in (math.inf, -math.inf, math.nan):
+        # in dy: its row of dx, its column of the sums
+        bad = dy.clone()
+        bad[17, last] = value
+        dx, dr, dw, db = grads(x, r, bad, ds)
+        other, column = torch.arange(rows, device=gpu_device) != 17, torch.arange(cols, device=gpu_device) != last
+        assert torch.equal(dx[other], clean[0][other]) and torch.equal(dr[other], clean[0][other]) and not bool(dx[17].isfinite().any())
+        assert torch.equal(dw[column], clean[2][column]) and torch.equal(db[column], clean[3][column])
+        assert not bool(dw[last].isfinite()) and (bool(db[last].isnan()) if math.isnan(value) else float(db[last]) == value)
+        # in ds: one element of dx
+        bad = ds.clone()
+        bad[17, last] = value
+        dx, _, dw, db = grads(x, r, dy, bad)
+        assert not bool(dx[17, last].isfinite())
+        dx[17, last] = clean[0][17, last]
+        assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), (clean[0], clean[2], clean[3])))
+        # in the sum: its row of dx, all of dweight, nothing of dbias
+        bad = x.clone()
+        bad[17, last] = value
+        dx, _, dw, db = grads(bad, r, dy, ds)
+        assert torch.equal(dx[other], clean[0][other]) and bool(dx[17].isnan().all()) and bool(dw.isnan().all()) and torch.equal(db, clean[3])

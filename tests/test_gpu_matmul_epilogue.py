@@ -587,3 +587,53 @@ def test_prepared_weights_of_any_depth_on_more_rows_than_one_copy_holds(gpu_devi
         S = a[m].double().abs() @ b.double().abs()
         tol = K * U * S + HALF[torch.float16] * want[m] + TINY[torch.float16]
         assert bool(((y[m::7].double() - want[m]).abs() <= tol).all()) and bool(((one[m].double() - want[m]).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_slopes_at_infinite_z(gpu_device, path, dtype):
+    """Their limits: one and zero; a NaN stays one (of relu, whose slope asks for z <= 0 only, it passes the gradient on)."""
+    z = torch.tensor([math.inf, -math.inf, math.nan] * 9, dtype=dtype, device=gpu_device)
+    none = torch.zeros(1, 0, dtype=dtype, device=gpu_device), torch.zeros(0, z.numel(), dtype=dtype, device=gpu_device)
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        leaf = z.clone().requires_grad_()
+        (g,) = torch.autograd.grad(cascaded_lowp_matmul_epilogue(*none, bias=leaf, activation=act).sum(), leaf)
+        g = g.double().view(9, 3)
+        assert bool(((g[:, 0] - 1).abs() <= 8 * U).all()) and bool((g[:, 1].abs() <= 8 * U).all()), act
+        assert bool((g[:, 2] == 1).all()) if act == "relu" else bool(g[:, 2].isnan().all()), act
+
+
+@pytest.mark.parametrize("cascade", CASCADES)
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_tanh", "silu"])
+def test_infinities_and_nan_in_gradients_stay_in_their_rows_and_columns(gpu_device, path, cascade, act):
+    dtype, options, _ = CASCADES[cascade]
+    if cascade == "fp32x3":
+        return      # (the scale of an operand is one for all its rows there)
+    a, b, bias, residual, dy = operands(140, 136, 72, dtype, gpu_device)
+
+    def grads(a, dy):
+        leaves = [t.clone().requires_grad_() for t in (a, b, bias, residual)]
+        return torch.autograd.grad(cascaded_lowp_matmul_epilogue(leaves[0], leaves[1], bias=leaves[2], activation=act, residual=leaves[3], **options), leaves, dy)
+
+    a[37] = a[37].abs()
+    z = a.double() @ b.double() + bias.double()
+    j = int(z[37].argmax())         # (where every activation has a slope)
+    assert float(z[37, j]) > 0.5
+    clean = grads(a, dy)
+    other, column = torch.arange(140, device=gpu_device) != 37, torch.arange(72, device=gpu_device) != j
+    for value in (math.inf, -math.inf, math.nan):
+        bad = dy.clone()
+        bad[37, j] = value
+        da, db, dbias, dr = grads(a, bad)
+        assert torch.equal(da[other], clean[0][other]) and not bool(da[37].isfinite().any())
+        assert torch.equal(db[:, column], clean[1][:, column]) and not bool(db[:, j].isfinite().any())
+        assert torch.equal(dbias[column], clean[2][column]) and not bool(dbias[j].isfinite())
+        assert torch.equal(dr[other], dy[other]) and torch.equal(dr[37][column], dy[37][column])
+    # a NaN in a: its row of z, so of dz where the activation has a slope; all of db's row of that input
+    bad = a.clone()
+    bad[37, 5] = math.nan
+    da, db, dbias, dr = grads(bad, dy)
+    assert torch.equal(da[other], clean[0][other]) and torch.equal(dr, dy) and bool(db[5].isnan().all())
+    if act in (None, "relu"):
+        assert bool(da[37].isfinite().all()) and bool(dbias.isfinite().all())
+    else:
+        assert bool(da[37].isnan().all()) and bool(dbias.isnan().all()) and bool(db.isnan().all())
