@@ -17,7 +17,7 @@ import torch.nn as nn
 from ..cascaded_lowp_matmul import (ChainedWeight, PreparedWeight, cascaded_lowp_matmul_chained, cascaded_lowp_matmul_glu_chained,
                                     chained_supported, glu_chained_worthwhile)
 from .geglu import BasedXLLowPGEGLU
-from .gradients import differentiated, gradient_of, with_gradient
+from .gradients import gradient_of, with_gradient
 from .lowp_linear import BasedXLLowPLinear
 
 
@@ -61,7 +61,7 @@ class BasedXLChainedFeedForward(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not self._chain_ok(x):
             return self.linear(self.geglu(x))
-        if differentiated(x):
+        if x.requires_grad and torch.is_grad_enabled():
             return with_gradient(self, x)
         dev = self.linear.weight.device
         if self._chained_weight is None or self._chained_weight.device != dev:

@@ -17,7 +17,7 @@ import torch.nn.functional as F
 from .. import _lib
 from ..cascaded_lowp_matmul import PreparedWeight, cascaded_lowp_matmul, cascaded_lowp_matmul_glu, default_cascade, gate_product, gated_variant
 from ..matmul_epilogue import cascaded_lowp_matmul_epilogue
-from .gradients import differentiated, gradient_of, with_gradient
+from .gradients import gradient_of, with_gradient
 
 
 class BasedXLLowPGEGLU(nn.Module):
@@ -86,7 +86,7 @@ class BasedXLLowPGEGLU(nn.Module):
             h = cascade_linear(x, self.weight, None, self.bias, self.lowp, self.terms, self.products, False, None)
             value, gate = h.chunk(2, dim=-1)
             return value * F.gelu(gate)
-        if differentiated(x):
+        if x.requires_grad and torch.is_grad_enabled():
             return with_gradient(self, x)
         pw = self._prepared
         if self.prepared and pw is not None and pw.device == self.weight.device and x.dtype == self.weight.dtype:

@@ -8,10 +8,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 
-def differentiated(x: torch.Tensor) -> bool:
-    return x.requires_grad and torch.is_grad_enabled()
-
-
 class _ConstantWeights(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, module):

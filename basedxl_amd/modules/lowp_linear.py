@@ -9,7 +9,7 @@ from typing import Optional
 from .. import _lib
 from ..cascaded_lowp_matmul import PreparedWeight, cascaded_lowp_matmul, default_cascade, raw_is_faster, tensor_scale_exp
 from ..matmul_epilogue import cascaded_lowp_matmul_epilogue
-from .gradients import differentiated, with_gradient
+from .gradients import with_gradient
 
 
 class BasedXLLowPLinear(nn.Module):
@@ -64,7 +64,7 @@ class BasedXLLowPLinear(nn.Module):
             from ..compiled import cascade_linear_epilogue
             return cascade_linear_epilogue(x, self.weight, None if pw is None else pw.slots, self.bias, residual, self.activation, self.lowp, self.terms,
                                            self.products, self._weight_exp if pw is None else pw.exp)
-        constant = not differentiated(x) and (residual is None or not differentiated(residual))
+        constant = not torch.is_grad_enabled() or not (x.requires_grad or (residual is not None and residual.requires_grad))
         if self.prepared and x.is_cuda and x.dtype == self.weight.dtype and constant and not raw_is_faster(
                 x.numel() // max(self.in_features, 1), self.in_features, self.out_features, x.dtype, self.lowp, self.terms, self.products):
             if pw is None or pw.device != self.weight.device:
@@ -92,7 +92,7 @@ class BasedXLLowPLinear(nn.Module):
             pw = self._prepared_weight
             return cascade_linear(x, self.weight, None if pw is None else pw.slots, self.bias, self.lowp, self.terms,
                                   self.products, False, self._weight_exp if pw is None else pw.exp)
-        if differentiated(x):
+        if x.requires_grad and torch.is_grad_enabled():
             return with_gradient(self, x)
         # the ordinary eager call in one native function; None: whatever is not ordinary about it is decided below
         pw, raw = self._prepared_weight, not self.prepared
