@@ -35,6 +35,19 @@ at::Tensor as_rows(const at::Tensor& t, int64_t& rows, int64_t& cols, int64_t& l
   return c;
 }
 
+// 16-bit operands off dwords: what the library copies of them beyond what cascmm_workspace_bytes counts, and copies made here where the library makes none (_copied_bytes
+// and _kernel_rows of matmul_epilogue.py)
+bool off_dwords(const at::Tensor& t, int64_t cols, int64_t ld, int unit) {
+  return t.element_size() == 2 && cols % unit == 0 && ((uintptr_t)t.const_data_ptr() % 4 != 0 || ld % 2 != 0);
+}
+int64_t copied_rows(const at::Tensor& a, int64_t M, int64_t K, int64_t lda) { return off_dwords(a, K, lda, 8) ? M * ((2 * K + 127) / 128 * 128) + 256 : 0; }
+int64_t copied_weight(const at::Tensor& b, int64_t K, int64_t N) { return off_dwords(b, N, N, 2) ? (K + 31) / 32 * 64 * N + 256 : 0; }
+at::Tensor kernel_rows(const at::Tensor& t, int64_t cols, int64_t& ld, bool copy) {
+  if (t.element_size() != 2 || (!copy && (ld == cols || ld * 2 * 512 < INT32_MAX))) return t;
+  ld = cols;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
 bool differentiated(std::initializer_list<const at::Tensor*> tensors) {
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : tensors)
@@ -211,14 +224,15 @@ struct EpilogueNode : torch::autograd::Function<EpilogueNode> {
     const at::Tensor bias = tensor_of(bias_in), residual = tensor_of(residual_in);
     int64_t M, K, lda, rows_r, cols_r, ldr = 0;
     rows_of(a, M, K, lda);
-    const int64_t N = b.size(1);
+    int64_t N = b.size(1), ldb = N;
+    const at::Tensor a_rows = kernel_rows(a, K, lda, copied_rows(a, M, K, lda) > INT32_MAX), b_rows = kernel_rows(b, N, ldb, copied_weight(b, K, N) > INT32_MAX);
     if (residual.defined()) rows_of(residual, rows_r, cols_r, ldr);
     at::Tensor out = result_like(a, N), preact, ws;
     if (act) preact = fresh({M, N}, a);
     const int dt = dtype_code(a);
-    const size_t need = workspace_need_anywhere({M, N, K, dt, (int)fmt, (int)terms, (int)products});
+    const size_t need = workspace_need_anywhere({M, N, K, dt, (int)fmt, (int)terms, (int)products}) + copied_rows(a_rows, M, K, lda) + copied_weight(b_rows, K, N);
     if (need) ws = scratch(need, a);
-    check(cascmm_gemm_epilogue(a.const_data_ptr(), b.const_data_ptr(), 0, out.data_ptr(), data_of(bias), data_of(residual), act ? preact.data_ptr() : nullptr, M, N, K, lda, N,
+    check(cascmm_gemm_epilogue(a_rows.const_data_ptr(), b_rows.const_data_ptr(), 0, out.data_ptr(), data_of(bias), data_of(residual), act ? preact.data_ptr() : nullptr, M, N, K, lda, N,
                                N, ldr, N, dt, (int)fmt, (int)terms, (int)products, (int)act, nullptr, need ? ws.data_ptr() : nullptr, need, stream_of(a)),
           "cascmm_gemm_epilogue");
     ctx->save_for_backward({a, b, preact});
@@ -257,6 +271,7 @@ struct EpilogueNode : torch::autograd::Function<EpilogueNode> {
       check(cascmm_epilogue_backward_operands(dy.const_data_ptr(), data_of(v[2]), slope ? dz.data_ptr() : nullptr, ptr(out[2]), a.const_data_ptr(), ptr(at), b.const_data_ptr(),
                                               ptr(bt), M, N, K, lddy, N, N, lda, M, N, K, act, dt, ptr(ws), ws.defined() ? ws.nbytes() : 0, stream),
             "cascmm_epilogue_backward_operands");
+      if (want_a || want_b) dz = kernel_rows(dz, N, lddz, off_dwords(dz, N, lddz, 2));
       if (want_a) {
         out[0] = fresh(v[0].sizes(), a);
         product(dz.const_data_ptr(), lddz, bt.const_data_ptr(), K, out[0], M, K, N, fmt, terms, products);
@@ -297,14 +312,17 @@ bool result_arguments(Product& p, int64_t N) {
     if (p.residual.size(d) != a.size(d)) return false;
   return true;
 }
-PyObject* run_product(const Product& p, const void* B, int prepared, int64_t N, int fmt, int terms, int products, int device) {
+// (copied: bytes of the workspace for a copy of B)
+PyObject* run_product(Product& p, const void* B, int prepared, int64_t copied, int64_t N, int fmt, int terms, int products, int device) {
   const hipStream_t stream = c10::hip::getCurrentHIPStream(device).stream();
   at::Tensor hold;
   void* ws;
   size_t ws_bytes;
-  if (!workspace_of(workspace_need({p.M, N, p.K, p.dt, fmt, terms, products}), device, stream, hold, ws, ws_bytes)) Py_RETURN_NONE;
+  const at::Tensor rows = kernel_rows(*p.a, p.K, p.lda, copied_rows(*p.a, p.M, p.K, p.lda) > INT32_MAX);
+  copied += copied_rows(rows, p.M, p.K, p.lda);
+  if (!workspace_of(workspace_need({p.M, N, p.K, p.dt, fmt, terms, products}) + copied, device, stream, hold, ws, ws_bytes)) Py_RETURN_NONE;
   at::Tensor out = result_like(*p.a, N);
-  const void *A = p.a->const_data_ptr(), *bias = data_of(p.bias), *residual = data_of(p.residual);
+  const void *A = rows.const_data_ptr(), *bias = data_of(p.bias), *residual = data_of(p.residual);
   void* C = out.data_ptr();
   int st;
   Py_BEGIN_ALLOW_THREADS
@@ -384,7 +402,9 @@ PyObject* epilogue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (fmt < 0 || terms < 1 || products < 0 || !result_arguments(p, N) || dual({b})) Py_RETURN_NONE;
     if (differentiated({p.a, b, &p.bias, &p.residual}))
       return THPVariable_Wrap(EpilogueNode::apply(*p.a, *b, optional_of(p.bias), optional_of(p.residual), (int64_t)p.act, (int64_t)fmt, (int64_t)terms, (int64_t)products));
-    return run_product(p, b->const_data_ptr(), 0, N, fmt, terms, products, device);
+    int64_t ldb = N;
+    const at::Tensor weight = kernel_rows(*b, N, ldb, copied_weight(*b, p.K, N) > INT32_MAX);
+    return run_product(p, weight.const_data_ptr(), 0, copied_weight(weight, p.K, N), N, fmt, terms, products, device);
   } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;
@@ -409,10 +429,10 @@ PyObject* epilogue_prepared(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
     if (p.dt == CASCMM_DT_F32) {
       if ((uintptr_t)p.a->const_data_ptr() % 16 != 0 || p.lda % 4 != 0) Py_RETURN_NONE;   // (the wrapper copies such rows)
       if (!(fmt == CASCMM_FMT_BF16 && terms == 2 && p.K % 8 == 0) && (p.K % 64 != 0 || N % 4 != 0)) Py_RETURN_NONE;
-    } else if (terms != 1 || fmt != (p.dt == CASCMM_DT_F16 ? CASCMM_FMT_FP16 : CASCMM_FMT_BF16)) {   // (rows of any alignment: the library copies what it has to)
+    } else if (terms != 1 || fmt != (p.dt == CASCMM_DT_F16 ? CASCMM_FMT_FP16 : CASCMM_FMT_BF16)) {   // (rows of any alignment)
       Py_RETURN_NONE;
     }
-    return run_product(p, slots->const_data_ptr(), 1, N, fmt, terms, products, device);
+    return run_product(p, slots->const_data_ptr(), 1, 0, N, fmt, terms, products, device);
   } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;

@@ -39,6 +39,31 @@ def _overlap(p: torch.Tensor, q: torch.Tensor) -> bool:
     return True
 
 
+_COPIES_END = 2 ** 31 - 1     # (the library's copies of operands stay below 2 GiB)
+
+
+def _off_dwords(t2: torch.Tensor, unit: int) -> bool:
+    """16-bit rows that start between dwords and whose length, a multiple of ``unit``, would not have the library count a copy of them anyway."""
+    return t2.element_size() == 2 and t2.shape[1] % unit == 0 and (t2.data_ptr() % 4 != 0 or (t2.shape[0] > 1 and t2.stride(0) % 2 != 0))
+
+
+def _copied_bytes(a2: torch.Tensor, b: Optional[torch.Tensor]) -> int:
+    """What the library copies of 16-bit operands off dwords: cascmm_workspace_bytes, which sees no addresses, does not count it, and without room for it the
+    kernels that read element by element would run, or not, as the stream's workspace has grown."""
+    (M, K), need = a2.shape, 0
+    if _off_dwords(a2, 8):
+        need += M * (-(-2 * K // 128) * 128) + 256
+    if b is not None and _off_dwords(b, 2):
+        need += -(-K // 32) * 64 * b.shape[1] + 256
+    return need
+
+
+def _kernel_rows(t2: torch.Tensor, copy: bool) -> torch.Tensor:
+    """``t2``, or a copy: if ``copy``, and of rows 2^21 16-bit (2^20 fp32) elements apart and more, which the offsets of the kernels do not span."""
+    far = t2.shape[0] > 1 and t2.stride(0) != t2.shape[1] and t2.stride(0) * t2.element_size() * 512 >= 2 ** 31 - 1
+    return t2.clone(memory_format=torch.contiguous_format) if copy or far else t2
+
+
 def _residual_rows(residual: torch.Tensor, M: int, N: int) -> Tuple[torch.Tensor, int]:
     """The residual (of the result's shape, expanded perhaps) as rows and their distance; 0: the same row for all."""
     if M > 1 and all(st == 0 or n == 1 for n, st in zip(residual.shape[:-1], residual.stride()[:-1])):
@@ -55,12 +80,16 @@ def _product(a2, b, bias, residual, preact, out2, activation, lowp, terms, produ
     N = b.N if prepared else b.shape[1]
     if M == 0 or N == 0:
         return
+    if a2.element_size() == 2 or prepared:
+        a2 = _kernel_rows(a2, _copied_bytes(a2, None) > _COPIES_END)
+    if not prepared and _off_dwords(b, 2) and _copied_bytes(a2, b) - _copied_bytes(a2, None) > _COPIES_END:
+        b = b.clone()
     dt, fmt, prod = _DTYPES[a2.dtype], _lib.FMT_BY_NAME[lowp], _lib.PROD_BY_NAME[products]
     dev, l = a2.device, _lib.lib()
     with torch.cuda.device(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream
         r2, ldr = (None, 0) if residual is None else _residual_rows(residual, M, N)
-        ws = _workspace(dev, stream, _workspace_bytes(M, N, K, dt, fmt, terms, prod))
+        ws = _workspace(dev, stream, _workspace_bytes(M, N, K, dt, fmt, terms, prod) + _copied_bytes(a2, None if prepared else b))
         exps = None
         if fmt == _lib.FMT_FP8:
             exps = torch.empty(2, dtype=torch.int32, device=dev)
@@ -117,6 +146,8 @@ class _EpilogueProduct(torch.autograd.Function):
                 dy2.data_ptr(), _ptr(preact), dz.data_ptr() if slope else None, _ptr(dbias), a2.data_ptr(), _ptr(at), b.data_ptr(), _ptr(bt), M, N, K, _ld(dy2), N, N,
                 _ld(a2), M, N, K, _lib.ACT_BY_NAME[activation], dt, _ptr(ws), 0 if ws is None else ws.numel(), torch.cuda.current_stream(dev).cuda_stream),
                 "cascmm_epilogue_backward_operands")
+            if (want_a or want_b) and dz.element_size() == 2:
+                dz = _kernel_rows(dz, _off_dwords(dz, 2))
             if want_a:
                 da = cascaded_lowp_matmul(dz, bt, lowp=lowp, terms=terms, products=products).reshape(a.shape)
             if want_b:
@@ -130,7 +161,8 @@ def cascaded_lowp_matmul_epilogue(a: torch.Tensor, b, *, bias: Optional[torch.Te
     """``activation(a @ b + bias) + residual``: :func:`cascaded_lowp_matmul` of ``a`` [..., K] and a 2-D ``b`` [K, N] (or a plain
     :class:`PreparedWeight`; of fp32 one whose K and N its kernels take, see ``usable_with``) with what follows a Linear layer.  ``activation``: None, "relu", "gelu" (erf), "gelu_tanh" or "silu", in fp32.
     ``residual``: of the result's dtype and of a shape that broadcasts to the result's.  ``lowp`` / ``terms`` / ``products`` / ``b_exp`` as there.
-    ``out``: [M, N] rows or the result's shape; it overlaps no operand.
+    ``out``: [M, N] rows or the result's shape; it overlaps no operand.  The result is rounded once; 16-bit tensors in another cascade than one term of
+    their own format, or with a raw weight beyond 2 GiB, have ``a @ b + bias`` rounded to their dtype on the way.
 
     Differentiable once in ``a``, ``b`` (a tensor: a prepared weight is a constant that no gradient passes through), ``bias`` and
     ``residual``; the gradients' products run with the cascade of the product itself, and sums over rows in a fixed order.  With an

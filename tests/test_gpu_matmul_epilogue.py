@@ -637,3 +637,61 @@ def test_infinities_and_nan_in_gradients_stay_in_their_rows_and_columns(gpu_devi
         assert bool(da[37].isfinite().all()) and bool(dbias.isfinite().all())
     else:
         assert bool(da[37].isnan().all()) and bool(dbias.isnan().all()) and bool(db.isnan().all())
+
+
+def off_dwords(t, how):
+    """The same values in rows that start between dwords, or lie too far apart for 32-bit offsets."""
+    M, N = t.shape
+    if how == "start":          # dense, one element off
+        v = torch.empty(M * N + 1, dtype=t.dtype, device=t.device)[1:].view(M, N)
+    elif how == "rows":         # odd distances
+        v = torch.full((M, N + 3), math.nan, dtype=t.dtype, device=t.device)[:, 2:2 + N]
+    else:
+        far = 2_200_000
+        v = torch.empty((M - 1) * far + N, dtype=t.dtype, device=t.device).as_strided((M, N), (far, 1))
+    v.copy_(t)
+    return v
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("how", ["start", "rows", "far"])
+@pytest.mark.parametrize("M, K, N", [(4, 8, 46), (85, 64, 1000), (300, 640, 320), (700, 72, 1700), (2, 5120, 64)])
+def test_rows_off_dwords_are_rounded_once_too(gpu_device, path, dtype, how, M, K, N):
+    """z is not rounded on its way to the result, whatever the rows: a residual that takes nearly all of z away shows it."""
+    a, b, bias, _, dy = operands(M, K, N, dtype, gpu_device)
+    pw = PreparedWeight(b)
+    b1 = off_dwords(b.view(1, -1), "start").view(K, N)
+    rows = off_dwords(a, how)
+    for act in ACTIVATIONS:
+        residual = -ACTIVATIONS[act](z_of(a, b, bias, dtype, 0.0)[0]).to(dtype)
+        for w in (b, b1, pw):
+            y = cascaded_lowp_matmul_epilogue(rows, w, bias=bias, activation=act, residual=residual)
+            check_forward(y, a, b, bias, act, residual, dtype, 0.0, f"{act} {type(w).__name__}", fused=True)
+        leaves = [t.detach().requires_grad_() for t in (rows, b1, bias, residual)]
+        y = cascaded_lowp_matmul_epilogue(leaves[0], leaves[1], bias=leaves[2], activation=act, residual=leaves[3])
+        check_forward(y, a, b, bias, act, residual, dtype, 0.0, f"{act} differentiated", fused=True)
+        grads = torch.autograd.grad(y, leaves, off_dwords(dy, "rows"))
+        check_backward(grads, dy, a, b, bias, act, residual, dtype, 0.0, f"{act}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_the_same_bits_whatever_the_workspace_has_grown_to(gpu_device, path, dtype):
+    # (a workspace of 10 MB by the library's own count, 26 MB of rows)
+    a, b, bias, residual, dy = operands(20000, 640, 64, dtype, gpu_device)
+    pw, rows, b1 = PreparedWeight(b), off_dwords(a, "rows"), off_dwords(b.view(1, -1), "start").view(640, 64)
+    big = torch.zeros(40_000, 1283, dtype=dtype, device=gpu_device), torch.zeros(1283, 64, dtype=dtype, device=gpu_device)
+
+    def calls():
+        leaf, wide = rows.detach().requires_grad_(), off_dwords(dy, "rows")
+        y = cascaded_lowp_matmul_epilogue(leaf, b1, bias=bias, residual=residual)
+        with torch.no_grad():
+            return [cascaded_lowp_matmul_epilogue(rows, w, bias=bias, activation="gelu", residual=residual) for w in (b, b1, pw)] + list(torch.autograd.grad(y, leaf, wide))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        before = calls()
+        cascaded_lowp_matmul(*big)         # (rows copied first: 100 MB of workspace on this stream)
+        after = calls()
+        torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(before, after))
