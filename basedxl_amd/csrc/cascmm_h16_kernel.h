@@ -589,7 +589,8 @@ __global__ __launch_bounds__(T::NT, 1) void cascmm_h16_kernel(const GroupParams 
             llvm_raw_buffer_store_v4f32(__builtin_bit_cast(f32x4, y), rc, offset(mi, gr, it, ldc), 0, 0);
           }
         } else {
-          // rows off 16-byte chunks, or too far apart for 32-bit offsets: an element a lane, eight of them at a time
+          // rows off 16-byte chunks, or too far apart for 32-bit offsets: an element a lane, eight of them at a time (8192 x 640 x 2556 fp16, gelu and
+          // residual, 162 us; 2560, by chunks, 50)
 #pragma unroll 1
           for (int i0 = lane; i0 < 32 * CB * 32; i0 += 8 * 64) {
             float v[8], r[8];
