@@ -398,3 +398,45 @@ def test_sums_of_two_dtypes_are_promoted_as_torch_does(gpu_device):
     layer = linear(gpu_device, 64, 96, torch.float16)
     a, r = torch.randn(5, 64, device=gpu_device).half(), torch.randn(5, 96, device=gpu_device)
     assert torch.equal(last_layer(layer, a, r), r + layer(a)) and last_layer(layer, a, r).dtype == torch.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_recorded_gradients_of_modules(gpu_device, dtype):
+    """Forward and backward through routed modules in a graph, replayed between eager work of their own."""
+    torch.manual_seed(14)
+    first, gated, conv = linear(gpu_device, 64, 96, dtype), BasedXLLowPGEGLU(nn.Linear(96, 128).to(device=gpu_device, dtype=dtype)), \
+        BasedXLLowPConv1x1(nn.Conv2d(64, 32, 1).to(device=gpu_device, dtype=dtype))
+    norm = BasedXLLayerNorm(nn.LayerNorm(64).to(device=gpu_device, dtype=dtype))
+
+    def step(x, dy, w, b):
+        norm.weight, norm.bias = w, b
+        h = gated(first(norm(x)))
+        y = conv(h.view(2, 5, 10, 64).permute(0, 3, 1, 2))
+        return (y, *torch.autograd.grad(y, (x, w, b), dy))
+
+    def inputs(seed):
+        gen = torch.Generator().manual_seed(seed)
+        r = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(gpu_device)   # noqa: E731
+        return [r(100, 64).requires_grad_(), r(2, 32, 5, 10), r(64).requires_grad_(), r(64).requires_grad_()]
+
+    norm.weight = norm.bias = None
+    side, ins = torch.cuda.Stream(), inputs(0)
+    ins = [nn.Parameter(t.detach()) if t.requires_grad else t for t in ins]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*ins)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*ins)
+    for seed in range(1, 5):
+        fresh = inputs(seed)
+        with torch.no_grad():
+            for t, f in zip(ins, fresh):
+                t.copy_(f)
+        graph.replay()
+        got = [t.detach().clone() for t in outs]
+        want = step(*[nn.Parameter(f.detach()) if f.requires_grad else f for f in fresh])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
