@@ -9,7 +9,7 @@ import ctypes
 import importlib
 import os
 import warnings
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p, POINTER
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcascmm.so")
@@ -80,6 +80,8 @@ SIGNATURES = {
     "cascmm_layer_norm": (c_int, [c_void_p] * 8 + [c_int64] * 6 + [c_float, c_int, c_int, c_void_p]),
     "cascmm_layer_norm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
     "cascmm_layer_norm_backward": (c_int, [c_void_p] * 9 + [c_int64] * 6 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "cascmm_gradients_workspace_bytes": (c_size_t, [c_int, c_void_p]),
+    "cascmm_clip_gradients": (c_int, [c_int, c_void_p, c_int, c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
     "cascmm_split_terms": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "cascmm_selftest": (c_int, []),
     "cascmm_strerror": (c_char_p, [c_int]),

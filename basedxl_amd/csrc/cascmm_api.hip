@@ -1824,6 +1824,7 @@ const char* cascmm_strerror(int status) {
     case CASCMM_ERR_LAUNCH: return "HIP launch failed";
     case CASCMM_ERR_BAD_VARIANT: return "kernel variant unknown or unable to run this problem";
     case CASCMM_ERR_TOO_LARGE: return "dimension too large";
+    case CASCMM_ERR_OVERLAP: return "a result shares memory with another result or with an operand";
     case CASCMM_ERR_SCRATCH_LIMIT: return "problem needs more scratch than the library's built-in buffer holds (use cascmm_gemm with a workspace)";
     default: return "unknown status";
   }

@@ -1,0 +1,128 @@
+"""The norm of a model's gradients taken together, and their clipping by it: what stands between the backward pass of the operators here and
+the step that uses their gradients.  (The reference, basedxl/unet.py:65-87, runs its model without gradients.)  Kernels:
+csrc/cascmm_gradients_kernel.h.
+"""
+from __future__ import annotations
+
+import math
+from array import array
+from typing import Iterable, Optional, Sequence, Union
+
+import torch
+
+from . import _lib
+from .cascaded_lowp_matmul import _DTYPES
+
+_NORM_TYPES = {1.0: 1, 2.0: 2, math.inf: 0}
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements of ``t``, in whatever order, fill a range of memory once."""
+    if t.is_contiguous():
+        return True
+    span = 1
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n != 1):
+        if stride != span:
+            return False
+        span *= size
+    return True
+
+
+def _check(gradients: Sequence[torch.Tensor], norm_type: float, name: str) -> int:
+    kind = _NORM_TYPES.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"{name}: norm_type must be 1, 2 or inf, got {norm_type}")
+    if not gradients:
+        raise ValueError(f"{name}: there are no gradients")
+    device = gradients[0].device
+    for i, g in enumerate(gradients):
+        if not g.is_cuda:
+            raise RuntimeError(f"{name}: gradient {i} is on {g.device}; the operator only runs on an AMD GPU (there is no CPU fallback)")
+        if g.device != device:
+            raise ValueError(f"{name}: gradient {i} is on {g.device} but the first on {device}")
+        if g.layout != torch.strided or g.dtype not in _DTYPES:
+            raise TypeError(f"{name}: gradient {i} must be a dense fp32, fp16 or bf16 tensor, got {g.layout} {g.dtype}")
+    return kind
+
+
+def _run(gradients, outs, kind: int, max_norm: float) -> torch.Tensor:
+    """One cascmm_clip_gradients over tensors that are dense, each like its result in shape and strides (``outs`` None: the norm alone)."""
+    device = gradients[0].device
+    table = array("q")
+    for i, g in enumerate(gradients):
+        code, out = _DTYPES[g.dtype], 0
+        if outs is not None:
+            out, code = outs[i].data_ptr(), code | _DTYPES[outs[i].dtype] << 32
+        table.extend((g.data_ptr(), out, g.numel(), code))
+    at, count, l = table.buffer_info()[0], len(gradients), _lib.lib()
+    with torch.cuda.device(device):
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        ws = torch.empty(l.cascmm_gradients_workspace_bytes(count, at), dtype=torch.uint8, device=device)   # (a temporary of the call)
+        _lib.check(l.cascmm_clip_gradients(count, at, kind, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(),
+                                           torch.cuda.current_stream(device).cuda_stream), "cascmm_clip_gradients")
+    return norm
+
+
+@torch.no_grad()
+def gradient_norm(gradients: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm (1, 2 or inf) of all elements of all ``gradients`` taken together, a device scalar in fp32; nothing waits for it.  fp32, fp16 and bf16
+    tensors of any strides on one GPU, the types mixed at will.  Squares and sums are fp64 in a fixed order: the same call gives the same bits."""
+    gradients = list(gradients)
+    kind = _check(gradients, norm_type, "gradient_norm")
+    return _run([g if _dense(g) else g.contiguous() for g in gradients], None, kind, 0.0)
+
+
+@torch.no_grad()
+def clip_gradients(gradients: Iterable[torch.Tensor], max_norm: float, *, norm_type: float = 2.0,
+                   out: Optional[Iterable[torch.Tensor]] = None) -> torch.Tensor:
+    """``g * min(1, max_norm / (norm + 1e-6))`` for every gradient, in place or into ``out`` (a tensor for each, of its shape and of its type or
+    fp32), and the norm of all of them together as :func:`gradient_norm` returns it.  Nothing waits for the GPU: the factor stays there, and gradients
+    in place that need no clipping are not written.  A NaN among the gradients makes all of them NaN; an infinity makes the factor 0 and itself NaN.  A result shares memory
+    with no other result and no gradient but its own (CascmmError): a tensor that is listed twice would be scaled twice."""
+    gradients = list(gradients)
+    kind = _check(gradients, norm_type, "clip_gradients")
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"clip_gradients: max_norm must be a number from 0 on, got {max_norm}")
+    results = gradients if out is None else list(out)
+    if len(results) != len(gradients):
+        raise ValueError(f"clip_gradients: {len(gradients)} gradients but {len(results)} results")
+    sources, targets, copied = [], [], []
+    for i, (g, o) in enumerate(zip(gradients, results)):
+        if o is not g:
+            if o.device != g.device or o.shape != g.shape or o.layout != torch.strided or o.dtype not in (g.dtype, torch.float32):
+                raise ValueError(f"clip_gradients: out[{i}] must be {tuple(g.shape)}, {g.dtype} or float32, on {g.device}, got {tuple(o.shape)} {o.dtype} on {o.device}")
+            if o.requires_grad and o.is_leaf:
+                raise ValueError(f"clip_gradients: out[{i}] is a leaf that requires a gradient")
+        if _dense(g) and (o is g or (_dense(o) and o.stride() == g.stride())):
+            sources.append(g)
+            targets.append(o)
+        else:   # (orders of elements that differ, or gaps between them: the scaled elements are put in place behind the call)
+            if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+                raise ValueError(f"clip_gradients: elements of result {i} share memory")
+            if any(o.data_ptr() == other.data_ptr() for k, other in enumerate(results) if k != i and other.numel() > 0) and o.numel() > 0:
+                raise ValueError(f"clip_gradients: result {i} shares memory with another")
+            sources.append(g.contiguous())
+            targets.append(torch.empty(g.shape, dtype=o.dtype, device=g.device))
+            copied.append((o, targets[-1]))
+    norm = _run(sources, targets, kind, max_norm)
+    for o, t in copied:
+        o.copy_(t)
+    torch.autograd.graph.increment_version([o for o in results if not o.is_inference()])   # (written behind autograd's back)
+    return norm
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` on this package's kernels: clips the ``grad`` of ``parameters`` in place and returns their norm.
+    ``error_if_nonfinite`` waits for the norm and raises before any gradient is touched."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    gradients = [p.grad for p in parameters if p.grad is not None]
+    if not gradients:
+        return torch.tensor(0.0)
+    if error_if_nonfinite:
+        norm = gradient_norm(gradients, norm_type)
+        if not math.isfinite(norm.item()):
+            raise RuntimeError(f"The total norm of order {norm_type} for gradients is non-finite, so it cannot be clipped: disable this error with error_if_nonfinite=False")
+    return clip_gradients(gradients, max_norm, norm_type=norm_type)

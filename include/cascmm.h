@@ -60,7 +60,8 @@ enum cascmm_status {
   CASCMM_ERR_LAUNCH = -7,        /* the HIP runtime refused the launch */
   CASCMM_ERR_BAD_VARIANT = -8,   /* forced kernel variant unknown or unable to run this problem */
   CASCMM_ERR_TOO_LARGE = -9,     /* a dimension exceeds 2^31 - 1 or a product overflows */
-  CASCMM_ERR_SCRATCH_LIMIT = -10 /* cascmm_gemm_noalloc: the problem needs more than CASCMM_NOALLOC_SCRATCH_BYTES */
+  CASCMM_ERR_SCRATCH_LIMIT = -10, /* cascmm_gemm_noalloc: the problem needs more than CASCMM_NOALLOC_SCRATCH_BYTES */
+  CASCMM_ERR_OVERLAP = -11       /* a result shares memory with another result or with an operand */
 };
 
 /*
@@ -381,6 +382,27 @@ int cascmm_layer_norm_backward(const void* dy, const void* ds, const void* x, co
                                const float* rstd, void* dx, void* dweight, void* dbias, int64_t rows, int64_t cols,
                                int64_t lddy, int64_t ldds, int64_t ldx, int64_t lddx, int dtype, int weight_dtype,
                                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The norm of many gradients taken together and their clipping by it, what stands between a backward pass and the step that uses it (no
+ * counterpart in the reference, which does not train):
+ *     norm = (sum over all elements of all tensors of |g|^p)^(1/p);   factor = min(1, max_norm / (norm + 1e-6));   out = g * factor
+ * norm_type: 1 and 2 are p, 0 is the largest |g|.  `gradients` is a HOST array, read during the call only: `elements` consecutive elements of
+ * `dtype` at `data`; `out`, of `out_dtype` (the gradient's own or fp32), is NULL in every entry (the norm alone is wanted) or in none with
+ * elements.  out == data clips in place (of the same type); otherwise results share memory with no gradient and no other result
+ * (CASCMM_ERR_OVERLAP).  *norm (device) receives the norm.  Sums are fp64 in a fixed order, results are rounded once; a NaN makes the norm and
+ * all results NaN, an infinity the norm infinite and the factor 0.  In place a factor of 1 writes nothing.  The workspace needs no initialisation
+ * and is 16-byte aligned; nothing is launched per tensor, and a recorded call replays on the same addresses.
+ */
+typedef struct cascmm_gradient {
+  const void* data;
+  void* out;
+  int64_t elements;
+  int32_t dtype, out_dtype;
+} cascmm_gradient;
+size_t cascmm_gradients_workspace_bytes(int count, const cascmm_gradient* gradients);
+int cascmm_clip_gradients(int count, const cascmm_gradient* gradients, int norm_type, double max_norm, float* norm,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* The operand split alone (a test hook for parity of the split with the CPU oracle):
  * out is fp32 [terms][n]; term i holds lowp(r_i * 2^(tensor_exp + shift*i)) upcast to fp32
