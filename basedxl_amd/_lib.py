@@ -82,6 +82,11 @@ SIGNATURES = {
     "cascmm_layer_norm_backward": (c_int, [c_void_p] * 9 + [c_int64] * 6 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "cascmm_gradients_workspace_bytes": (c_size_t, [c_int, c_void_p]),
     "cascmm_clip_gradients": (c_int, [c_int, c_void_p, c_int, c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cascmm_block_values_bytes": (c_size_t, [c_int64, c_int64]),
+    "cascmm_block_scales_bytes": (c_size_t, [c_int64, c_int64]),
+    "cascmm_block_round_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "cascmm_block_round": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_int] + [c_void_p] * 6 + [c_size_t, c_void_p]),
+    "cascmm_block_gemm": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_int, c_void_p]),
     "cascmm_split_terms": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "cascmm_selftest": (c_int, []),
     "cascmm_strerror": (c_char_p, [c_int]),

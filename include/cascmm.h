@@ -404,6 +404,29 @@ size_t cascmm_gradients_workspace_bytes(int count, const cascmm_gradient* gradie
 int cascmm_clip_gradients(int count, const cascmm_gradient* gradients, int norm_type, double max_norm, float* norm,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Products of operands held in 8-bit floating point (e4m3) with a power of two as the scale of each block of 128 (the layer's counterpart in the
+ * reference is basedxl/modules/lowp_linear.py:7-20):
+ *     C[m][n] = sum over blocks of k of 2^(ea + eb) * sum over the block of qa[m][k] qb[n][k]   (+ bias[n])
+ * A held operand is `values`, bytes [rows][k rounded up to 128] with zeros behind k, and `scales`, bytes [blocks / 4, rounded up][rows][4]: block i of row r has the
+ * scale 2^(byte - 127) of byte [i / 4][r][i % 4]; cascmm_block_values_bytes and cascmm_block_scales_bytes are their sizes.
+ * cascmm_block_round rounds x [rows, cols] (leading dimension ldx): `values` with blocks of 128 along a row's columns, and / or `values_t`, x transposed, with blocks of 128
+ * along a column's rows; square != 0: one scale for every 128 x 128 elements in both.  The scale of a block is the smallest power of two, from 2^-127 on, with
+ * max|x| <= 448 * 2^e over its finite elements (1 where those are zeros or none); the quotient, which is exact, is rounded to nearest, ties to even; infinities
+ * and NaN become NaN.  `sums` (NULL, or [cols] of `dtype`): sums over the rows of x itself, in fp32 in a fixed order, for which the workspace (16-byte
+ * aligned, no initialisation) holds cascmm_block_round_workspace_bytes.  values and values_t are 16-byte aligned.
+ * cascmm_block_gemm: a [M rows][K], b [N rows][K], C [M, N] (leading dimension ldc) and bias (NULL or [N]) of `dtype`.  16-bit results come from the 8-bit matrix
+ * instruction, fp32 results from the 16-bit one on the same values, with fp32's accuracy (rounded elements below 2^-126 count as zeros).  K up to 2^22.
+ */
+size_t cascmm_block_values_bytes(int64_t rows, int64_t k);
+size_t cascmm_block_scales_bytes(int64_t rows, int64_t k);
+size_t cascmm_block_round_workspace_bytes(int64_t rows, int64_t cols);
+int cascmm_block_round(const void* x, int64_t rows, int64_t cols, int64_t ldx, int dtype, int square, void* values,
+                       void* scales, void* values_t, void* scales_t, void* sums, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int cascmm_block_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, void* C, const void* bias,
+                      int64_t M, int64_t N, int64_t K, int64_t ldc, int dtype, void* stream);
+
 /* The operand split alone (a test hook for parity of the split with the CPU oracle):
  * out is fp32 [terms][n]; term i holds lowp(r_i * 2^(tensor_exp + shift*i)) upcast to fp32
  * with r_0 = x, r_{i+1} = r_i - t_i / 2^(tensor_exp + shift*i); shift = 0 / 11 / 4 for
