@@ -3,6 +3,7 @@ from .cascaded_lowp_matmul import (cascaded_lowp_matmul, cascaded_lowp_matmul_gr
                                    cascaded_lowp_matmul_prepared, PreparedWeight, tensor_scale_exp,
                                    LeftSlots, ChainedWeight, cascaded_lowp_matmul_chained, cascaded_lowp_matmul_glu_chained)
 from .block_scaled import BlockScaledWeight, block_scaled_matmul  # noqa: F401
+from .gated_norm import gated_add_norm  # noqa: F401
 from .gradient_clip import clip_grad_norm_, clip_gradients, gradient_norm  # noqa: F401
 from .layer_norm import add_layer_norm, layer_norm  # noqa: F401
 from .matmul_epilogue import cascaded_lowp_matmul_epilogue  # noqa: F401
@@ -14,5 +15,5 @@ __all__ = ["cascaded_lowp_matmul", "cascaded_lowp_matmul_grouped", "cascaded_low
            "BasedXLChainedFeedForward", "chain_feed_forward_layers",
            "BasedXLLowPLinear", "BasedXLLowPConv1x1", "BasedXLLowPGEGLU", "BasedXLFusedKV",
            "patch_linear_layers", "patch_pointwise_convs", "layer_norm", "add_layer_norm", "cascaded_lowp_matmul_epilogue",
-           "BasedXLLayerNorm", "patch_layer_norms", "BlockScaledWeight", "block_scaled_matmul", "gradient_norm",
+           "BasedXLLayerNorm", "patch_layer_norms", "gated_add_norm", "BlockScaledWeight", "block_scaled_matmul", "gradient_norm",
            "clip_gradients", "clip_grad_norm_"]

@@ -80,6 +80,9 @@ SIGNATURES = {
     "cascmm_layer_norm": (c_int, [c_void_p] * 8 + [c_int64] * 6 + [c_float, c_int, c_int, c_void_p]),
     "cascmm_layer_norm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
     "cascmm_layer_norm_backward": (c_int, [c_void_p] * 9 + [c_int64] * 6 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "cascmm_gated_norm_forward": (c_int, [c_void_p, c_void_p]),
+    "cascmm_gated_norm_workspace_bytes": (c_size_t, [c_void_p]),
+    "cascmm_gated_norm_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "cascmm_gradients_workspace_bytes": (c_size_t, [c_int, c_void_p]),
     "cascmm_clip_gradients": (c_int, [c_int, c_void_p, c_int, c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
     "cascmm_block_values_bytes": (c_size_t, [c_int64, c_int64]),
@@ -92,6 +95,16 @@ SIGNATURES = {
     "cascmm_strerror": (c_char_p, [c_int]),
     "cascmm_version": (c_int, []),
 }
+
+
+class GatedNorm(ctypes.Structure):
+    """cascmm_gated_norm of include/cascmm.h."""
+    _fields_ = ([(name, c_void_p) for name in ("x", "residual", "gate", "scale", "post_weight", "post_bias", "weight", "bias", "y", "sum", "stats", "dy", "ds", "dx",
+                                               "dresidual", "dgate", "dscale", "dpost_weight", "dpost_bias", "dweight", "dbias")]
+                + [(name, c_int64) for name in ("rows", "cols", "group_rows", "ldx", "ldr", "ldy", "lds", "lddy", "ldds", "lddx", "lddr", "gate_ld", "scale_ld",
+                                                "weight_ld", "bias_ld")]
+                + [(name, c_double) for name in ("residual_scale", "eps")]
+                + [(name, c_int32) for name in ("norm", "post", "dtype", "weight_dtype")])
 
 
 class CascmmError(RuntimeError):

@@ -384,6 +384,38 @@ int cascmm_layer_norm_backward(const void* dy, const void* ds, const void* x, co
                                void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * The norms on both sides of a block's residual add, with the add, its gate and the residual's scale (a transformer block's counterpart in the model that
+ * the reference wraps at basedxl/unet.py:65-87 is torch's):
+ *     p = norm(x) post_weight + post_bias with `post`, else x;   s = scale * residual + gate * p, rounded to `dtype`;   y = norm(s) weight + bias
+ *     norm(v) = (v - mean) / sqrt(var + eps) (CASCMM_NORM_LAYER) or v / sqrt(mean of v^2 + eps) (CASCMM_NORM_RMS), over a row
+ * Tensors are [rows, cols] with leading dimensions in elements.  gate, scale, weight and bias are one row of [cols] (leading dimension 0) or one for each group_rows
+ * consecutive rows (rows is a multiple of group_rows); post_weight and post_bias one row; all of weight_dtype (`dtype` or fp32), NULL: ones, for a bias zeros,
+ * for scale residual_scale.  stats: fp32 [4][rows] for the backward pass, or NULL.  Statistics and everything between a load and a store are fp32,
+ * each result is rounded once; y and sum overlap no operand.
+ * Backward, from the gradients dy of y and ds of s (NULL: zeros): dx, dresidual, and of those operands that are there dgate, dscale, dpost_weight, dpost_bias, dweight and
+ * dbias, [cols] or, where the operand's leading dimension is not 0, [groups][cols]; each NULL if it is not wanted.  It reads sum and stats of the forward pass, x with
+ * `post` or a gate, residual with a scale.  Sums over rows are fp32 in a fixed order, without atomics.  The workspace (16-byte aligned, no initialisation) holds
+ * cascmm_gated_norm_workspace_bytes: five rows of sums for each of up to 1024 workgroups, and at least one workgroup to a group.
+ * The struct is read during the call only.
+ */
+typedef enum cascmm_norm_kind { CASCMM_NORM_LAYER = 0, CASCMM_NORM_RMS = 1 } cascmm_norm_kind;
+typedef struct cascmm_gated_norm {
+  const void *x, *residual, *gate, *scale, *post_weight, *post_bias, *weight, *bias;
+  void *y, *sum;
+  float* stats;
+  const void *dy, *ds;
+  void *dx, *dresidual, *dgate, *dscale, *dpost_weight, *dpost_bias, *dweight, *dbias;
+  int64_t rows, cols, group_rows;
+  int64_t ldx, ldr, ldy, lds, lddy, ldds, lddx, lddr;
+  int64_t gate_ld, scale_ld, weight_ld, bias_ld;
+  double residual_scale, eps;
+  int32_t norm, post, dtype, weight_dtype;
+} cascmm_gated_norm;
+int cascmm_gated_norm_forward(const cascmm_gated_norm* args, void* stream);
+size_t cascmm_gated_norm_workspace_bytes(const cascmm_gated_norm* args);
+int cascmm_gated_norm_backward(const cascmm_gated_norm* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * The norm of many gradients taken together and their clipping by it, what stands between a backward pass and the step that uses it (no
  * counterpart in the reference, which does not train):
  *     norm = (sum over all elements of all tensors of |g|^p)^(1/p);   factor = min(1, max_norm / (norm + 1e-6));   out = g * factor
