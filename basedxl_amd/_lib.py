@@ -90,6 +90,8 @@ SIGNATURES = {
     "cascmm_block_round_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "cascmm_block_round": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_int] + [c_void_p] * 6 + [c_size_t, c_void_p]),
     "cascmm_block_gemm": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_int, c_void_p]),
+    "cascmm_block_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "cascmm_block_linear": (c_int, [c_void_p] * 5 + [c_int64] * 5 + [c_int, c_void_p, c_size_t, c_void_p]),
     "cascmm_split_terms": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "cascmm_selftest": (c_int, []),
     "cascmm_strerror": (c_char_p, [c_int]),

@@ -169,7 +169,11 @@ def block_scaled_matmul(a: torch.Tensor, b, *, bias: Optional[torch.Tensor] = No
     out = torch.empty(*a.shape[:-1], N, dtype=a.dtype, device=a.device)
     if out.numel() == 0:
         return out
-    left = _round(a2, False, True, False)[0]
+    (M, _), dev, l = a2.shape, a2.device, _lib.lib()
     right = (b.values, b.scales) if held else _round_weight(b, True, False)[0]
-    _multiply(left, right, out.view(a2.shape[0], N), bias, K)
+    with torch.cuda.device(dev):
+        need = l.cascmm_block_linear_workspace_bytes(M, K, _DTYPES[a.dtype])
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None      # (a temporary of the call)
+        _lib.check(l.cascmm_block_linear(a2.data_ptr(), right[0].data_ptr(), right[1].data_ptr(), out.data_ptr(), _ptr(bias), M, N, K, _ld(a2), N, _DTYPES[a.dtype], _ptr(ws), need,
+                                         torch.cuda.current_stream(dev).cuda_stream), "cascmm_block_linear")
     return out

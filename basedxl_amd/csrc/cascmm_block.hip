@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "cascmm_norm_kernel.h"
+#include "cascmm_variants.h"
 
 namespace cascmm {
 
@@ -21,14 +22,63 @@ template <int IODT> static hipError_t block_round(const BlockRoundParams& p, boo
   return err;
 }
 
-template <int IODT, int MT, int NT> static hipError_t block_gemm(BlockGemmParams p, hipStream_t s) {
+// The tiles: estimated microseconds from what was measured (us, 8192 x 8192 x 8192 bf16 / 2048 x 10240 x 1280 / 1024 x 1280 x 5120 / 154 x 5120 x 1280): 256 x 256 on eight waves, one
+// workgroup on a CU, 394 / 37.2 / 48.6 / 15.6; 128 x 128, two on a CU, so that one's stores hide behind the other's products, 486 / 35.2 / 31.1 / 8.2; 128 x 64, three stages
+// deep, 640 / 46.2 / 17.9 / 7.3; 64 x 64 821 / 53.6 / 23.5 / 6.1; 64 x 64 with k dealt to two groups of waves, four stages deep, 989 / 97.8 / 24.2 / 6.4, and for 640 x 640 x 8192 17.1 where
+// the others take 70, 41, 24 and 34.  `t`: of a block of k, `o`: of a tile's beginning and end, of the tiles that fall to a CU.
+typedef BlockTile<2, 2, 1, 1, 2, 1> BlockTile64;
+typedef BlockTile<2, 2, 1, 1, 4, 2> BlockTile64Shares;
+typedef BlockTile<2, 2, 2, 1, 3, 1> BlockTile128x64;
+typedef BlockTile<2, 2, 2, 2, 2, 1> BlockTile128;
+typedef BlockTile<2, 4, 4, 2, 2, 1> BlockTile256;
+enum { kTile64, kTile64Shares, kTile128x64, kTile128, kTile256, kTiles };
+static int block_tile(int64_t M, int64_t N, int64_t blocks, bool fine) {
+  const auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  const double k = (double)blocks;
+  double cost[kTiles];
+  const int64_t small = tiles(64, 64), n64 = (small + 255) / 256, n128x64 = (tiles(128, 64) + 255) / 256, n128 = (tiles(128, 128) + 255) / 256, t256 = tiles(256, 256), n256 = (t256 + 255) / 256;
+  cost[kTile64] = std::max(n64 * (0.22 * k + 0.9), 0.3 * k + 1.0);
+  cost[kTile64Shares] = n64 * (0.23 * k + 1.9);
+  cost[kTile128x64] = n128x64 <= 1 ? 0.36 * k + 1.2 : n128x64 * (0.31 * k + 1.0);
+  cost[kTile128] = n128 <= 1 ? 0.62 * k + 1.5 : n128 * (0.45 * k + 1.5);
+  cost[kTile256] = n256 * ((t256 <= 128 ? 1.05 : t256 <= 256 ? 1.2 : 1.45) * k + 3.5);
+  int best = kTile64;
+  for (int i = 0; i < kTiles; ++i)
+    if (cost[i] < cost[best] && !(fine && i == kTile256)) best = i;     // (widened fragments do not fit beside 128 x 64 sums of a wave)
+  return best;
+}
+
+template <int IODT, typename T> static hipError_t block_gemm_tile(BlockGemmParams p, hipStream_t s) {
   hipError_t err = hipSuccess;
-  constexpr int BM = 64 * MT, BN = 64 * NT, LDS = 2 * (BM + BN) * 128;
-  p.tiles_m = (p.M + BM - 1) / BM;
-  p.tiles_n = (p.N + BN - 1) / BN;
-  CASCMM_LAUNCH(err, (cascmm_block_gemm_kernel<IODT, MT, NT, IODT == CASCMM_DT_F32>), dim3((unsigned)p.tiles_m * (unsigned)p.tiles_n), dim3(256), LDS, s, p);
+  constexpr bool FINE = IODT == CASCMM_DT_F32;
+  static LdsFlags done;
+  if (T::LDS > 64 * 1024 && !ensure_lds((const void*)cascmm_block_gemm_kernel<IODT, T, FINE>, T::LDS, done)) return hipErrorInvalidValue;
+  p.tiles_m = (p.M + T::BM - 1) / T::BM;
+  p.tiles_n = (p.N + T::BN - 1) / T::BN;
+  CASCMM_LAUNCH(err, (cascmm_block_gemm_kernel<IODT, T, FINE>), dim3((unsigned)p.tiles_m * (unsigned)p.tiles_n), dim3(T::THREADS), T::LDS, s, p);
   return err;
 }
+template <int IODT> static hipError_t block_gemm(const BlockGemmParams& p, hipStream_t s) {
+  constexpr bool FINE = IODT == CASCMM_DT_F32;
+  switch (block_tile(p.M, p.N, p.blocks, FINE)) {
+    case kTile64: return block_gemm_tile<IODT, BlockTile64>(p, s);
+    case kTile64Shares: return block_gemm_tile<IODT, BlockTile64Shares>(p, s);
+    case kTile128x64: return block_gemm_tile<IODT, BlockTile128x64>(p, s);
+    case kTile128: return block_gemm_tile<IODT, BlockTile128>(p, s);
+    default:
+      if constexpr (!FINE) return block_gemm_tile<IODT, BlockTile256>(p, s);
+      return hipErrorInvalidValue;
+  }
+}
+
+template <int IODT> static hipError_t block_rows(const BlockRowsParams& p, hipStream_t s) {
+  hipError_t err = hipSuccess;
+  CASCMM_LAUNCH(err, (cascmm_block_rows_kernel<IODT, 16>), dim3((unsigned)(p.N + 15) / 16), dim3(1024), 0, s, p);
+  return err;
+}
+// (fp32 results come from the 16-bit instruction, which the kernel of few rows does not use)
+static bool block_few_rows(int64_t M, int64_t K, int dtype) { return M <= 16 && K > 0 && dtype != CASCMM_DT_F32; }
+static size_t block_slice(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace cascmm
 
@@ -100,16 +150,51 @@ int cascmm_block_gemm(const void* a, const void* a_scales, const void* b, const 
   const size_t es = block_size(dtype);
   if (!block_aligned(C, es) || !block_aligned(bias, es) || !block_aligned(a, 16) || !block_aligned(b, 16) || !block_aligned(a_scales, 4) || !block_aligned(b_scales, 4))
     return CASCMM_ERR_ALIGNMENT;
-  if ((M + 127) / 128 * ((N + 127) / 128) > (1 << 24) - 1) return CASCMM_ERR_TOO_LARGE;
+  if ((M + 63) / 64 * ((N + 63) / 64) > (1 << 22) - 1) return CASCMM_ERR_TOO_LARGE;      // (a launch has fewer than 2^32 threads)
   BlockGemmParams p;
   memset(&p, 0, sizeof(p));
   p.a = (const unsigned char*)a; p.b = (const unsigned char*)b; p.sa = (const unsigned*)a_scales; p.sb = (const unsigned*)b_scales;
   p.c = C; p.bias = bias; p.ldc = ldc;
   p.M = (int)M; p.N = (int)N; p.blocks = (int)(block_padded(K) / kBlock);
   const hipStream_t s = (hipStream_t)stream;
-  const hipError_t err = dtype == CASCMM_DT_F32   ? block_gemm<CASCMM_DT_F32, 2, 2>(p, s)
-                         : dtype == CASCMM_DT_F16 ? block_gemm<CASCMM_DT_F16, 2, 2>(p, s)
-                                                  : block_gemm<CASCMM_DT_BF16, 2, 2>(p, s);
+  const hipError_t err = dtype == CASCMM_DT_F32   ? block_gemm<CASCMM_DT_F32>(p, s)
+                         : dtype == CASCMM_DT_F16 ? block_gemm<CASCMM_DT_F16>(p, s)
+                                                  : block_gemm<CASCMM_DT_BF16>(p, s);
+  return err == hipSuccess ? CASCMM_OK : CASCMM_ERR_LAUNCH;
+}
+
+size_t cascmm_block_linear_workspace_bytes(int64_t M, int64_t K, int dtype) {
+  if (M < 0 || K < 0 || M > INT32_MAX || K > kBlockMostK || !block_dtype(dtype) || block_few_rows(M, K, dtype)) return 0;
+  return block_slice((size_t)(M * block_padded(K))) + (size_t)block_scale_bytes(M, K);
+}
+
+int cascmm_block_linear(const void* x, const void* b, const void* b_scales, void* C, const void* bias, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldc, int dtype,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (!block_dtype(dtype)) return CASCMM_ERR_BAD_DTYPE;
+  if (M < 0 || N < 0 || K < 0 || ldx < K || ldc < N) return CASCMM_ERR_BAD_SHAPE;
+  if (M > INT32_MAX || N > INT32_MAX || K > kBlockMostK) return CASCMM_ERR_TOO_LARGE;
+  if (M == 0 || N == 0) return CASCMM_OK;
+  if (!block_few_rows(M, K, dtype)) {
+    if (!workspace && M * K > 0) return CASCMM_ERR_WORKSPACE;
+    if (workspace_bytes < cascmm_block_linear_workspace_bytes(M, K, dtype)) return CASCMM_ERR_WORKSPACE;
+    if (!block_aligned(workspace, 16)) return CASCMM_ERR_ALIGNMENT;
+    void* const scales = (char*)workspace + block_slice((size_t)(M * block_padded(K)));
+    // (everything is checked before the first launch: the product's own checks see the same arguments)
+    if (!C || (K > 0 && (!x || !b || !b_scales))) return CASCMM_ERR_NULL_POINTER;
+    if ((M + 63) / 64 * ((N + 63) / 64) > (1 << 22) - 1) return CASCMM_ERR_TOO_LARGE;
+    if (!block_aligned(C, block_size(dtype)) || !block_aligned(bias, block_size(dtype)) || !block_aligned(b, 16) || !block_aligned(b_scales, 4)) return CASCMM_ERR_ALIGNMENT;
+    const int st = K > 0 ? cascmm_block_round(x, M, K, ldx, dtype, 0, workspace, scales, nullptr, nullptr, nullptr, nullptr, 0, stream) : (int)CASCMM_OK;
+    return st != CASCMM_OK ? st : cascmm_block_gemm(workspace, scales, b, b_scales, C, bias, M, N, K, ldc, dtype, stream);
+  }
+  if (!C || !x || !b || !b_scales) return CASCMM_ERR_NULL_POINTER;
+  const size_t es = block_size(dtype);
+  if (!block_aligned(C, es) || !block_aligned(bias, es) || !block_aligned(x, es) || !block_aligned(b, 16) || !block_aligned(b_scales, 4)) return CASCMM_ERR_ALIGNMENT;
+  if ((N + 15) / 16 > (1 << 22) - 1) return CASCMM_ERR_TOO_LARGE;
+  BlockRowsParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = x; p.b = (const unsigned char*)b; p.sb = (const unsigned*)b_scales; p.c = C; p.bias = bias; p.ldx = ldx; p.ldc = ldc;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K; p.blocks = (int)(block_padded(K) / kBlock);
+  const hipError_t err = dtype == CASCMM_DT_F16 ? block_rows<CASCMM_DT_F16>(p, (hipStream_t)stream) : block_rows<CASCMM_DT_BF16>(p, (hipStream_t)stream);
   return err == hipSuccess ? CASCMM_OK : CASCMM_ERR_LAUNCH;
 }
 

@@ -185,50 +185,80 @@ __device__ __forceinline__ void block_load_lds(__amdgpu_buffer_rsrc_t rsrc, unsi
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (block_lds_ptr)dst, 16, voffset, soffset, 0, 0);
 }
 
-// 2 x 2 waves, each MT x NT blocks of 32 x 32.  A stage is one block of k: rows of 128 bytes in LDS, the eight 16-byte pieces of row r in the order i ^ (r % 8), so that
-// the lanes of a fragment read, 32 rows apart by 128 bytes, hit all banks.  The copy to LDS writes in order; the order is made by the addresses it reads.
+// WM x WN waves, each MT x NT blocks of 32 x 32.  A stage is one block of k: rows of 128 bytes in LDS, the eight 16-byte pieces of row r in the order i ^ (r % 8), so that
+// the lanes of a fragment read, 32 rows apart by 128 bytes, hit all banks, and the rows' scales of the block's four.  The copy to LDS writes in order; the order is made by the
+// addresses it reads.
+// A stage is multiplied in two halves of 64 k.  The fragments of one half are read behind the matrix instructions of the other, so that no wave waits for LDS: behind the first
+// half's the second's; then the barrier, which the stage has been read in front of and the next one has landed at; behind the second half's instructions the next stage's first
+// fragments, and the loads of the stage DEEP on, into the place of the one just read: they have DEEP - 1 stages' instructions to land.
+// SHARES: the blocks of k are dealt to as many groups of WM x WN waves, each with stages of its own, for few tiles and a long k; their sums meet in LDS, in order.
 // FINE: products and sums by the 16-bit matrix instruction, to fp32's accuracy.  The 8-bit one cuts the products inside an instruction at about 2^-15 of the largest: 1.5e-5
 // of the result's size, unbiased and the same for every depth, which 16-bit results do not show and fp32 ones would.  (bf16 holds the scaled values exactly, but for those
 // below 2^-126, which the instruction takes as zeros.)
-template <int IODT, int MT, int NT, bool FINE>
-__global__ __launch_bounds__(256) void cascmm_block_gemm_kernel(const BlockGemmParams p) {
+constexpr int block_waitcnt(int vm, int lgkm) { return 0x70 | (vm & 15) | (vm >> 4) << 14 | lgkm << 8; }
+template <int WM_, int WN_, int MT_, int NT_, int DEEP_, int SHARES_> struct BlockTile {
+  static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, DEEP = DEEP_, SHARES = SHARES_, WAVES = WM * WN, THREADS = 64 * WAVES * SHARES;
+  static constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, ROWS = BM + BN;
+  static constexpr int STAGE = ROWS * 132, LDS = DEEP * STAGE * SHARES, BAND = BM >= 256 ? 4 : 8;
+  static constexpr int LOADS = ROWS / 8 / WAVES, SCALES = (ROWS / 64 + WAVES - 1) / WAVES;    // a wave's, of a stage: 1 KB (256 bytes) each
+  static_assert(ROWS % (8 * WAVES) == 0 && ROWS % 64 == 0 && BM % 64 == 0 && LDS <= 160 * 1024, "tile");
+};
+
+// Workgroup w runs on die w % 8, each with a cache of its own: a die takes tiles that follow each other, in bands of `band` tiles down and all the way across, so that those at work
+// at a time share rows of both operands
+__device__ __forceinline__ void block_place(unsigned w, int tiles_m, int tiles_n, int band, int& tile_m, int& tile_n) {
+  const unsigned total = gridDim.x, die = w & 7u, each = total >> 3, more = total & 7u;
+  const unsigned id = die * each + (die < more ? die : more) + (w >> 3);
+  const unsigned across = (unsigned)band * (unsigned)tiles_n, which = id / across, in = id % across;
+  const unsigned down = (unsigned)tiles_m - which * band < (unsigned)band ? (unsigned)tiles_m - which * band : (unsigned)band;    // (the last band may be lower)
+  tile_m = (int)(which * band + in % down);
+  tile_n = (int)(in / down);
+}
+
+template <int IODT, typename T, bool FINE>
+__global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const BlockGemmParams p) {
   typedef typename IoType<IODT>::T E;
-  constexpr int BM = 64 * MT, BN = 64 * NT, STAGE = (BM + BN) * 128, LOADS = (BM + BN) / 8 / 4;
+  constexpr int MT = T::MT, NT = T::NT, BM = T::BM, BN = T::BN;
   extern __shared__ __attribute__((aligned(1024))) unsigned char block_smem[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x % p.tiles_n;
-  const int m0 = tile_m * BM, n0 = tile_n * BN, wm = (wave >> 1) * 32 * MT, wn = (wave & 1) * 32 * NT;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % T::WAVES, share = __builtin_amdgcn_readfirstlane(tid >> 6) / T::WAVES;
+  int tile_m, tile_n;
+  block_place(blockIdx.x, p.tiles_m, p.tiles_n, T::BAND, tile_m, tile_n);
+  const int m0 = tile_m * BM, n0 = tile_n * BN, wm = (wave / T::WN) * 32 * MT, wn = (wave % T::WN) * 32 * NT;
   const int64_t kp = (int64_t)p.blocks * kBlock;
   // (a tile's rows lie below 2 GiB from its first: host-checked)
   const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + m0 * kp), 0, 0x7FFFFFFF, 0x00020000);
   const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.b + n0 * kp), 0, 0x7FFFFFFF, 0x00020000);
-  int from[LOADS];
+  const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc((void*)(p.sa + m0), 0, 0x7FFFFFFF, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.sb + n0), 0, 0x7FFFFFFF, 0x00020000);
+  const int last_m = p.M - m0 - 1, last_n = p.N - n0 - 1;     // (rows past the edge: the last one again)
+  int from[T::LOADS], scale_from[T::SCALES];
 #pragma unroll
-  for (int j = 0; j < LOADS; ++j) {
-    int r = (wave + 4 * j) * 8 + (lane >> 3);
-    const bool second = r >= BM;
-    r -= second ? BM : 0;
-    const int last = (second ? p.N - n0 : p.M - m0) - 1, row = r < last ? r : last;     // (rows past the edge: the last one again)
+  for (int j = 0; j < T::LOADS; ++j) {
+    const int r = (wave + T::WAVES * j) * 8 + (lane >> 3), row = r < BM ? (r < last_m ? r : last_m) : (r - BM < last_n ? r - BM : last_n);
     from[j] = (int)(row * kp) + (((lane & 7) ^ (r & 7)) << 4);
   }
-  auto issue = [&](int step) {
-    unsigned char* to = block_smem + (step & 1) * STAGE;
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) block_load_lds((wave + 4 * j) * 8 >= BM ? rb : ra, to + (wave + 4 * j) * 1024, from[j], step * kBlock);
+  for (int j = 0; j < T::SCALES; ++j) {
+    const int run = (wave + T::WAVES * j) % (T::ROWS / 64), r = run * 64 + lane;
+    scale_from[j] = 4 * (r < BM ? (r < last_m ? r : last_m) : (r - BM < last_n ? r - BM : last_n));
+  }
+  // this share's blocks; all shares take as many steps, those past the last block without products
+  const int steps = (p.blocks + T::SHARES - 1) / T::SHARES, first = share * steps, live = p.blocks - first < steps ? p.blocks - first : steps;
+  unsigned char* const ring = block_smem + share * T::DEEP * T::STAGE;
+  // load j of a stage, the first ones of the rows' scales; `to`: the stage's place
+  auto issue = [&](int step, unsigned char* to, int j) {
+    step = first + step < p.blocks ? first + step : p.blocks - 1;     // (past the end: the last one again, so that every share waits for as many)
+    if (j < T::SCALES) {
+      const int run = (wave + T::WAVES * j) % (T::ROWS / 64);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(run * 64 < BM ? rsa : rsb, (block_lds_ptr)(to + T::ROWS * 128 + run * 256), 4, scale_from[j],
+                                               (step >> 2) * 4 * (run * 64 < BM ? p.M : p.N), 0, 0);
+    } else {
+      j -= T::SCALES;
+      block_load_lds((wave + T::WAVES * j) * 8 < BM ? ra : rb, to + (wave + T::WAVES * j) * 1024, from[j], step * kBlock);
+    }
   };
-  const unsigned *sa[MT], *sb[NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) sa[i] = p.sa + (m0 + wm + 32 * i + l31 < p.M ? m0 + wm + 32 * i + l31 : p.M - 1);
-#pragma unroll
-  for (int i = 0; i < NT; ++i) sb[i] = p.sb + (n0 + wn + 32 * i + l31 < p.N ? n0 + wn + 32 * i + l31 : p.N - 1);
-  unsigned a_scale[MT], b_scale[NT], a_next[MT], b_next[NT];
-  auto scales = [&](int four) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) a_next[i] = sa[i][(int64_t)four * p.M];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) b_next[i] = sb[i][(int64_t)four * p.N];
-  };
+  constexpr int ISSUES = T::LOADS + T::SCALES, GAPS = MT * NT, READS = 2 * (MT + NT);
   f32x16 acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -236,103 +266,251 @@ __global__ __launch_bounds__(256) void cascmm_block_gemm_kernel(const BlockGemmP
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  u32x4 f[2][MT + NT][2];              // fragments of both halves: rows of a, then of b; 32 k in two pieces
+  unsigned scale[MT + NT], scale_next[MT + NT];
+  // read k of a half: the pieces of b and a in turn, as the instructions want them
+  const int at[2] = {(wm + l31) * 128, (BM + wn + l31) * 128}, turn = l31 & 7;
+  auto read = [&](const unsigned char* stage, int half, int k) {
+    const int g = k >> 1, piece = k & 1;
+    const int base = g < MT ? at[0] + g * 4096 : at[1] + (g - MT) * 4096;
+    f[half][g][piece] = *(const u32x4*)(stage + base + (((4 * half + 2 * h + piece) ^ turn) << 4));
+  };
+  auto read_scale = [&](const unsigned char* stage, int g) {
+    scale_next[g] = *(const unsigned*)(stage + T::ROWS * 128 + (g < MT ? wm + 32 * g + l31 : BM + wn + 32 * (g - MT) + l31) * 4);
+  };
+  auto whole = [&](int half, int g) {
+    const u32x4 lo = f[half][g][0], hi = f[half][g][1];
+    return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  };
+  // product t of a half
+  auto multiply = [&](int half, int t) {
+    const int i = t / NT, j = t % NT;
+    if constexpr (!FINE) {
+      // (the right operand first: a lane's registers are then neighbours along a row of c)
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(half, MT + j), whole(half, i), acc[i][j], 0, 0, 0, (int)scale[MT + j], 0, (int)scale[i]);
+    } else {
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      auto wide = [&](int g, int part) {     // eight values, scaled
+        const float s = __builtin_bit_cast(float, (scale[g] & 255u) << 23);
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned word = f[half][g][part >> 1][2 * (part & 1) + (e >> 1)];
+          const bf16x2 two = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, s, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, s, false);
+          w[e] = __builtin_bit_cast(unsigned, two);
+        }
+        return __builtin_bit_cast(bf16x8, w);
+      };
+#pragma unroll
+      for (int part = 0; part < 4; ++part) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wide(MT + j, part), wide(i, part), acc[i][j], 0, 0, 0);
+    }
+  };
+#define BLOCK_FENCE() __builtin_amdgcn_sched_barrier(0)
   if (p.blocks > 0) {     // (else: nothing but the bias)
-    issue(0);
-    scales(0);
+#pragma unroll
+    for (int s = 0; s < T::DEEP; ++s)
+#pragma unroll
+      for (int j = 0; j < ISSUES; ++j) issue(s, ring + s * T::STAGE, j);
+    __builtin_amdgcn_s_waitcnt(block_waitcnt(ISSUES * (T::DEEP - 1), 15));
+    __builtin_amdgcn_s_barrier();
+    BLOCK_FENCE();
+#pragma unroll
+    for (int g = 0; g < MT + NT; ++g) read_scale(ring, g);
+#pragma unroll
+    for (int k = 0; k < READS; ++k) read(ring, 0, k);
+    int here = 0;
+    for (int step = 0; step < steps; ++step) {
+      unsigned char* const stage = ring + here;
+      here = here + T::STAGE < T::DEEP * T::STAGE ? here + T::STAGE : 0;
+      unsigned char* const other = ring + here;
+      const bool counts = T::SHARES == 1 || step < live;
+#pragma unroll
+      for (int g = 0; g < MT + NT; ++g) scale[g] = scale_next[g] >> (((first + step) & 3) * 8);
+#pragma unroll
+      for (int t = 0; t < GAPS; ++t) {
+        if (counts) multiply(0, t);
+        BLOCK_FENCE();
+#pragma unroll
+        for (int k = READS * t / GAPS; k < READS * (t + 1) / GAPS; ++k) read(stage, 1, k);
+        BLOCK_FENCE();
+      }
+      __builtin_amdgcn_s_waitcnt(block_waitcnt(ISSUES * (T::DEEP - 2), 0));    // own loads of the next stage have landed, own reads of this one are back
+      __builtin_amdgcn_s_barrier();          // everybody's
+      BLOCK_FENCE();
+#pragma unroll
+      for (int t = 0; t < GAPS; ++t) {
+        if (counts) multiply(1, t);
+        BLOCK_FENCE();
+#pragma unroll
+        for (int k = READS * t / GAPS; k < READS * (t + 1) / GAPS; ++k) read(other, 0, k);
+#pragma unroll
+        for (int g = (MT + NT) * t / GAPS; g < (MT + NT) * (t + 1) / GAPS; ++g) read_scale(other, g);
+#pragma unroll
+        for (int j = ISSUES * t / GAPS; j < ISSUES * (t + 1) / GAPS; ++j) issue(step + T::DEEP, stage, j);
+        BLOCK_FENCE();
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);      // (the redundant loads land before LDS is given up)
   }
-  for (int step = 0; step < p.blocks; ++step) {
-    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0), lgkmcnt(0): this stage has landed, the last one is read
+#undef BLOCK_FENCE
+  // A lane holds row l31 of a block, columns 8 q + 4 h + e: sixteen bytes of a row and less.  Through LDS, in a place of each wave's own, 32 rows of the wave's width at a time, so that
+  // what is stored are whole pieces of rows.
+  typedef E four __attribute__((ext_vector_type(4), aligned(4 * sizeof(E))));
+  constexpr int VEC = 16 / (int)sizeof(E), WIDTH = 32 * NT, PITCH = WIDTH + VEC, LANES = WIDTH / VEC, AT_ONCE = 64 / LANES;   // (elements; lanes of a row; rows of a store)
+  static_assert(64 % LANES == 0 && T::WAVES * 32 * PITCH * (int)sizeof(E) <= T::LDS, "the rows of a store");
+  typedef E chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
+  __syncthreads();
+  if constexpr (T::SHARES > 1) {
+    float* const meet = (float*)block_smem + (wave * MT * NT * 16) * 64 + lane;
+    constexpr int ALL = T::WAVES * MT * NT * 16 * 64;
+    static_assert((T::SHARES - 1) * ALL * 4 <= T::LDS, "the sums of the shares");
+    if (share > 0) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) meet[(share - 1) * ALL + ((i * NT + j) * 16 + e) * 64] = acc[i][j][e];
+    }
     __syncthreads();
-    if ((step & 3) == 0) {
+    if (share == 0) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) a_scale[i] = a_next[i];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) b_scale[i] = b_next[i];
-    }
-    if (step + 1 < p.blocks) {
-      issue(step + 1);
-      if ((step & 3) == 0 && step + 4 < p.blocks) scales((step >> 2) + 1);
-    }
-    const unsigned char* stage = block_smem + (step & 1) * STAGE;
-    auto fragment = [&](int r, int half) {
-      const u32x4 lo = *(const u32x4*)(stage + r * 128 + (((4 * half + 2 * h) ^ (r & 7)) << 4));
-      const u32x4 hi = *(const u32x4*)(stage + r * 128 + (((4 * half + 2 * h + 1) ^ (r & 7)) << 4));
-      return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-    };
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      i32x8 a[MT], b[NT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[i] = fragment(wm + 32 * i + l31, half);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) b[j] = fragment(BM + wn + 32 * j + l31, half);
-      if constexpr (!FINE) {
-        // (the right operand first: a lane's registers are then neighbours along a row of c)
+      for (int o = 0; o < T::SHARES - 1; ++o)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int j = 0; j < NT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 0, 0, 0, (int)b_scale[j], 0, (int)a_scale[i]);
-      } else {
-        auto wide = [&](i32x8 q, int g, unsigned byte) {     // eight values, scaled
-          const float f = __builtin_bit_cast(float, byte << 23);
-          typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-          u32x4 w;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const unsigned word = (unsigned)q[2 * g + (e >> 1)];
-            const bf16x2 two = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, f, false);
-            w[e] = __builtin_bit_cast(unsigned, two);
-          }
-          return __builtin_bit_cast(bf16x8, w);
-        };
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          bf16x8 aw[MT], bw[NT];
-#pragma unroll
-          for (int i = 0; i < MT; ++i) aw[i] = wide(a[i], g, a_scale[i] & 255u);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) bw[j] = wide(b[j], g, b_scale[j] & 255u);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bw[j], aw[i], acc[i][j], 0, 0, 0);
-        }
-      }
+            for (int e = 0; e < 16; ++e) acc[i][j][e] += meet[o * ALL + ((i * NT + j) * 16 + e) * 64];
     }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) a_scale[i] >>= 8;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) b_scale[i] >>= 8;
+    __syncthreads();
+    if (share > 0) return;
   }
-  // a lane holds row l31 of a block of c, columns 8 q + 4 h + e
-  typedef E four __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+  E* const mine = (E*)block_smem + wave * 32 * PITCH;
+  float bias[NT][4][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int n = n0 + wn + 32 * j + 8 * q + 4 * h;
-      float bias[4] = {0.f, 0.f, 0.f, 0.f};
-      if (p.bias) {
+    for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bias[e] = IoType<IODT>::load((const E*)p.bias + (n + e < p.N ? n + e : p.N - 1));
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + wn + 32 * j + 8 * q + 4 * h + e;
+        bias[j][q][e] = p.bias ? IoType<IODT>::load((const E*)p.bias + (n < p.N ? n : p.N - 1)) : 0.f;
       }
+  const int column = n0 + wn + lane % LANES * VEC;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int m = m0 + wm + 32 * i + l31;
-        E* row = (E*)p.c + m * p.ldc;
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
         four o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (E)(acc[i][j][4 * q + e] + bias[e]);
-        if (m < p.M && n + 4 <= p.N) {
-          *(four*)(row + n) = o;
-        } else if (m < p.M) {
+        for (int e = 0; e < 4; ++e) o[e] = (E)(acc[i][j][4 * q + e] + bias[j][q][e]);
+        *(four*)(mine + l31 * PITCH + 32 * j + 8 * q + 4 * h) = o;
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < p.N) row[n + e] = o[e];
-        }
+    for (int k = 0; k < 32 / AT_ONCE; ++k) {
+      const int r = k * AT_ONCE + lane / LANES, m = m0 + wm + 32 * i + r;
+      const chunk o = *(const chunk*)__builtin_assume_aligned(mine + r * PITCH + lane % LANES * VEC, 16);
+      E* to = (E*)p.c + m * p.ldc + column;
+      if (m < p.M && column + VEC <= p.N) {
+        *(chunk*)to = o;
+      } else if (m < p.M) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (column + e < p.N) to[e] = o[e];
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// few rows: c [M][N] of up to sixteen rows of x, rounded here
+// ---------------------------------------------------------------------------------------
+// Sixteen columns a workgroup, a block of k at a time a wave: its fragments come straight from memory, sixteen bytes a lane of four neighbours along a row; every workgroup rounds
+// the rows itself, which costs less than a launch in front of it.  The waves' sums meet in LDS, in order.  A lane's 32 k are the pieces i and i + 4 of a block's eight, of both operands.
+struct BlockRowsParams {
+  const void* x;                   // [M][K], row stride ldx
+  const unsigned char* b;
+  const unsigned* sb;
+  void* c;
+  const void* bias;
+  int64_t ldx, ldc;
+  int M, N, K, blocks;
+};
+template <int IODT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void cascmm_block_rows_kernel(const BlockRowsParams p) {
+  typedef typename IoType<IODT>::T E;
+  typedef E eight __attribute__((ext_vector_type(8), aligned(sizeof(E))));
+  __shared__ f32x4 meet[WAVES][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, part = lane >> 4;
+  const int n = blockIdx.x * 16 + l15, row_b = n < p.N ? n : p.N - 1, row_a = l15 < p.M ? l15 : p.M - 1;
+  const unsigned char* const b = p.b + (int64_t)row_b * p.blocks * kBlock + part * 16;
+  const E* const x = (const E*)p.x + row_a * p.ldx + part * 16;
+  struct Piece {
+    u32x4 b[2];
+    unsigned scale;
+    eight x[4];
+  } next;
+  auto fetch = [&](int block) {
+    next.b[0] = *(const u32x4*)(b + (int64_t)block * kBlock);
+    next.b[1] = *(const u32x4*)(b + (int64_t)block * kBlock + 64);
+    next.scale = p.sb[(int64_t)(block >> 2) * p.N + row_b] >> ((block & 3) * 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = block * kBlock + (i >> 1) * 64 + (i & 1) * 8;     // (of this lane's: + part * 16)
+      if (k + part * 16 + 8 <= p.K) {
+        next.x[i] = *(const eight*)(x + k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) next.x[i][e] = k + part * 16 + e < p.K ? x[k + e] : (E)0.f;
+      }
+    }
+  };
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  int block = wave;
+  if (block < p.blocks) fetch(block);
+  while (block < p.blocks) {
+    const Piece cur = next;
+    block += WAVES;
+    if (block < p.blocks) fetch(block);
+    float v[4][8];
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[i][e] = (float)cur.x[i][e];
+        const unsigned bits = __builtin_bit_cast(unsigned, v[i][e]) & 0x7FFFFFFFu;
+        const bool finite = bits < 0x7F800000u;
+        v[i][e] = finite ? v[i][e] : __builtin_nanf("");
+        most = block_larger(most, finite ? bits : 0u);
+      }
+    most = block_larger(most, (unsigned)__shfl_xor((int)most, 16, 64));
+    most = block_larger(most, (unsigned)__shfl_xor((int)most, 32, 64));
+    const unsigned byte = block_scale(most);
+    const float f = block_inverse(byte);
+    const u32x2 q0 = block_pack(v[0], f), q1 = block_pack(v[1], f), q2 = block_pack(v[2], f), q3 = block_pack(v[3], f);
+    const i32x8 a = {(int)q0[0], (int)q0[1], (int)q1[0], (int)q1[1], (int)q2[0], (int)q2[1], (int)q3[0], (int)q3[1]};
+    const i32x8 w = {(int)cur.b[0][0], (int)cur.b[0][1], (int)cur.b[0][2], (int)cur.b[0][3], (int)cur.b[1][0], (int)cur.b[1][1], (int)cur.b[1][2], (int)cur.b[1][3]};
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, (int)cur.scale, 0, (int)byte);
+  }
+  meet[wave][lane] = acc;
+  __syncthreads();
+  // a lane holds row l15 of c, columns 4 part + e: a thread for each of the 256
+  if (tid < 256) {
+    const int from = tid >> 2, e = tid & 3, m = from & 15, column = blockIdx.x * 16 + 4 * (from >> 4) + e;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += meet[w][from][e];
+    if (m < p.M && column < p.N) {
+      if (p.bias) s += IoType<IODT>::load((const E*)p.bias + column);
+      IoType<IODT>::store((E*)p.c + m * p.ldc + column, s);
+    }
+  }
 }
 
 }  // namespace cascmm

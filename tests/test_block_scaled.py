@@ -35,6 +35,26 @@ def test_product_arguments(change, status):
     assert product(**change) == status
 
 
+def linear(x=P, b=P, sb=P, c=P, bias=None, M=4, N=8, K=16, ldx=16, ldc=8, dtype=F16, workspace=P, nbytes=1 << 20):
+    return _lib.lib().cascmm_block_linear(x, b, sb, c, bias, M, N, K, ldx, ldc, dtype, workspace, nbytes, None)
+
+
+@pytest.mark.parametrize("rows", [4, 20])     # (one launch, and two with a workspace)
+@pytest.mark.parametrize("change, status", [
+    (dict(dtype=4), -3), (dict(M=-1), -2), (dict(N=-1), -2), (dict(K=-1), -2), (dict(ldx=15), -2), (dict(ldc=7), -2), (dict(M=2 ** 31), -9), (dict(N=2 ** 31, ldc=2 ** 31), -9),
+    (dict(K=2 ** 22 + 1, ldx=2 ** 23), -9), (dict(x=None), -1), (dict(b=None), -1), (dict(sb=None), -1), (dict(c=None), -1), (dict(x=P + 1), -6), (dict(b=P + 8), -6),
+    (dict(sb=P + 2), -6), (dict(c=P + 1), -6), (dict(bias=P + 1), -6), (dict(M=0, x=None, c=None), 0), (dict(N=0, ldc=0, c=None), 0)])
+def test_linear_arguments(rows, change, status):
+    assert linear(**{"M": rows, **change}) == status
+
+
+def test_linear_workspace():
+    need = _lib.lib().cascmm_block_linear_workspace_bytes
+    assert need(16, 5120, F16) == 0 and need(17, 300, BF16) >= 17 * 384 + 17 * 4 and need(1, 300, F32) >= 384 + 4 and need(-1, 5, F16) == 0 and need(20, 2 ** 22 + 1, F16) == 0
+    for workspace, nbytes, status in ((None, 1 << 20, -5), (P, need(20, 16, F16) - 1, -5), (P + 8, 1 << 20, -6)):
+        assert linear(M=20, workspace=workspace, nbytes=nbytes) == status
+
+
 def test_sizes():
     values, scales, ws = (getattr(_lib.lib(), f"cascmm_block_{n}_bytes") for n in ("values", "scales", "round_workspace"))
     assert values(3, 1) == 3 * 128 and values(3, 128) == 3 * 128 and values(3, 129) == 3 * 256 and values(0, 5) == 0 and values(5, 0) == 0 and values(-1, 5) == 0

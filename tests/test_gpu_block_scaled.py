@@ -144,7 +144,7 @@ def check_product(got, a, b, bias, what):
         assert rms(off) <= most * rms(want) + (rms(lost) if got.dtype == torch.float32 else 0), f"{what}: rms {rms(off) / rms(want)}"
 
 
-SIZES = [(1, 1, 1), (1, 5120, 130), (2, 128, 64), (3, 127, 129), (17, 130, 5), (64, 640, 128), (127, 384, 255), (129, 1000, 131), (260, 513, 320), (300, 1280, 640)]
+SIZES = [(1, 1, 1), (1, 5120, 130), (16, 2049, 47), (5, 4096, 16), (2, 128, 64), (3, 127, 129), (17, 130, 5), (64, 640, 128), (127, 384, 255), (129, 1000, 131), (260, 513, 320), (300, 1280, 640)]
 
 
 @pytest.mark.parametrize("dtype", HALF)
@@ -172,6 +172,23 @@ def test_product_and_gradients(gpu_device, M, K, N, dtype):
         check_product(gb, held(a, "columns")[0].t(), held(dy, "columns")[0], None, "db")
         want = dy.double().sum(0)
         assert bool(((gbias.cpu().double() - want).abs() <= half_of(dtype) * want.abs() + TINY[dtype] + (16 + M // 128) * U * dy.double().abs().sum(0)).all())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M, K, N", [(65, 2500, 70), (400, 700, 129), (500, 260, 1300), (520, 1100, 5130), (1030, 5000, 1290), (2100, 257, 2570), (4100, 600, 2500)])
+def test_every_tile(gpu_device, M, K, N, dtype):
+    """Sizes that the rule gives to each of its tiles, with rows, columns and k past their edges."""
+    gen = torch.Generator(device=gpu_device).manual_seed(M)
+    a, b = (torch.randn(M, K, generator=gen, device=gpu_device) * 3).to(dtype), torch.randn(K, N, generator=gen, device=gpu_device).to(dtype)
+    bias = torch.randn(N, generator=gen, device=gpu_device).to(dtype)
+    weight = BlockScaledWeight(b)
+    y = block_scaled_matmul(a, weight, bias=bias)
+    rows = sorted({0, 1, 31, 32, 63, 64, 127, 128, 129, 255, 256, 257, M // 2, M - 65, M - 2, M - 1} & set(range(M)))
+    pick = torch.tensor(rows, device=gpu_device)
+    wide = seen(_round(a[pick].contiguous(), False, True, False)[0], len(rows), K)[0]
+    check_product(y[pick], wide, weight.dequantized().cpu().double(), bias, "rows")
+    want = seen(_round(a, False, True, False)[0], M, K)[0].float().to(gpu_device) @ weight.dequantized()
+    assert bool(((y.float() - want - bias.float()).abs() <= 2 * half_of(dtype) * want.abs() + 2e-3 * want.pow(2).mean().sqrt()).all())
 
 
 def test_each_gradient_alone_and_other_shapes(gpu_device):
@@ -215,7 +232,7 @@ def test_differences(gpu_device):
             step[which][at] -= 2
             difference = float((up - f(*step)).detach()) / 2
             # (16-bit results of these sums are rounded: each of the results that changed by half a step)
-            most = float(block_scaled_matmul(a, b).abs().max() + 7) * 7 * 9 * half_of(dtype) if dtype != torch.float32 else 0.0
+            most = float(block_scaled_matmul(a, b).detach().abs().max() + 7) * 7 * 9 * half_of(dtype) if dtype != torch.float32 else 0.0
             assert abs(difference - float(grads[which][at])) <= most + half_of(dtype) * abs(difference), (dtype, which, at)
 
 
