@@ -59,31 +59,147 @@ __device__ __forceinline__ u32x2 block_pack(const float (&v)[8], float f) {
   return (u32x2){(unsigned)lo, (unsigned)hi};
 }
 
+// Eight elements, as the rounding handles them.  fp32: numbers; 16 bits: pairs, whose magnitudes are compared as whole numbers two at a time and which an instruction divides by the
+// scale and rounds two at a time (all patterns under all scales: the same bytes as by fp32; infinities become NaN there too).
+template <int IODT> struct BlockEight {
+  typedef typename IoType<IODT>::T E;
+  typedef float Values[8];
+  typedef unsigned Most[8];                   // magnitudes of eight columns
+  static __device__ __forceinline__ void clear(Most& m) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m[e] = 0;
+  }
+  static __device__ __forceinline__ void load(Values& v, const E* src, bool whole, int left) {
+    typedef E chunk __attribute__((ext_vector_type(8), aligned(sizeof(E))));   // (rows start on elements, not on 16 bytes)
+    if (whole) {
+      const chunk c = *(const chunk*)src;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < left ? src[e] : 0.f;
+    }
+  }
+  static __device__ __forceinline__ float value(const Values& v, int e) { return v[e]; }
+  // folds the finite magnitudes into those of the columns; returns the largest of the eight, as bits of a float
+  static __device__ __forceinline__ unsigned fold(Values& v, Most& columns) {
+    unsigned most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned bits = __builtin_bit_cast(unsigned, v[e]) & 0x7FFFFFFFu;
+      const bool finite = bits < 0x7F800000u;
+      v[e] = finite ? v[e] : __builtin_nanf("");
+      const unsigned b = finite ? bits : 0u;
+      columns[e] = block_larger(columns[e], b);
+      most = block_larger(most, b);
+    }
+    return most;
+  }
+  static __device__ __forceinline__ unsigned column(const Most& m, int e) { return m[e]; }
+  static __device__ __forceinline__ u32x2 pack(const Values& v, unsigned byte) { return block_pack(v, block_inverse(byte)); }
+  static __device__ __forceinline__ u32x2 pack_column(const Values (&v)[8], int e, unsigned byte) {
+    const float column[8] = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
+    return block_pack(column, block_inverse(byte));
+  }
+};
+template <int IODT> struct BlockEight16 {
+  typedef typename IoType<IODT>::T E;
+  typedef E pair __attribute__((ext_vector_type(2)));
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  typedef u32x4 Values;
+  typedef unsigned Most[4];
+  static constexpr unsigned kInf = IODT == CASCMM_DT_BF16 ? 0x7F80u : 0x7C00u;
+  static __device__ __forceinline__ void clear(Most& m) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m[c] = 0;
+  }
+  static __device__ __forceinline__ void load(Values& v, const E* src, bool whole, int left) {
+    typedef E chunk __attribute__((ext_vector_type(8), aligned(sizeof(E))));
+    chunk c;
+    if (whole) {
+      c = *(const chunk*)src;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e] = e < left ? src[e] : (E)0.f;
+    }
+    v = __builtin_bit_cast(u32x4, c);
+  }
+  static __device__ __forceinline__ float value(const Values& v, int e) {
+    const unsigned w = v[e >> 1];      // (a number of its own: a cast of a vector's element takes the vector's first)
+    return (float)__builtin_bit_cast(pair, w)[e & 1];
+  }
+  static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+  }
+  static __device__ __forceinline__ unsigned bits(unsigned half) {   // of the float
+    return IODT == CASCMM_DT_BF16 ? half << 16 : __builtin_bit_cast(unsigned, (float)__builtin_bit_cast(_Float16, (unsigned short)half));
+  }
+  static __device__ __forceinline__ unsigned fold(Values& v, Most& columns) {
+    unsigned m[4], most = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      m[c] = v[c] & 0x7FFF7FFFu;
+      most = larger(most, m[c]);
+    }
+    if ((most >> 16) >= kInf || (most & 0xFFFFu) >= kInf) {   // (hardly ever)
+      most = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        m[c] = ((m[c] >> 16) >= kInf ? 0u : m[c] & 0xFFFF0000u) | ((m[c] & 0xFFFFu) >= kInf ? 0u : m[c] & 0xFFFFu);
+        most = larger(most, m[c]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) columns[c] = larger(columns[c], m[c]);
+    return bits((most >> 16) > (most & 0xFFFFu) ? most >> 16 : most & 0xFFFFu);
+  }
+  static __device__ __forceinline__ unsigned column(const Most& m, int e) { return bits(e & 1 ? m[e >> 1] >> 16 : m[e >> 1] & 0xFFFFu); }
+  static __device__ __forceinline__ s16x2 two(s16x2 old, unsigned w, float scale, bool high) {
+    if constexpr (IODT == CASCMM_DT_BF16)
+      return high ? __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(old, __builtin_bit_cast(pair, w), scale, true) : __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(old, __builtin_bit_cast(pair, w), scale, false);
+    else
+      return high ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(old, __builtin_bit_cast(pair, w), scale, true) : __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(old, __builtin_bit_cast(pair, w), scale, false);
+  }
+  static __device__ __forceinline__ u32x2 pack4(unsigned w0, unsigned w1, unsigned w2, unsigned w3, unsigned byte) {
+    const float scale = __builtin_bit_cast(float, byte << 23);      // (its exponent is the scale: a byte of 0 is 2^-127)
+    const s16x2 zero = {0, 0};
+    return (u32x2){__builtin_bit_cast(unsigned, two(two(zero, w0, scale, false), w1, scale, true)), __builtin_bit_cast(unsigned, two(two(zero, w2, scale, false), w3, scale, true))};
+  }
+  static __device__ __forceinline__ u32x2 pack(const Values& v, unsigned byte) { return pack4(v[0], v[1], v[2], v[3], byte); }
+  static __device__ __forceinline__ u32x2 pack_column(const Values (&v)[8], int e, unsigned byte) {
+    const unsigned which = e & 1 ? 0x07060302u : 0x05040100u;
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], which);
+    return pack4(w[0], w[1], w[2], w[3], byte);
+  }
+};
+template <> struct BlockEight<CASCMM_DT_F16> : BlockEight16<CASCMM_DT_F16> {};
+template <> struct BlockEight<CASCMM_DT_BF16> : BlockEight16<CASCMM_DT_BF16> {};
+
 // A tile of 128 x 128 a workgroup, read once: a thread holds 8 rows of 8 columns, sixteen threads a row of the tile.
 // SQUARE: one scale for the whole tile; else one for each of its rows (q) and of its columns (qt).
 template <int IODT, bool SQUARE>
 __global__ __launch_bounds__(256) void cascmm_block_round_kernel(const BlockRoundParams p) {
-  typedef typename IoType<IODT>::T E;
-  typedef E chunk __attribute__((ext_vector_type(8), aligned(sizeof(E))));   // (rows start on elements, not on 16 bytes)
-  __shared__ unsigned col_most[4][kBlock];
+  typedef BlockEight<IODT> V;
+  typedef typename V::E E;
+  constexpr int MOST = sizeof(typename V::Most) / 4;      // words of eight columns' magnitudes
+  __shared__ unsigned col_most[4][16][MOST];
   __shared__ float col_sum[4][kBlock];
   __shared__ u32x2 turned[kBlock][16];       // [column][eight rows], the eights of a column in the order i ^ (column / 8): writes and reads without conflicts
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, wave = tid >> 6;
   const int64_t tile_row = blockIdx.x / p.across, tile_col = blockIdx.x % p.across;
   const int64_t row0 = tile_row * kBlock + ty * 8, col0 = tile_col * kBlock + tx * 8;
   const E* src = (const E*)p.x + row0 * p.ldx + col0;
-  float v[8][8];
-  const int64_t left = p.cols - col0;
+  typename V::Values v[8];
+  const int left = p.cols - col0 < 8 ? (int)(p.cols - col0) : 8, down = p.rows - row0 < 8 ? (int)(p.rows - row0) : 8;
+  if (left == 8 && down == 8) {
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    if (row0 + r < p.rows && left >= 8) {
-      const chunk c = *(const chunk*)(src + r * p.ldx);
+    for (int r = 0; r < 8; ++r) V::load(v[r], src + r * p.ldx, true, 8);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[r][e] = (float)c[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[r][e] = row0 + r < p.rows && e < left ? (float)src[r * p.ldx + e] : 0.f;
-    }
+    for (int r = 0; r < 8; ++r) V::load(v[r], src + r * p.ldx, r < down && left == 8, r < down ? left : 0);
   }
   if (p.sums) {
     // sums over the tile's rows: eight in a thread, four threads of a wave, four waves, in this order
@@ -91,70 +207,66 @@ __global__ __launch_bounds__(256) void cascmm_block_round_kernel(const BlockRoun
     for (int e = 0; e < 8; ++e) {
       float s = 0.f;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) s += v[r][e];
+      for (int r = 0; r < 8; ++r) s += V::value(v[r], e);
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
       if ((tid & 63) < 16) col_sum[wave][tx * 8 + e] = s;
     }
   }
-  unsigned row_most[8], most[8];
+  unsigned row_most[8];
+  typename V::Most most;
+  V::clear(most);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) most[e] = 0;
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    row_most[r] = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned bits = __builtin_bit_cast(unsigned, v[r][e]) & 0x7FFFFFFFu;
-      const bool finite = bits < 0x7F800000u;
-      v[r][e] = finite ? v[r][e] : __builtin_nanf("");
-      const unsigned b = finite ? bits : 0u;
-      row_most[r] = block_larger(row_most[r], b);
-      most[e] = block_larger(most[e], b);
-    }
-  }
+  for (int r = 0; r < 8; ++r) row_most[r] = V::fold(v[r], most);
   unsigned square = 0;
   if (SQUARE) {
+    __shared__ unsigned all[4];
 #pragma unroll
     for (int r = 0; r < 8; ++r) square = block_larger(square, row_most[r]);
     square = block_row_max(square);
     square = block_larger(square, (unsigned)__shfl_xor((int)square, 16, 64));
     square = block_larger(square, (unsigned)__shfl_xor((int)square, 32, 64));
-    if ((tid & 63) == 0) col_most[wave][0] = square;
+    if ((tid & 63) == 0) all[wave] = square;
     __syncthreads();
-    square = block_scale(block_larger(block_larger(col_most[0][0], col_most[1][0]), block_larger(col_most[2][0], col_most[3][0])));
+    square = block_scale(block_larger(block_larger(all[0], all[1]), block_larger(all[2], all[3])));
   }
   if (p.q) {
     const int64_t padded = block_padded(p.cols);
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const unsigned byte = SQUARE ? square : block_scale(block_row_max(row_most[r]));
-      if (row0 + r < p.rows) {
-        *(u32x2*)(p.q + (row0 + r) * padded + col0) = block_pack(v[r], block_inverse(byte));
+      if (r < down) {
+        *(u32x2*)(p.q + (row0 + r) * padded + col0) = V::pack(v[r], byte);
         if (tx == 0) p.s[((tile_col >> 2) * p.rows + row0 + r) * 4 + (tile_col & 3)] = (unsigned char)byte;
       }
     }
   }
   if (!p.qt && !p.sums) return;
+  auto join = [&](unsigned a, unsigned b) {
+    if constexpr (MOST == 4) return V::larger(a, b);
+    else return block_larger(a, b);
+  };
   if (!SQUARE && p.qt) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      most[e] = block_larger(most[e], (unsigned)__shfl_xor((int)most[e], 16, 64));
-      most[e] = block_larger(most[e], (unsigned)__shfl_xor((int)most[e], 32, 64));
-      if ((tid & 63) < 16) col_most[wave][tx * 8 + e] = most[e];
+    for (int c = 0; c < MOST; ++c) {
+      most[c] = join(most[c], (unsigned)__shfl_xor((int)most[c], 16, 64));
+      most[c] = join(most[c], (unsigned)__shfl_xor((int)most[c], 32, 64));
+      if ((tid & 63) < 16) col_most[wave][tx][c] = most[c];
     }
   }
   __syncthreads();
   if (p.sums && tid < kBlock && tile_col * kBlock + tid < p.cols)
     p.sums[tile_row * p.cols + tile_col * kBlock + tid] = (col_sum[0][tid] + col_sum[1][tid]) + (col_sum[2][tid] + col_sum[3][tid]);
   if (!p.qt) return;
+  if (!SQUARE) {
+#pragma unroll
+    for (int c = 0; c < MOST; ++c) most[c] = join(join(col_most[0][tx][c], col_most[1][tx][c]), join(col_most[2][tx][c], col_most[3][tx][c]));
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int c = tx * 8 + e;
-    const unsigned byte = SQUARE ? square : block_scale(block_larger(block_larger(col_most[0][c], col_most[1][c]), block_larger(col_most[2][c], col_most[3][c])));
-    const float column[8] = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
-    turned[c][ty ^ tx] = block_pack(column, block_inverse(byte));
-    if (ty == 0 && col0 + e < p.cols) p.st[((tile_row >> 2) * p.cols + col0 + e) * 4 + (tile_row & 3)] = (unsigned char)byte;
+    const unsigned byte = SQUARE ? square : block_scale(V::column(most, e));
+    turned[tx * 8 + e][ty ^ tx] = V::pack_column(v, e, byte);
+    if (ty == 0 && e < left) p.st[((tile_row >> 2) * p.cols + col0 + e) * 4 + (tile_row & 3)] = (unsigned char)byte;
   }
   __syncthreads();
   const int64_t padded = block_padded(p.rows);
@@ -443,8 +555,8 @@ struct BlockRowsParams {
 };
 template <int IODT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void cascmm_block_rows_kernel(const BlockRowsParams p) {
-  typedef typename IoType<IODT>::T E;
-  typedef E eight __attribute__((ext_vector_type(8), aligned(sizeof(E))));
+  typedef BlockEight<IODT> V;
+  typedef typename V::E E;
   __shared__ f32x4 meet[WAVES][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, part = lane >> 4;
   const int n = blockIdx.x * 16 + l15, row_b = n < p.N ? n : p.N - 1, row_a = l15 < p.M ? l15 : p.M - 1;
@@ -453,7 +565,7 @@ __global__ __launch_bounds__(64 * WAVES) void cascmm_block_rows_kernel(const Blo
   struct Piece {
     u32x4 b[2];
     unsigned scale;
-    eight x[4];
+    typename V::Values x[4];
   } next;
   auto fetch = [&](int block) {
     next.b[0] = *(const u32x4*)(b + (int64_t)block * kBlock);
@@ -462,38 +574,26 @@ __global__ __launch_bounds__(64 * WAVES) void cascmm_block_rows_kernel(const Blo
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int k = block * kBlock + (i >> 1) * 64 + (i & 1) * 8;     // (of this lane's: + part * 16)
-      if (k + part * 16 + 8 <= p.K) {
-        next.x[i] = *(const eight*)(x + k);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) next.x[i][e] = k + part * 16 + e < p.K ? x[k + e] : (E)0.f;
-      }
+      const int left = p.K - k - part * 16;
+      V::load(next.x[i], x + k, left >= 8, left);
     }
   };
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   int block = wave;
   if (block < p.blocks) fetch(block);
   while (block < p.blocks) {
-    const Piece cur = next;
+    Piece cur = next;
     block += WAVES;
     if (block < p.blocks) fetch(block);
-    float v[4][8];
+    typename V::Most columns;
+    V::clear(columns);
     unsigned most = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[i][e] = (float)cur.x[i][e];
-        const unsigned bits = __builtin_bit_cast(unsigned, v[i][e]) & 0x7FFFFFFFu;
-        const bool finite = bits < 0x7F800000u;
-        v[i][e] = finite ? v[i][e] : __builtin_nanf("");
-        most = block_larger(most, finite ? bits : 0u);
-      }
+    for (int i = 0; i < 4; ++i) most = block_larger(most, V::fold(cur.x[i], columns));
     most = block_larger(most, (unsigned)__shfl_xor((int)most, 16, 64));
     most = block_larger(most, (unsigned)__shfl_xor((int)most, 32, 64));
     const unsigned byte = block_scale(most);
-    const float f = block_inverse(byte);
-    const u32x2 q0 = block_pack(v[0], f), q1 = block_pack(v[1], f), q2 = block_pack(v[2], f), q3 = block_pack(v[3], f);
+    const u32x2 q0 = V::pack(cur.x[0], byte), q1 = V::pack(cur.x[1], byte), q2 = V::pack(cur.x[2], byte), q3 = V::pack(cur.x[3], byte);
     const i32x8 a = {(int)q0[0], (int)q0[1], (int)q1[0], (int)q1[1], (int)q2[0], (int)q2[1], (int)q3[0], (int)q3[1]};
     const i32x8 w = {(int)cur.b[0][0], (int)cur.b[0][1], (int)cur.b[0][2], (int)cur.b[0][3], (int)cur.b[1][0], (int)cur.b[1][1], (int)cur.b[1][2], (int)cur.b[1][3]};
     acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, (int)cur.scale, 0, (int)byte);

@@ -119,6 +119,27 @@ def test_rounding_at_every_border(gpu_device):
     assert same(got, want) and torch.equal(exps, we) and we[:5, 0].tolist() == [0, 1, 0, -1, 0] and we[8, 0] == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rounding_of_every_pattern(gpu_device, dtype):
+    """All numbers of a 16-bit type, each in a block whose largest element is one of their own size or larger, along rows and along columns, by tiles and by the product's own rounding."""
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    order = torch.argsort(x.float().abs().nan_to_num(posinf=0.0, nan=0.0))
+    for spread in (1, 37, 4099):
+        v = x[order][torch.arange(65536) * spread % 65536].view(512, 128)
+        d = v.to(gpu_device)
+        q, qt, _ = _round(d, False, True, True)
+        for pair, how, turn in ((q, "rows", False), (qt, "columns", True)):
+            want, we = held(v, how)
+            got, exps, _ = seen(pair, *(want.t() if turn else want).shape)
+            assert same(got, want.t() if turn else want) and torch.equal(exps, we.t() if turn else we)
+        eye = torch.eye(128, dtype=dtype, device=gpu_device)      # (held exactly: the product with it is the rounded block; what is not finite spoils its row, a sum of one)
+        clean = v.clone()
+        clean[~clean.isfinite()] = 0
+        for r in range(0, 512, 16):
+            got = block_scaled_matmul(clean[r:r + 16].to(gpu_device), eye)
+            assert same(got.cpu().double(), held(clean[r:r + 16], "rows")[0].to(dtype).double())
+
+
 def check_product(got, a, b, bias, what):
     """``a`` [M, K], ``b`` [K, N]: rounded operands in 64 bits."""
     M, K = a.shape
