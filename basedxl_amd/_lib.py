@@ -156,7 +156,8 @@ def native():
             module = importlib.import_module("._native", __package__)
             module.init(workspaces)
             module.init_scales(scale_scratch)
-            if any(not hasattr(module, name) for name in ("matmul", "prepared", "fp8", "layer_norm", "add_layer_norm", "epilogue", "epilogue_prepared")):
+            if any(not hasattr(module, name) for name in ("matmul", "prepared", "fp8", "layer_norm", "add_layer_norm", "epilogue", "epilogue_prepared",
+                                                          "block_scaled", "gated_add_norm", "clip_gradients")):
                 raise AttributeError("a function is missing")
         except (ImportError, AttributeError) as e:      # (AttributeError: the extension of an earlier build)
             raise ImportError(f"the host extension {os.path.join(_HERE, '_native.so')} is not built or does not load: {e}. "
@@ -172,7 +173,7 @@ class _NoShortCut:
     def matmul(*_args):
         return None
 
-    prepared = fp8 = layer_norm = add_layer_norm = epilogue = epilogue_prepared = matmul
+    prepared = fp8 = layer_norm = add_layer_norm = epilogue = epilogue_prepared = block_scaled = gated_add_norm = clip_gradients = matmul
 
 
 _short_cut = None

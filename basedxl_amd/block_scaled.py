@@ -140,6 +140,13 @@ def block_scaled_matmul(a: torch.Tensor, b, *, bias: Optional[torch.Tensor] = No
     Differentiable once in ``a``, ``b`` (a tensor: a held weight is a constant that no gradient passes through) and ``bias``, by products of the same kind, with the
     rounding passed over: ``dy`` in blocks of 128 along N times the same rounded ``b``; ``a`` and ``dy`` both in blocks of 128 rows; ``dbias`` from ``dy`` itself."""
     held = isinstance(b, BlockScaledWeight)
+    # the ordinary eager call in one native function; None: whatever is not ordinary about it is decided below
+    if not held:
+        y = _lib.short_cut().block_scaled(a, b, None, 0, 0, 0, bias)
+    else:
+        y = _lib.short_cut().block_scaled(a, b.values, b.scales, b.K, b.N, _DTYPES[b.dtype], bias)
+    if y is not None:
+        return y
     _check_operand(a, "a")
     if a.dim() < 1:
         raise ValueError("block_scaled_matmul: a needs at least one dimension")

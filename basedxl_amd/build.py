@@ -44,7 +44,7 @@ def _compile(src: str) -> str:
     return obj
 
 
-HOST_SOURCES = ("native.cpp", "native_operators.cpp")
+HOST_SOURCES = ("native.cpp", "native_operators.cpp", "native_blocks.cpp")
 
 
 def _compile_native(src: str) -> str:

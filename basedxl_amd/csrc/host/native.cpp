@@ -196,6 +196,9 @@ PyMethodDef kMethods[] = {
     {"add_layer_norm", (PyCFunction)(void (*)(void))add_layer_norm, METH_FASTCALL, "residual add and layer norm, differentiable; None: not the ordinary case"},
     {"epilogue", (PyCFunction)(void (*)(void))epilogue, METH_FASTCALL, "raw operands and an epilogue, differentiable; None: not the ordinary case"},
     {"epilogue_prepared", (PyCFunction)(void (*)(void))epilogue_prepared, METH_FASTCALL, "prepared weight and an epilogue; None: not the ordinary case"},
+    {"block_scaled", (PyCFunction)(void (*)(void))block_scaled, METH_FASTCALL, "block-scaled product, differentiable; None: not the ordinary case"},
+    {"gated_add_norm", (PyCFunction)(void (*)(void))gated_add_norm, METH_FASTCALL, "norms around a residual add, differentiable; None: not the ordinary case"},
+    {"clip_gradients", (PyCFunction)(void (*)(void))clip_gradients, METH_FASTCALL, "gradients' norm and clipping; None: not the ordinary case"},
     {"init_scales", init_scales, METH_O, "hands over the dict of the scale searches' scratch"},
     {"init", init, METH_O, "hands over the workspaces' dict"},
     {nullptr, nullptr, 0, nullptr},

@@ -4,36 +4,14 @@
 // time, and a forward and backward pass through Python autograd functions 180.  As in native.cpp everything here is a short cut: a function
 // returns None whenever a call is not the ordinary case and the Python code, which holds all rules and raises all errors, takes it from the start.
 // The gradients' nodes are the counterparts of the Python autograd functions (layer_norm.py, matmul_epilogue.py), and like them differentiable once.
-#include "native_common.h"
+#include "native_autograd.h"
 
 #include "native_operators.h"
 
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-
 #include <mutex>
-#include <optional>
 
 namespace native {
 namespace {
-
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-void check(int st, const char* where) { TORCH_CHECK(st == CASCMM_OK, where, " failed: ", cascmm_strerror(st), " (status ", st, ")"); }
-
-hipStream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-const void* data_of(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-at::Tensor scratch(size_t bytes, const at::Tensor& like) { return at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(like.device())); }
-at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor& like) { return at::empty(sizes, at::TensorOptions().dtype(like.scalar_type()).device(like.device())); }
-
-// rows of `t` (all of it known not to be empty), copied where its strides are not those of rows
-at::Tensor as_rows(const at::Tensor& t, int64_t& rows, int64_t& cols, int64_t& ld) {
-  if (rows_of(t, rows, cols, ld)) return t;
-  at::Tensor c = t.contiguous();
-  rows_of(c, rows, cols, ld);
-  return c;
-}
 
 // 16-bit operands off dwords: what the library copies of them beyond what cascmm_workspace_bytes counts, and copies made here where the library makes none (_copied_bytes
 // and _kernel_rows of matmul_epilogue.py)
@@ -46,48 +24,6 @@ at::Tensor kernel_rows(const at::Tensor& t, int64_t cols, int64_t& ld, bool copy
   if (t.element_size() != 2 || (!copy && (ld == cols || ld * 2 * 512 < INT32_MAX))) return t;
   ld = cols;
   return t.clone(at::MemoryFormat::Contiguous);
-}
-
-bool differentiated(std::initializer_list<const at::Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const at::Tensor* t : tensors)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
-// gradients that are asked to be differentiated again say so when they are (what once_differentiable does for a Python function)
-variable_list once(variable_list grads, const char* name, bool again) {
-  if (!again) return grads;
-  at::AutoGradMode enabled(true);
-  for (at::Tensor& g : grads)
-    if (g.defined()) g = g.detach().set_requires_grad(true);
-  auto raise = std::make_shared<torch::autograd::DelayedError>(std::string("trying to differentiate twice a function that is differentiable once: ") + name, (int64_t)grads.size());
-  return (*raise)(std::move(grads));
-}
-
-// An optional input of a node: those that are there count among the node's edges, in the order of the arguments
-typedef std::optional<at::Tensor> Optional;
-Optional optional_of(const at::Tensor& t) { return t.defined() ? Optional(t) : std::nullopt; }
-at::Tensor tensor_of(const Optional& t) { return t ? *t : at::Tensor(); }
-struct Wanted {
-  AutogradContext* ctx;
-  size_t edge = 0;
-  bool next(bool there = true) { return there && ctx->needs_input_grad(edge++); }
-};
-
-// a tensor whose forward-mode tangent would be lost here (the wrapper raises)
-bool dual(std::initializer_list<const at::Tensor*> tensors) {
-  for (const at::Tensor* t : tensors)
-    if (t->defined() && t->_fw_grad(0).defined()) return true;
-  return false;
-}
-
-// a tensor or None (undefined); false: not the ordinary case
-bool optional_tensor(PyObject* o, int device, at::Tensor& t) {
-  if (o == Py_None) return true;
-  const at::Tensor* p = gpu_tensor(o, device);
-  if (!p) return false;
-  t = *p;
-  return true;
 }
 
 // ---------------------------------------------------------------------------------------

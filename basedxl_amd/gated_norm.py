@@ -142,6 +142,10 @@ def gated_add_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[tor
     pass holds five rows of sums for each); gate and scale may be scalars too; ``post_weight`` and ``post_bias`` are [C].  All of the dtype of ``x`` or fp32; None: ones, for a bias
     zeros.  The norm is of ``s`` as it is returned, rounded to the tensors' dtype; statistics and arithmetic are fp32, each result is rounded once.
     Differentiable once in all tensors, through both results; sums over rows are added in a fixed order, so the same call gives the same bits."""
+    # the ordinary eager call in one native function; None: whatever is not ordinary about it is decided below
+    both = _lib.short_cut().gated_add_norm(x, residual, weight, bias, gate, residual_scale, post_weight, post_bias, post_norm, _NORMS.get(norm, -1) if type(norm) is str else -1, eps)
+    if both is not None:
+        return both
     if not x.is_cuda:
         raise RuntimeError(f"gated_add_norm: x is on {x.device}; the operator only runs on an AMD GPU (there is no CPU fallback)")
     if x.dtype not in _DTYPES:

@@ -68,6 +68,9 @@ def gradient_norm(gradients: Iterable[torch.Tensor], norm_type: float = 2.0) -> 
     """The norm (1, 2 or inf) of all elements of all ``gradients`` taken together, a device scalar in fp32; nothing waits for it.  fp32, fp16 and bf16
     tensors of any strides on one GPU, the types mixed at will.  Squares and sums are fp64 in a fixed order: the same call gives the same bits."""
     gradients = list(gradients)
+    norm = _lib.short_cut().clip_gradients(gradients, None, _NORM_TYPES.get(norm_type, -1), 0.0)   # the ordinary call in one native function; None: it is decided below
+    if norm is not None:
+        return norm
     kind = _check(gradients, norm_type, "gradient_norm")
     return _run([g if _dense(g) else g.contiguous() for g in gradients], None, kind, 0.0)
 
@@ -80,11 +83,14 @@ def clip_gradients(gradients: Iterable[torch.Tensor], max_norm: float, *, norm_t
     in place that need no clipping are not written.  A NaN among the gradients makes all of them NaN; an infinity makes the factor 0 and itself NaN.  A result shares memory
     with no other result and no gradient but its own (CascmmError): a tensor that is listed twice would be scaled twice."""
     gradients = list(gradients)
+    results = gradients if out is None else list(out)
+    norm = _lib.short_cut().clip_gradients(gradients, results, _NORM_TYPES.get(norm_type, -1), max_norm)
+    if norm is not None:
+        return norm
     kind = _check(gradients, norm_type, "clip_gradients")
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_gradients: max_norm must be a number from 0 on, got {max_norm}")
-    results = gradients if out is None else list(out)
     if len(results) != len(gradients):
         raise ValueError(f"clip_gradients: {len(gradients)} gradients but {len(results)} results")
     sources, targets, copied = [], [], []

@@ -11,10 +11,19 @@ import math
 import pytest
 import torch
 
-from basedxl_amd import BlockScaledWeight, block_scaled_matmul
+from basedxl_amd import _lib, BlockScaledWeight, block_scaled_matmul
 from basedxl_amd.block_scaled import _round
 
 pytestmark = pytest.mark.gpu
+
+@pytest.fixture(params=["native", "python"], autouse=True)
+def path(request, monkeypatch):
+    """Ordinary eager calls by the host extension, and everything by the Python code."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_short_cut", _lib._NoShortCut)
+    else:
+        assert _lib.short_cut() is _lib.native()
+    return request.param
 
 U = 2.0 ** -24
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
@@ -282,6 +291,17 @@ def test_scales_far_apart(gpu_device, ea, eb):
     check_product(block_scaled_matmul(a.to(gpu_device), b.to(gpu_device)), held(a, "rows")[0], held(b, "square")[0], None, "fp32")
     a16, b16 = a.bfloat16(), b.bfloat16()
     check_product(block_scaled_matmul(a16.to(gpu_device), b16.to(gpu_device)), held(a16, "rows")[0], held(b16, "square")[0], None, "bf16")
+
+
+def test_ordinary_calls_are_one_native_function(gpu_device):
+    x, w, b = (torch.ones(s, device=gpu_device, dtype=torch.bfloat16) for s in ((4, 20, 64), (64, 32), (32,)))
+    held = BlockScaledWeight(w)
+    f = _lib.native().block_scaled
+    for args in ((x, w, None, 0, 0, 0, b), (x, w.t().contiguous().t(), None, 0, 0, 0, None), (x, held.values, held.scales, 64, 32, _lib.DT_BF16, b), (x.clone().requires_grad_(), w, None, 0, 0, 0, b)):
+        assert f(*args).shape == (4, 20, 32)
+    for args in ((x, w.half(), None, 0, 0, 0, b), (x, w, None, 0, 0, 0, b[:31]), (x, held.values, held.scales, 63, 32, _lib.DT_BF16, b), (x, held.values, held.scales, 64, 33, _lib.DT_BF16, None),
+                 (x, held.values[:1], held.scales, 64, 32, _lib.DT_BF16, b), (x, held.values, held.scales, 64, 32, _lib.DT_F16, b), (x.cpu(), w, None, 0, 0, 0, b), (x, w, None, 0, 0, 0), (x[:0], w, None, 0, 0, 0, b)):
+        assert f(*args) is None
 
 
 def test_nothing_to_do(gpu_device):

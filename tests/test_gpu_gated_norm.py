@@ -10,9 +10,18 @@ import math
 import pytest
 import torch
 
-from basedxl_amd import add_layer_norm, gated_add_norm
+from basedxl_amd import _lib, add_layer_norm, gated_add_norm
 
 pytestmark = pytest.mark.gpu
+
+@pytest.fixture(params=["native", "python"], autouse=True)
+def path(request, monkeypatch):
+    """Ordinary eager calls by the host extension, and everything by the Python code."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_short_cut", _lib._NoShortCut)
+    else:
+        assert _lib.short_cut() is _lib.native()
+    return request.param
 
 U = 2.0 ** -24
 TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}
@@ -268,6 +277,18 @@ def test_rows_that_are_not_finite_stay_alone(gpu_device, cols, dtype):
     keep[touched] = False
     assert torch.equal(y[0][keep], clean[0][0][keep]) and torch.equal(s[0][keep], clean[1][0][keep])
     assert bool(y[0, 3].isnan().all() and y[0, 7].isnan().all() and y[0, 9].isfinite().all())
+
+
+def test_ordinary_calls_are_one_native_function(gpu_device):
+    x, c, g = torch.ones(3, 4, 64, device=gpu_device), torch.ones(64, device=gpu_device), torch.ones(3, 1, 64, device=gpu_device)
+    f = _lib.native().gated_add_norm
+    for args in ((x, x, c, c, g, 1.0, None, None, False, 0, 1e-5), (x, x, None, None, None, g, c, c, True, 1, 1e-5), (x.clone().requires_grad_(), x, g, g, c, 0.5, None, None, False, 1, 0.0)):
+        y, s = f(*args)
+        assert y.shape == s.shape == x.shape
+    for args in ((x, x, c, c, g[:2], 1.0, None, None, False, 0, 1e-5), (x, x, c.half(), c, g, 1.0, None, None, False, 0, 1e-5), (x, x, c, c, g, 1.0, c, None, False, 0, 1e-5),
+                 (x, x, c, c, g, 1.0, None, None, False, 2, 1e-5), (x, x, c, c, g, 1.0, None, None, False, 0, -1.0), (x, x, c, c, g, math.inf, None, None, False, 0, 1e-5),
+                 (x, x, c, c, g, 1.0, g, None, True, 0, 1e-5), (x, x[:2], c, c, g, 1.0, None, None, False, 0, 1e-5), (x, x, c, c, g, 1.0, None, None, False, 0)):
+        assert f(*args) is None
 
 
 def test_nothing_to_do(gpu_device):

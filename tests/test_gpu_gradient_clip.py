@@ -12,6 +12,15 @@ from basedxl_amd import _lib, clip_grad_norm_, clip_gradients, gradient_norm
 
 pytestmark = pytest.mark.gpu
 
+@pytest.fixture(params=["native", "python"], autouse=True)
+def path(request, monkeypatch):
+    """Ordinary eager calls by the host extension, and everything by the Python code."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_short_cut", _lib._NoShortCut)
+    else:
+        assert _lib.short_cut() is _lib.native()
+    return request.param
+
 U = 2.0 ** -24
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}
@@ -150,6 +159,15 @@ def test_refusals(gpu_device):
         gradient_norm([g, torch.ones(3)])
     assert bool((g == 1).all() and (h == 1).all())
     assert torch.equal(gradient_norm([g, g]), gradient_norm([g, h]))                   # (a norm reads only)
+
+
+def test_ordinary_calls_are_one_native_function(gpu_device):
+    g, h = torch.ones(8, 3, device=gpu_device), torch.ones(8, 3, device=gpu_device, dtype=torch.bfloat16)
+    f = _lib.native().clip_gradients
+    assert f([g, h], None, 2, 0.0).shape == () and f([g, h], [g, h], 0, 1.0).shape == () and f([g.t(), h], [torch.ones_like(g).t(), torch.ones_like(g)], 2, 1.0).shape == ()
+    for args in (([], None, 2, 0.0), ([g, g], [g, g], 2, 1.0), ([g], [g[:4]], 2, 1.0), ([g], [h], 2, 1.0), ([g], [g], 3, 1.0), ([g], [g], 2, -1.0), ([g.cpu()], None, 2, 0.0), ([g[:, :2]], None, 2, 0.0),
+                 ([g], [g.t().contiguous().t()], 2, 1.0), ((g,), None, 2, 0.0), ([g], [g, g], 2, 1.0), ([g.double()], None, 2, 0.0), ([g], [None], 2, 1.0)):
+        assert f(*args) is None
 
 
 def test_parameters(gpu_device):
