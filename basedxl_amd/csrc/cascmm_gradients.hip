@@ -13,7 +13,7 @@ namespace cascmm {
 static int64_t grad_size(int dtype) { return dtype == CASCMM_DT_F32 ? 4 : 2; }
 static bool grad_dtype(int dtype) { return dtype == CASCMM_DT_F32 || dtype == CASCMM_DT_F16 || dtype == CASCMM_DT_BF16; }
 
-// Elements of a chunk: about 8192 chunks of what there is, 4096 elements at least
+// Elements of a chunk: about 2048 chunks of what there is, 4096 elements at least; of more than 2^26 elements 8192 chunks, which balance better over several launches
 struct GradPlan { int64_t chunk, parts; };
 static int grad_plan(int count, const cascmm_gradient* list, GradPlan& plan) {
   if (count < 0) return CASCMM_ERR_BAD_SHAPE;
@@ -23,7 +23,8 @@ static int grad_plan(int count, const cascmm_gradient* list, GradPlan& plan) {
     if (list[i].elements < 0) return CASCMM_ERR_BAD_SHAPE;
     if (__builtin_add_overflow(total, list[i].elements, &total) || total > (int64_t)1 << 48) return CASCMM_ERR_TOO_LARGE;
   }
-  plan.chunk = std::max<int64_t>(kGradChunk, ((total + 8191) / 8192 + kGradChunk - 1) / kGradChunk * kGradChunk);
+  const int64_t most = total > ((int64_t)1 << 26) ? 8192 : 2048;
+  plan.chunk = std::max<int64_t>(kGradChunk, ((total + most - 1) / most + 255) / 256 * 256);
   plan.parts = 0;
   for (int i = 0; i < count; ++i) plan.parts += (list[i].elements + plan.chunk - 1) / plan.chunk;
   return plan.parts > (1 << 24) ? CASCMM_ERR_TOO_LARGE : CASCMM_OK;   // (a launch has fewer than 2^32 threads)

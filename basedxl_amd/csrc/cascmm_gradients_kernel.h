@@ -15,7 +15,7 @@ namespace cascmm {
 
 constexpr int kGradTensors = 96;          // of one launch (arguments of 2.7 KB)
 constexpr int64_t kGradChunk = 4096;      // elements of a chunk, at least
-constexpr int kGradMerged = 512;          // partial sums that every workgroup of the second pass adds itself
+constexpr int kGradMerged = 2560;         // partial sums that every workgroup of the second pass adds itself
 struct GradBatch {
   int64_t chunk;
   double* parts;        // of all chunks of the call

@@ -32,7 +32,8 @@ LISTS = {
     "all_empty": [(0,), (0, 5)],
     "chunk_edges": [(4095,), (4096,), (4097,), (8192,), (4096 * 3 + 1,)],
     "many": [(1 + i % 37,) for i in range(301)],
-    "more_parts_than_merged": [(4096 * 600 + 5,), (77,)],
+    "chunks_of_other_sizes": [(4096 * 2100 + 5,), (77,), (4096 * 300,)],
+    "more_parts_than_merged": [(1 + i % 9,) for i in range(2700)],
     "large": [(4097, 8195), (129,), (1000, 1000)],
 }
 
