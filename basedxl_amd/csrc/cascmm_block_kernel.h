@@ -327,9 +327,94 @@ __device__ __forceinline__ void block_place(unsigned w, int tiles_m, int tiles_n
   tile_n = (int)(in / down);
 }
 
+// A wave's loads of a stage: 1 KB of rows each, and 256 bytes of scales
+template <typename T> struct BlockLoads {
+  __amdgpu_buffer_rsrc_t ra, rb, rsa, rsb;
+  int from[T::LOADS], scale_from[T::SCALES], wave;
+  __device__ __forceinline__ BlockLoads(const BlockGemmParams& p, int m0, int n0, int wave_, int lane) : wave(wave_) {
+    const int64_t kp = (int64_t)p.blocks * kBlock;
+    // (a tile's rows lie below 2 GiB from its first: host-checked)
+    ra = __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + m0 * kp), 0, 0x7FFFFFFF, 0x00020000);
+    rb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.b + n0 * kp), 0, 0x7FFFFFFF, 0x00020000);
+    rsa = __builtin_amdgcn_make_buffer_rsrc((void*)(p.sa + m0), 0, 0x7FFFFFFF, 0x00020000);
+    rsb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.sb + n0), 0, 0x7FFFFFFF, 0x00020000);
+    const int last_m = p.M - m0 - 1, last_n = p.N - n0 - 1;     // (rows past the edge: the last one again)
+#pragma unroll
+    for (int j = 0; j < T::LOADS; ++j) {
+      const int r = (wave + T::WAVES * j) * 8 + (lane >> 3), row = r < T::BM ? (r < last_m ? r : last_m) : (r - T::BM < last_n ? r - T::BM : last_n);
+      from[j] = (int)(row * kp) + (((lane & 7) ^ (r & 7)) << 4);
+    }
+#pragma unroll
+    for (int j = 0; j < T::SCALES; ++j) {
+      const int r = (wave + T::WAVES * j) % (T::ROWS / 64) * 64 + lane;
+      scale_from[j] = 4 * (r < T::BM ? (r < last_m ? r : last_m) : (r - T::BM < last_n ? r - T::BM : last_n));
+    }
+  }
+  // load j of block `block` of k to the stage at `to`, the first ones those of the scales
+  __device__ __forceinline__ void issue(const BlockGemmParams& p, int block, unsigned char* to, int j) const {
+    if (j < T::SCALES) {
+      const int run = (wave + T::WAVES * j) % (T::ROWS / 64);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(run * 64 < T::BM ? rsa : rsb, (block_lds_ptr)(to + T::ROWS * 128 + run * 256), 4, scale_from[j], (block >> 2) * 4 * (run * 64 < T::BM ? p.M : p.N), 0, 0);
+    } else {
+      const int run = wave + T::WAVES * (j - T::SCALES);
+      block_load_lds(run * 8 < T::BM ? ra : rb, to + run * 1024, from[j - T::SCALES], block * kBlock);
+    }
+  }
+};
+
+template <int IODT, typename T>
+__device__ __forceinline__ void block_store(const BlockGemmParams& p, const f32x16 (&acc)[T::MT][T::NT], unsigned char* smem, int m0, int n0, int wave, int lane) {
+  typedef typename IoType<IODT>::T E;
+  constexpr int MT = T::MT, NT = T::NT;
+  const int l31 = lane & 31, h = lane >> 5, wm = (wave / T::WN) * 32 * MT, wn = (wave % T::WN) * 32 * NT;
+  // A lane holds row l31 of a block, columns 8 q + 4 h + e: sixteen bytes of a row and less.  Through LDS, in a place of each wave's own, 32 rows of the wave's width at a time, so that
+  // what is stored are whole pieces of rows.
+  typedef E four __attribute__((ext_vector_type(4), aligned(4 * sizeof(E))));
+  constexpr int VEC = 16 / (int)sizeof(E), WIDTH = 32 * NT, PITCH = WIDTH + VEC, PIECES = WIDTH / VEC, STORES = 32 * PIECES / 64;   // (elements; pieces of a row; stores of a lane)
+  static_assert(32 * PIECES % 64 == 0 && T::WAVES * 32 * PITCH * (int)sizeof(E) <= T::LDS, "the rows of a store");
+  typedef E chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
+  E* const mine = (E*)smem + wave * 32 * PITCH;
+  float bias[NT][4][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + wn + 32 * j + 8 * q + 4 * h + e;
+        bias[j][q][e] = p.bias ? IoType<IODT>::load((const E*)p.bias + (n < p.N ? n : p.N - 1)) : 0.f;
+      }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        four o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (E)(acc[i][j][4 * q + e] + bias[j][q][e]);
+        *(four*)(mine + l31 * PITCH + 32 * j + 8 * q + 4 * h) = o;
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int k = 0; k < STORES; ++k) {
+      const int id = k * 64 + lane, r = id / PIECES, m = m0 + wm + 32 * i + r, column = n0 + wn + id % PIECES * VEC;
+      const chunk o = *(const chunk*)__builtin_assume_aligned(mine + r * PITCH + id % PIECES * VEC, 16);
+      E* to = (E*)p.c + m * p.ldc + column;
+      if (m < p.M && column + VEC <= p.N) {
+        *(chunk*)to = o;
+      } else if (m < p.M) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (column + e < p.N) to[e] = o[e];
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
 template <int IODT, typename T, bool FINE>
 __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const BlockGemmParams p) {
-  typedef typename IoType<IODT>::T E;
   constexpr int MT = T::MT, NT = T::NT, BM = T::BM, BN = T::BN;
   extern __shared__ __attribute__((aligned(1024))) unsigned char block_smem[];
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
@@ -337,39 +422,12 @@ __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const Blo
   int tile_m, tile_n;
   block_place(blockIdx.x, p.tiles_m, p.tiles_n, T::BAND, tile_m, tile_n);
   const int m0 = tile_m * BM, n0 = tile_n * BN, wm = (wave / T::WN) * 32 * MT, wn = (wave % T::WN) * 32 * NT;
-  const int64_t kp = (int64_t)p.blocks * kBlock;
-  // (a tile's rows lie below 2 GiB from its first: host-checked)
-  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + m0 * kp), 0, 0x7FFFFFFF, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.b + n0 * kp), 0, 0x7FFFFFFF, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc((void*)(p.sa + m0), 0, 0x7FFFFFFF, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.sb + n0), 0, 0x7FFFFFFF, 0x00020000);
-  const int last_m = p.M - m0 - 1, last_n = p.N - n0 - 1;     // (rows past the edge: the last one again)
-  int from[T::LOADS], scale_from[T::SCALES];
-#pragma unroll
-  for (int j = 0; j < T::LOADS; ++j) {
-    const int r = (wave + T::WAVES * j) * 8 + (lane >> 3), row = r < BM ? (r < last_m ? r : last_m) : (r - BM < last_n ? r - BM : last_n);
-    from[j] = (int)(row * kp) + (((lane & 7) ^ (r & 7)) << 4);
-  }
-#pragma unroll
-  for (int j = 0; j < T::SCALES; ++j) {
-    const int run = (wave + T::WAVES * j) % (T::ROWS / 64), r = run * 64 + lane;
-    scale_from[j] = 4 * (r < BM ? (r < last_m ? r : last_m) : (r - BM < last_n ? r - BM : last_n));
-  }
   // this share's blocks; all shares take as many steps, those past the last block without products
   const int steps = (p.blocks + T::SHARES - 1) / T::SHARES, first = share * steps, live = p.blocks - first < steps ? p.blocks - first : steps;
   unsigned char* const ring = block_smem + share * T::DEEP * T::STAGE;
-  // load j of a stage, the first ones of the rows' scales; `to`: the stage's place
-  auto issue = [&](int step, unsigned char* to, int j) {
-    step = first + step < p.blocks ? first + step : p.blocks - 1;     // (past the end: the last one again, so that every share waits for as many)
-    if (j < T::SCALES) {
-      const int run = (wave + T::WAVES * j) % (T::ROWS / 64);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(run * 64 < BM ? rsa : rsb, (block_lds_ptr)(to + T::ROWS * 128 + run * 256), 4, scale_from[j],
-                                               (step >> 2) * 4 * (run * 64 < BM ? p.M : p.N), 0, 0);
-    } else {
-      j -= T::SCALES;
-      block_load_lds((wave + T::WAVES * j) * 8 < BM ? ra : rb, to + (wave + T::WAVES * j) * 1024, from[j], step * kBlock);
-    }
-  };
+  const BlockLoads<T> loads(p, m0, n0, wave, lane);
+  // (past the end: the last block again, so that every share waits for as many)
+  auto issue = [&](int step, unsigned char* to, int j) { loads.issue(p, first + step < p.blocks ? first + step : p.blocks - 1, to, j); };
   constexpr int ISSUES = T::LOADS + T::SCALES, GAPS = MT * NT, READS = 2 * (MT + NT);
   f32x16 acc[MT][NT];
 #pragma unroll
@@ -465,12 +523,6 @@ __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const Blo
     __builtin_amdgcn_s_waitcnt(0x0F70);      // (the redundant loads land before LDS is given up)
   }
 #undef BLOCK_FENCE
-  // A lane holds row l31 of a block, columns 8 q + 4 h + e: sixteen bytes of a row and less.  Through LDS, in a place of each wave's own, 32 rows of the wave's width at a time, so that
-  // what is stored are whole pieces of rows.
-  typedef E four __attribute__((ext_vector_type(4), aligned(4 * sizeof(E))));
-  constexpr int VEC = 16 / (int)sizeof(E), WIDTH = 32 * NT, PITCH = WIDTH + VEC, LANES = WIDTH / VEC, AT_ONCE = 64 / LANES;   // (elements; lanes of a row; rows of a store)
-  static_assert(64 % LANES == 0 && T::WAVES * 32 * PITCH * (int)sizeof(E) <= T::LDS, "the rows of a store");
-  typedef E chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(E))));
   __syncthreads();
   if constexpr (T::SHARES > 1) {
     float* const meet = (float*)block_smem + (wave * MT * NT * 16) * 64 + lane;
@@ -498,45 +550,7 @@ __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const Blo
     __syncthreads();
     if (share > 0) return;
   }
-  E* const mine = (E*)block_smem + wave * 32 * PITCH;
-  float bias[NT][4][4];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = n0 + wn + 32 * j + 8 * q + 4 * h + e;
-        bias[j][q][e] = p.bias ? IoType<IODT>::load((const E*)p.bias + (n < p.N ? n : p.N - 1)) : 0.f;
-      }
-  const int column = n0 + wn + lane % LANES * VEC;
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        four o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (E)(acc[i][j][4 * q + e] + bias[j][q][e]);
-        *(four*)(mine + l31 * PITCH + 32 * j + 8 * q + 4 * h) = o;
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int k = 0; k < 32 / AT_ONCE; ++k) {
-      const int r = k * AT_ONCE + lane / LANES, m = m0 + wm + 32 * i + r;
-      const chunk o = *(const chunk*)__builtin_assume_aligned(mine + r * PITCH + lane % LANES * VEC, 16);
-      E* to = (E*)p.c + m * p.ldc + column;
-      if (m < p.M && column + VEC <= p.N) {
-        *(chunk*)to = o;
-      } else if (m < p.M) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (column + e < p.N) to[e] = o[e];
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  }
+  block_store<IODT, T>(p, acc, block_smem, m0, n0, wave, lane);
 }
 
 // ---------------------------------------------------------------------------------------

@@ -137,13 +137,15 @@ int cascmm_gated_norm_backward(const cascmm_gated_norm* args, void* workspace, s
     f.gate_ld = a.gate_ld;
     f.parts = a.rows > 0 ? plan.parts : 0;
     f.cols = (int)a.cols;
-    f.rich = plan.lanes == 0 || plan.rich;     // (the sums of rows without registers are always five)
-    f.share = 32;
-    while (f.share > 1 && 32 / f.share < plan.groups) f.share /= 2;
+    const bool rich = plan.lanes == 0 || plan.rich;     // (the sums of rows without registers are always five)
     f.gate_grouped = a.gate_ld != 0; f.scale_grouped = a.scale_ld != 0; f.weight_grouped = a.weight_ld != 0; f.bias_grouped = a.bias_ld != 0;
-    err = a.weight_dtype == CASCMM_DT_F32   ? gated_finish<CASCMM_DT_F32>(f, s)
-          : a.weight_dtype == CASCMM_DT_F16 ? gated_finish<CASCMM_DT_F16>(f, s)
-                                            : gated_finish<CASCMM_DT_BF16>(f, s);
+    f.shared = a.dpost_weight || a.dpost_bias || (a.dgate && !f.gate_grouped) || (a.dscale && !f.scale_grouped) || (a.dweight && !f.weight_grouped) || (a.dbias && !f.bias_grouped);
+    // (rows of threads on a group: as many as leave one for each group; where no gradient runs over the groups there are more workgroups, and eight rows add the parts of each of four groups)
+    f.share = f.shared ? 32 : plan.parts >= 4 ? 8 : 1;
+    while (f.shared && f.share > 1 && 32 / f.share < plan.groups) f.share /= 2;
+    err = a.weight_dtype == CASCMM_DT_F32   ? gated_finish<CASCMM_DT_F32>(f, rich, s)
+          : a.weight_dtype == CASCMM_DT_F16 ? gated_finish<CASCMM_DT_F16>(f, rich, s)
+                                            : gated_finish<CASCMM_DT_BF16>(f, rich, s);
   }
   return err == hipSuccess ? CASCMM_OK : CASCMM_ERR_LAUNCH;
 }

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void cascmm_gated_norm_kernel(const GatedParam
   }
 }
 
-// RICH: five sums, else S1, S4 and S5
+// RICH: five sums, else S1, S4 and S5.
 template <int IODT, int NV, int LPR, bool POST, bool RICH>
 __global__ __launch_bounds__(256) void cascmm_gated_norm_backward_kernel(const GatedParams p) {
   typedef GatedRow<IODT, LPR, NV, POST, RICH> G;
@@ -260,10 +260,10 @@ __global__ __launch_bounds__(256) void cascmm_gated_norm_backward_kernel(const G
       }
     norm_sums<LPR>(means, slots, turn);
     const float c1 = p.centred ? means[0] * p.inv_cols : 0.f, c2 = means[1] * p.inv_cols;
-    float D[CH][VEC], post[2] = {0.f, 0.f};
+    float D[POST ? CH : 1][VEC], post[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      chunk out;
+      chunk out, dx;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float shat = ((float)cur.s[c][e] - cur.mean2) * cur.rstd2;
@@ -275,34 +275,33 @@ __global__ __launch_bounds__(256) void cascmm_gated_norm_backward_kernel(const G
           sum[1][c][e] += d;
           sum[2][c][e] = __builtin_fmaf(d, (float)cur.r[c][e], sum[2][c][e]);
         }
-        D[c][e] = d * g.P[c][e];
+        const float q = d * g.P[c][e];
         if constexpr (POST) {
-          post[0] += D[c][e];
-          post[1] = __builtin_fmaf(D[c][e], xhat, post[1]);
+          D[c][e] = q;
+          post[0] += q;
+          post[1] = __builtin_fmaf(q, xhat, post[1]);
+        } else {
+          dx[e] = (E)q;
         }
       }
       if (p.dresidual) R::store((E*)p.dresidual + at * p.lddr, col0 + c * STEP, cols, out, c < FULL);
+      if constexpr (!POST)
+        if (p.dx) R::store((E*)p.dx + at * p.lddx, col0 + c * STEP, cols, dx, c < FULL);
     }
-    if (!p.dx) continue;   // (of all lanes)
-    float c3 = 0.f, c4 = 0.f;
     if constexpr (POST) {
+      if (!p.dx) continue;   // (of all lanes)
       norm_sums<LPR>(post, slots, turn);
-      c3 = p.centred ? post[0] * p.inv_cols : 0.f;
-      c4 = post[1] * p.inv_cols;
-    }
+      const float c3 = p.centred ? post[0] * p.inv_cols : 0.f, c4 = post[1] * p.inv_cols;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      chunk out;
+      for (int c = 0; c < CH; ++c) {
+        chunk out;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if constexpr (POST) {
+        for (int e = 0; e < VEC; ++e) {
           const float xhat = ((float)cur.x[c][e] - cur.mean1) * cur.rstd1;
           out[e] = (E)(cur.rstd1 * (D[c][e] - c3 - xhat * c4));
-        } else {
-          out[e] = (E)D[c][e];
         }
+        R::store((E*)p.dx + at * p.lddx, col0 + c * STEP, cols, out, c < FULL);
       }
-      R::store((E*)p.dx + at * p.lddx, col0 + c * STEP, cols, out, c < FULL);
     }
   }
   if (!p.partials) return;
@@ -551,53 +550,56 @@ struct GatedFinish {
   const void *gate, *post_weight, *post_bias;
   void *dgate, *dscale, *dpost_weight, *dpost_bias, *dweight, *dbias;   // NULL: not wanted
   int64_t groups, gate_ld;
-  int parts, cols, rich, share;  // parts 0: there are no rows
+  int parts, cols, share;        // parts 0: there are no rows
+  int shared;                    // a gradient over all groups is wanted: one workgroup of the grid's second axis, else 32 / share groups each
   int gate_grouped, scale_grouped, weight_grouped, bias_grouped;        // a gradient for each group
 };
-template <int ODT>
+template <int ODT, bool RICH>
 __global__ __launch_bounds__(1024) void cascmm_gated_norm_finish_kernel(const GatedFinish p) {
   typedef typename IoType<ODT>::T E;
-  __shared__ float meet[5][32][33];
+  constexpr int NS = RICH ? 5 : 3;
+  __shared__ float meet[NS][32][33];
   const int c = threadIdx.x & 31, r = threadIdx.x >> 5, slot = r / p.share, sub = r % p.share, at_a_time = 32 / p.share;
   const int64_t col = (int64_t)blockIdx.x * 32 + c;
   const bool in = col < p.cols;
-  const int ns = p.rich ? 5 : 3;
   float total[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};    // gate, scale, post_weight, post_bias, weight, bias
   const float w1 = in && p.post_weight ? (float)((const E*)p.post_weight)[col] : 1.f, b1 = in && p.post_bias ? (float)((const E*)p.post_bias)[col] : 0.f;
   auto store = [&](void* to, int64_t at, float v) {
     if (to && in) IoType<ODT>::store((E*)to + at, v);
   };
-  for (int64_t base = 0; base < p.groups; base += at_a_time) {
+  for (int64_t base = p.shared ? 0 : (int64_t)blockIdx.y * at_a_time; base < p.groups; base += p.shared ? at_a_time : (int64_t)gridDim.y * at_a_time) {
     const int64_t group = base + slot;
-    float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+    float s[NS], gate = 1.f;
+#pragma unroll
+    for (int k = 0; k < NS; ++k) s[k] = 0.f;
     if (in && group < p.groups) {
-      const float* src = p.partials + group * p.parts * ns * p.cols + col;
-      for (int i = sub; i < p.parts; i += p.share * 4) {   // (loads of four parts in flight)
-        float v[4][5];
+      if (p.gate) gate = (float)((const E*)p.gate)[group * p.gate_ld + col];
+      const float* src = p.partials + group * p.parts * NS * p.cols + col;
+      for (int i = sub; i < p.parts; i += p.share * 8) {   // (loads of eight parts in flight, the last part again past the end: a load under a condition is waited for by itself)
+        float v[8][NS];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 8; ++u)
 #pragma unroll
-          for (int k = 0; k < 5; ++k) v[u][k] = k < ns && i + u * p.share < p.parts ? src[((int64_t)(i + u * p.share) * ns + k) * p.cols] : 0.f;
+          for (int k = 0; k < NS; ++k) v[u][k] = src[((int64_t)(i + u * p.share < p.parts ? i + u * p.share : p.parts - 1) * NS + k) * p.cols];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 8; ++u)
 #pragma unroll
-          for (int k = 0; k < 5; ++k) s[k] += v[u][k];
+          for (int k = 0; k < NS; ++k) s[k] += i + u * p.share < p.parts ? v[u][k] : 0.f;
       }
     }
     if (p.share > 1) {
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 5; ++k) meet[k][r][c] = s[k];
+      for (int k = 0; k < NS; ++k) meet[k][r][c] = s[k];
       __syncthreads();
       if (sub == 0) {
 #pragma unroll
-        for (int k = 0; k < 5; ++k)
+        for (int k = 0; k < NS; ++k)
           for (int i = 1; i < p.share; ++i) s[k] += meet[k][r + i][c];
       }
     }
     if (sub == 0 && group < p.groups) {
-      const float s2 = p.rich ? s[1] : 0.f, s3 = p.rich ? s[2] : 0.f, s4 = p.rich ? s[3] : s[1], s5 = p.rich ? s[4] : s[2];
-      const float gate = in && p.gate ? (float)((const E*)p.gate)[group * p.gate_ld + col] : 1.f;
+      const float s2 = RICH ? s[1] : 0.f, s3 = RICH ? s[2] : 0.f, s4 = s[NS - 2], s5 = s[NS - 1];
       const float dgate = w1 * s[0] + b1 * s2;
       if (p.gate_grouped) store(p.dgate, group * p.cols + col, dgate);
       if (p.scale_grouped) store(p.dscale, group * p.cols + col, s3);
@@ -610,6 +612,15 @@ __global__ __launch_bounds__(1024) void cascmm_gated_norm_finish_kernel(const Ga
       total[4] += s4;
       total[5] += s5;
     }
+  }
+  if (!p.shared) return;
+  if (p.groups <= 1) {
+    if (r != 0) return;
+    void* const to[6] = {p.gate_grouped ? nullptr : p.dgate, p.scale_grouped ? nullptr : p.dscale, p.dpost_weight, p.dpost_bias, p.weight_grouped ? nullptr : p.dweight,
+                         p.bias_grouped ? nullptr : p.dbias};
+#pragma unroll
+    for (int k = 0; k < 6; ++k) store(to[k], col, total[k]);
+    return;
   }
   // over the groups, one gradient at a time (they share the first slots of the memory)
 #pragma unroll

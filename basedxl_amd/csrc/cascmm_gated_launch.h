@@ -7,7 +7,7 @@
 namespace cascmm {
 
 // The lanes of a row and the elements of a lane: sixteen lanes take rows of up to 256 columns, a wave up to 2048 (in the backward pass, which holds the sums beside a
-// row, 1536), four of them up to 8192 (backward 6144: beyond, five sums do not fit beside a row); none: longer rows, and rows shorter than 16 bytes
+// row, 1536; with four waves on rows of 1025 to 1536 columns 32768 x 1280 bf16 takes 151 us for 112), four of them up to 8192 (backward 6144: beyond, five sums do not fit beside a row); none: longer rows, and rows shorter than 16 bytes
 struct GatedShape { int lanes, values; };
 inline GatedShape gated_shape(int64_t cols, bool backward, int64_t chunk) {
   const auto fit = [&](int lanes) { return (int)std::min<int64_t>((cols + 8 * lanes - 1) / (8 * lanes) * 8, 1 << 20); };
@@ -17,9 +17,10 @@ inline GatedShape gated_shape(int64_t cols, bool backward, int64_t chunk) {
   if (fit(256) <= (backward ? 24 : 32)) return {256, fit(256)};
   return {0, 0};
 }
-// Workgroups of a group: in all as many as layer norm's (its figures: norm_groups), at least one to a group
+// Workgroups of a group: in all four on a CU forward (as layer norm's), backward one, as many as the registers of the longer rows leave room for (32768 x 1280 bf16, gated and
+// modulated, with the sums' kernel 112 us; 512 workgroups 121, 768 127, 1024 130; 8 x 1024 x 1280 fp32 57, 61, 67, 70; 32768 x 1024 bf16 85, 86, 97, 93), at least one to a group
 inline void gated_parts(int64_t groups, int64_t group_rows, int lanes, bool backward, int& parts, int64_t& part_rows) {
-  const int64_t at_a_time = lanes ? 256 / lanes * (backward ? 2 : 1) : 16, most = !lanes ? 512 : !backward ? 1024 : lanes == 256 ? 256 : lanes == 64 ? 512 : 1024;
+  const int64_t at_a_time = lanes ? 256 / lanes * (backward ? 2 : 1) : 16, most = !lanes ? 512 : !backward ? 1024 : lanes >= 64 ? 256 : 1024;
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>((group_rows + at_a_time - 1) / at_a_time, most / std::max<int64_t>(groups, 1)));
   part_rows = std::max<int64_t>(1, (group_rows + want - 1) / want);
   parts = (int)std::max<int64_t>(1, (group_rows + part_rows - 1) / part_rows);
@@ -90,15 +91,16 @@ template <int IODT> hipError_t gated_backward(const GatedParams& p, int64_t grou
   if (post) return rich ? gated_backward_of<IODT, true, true>(p, (unsigned)groups, s) : gated_backward_of<IODT, true, false>(p, (unsigned)groups, s);
   return rich ? gated_backward_of<IODT, false, true>(p, (unsigned)groups, s) : gated_backward_of<IODT, false, false>(p, (unsigned)groups, s);
 }
-template <int ODT> hipError_t gated_finish(const GatedFinish& p, hipStream_t s) {
+template <int ODT> hipError_t gated_finish(const GatedFinish& p, bool rich, hipStream_t s) {
   hipError_t err = hipSuccess;
-  CASCMM_LAUNCH(err, cascmm_gated_norm_finish_kernel<ODT>, dim3((unsigned)((p.cols + 31) / 32)), dim3(1024), 0, s, p);
+  const int64_t turns = (p.groups + 32 / p.share - 1) / (32 / p.share);
+  CASCMM_LAUNCH(err, (rich ? cascmm_gated_norm_finish_kernel<ODT, true> : cascmm_gated_norm_finish_kernel<ODT, false>), dim3((unsigned)((p.cols + 31) / 32), p.shared ? 1u : (unsigned)std::max<int64_t>(1, std::min<int64_t>(turns, 4096))), dim3(1024), 0, s, p);
   return err;
 }
 
 #define CASCMM_GATED_OF(LINKAGE, DT)                                                                        \
   LINKAGE template hipError_t gated_forward<DT>(const GatedParams&, int64_t, bool, bool, hipStream_t);      \
   LINKAGE template hipError_t gated_backward<DT>(const GatedParams&, int64_t, bool, bool, hipStream_t);     \
-  LINKAGE template hipError_t gated_finish<DT>(const GatedFinish&, hipStream_t);
+  LINKAGE template hipError_t gated_finish<DT>(const GatedFinish&, bool, hipStream_t);
 
 }  // namespace cascmm
