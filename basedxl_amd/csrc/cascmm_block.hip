@@ -48,6 +48,14 @@ static int block_tile(int64_t M, int64_t N, int64_t blocks, bool fine) {
   return best;
 }
 
+// Launches of fewer than 2^32 threads, and scales that 31 bits of an offset span
+static bool block_too_large(int64_t M, int64_t N, int64_t K, bool fine) {
+  if (M > INT32_MAX || N > INT32_MAX || K > kBlockMostK || block_scale_bytes(std::max(M, N), K) > INT32_MAX) return true;
+  const int tile = block_tile(M, N, block_padded(K) / kBlock, fine);
+  const int64_t bm = tile <= kTile64Shares ? 64 : tile == kTile256 ? 256 : 128, bn = tile <= kTile128x64 ? 64 : tile == kTile256 ? 256 : 128;
+  return ((M + bm - 1) / bm) * ((N + bn - 1) / bn) > (int64_t)UINT32_MAX / 512;
+}
+
 template <int IODT, typename T> static hipError_t block_gemm_tile(BlockGemmParams p, hipStream_t s) {
   hipError_t err = hipSuccess;
   constexpr bool FINE = IODT == CASCMM_DT_F32;
@@ -144,13 +152,12 @@ int cascmm_block_gemm(const void* a, const void* a_scales, const void* b, const 
                       void* stream) {
   if (!block_dtype(dtype)) return CASCMM_ERR_BAD_DTYPE;
   if (M < 0 || N < 0 || K < 0 || ldc < N) return CASCMM_ERR_BAD_SHAPE;
-  if (M > INT32_MAX || N > INT32_MAX || K > kBlockMostK) return CASCMM_ERR_TOO_LARGE;
+  if (block_too_large(M, N, K, dtype == CASCMM_DT_F32)) return CASCMM_ERR_TOO_LARGE;
   if (M == 0 || N == 0) return CASCMM_OK;
   if (!C || (K > 0 && (!a || !a_scales || !b || !b_scales))) return CASCMM_ERR_NULL_POINTER;
   const size_t es = block_size(dtype);
   if (!block_aligned(C, es) || !block_aligned(bias, es) || !block_aligned(a, 16) || !block_aligned(b, 16) || !block_aligned(a_scales, 4) || !block_aligned(b_scales, 4))
     return CASCMM_ERR_ALIGNMENT;
-  if ((M + 63) / 64 * ((N + 63) / 64) > (1 << 22) - 1) return CASCMM_ERR_TOO_LARGE;      // (a launch has fewer than 2^32 threads)
   BlockGemmParams p;
   memset(&p, 0, sizeof(p));
   p.a = (const unsigned char*)a; p.b = (const unsigned char*)b; p.sa = (const unsigned*)a_scales; p.sb = (const unsigned*)b_scales;
@@ -181,7 +188,7 @@ int cascmm_block_linear(const void* x, const void* b, const void* b_scales, void
     void* const scales = (char*)workspace + block_slice((size_t)(M * block_padded(K)));
     // (everything is checked before the first launch: the product's own checks see the same arguments)
     if (!C || (K > 0 && (!x || !b || !b_scales))) return CASCMM_ERR_NULL_POINTER;
-    if ((M + 63) / 64 * ((N + 63) / 64) > (1 << 22) - 1) return CASCMM_ERR_TOO_LARGE;
+    if (block_too_large(M, N, K, dtype == CASCMM_DT_F32)) return CASCMM_ERR_TOO_LARGE;
     if (!block_aligned(C, block_size(dtype)) || !block_aligned(bias, block_size(dtype)) || !block_aligned(b, 16) || !block_aligned(b_scales, 4)) return CASCMM_ERR_ALIGNMENT;
     const int st = K > 0 ? cascmm_block_round(x, M, K, ldx, dtype, 0, workspace, scales, nullptr, nullptr, nullptr, nullptr, 0, stream) : (int)CASCMM_OK;
     return st != CASCMM_OK ? st : cascmm_block_gemm(workspace, scales, b, b_scales, C, bias, M, N, K, ldc, dtype, stream);

@@ -28,7 +28,7 @@ def test_rounding_arguments(change, status):
 
 @pytest.mark.parametrize("change, status", [
     (dict(dtype=-1), -3), (dict(M=-1), -2), (dict(N=-1), -2), (dict(K=-1), -2), (dict(ldc=7), -2), (dict(M=2 ** 31), -9), (dict(N=2 ** 31, ldc=2 ** 31), -9),
-    (dict(K=2 ** 22 + 1), -9), (dict(M=2 ** 20, N=2 ** 20, ldc=2 ** 20), -9), (dict(a=None), -1), (dict(sa=None), -1), (dict(b=None), -1), (dict(sb=None), -1),
+    (dict(K=2 ** 22 + 1), -9), (dict(M=2 ** 20, N=2 ** 20, ldc=2 ** 20), -9), (dict(M=2 ** 17, K=2 ** 21), -9), (dict(N=2 ** 17, ldc=2 ** 17, K=2 ** 21), -9), (dict(a=None), -1), (dict(sa=None), -1), (dict(b=None), -1), (dict(sb=None), -1),
     (dict(c=None), -1), (dict(a=P + 8), -6), (dict(b=P + 1), -6), (dict(sa=P + 2), -6), (dict(sb=P + 1), -6), (dict(c=P + 2), -6), (dict(bias=P + 2), -6),
     (dict(M=0, a=None, c=None), 0), (dict(N=0, ldc=0, b=None, c=None), 0)])
 def test_product_arguments(change, status):
