@@ -297,7 +297,7 @@ __device__ __forceinline__ void block_load_lds(__amdgpu_buffer_rsrc_t rsrc, unsi
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (block_lds_ptr)dst, 16, voffset, soffset, 0, 0);
 }
 
-// WM x WN waves, each MT x NT blocks of 32 x 32.  A stage is one block of k: rows of 128 bytes in LDS, the eight 16-byte pieces of row r in the order i ^ (r % 8), so that
+// WM x WN waves, each MT x NT blocks of 32 x 32.  A stage is one block of k: rows of 128 bytes in LDS, the eight 16-byte pieces of a row turned (block_turn), so that
 // the lanes of a fragment read, 32 rows apart by 128 bytes, hit all banks, and the rows' scales of the block's four.  The copy to LDS writes in order; the order is made by the
 // addresses it reads.
 // A stage is multiplied in two halves of 64 k.  The fragments of one half are read behind the matrix instructions of the other, so that no wave waits for LDS: behind the first
@@ -327,6 +327,10 @@ __device__ __forceinline__ void block_place(unsigned w, int tiles_m, int tiles_n
   tile_n = (int)(in / down);
 }
 
+// The order of a row's 16-byte pieces in LDS: piece i lies at i ^ turn.  Sixteen lanes are served at a time, from 64 banks: two rows side by side, and eight pairs of them in eight places (measured,
+// cycles of a read by sixteen waves: 4.4 so, 8.1 with r % 8)
+__device__ __forceinline__ int block_turn(int r) { return (r >> 1) & 7; }
+
 // A wave's loads of a stage: 1 KB of rows each, and 256 bytes of scales
 template <typename T> struct BlockLoads {
   __amdgpu_buffer_rsrc_t ra, rb, rsa, rsb;
@@ -342,7 +346,7 @@ template <typename T> struct BlockLoads {
 #pragma unroll
     for (int j = 0; j < T::LOADS; ++j) {
       const int r = (wave + T::WAVES * j) * 8 + (lane >> 3), row = r < T::BM ? (r < last_m ? r : last_m) : (r - T::BM < last_n ? r - T::BM : last_n);
-      from[j] = (int)(row * kp) + (((lane & 7) ^ (r & 7)) << 4);
+      from[j] = (int)(row * kp) + (((lane & 7) ^ block_turn(r)) << 4);
     }
 #pragma unroll
     for (int j = 0; j < T::SCALES; ++j) {
@@ -439,7 +443,7 @@ __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const Blo
   u32x4 f[2][MT + NT][2];              // fragments of both halves: rows of a, then of b; 32 k in two pieces
   unsigned scale[MT + NT], scale_next[MT + NT];
   // read k of a half: the pieces of b and a in turn, as the instructions want them
-  const int at[2] = {(wm + l31) * 128, (BM + wn + l31) * 128}, turn = l31 & 7;
+  const int at[2] = {(wm + l31) * 128, (BM + wn + l31) * 128}, turn = block_turn(l31);
   auto read = [&](const unsigned char* stage, int half, int k) {
     const int g = k >> 1, piece = k & 1;
     const int base = g < MT ? at[0] + g * 4096 : at[1] + (g - MT) * 4096;
