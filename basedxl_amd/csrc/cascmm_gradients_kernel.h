@@ -8,6 +8,9 @@
 //
 // Bound by memory: the gradients are read for the norm and again to be scaled, 12 bytes an fp32 element with the store.  The tensors' addresses travel in the
 // kernels' arguments, as many to a launch as fit: there is no table in memory to be kept, copied or outlived by a recorded graph.
+//
+// Measured (us among other calls): 786 M fp32 gradients in 400 tensors 1835 (the first pass at 5.9 TB/s, the second at 5.1; a large copy 4.9), 30 M bf16 into fp32 60.5, the 37 thousand
+// of 30 small tensors 11.7, two launches of 4 and what the host takes.
 #pragma once
 #include "cascmm_common.h"
 

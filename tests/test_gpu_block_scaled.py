@@ -13,6 +13,7 @@ import torch
 
 from basedxl_amd import _lib, BlockScaledWeight, block_scaled_matmul
 from basedxl_amd.block_scaled import _round
+from tests.side_streams import side_streams
 
 pytestmark = pytest.mark.gpu
 
@@ -349,7 +350,7 @@ def test_recorded_replayed_and_on_other_streams(gpu_device):
         with torch.cuda.graph(graph):
             y = block_scaled_matmul(a, right)
         graphs.append((graph, y, right))
-    side = torch.cuda.Stream()
+    side = side_streams()[0]
     for _ in range(4):
         a.normal_(generator=gen)
         eager = [block_scaled_matmul(a, right) for _, _, right in graphs]

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from basedxl_amd import _lib, add_layer_norm, gated_add_norm
+from tests.side_streams import side_streams
 
 pytestmark = pytest.mark.gpu
 
@@ -340,7 +341,7 @@ def test_recorded_replayed_and_on_other_streams(gpu_device):
         return [y.detach(), s.detach(), *torch.autograd.grad((y, s), list(leaves.values()), (t["dy"], t["ds"]))]
     graphs = []
     for _ in range(2):
-        side = torch.cuda.Stream()
+        side = side_streams()[0]
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             step()
@@ -351,7 +352,7 @@ def test_recorded_replayed_and_on_other_streams(gpu_device):
             out = step()
         graphs.append((graph, out))
     gen = torch.Generator(device=gpu_device).manual_seed(1)
-    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    streams = side_streams()
     for _ in range(4):
         for v in t.values():
             v.normal_(generator=gen)

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from basedxl_amd import _lib, clip_grad_norm_, clip_gradients, gradient_norm
+from tests.side_streams import side_streams
 
 pytestmark = pytest.mark.gpu
 
@@ -193,7 +194,7 @@ def test_recorded_and_replayed(gpu_device):
     shapes = [(50, 70), (4096 * 700,), (3,)]
     gradients, outs = make(shapes, (torch.float32, torch.bfloat16), gpu_device), []
     graphs = []
-    side = torch.cuda.Stream()
+    side = side_streams()[0]
     for kind in (2.0, math.inf):
         out = [torch.zeros_like(g) for g in gradients]
         clip_gradients(gradients, 0.5, norm_type=kind, out=out)
@@ -221,7 +222,7 @@ def test_recorded_and_replayed(gpu_device):
 def test_other_stream_and_same_bits(gpu_device):
     gradients = make([(4097, 8195), (129,)], (torch.bfloat16,), gpu_device)
     first = gradient_norm(gradients)
-    side = torch.cuda.Stream()
+    side = side_streams()[0]
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         again = [gradient_norm(gradients) for _ in range(3)]

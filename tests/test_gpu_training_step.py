@@ -8,6 +8,7 @@ import torch
 
 from basedxl_amd import BlockScaledWeight, _lib, block_scaled_matmul, clip_gradients, clip_grad_norm_, gated_add_norm
 from tests.test_gpu_block_scaled import held
+from tests.side_streams import side_streams
 
 pytestmark = pytest.mark.gpu
 
@@ -103,7 +104,7 @@ def test_recorded_steps_with_an_update_replay_like_eager_ones(gpu_device, dtype)
     (p, (y, s)), (q, (y2, s2)) = parameters(gpu_device, dtype), parameters(gpu_device, dtype)
     c = torch.randn(B, S, C, generator=torch.Generator().manual_seed(5)).to(dtype).to(gpu_device)
     mine, other = [v.float() for v in p.values()], [v.float() for v in q.values()]
-    side = torch.cuda.Stream()
+    side = side_streams()[0]
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         program(q, other, y2, s2, c)
