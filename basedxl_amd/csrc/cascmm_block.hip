@@ -18,6 +18,11 @@ constexpr int64_t kBlockMostK = 1 << 22;
 
 template <int IODT> static hipError_t block_round(const BlockRoundParams& p, bool square, unsigned tiles, hipStream_t s) {
   hipError_t err = hipSuccess;
+  const int64_t strips = (p.rows + 15) / 16 * p.across;
+  if (!square && !p.qt && !p.sums && strips < (1 << 24)) {
+    CASCMM_LAUNCH(err, cascmm_block_round_rows_kernel<IODT>, dim3((unsigned)strips), dim3(256), 0, s, p);
+    return err;
+  }
   CASCMM_LAUNCH(err, (square ? cascmm_block_round_kernel<IODT, true> : cascmm_block_round_kernel<IODT, false>), dim3(tiles), dim3(256), 0, s, p);
   return err;
 }

@@ -284,6 +284,25 @@ __global__ __launch_bounds__(256) void cascmm_block_round_kernel(const BlockRoun
   }
 }
 
+// Blocks along the rows alone: sixteen rows of one block of columns a workgroup, eight elements a thread.  Few and short loads for each, so that few rows are spread over many workgroups
+template <int IODT>
+__global__ __launch_bounds__(256) void cascmm_block_round_rows_kernel(const BlockRoundParams p) {
+  typedef BlockEight<IODT> V;
+  typedef typename V::E E;
+  const int tid = threadIdx.x, tx = tid & 15;
+  const int64_t tile_row = blockIdx.x / p.across, tile_col = blockIdx.x % p.across;
+  const int64_t row = tile_row * 16 + (tid >> 4), col0 = tile_col * kBlock + tx * 8;
+  if (row >= p.rows) return;       // (sixteen lanes of a row or none)
+  const int left = p.cols - col0 < 8 ? (int)(p.cols - col0) : 8;
+  typename V::Values v;
+  V::load(v, (const E*)p.x + row * p.ldx + col0, left == 8, left);
+  typename V::Most columns;
+  V::clear(columns);
+  const unsigned byte = block_scale(block_row_max(V::fold(v, columns)));
+  *(u32x2*)(p.q + row * block_padded(p.cols) + col0) = V::pack(v, byte);
+  if (tx == 0) p.s[((tile_col >> 2) * p.rows + row) * 4 + (tile_col & 3)] = (unsigned char)byte;
+}
+
 // ---------------------------------------------------------------------------------------
 // product
 // ---------------------------------------------------------------------------------------
