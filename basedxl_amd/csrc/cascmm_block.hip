@@ -29,10 +29,11 @@ template <int IODT> static hipError_t block_round(const BlockRoundParams& p, boo
 
 // The tiles: estimated microseconds from what was measured (us in a graph, 8192 x 8192 x 8192 bf16 / 8192 x 1280 x 5120 / 2048 x 10240 x 1280 / 1024 x 1280 x 5120 / 154 x 5120 x 1280):
 // 256 x 256 on eight waves, one workgroup on a CU, 409 / 52.6 / 37.0 / 48.1 / 15.1; 128 x 128, two on a CU, so that one's stores hide behind the other's products, 480 / 68.2 / 34.6 /
-// 31.2 / 7.9; 128 x 64, three stages deep, 640 / 68.2 / 42.8 / 17.4 / 6.7; 64 x 64 811 / 89.5 / 50.1 / 22.9 / 5.9; 64 x 64 with k dealt to two groups of waves, four stages deep, 977 / 115 /
-// 96.9 / 23.9 / 6.1, and for 640 x 640 x 8192 17.0 where the others take 70, 42, 24 and 34.  Of 25 sizes the estimate's tile is the best or within 5 % for 24, 13 % behind for one.  In the
-// terms: what a block of k and a tile's beginning and end take, times the tiles that fall to a CU.
-typedef BlockTile<2, 2, 1, 1, 2, 1> BlockTile64;
+// 31.2 / 7.9; 128 x 64, three stages deep, 640 / 68.2 / 42.8 / 17.4 / 6.7; 64 x 64, as deep, 825 / 90.5 / 51.3 / 18.8 / 5.7 (two deep 816 / 88.8 / 50.8 / 22.9 / 5.9 with the weights in the caches,
+// and 1.6 more of 154 x 5120 x 1280 with them in memory); 64 x 64 with k dealt to two groups of waves, four stages deep, 977 / 115 / 96.9 / 23.9 / 6.1, and for 640 x 640 x 8192 17.0 where the
+// others take 70, 42, 24 and 20.  Of 25 sizes the estimate's tile is the best or within 5 % for 24, 13 % behind for one.  In the terms: what a block of k and a tile's beginning and end take,
+// times the tiles that fall to a CU.
+typedef BlockTile<2, 2, 1, 1, 3, 1> BlockTile64;
 typedef BlockTile<2, 2, 1, 1, 4, 2> BlockTile64Shares;
 typedef BlockTile<2, 2, 2, 1, 3, 1> BlockTile128x64;
 typedef BlockTile<2, 2, 2, 2, 2, 1> BlockTile128;

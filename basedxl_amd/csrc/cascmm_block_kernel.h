@@ -7,8 +7,8 @@
 // Infinities and NaN become NaN.
 //
 // The rounding is bound by memory, the product by the clock that the card holds under it: 8192 x 1280 x 5120 takes the same time on 160 CUs (256 x 256 tiles) as on all 256 (256 x 160), at 1.75 GHz
-// from the busy cycles.  Measured (us in a graph): 8192 x 8192 x 8192 bf16 409 (2.7 PF; registers alone reach 4.1 to 4.4), 8192 x 5120 x 1280 60, 2048 x 10240 x 1280 34.6, 154 x 5120 x 1280 5.9;
-// rounding 8192 x 5120 bf16 in both orders with its sums 37.5 (168 MB, 4.5 TB/s), 2048 x 1280 in one 5.4.  Tried and left out: four waves on 256 x 320 (the sums no longer fit the
+// from the busy cycles.  Measured (us in a graph): 8192 x 8192 x 8192 bf16 409 (2.7 PF; registers alone reach 4.1 to 4.4), 8192 x 5120 x 1280 60, 2048 x 10240 x 1280 34.6, 154 x 5120 x 1280 5.7;
+// rounding 8192 x 5120 bf16 in both orders with its sums 37.5 (168 MB, 4.5 TB/s), 2048 x 1280 along rows 3.7 (a launch of 32 tiles, which turns them too, 5.4).  Tried and left out: four waves on 256 x 320 (the sums no longer fit the
 // accumulation registers and are moved about: 2.3 us a block of k for 1.25 of instructions), stages of half a block in deeper rings (8192 x 8192 x 8192 620), 256 x 128 tiles (490).
 //
 // Operands lie as rows of bytes along k, [rows][k rounded up to 128], what is behind k zero; the scales as bytes [block / 4][rows][4], so that a lane
