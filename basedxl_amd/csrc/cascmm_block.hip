@@ -86,10 +86,18 @@ template <int IODT> static hipError_t block_gemm(const BlockGemmParams& p, hipSt
   }
 }
 
-template <int IODT> static hipError_t block_rows(const BlockRowsParams& p, hipStream_t s) {
+template <int IODT, int WAVES> static hipError_t block_rows_waves(const BlockRowsParams& p, hipStream_t s) {
   hipError_t err = hipSuccess;
-  CASCMM_LAUNCH(err, (cascmm_block_rows_kernel<IODT, 16>), dim3((unsigned)(p.N + 15) / 16), dim3(1024), 0, s, p);
+  const dim3 grid((unsigned)(p.N + 15) / 16), threads(64 * WAVES);
+  if (p.M <= 4) CASCMM_LAUNCH(err, (cascmm_block_rows_kernel<IODT, WAVES, 1>), grid, threads, 0, s, p);
+  else if (p.M <= 8) CASCMM_LAUNCH(err, (cascmm_block_rows_kernel<IODT, WAVES, 2>), grid, threads, 0, s, p);
+  else CASCMM_LAUNCH(err, (cascmm_block_rows_kernel<IODT, WAVES, 4>), grid, threads, 0, s, p);
   return err;
+}
+// Sixteen waves where no CU gets a second workgroup, eight behind that (us, 16 waves / 8: 1 x 5120 x 1280 5.3 / 5.4, 16 x 5120 x 1280 8.2 / 9.2; 1 x 1280 x 10240 7.7 / 5.5, 16 x 1280 x 5120
+// 7.5 / 6.0, 8 x 10240 x 10240 33.5 / 29.9)
+template <int IODT> static hipError_t block_rows(const BlockRowsParams& p, hipStream_t s) {
+  return p.N <= 256 * 16 ? block_rows_waves<IODT, 16>(p, s) : block_rows_waves<IODT, 8>(p, s);
 }
 // (fp32 results come from the 16-bit instruction, which the kernel of few rows does not use)
 static bool block_few_rows(int64_t M, int64_t K, int dtype) { return M <= 16 && K > 0 && dtype != CASCMM_DT_F32; }

@@ -584,8 +584,11 @@ __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const Blo
 // ---------------------------------------------------------------------------------------
 // few rows: c [M][N] of up to sixteen rows of x, rounded here
 // ---------------------------------------------------------------------------------------
-// Sixteen columns a workgroup, a block of k at a time a wave: its fragments come straight from memory, sixteen bytes a lane of four neighbours along a row; every workgroup rounds
-// the rows itself, which costs less than a launch in front of it (1 x 5120 x 1280 bf16 7.1 us; a launch each 5 and 11).  The waves' sums meet in LDS, in order.  A lane's 32 k are the pieces i and i + 4 of a block's eight, of both operands.
+// Sixteen columns a workgroup, a block of k at a time a wave; every workgroup rounds the rows itself, which costs less than a launch in front of it (1 x 5120 x 1280 bf16 5.3 us a call in a
+// graph; a launch each 5 and 11).  Bound by what a CU's vector memory takes in: the weights' fragments come straight from memory, sixteen bytes a lane, and a load of the rows is four of
+// them whole, sixteen lanes a row, turned into fragments in the wave's own LDS (loaded as fragments, sixteen rows whatever M is, 6.9 us, and 43 instead of 30 for 8 x 10240 x 10240).  The
+// next block's loads are under way while one is multiplied, with no branch between them (a load that a branch may skip makes every wait one for all); two blocks ahead gain nothing (5.4).
+// The waves' sums meet in LDS, in order.  A lane's 32 k are the pieces i and i + 4 of a block's eight, of both operands.
 struct BlockRowsParams {
   const void* x;                   // [M][K], row stride ldx
   const unsigned char* b;
@@ -595,59 +598,84 @@ struct BlockRowsParams {
   int64_t ldx, ldc;
   int M, N, K, blocks;
 };
-template <int IODT, int WAVES>
+template <int IODT, int WAVES, int QUADS>
 __global__ __launch_bounds__(64 * WAVES) void cascmm_block_rows_kernel(const BlockRowsParams p) {
   typedef BlockEight<IODT> V;
   typedef typename V::E E;
-  __shared__ f32x4 meet[WAVES][64];
+  constexpr int PITCH = kBlock + 16;                // (the scale stands behind a row; sixteen rows' pieces on banks of their own)
+  __shared__ __attribute__((aligned(16))) unsigned char rounded[WAVES][16 * PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, part = lane >> 4;
-  const int n = blockIdx.x * 16 + l15, row_b = n < p.N ? n : p.N - 1, row_a = l15 < p.M ? l15 : p.M - 1;
+  const int n = blockIdx.x * 16 + l15, row_b = n < p.N ? n : p.N - 1;
   const unsigned char* const b = p.b + (int64_t)row_b * p.blocks * kBlock + part * 16;
-  const E* const x = (const E*)p.x + row_a * p.ldx + part * 16;
+  unsigned char* const mine = rounded[wave];
+  const E* x[QUADS];
+#pragma unroll
+  for (int i = 0; i < QUADS; ++i) {
+    const int row = 4 * i + part;
+    x[i] = (const E*)p.x + (row < p.M ? row : p.M - 1) * p.ldx + l15 * 8;
+  }
   struct Piece {
     u32x4 b[2];
     unsigned scale;
-    typename V::Values x[4];
-  } next;
-  auto fetch = [&](int block) {
-    next.b[0] = *(const u32x4*)(b + (int64_t)block * kBlock);
-    next.b[1] = *(const u32x4*)(b + (int64_t)block * kBlock + 64);
-    next.scale = p.sb[(int64_t)(block >> 2) * p.N + row_b] >> ((block & 3) * 8);
+    typename V::Values x[QUADS];
+  };
+  auto fetch = [&](Piece& to, int block, bool whole) {
+    to.b[0] = *(const u32x4*)(b + (int64_t)block * kBlock);
+    to.b[1] = *(const u32x4*)(b + (int64_t)block * kBlock + 64);
+    to.scale = p.sb[(int64_t)(block >> 2) * p.N + row_b] >> ((block & 3) * 8);
+    const int left = p.K - block * kBlock - l15 * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int k = block * kBlock + (i >> 1) * 64 + (i & 1) * 8;     // (of this lane's: + part * 16)
-      const int left = p.K - k - part * 16;
-      V::load(next.x[i], x + k, left >= 8, left);
-    }
+    for (int i = 0; i < QUADS; ++i) V::load(to.x[i], x[i] + (int64_t)block * kBlock, whole || left >= 8, left);
   };
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  int block = wave;
-  if (block < p.blocks) fetch(block);
-  while (block < p.blocks) {
-    Piece cur = next;
-    block += WAVES;
-    if (block < p.blocks) fetch(block);
-    typename V::Most columns;
-    V::clear(columns);
-    unsigned most = 0;
+  auto add = [&](Piece& cur) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) most = block_larger(most, V::fold(cur.x[i], columns));
-    most = block_larger(most, (unsigned)__shfl_xor((int)most, 16, 64));
-    most = block_larger(most, (unsigned)__shfl_xor((int)most, 32, 64));
-    const unsigned byte = block_scale(most);
-    const u32x2 q0 = V::pack(cur.x[0], byte), q1 = V::pack(cur.x[1], byte), q2 = V::pack(cur.x[2], byte), q3 = V::pack(cur.x[3], byte);
-    const i32x8 a = {(int)q0[0], (int)q0[1], (int)q1[0], (int)q1[1], (int)q2[0], (int)q2[1], (int)q3[0], (int)q3[1]};
+    for (int i = 0; i < QUADS; ++i) {
+      typename V::Most columns;
+      V::clear(columns);
+      unsigned most = V::fold(cur.x[i], columns);
+#pragma unroll
+      for (int o = 1; o < 16; o *= 2) most = block_larger(most, (unsigned)__shfl_xor((int)most, o, 64));
+      const unsigned byte = block_scale(most);
+      *(u32x2*)(mine + (4 * i + part) * PITCH + l15 * 8) = V::pack(cur.x[i], byte);
+      if (l15 == 0) mine[(4 * i + part) * PITCH + kBlock] = (unsigned char)byte;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const u32x4 a0 = *(const u32x4*)(mine + l15 * PITCH + part * 16), a1 = *(const u32x4*)(mine + l15 * PITCH + 64 + part * 16);
+    const unsigned byte = mine[l15 * PITCH + kBlock];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const i32x8 a = {(int)a0[0], (int)a0[1], (int)a0[2], (int)a0[3], (int)a1[0], (int)a1[1], (int)a1[2], (int)a1[3]};
     const i32x8 w = {(int)cur.b[0][0], (int)cur.b[0][1], (int)cur.b[0][2], (int)cur.b[0][3], (int)cur.b[1][0], (int)cur.b[1][1], (int)cur.b[1][2], (int)cur.b[1][3]};
     acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, (int)cur.scale, 0, (int)byte);
+  };
+  const int whole = p.K / kBlock;
+  int block = wave;
+  if (block < whole) {
+    Piece next;
+    fetch(next, block, true);
+    while ((block += WAVES) < whole) {
+      Piece cur = next;
+      fetch(next, block, true);
+      add(cur);
+    }
+    add(next);
   }
-  meet[wave][lane] = acc;
+  if (whole < p.blocks && wave == whole % WAVES) {
+    Piece last;
+    fetch(last, whole, false);
+    add(last);
+  }
+  f32x4* const sums = (f32x4*)mine;
+  sums[lane] = acc;
   __syncthreads();
   // a lane holds row l15 of c, columns 4 part + e: a thread for each of the 256
   if (tid < 256) {
     const int from = tid >> 2, e = tid & 3, m = from & 15, column = blockIdx.x * 16 + 4 * (from >> 4) + e;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) s += meet[w][from][e];
+    for (int w = 0; w < WAVES; ++w) s += ((const f32x4*)rounded[w])[from][e];
     if (m < p.M && column < p.N) {
       if (p.bias) s += IoType<IODT>::load((const E*)p.bias + column);
       IoType<IODT>::store((E*)p.c + m * p.ldc + column, s);

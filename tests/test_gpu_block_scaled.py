@@ -205,6 +205,24 @@ def test_product_and_gradients(gpu_device, M, K, N, dtype):
         assert bool(((gbias.cpu().double() - want).abs() <= half_of(dtype) * want.abs() + TINY[dtype] + (16 + M // 128) * U * dy.double().abs().sum(0)).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("K, N", [(100, 4100), (2200, 45), (2200, 4104), (1024, 4096), (128, 5000)])
+def test_few_rows(gpu_device, K, N, dtype):
+    """Every number of rows that has a kernel of its own, from rows inside larger ones: a row's results do not depend on the others, whatever those hold."""
+    gen = torch.Generator(device=gpu_device).manual_seed(K + N)
+    wide = torch.randn(18, K + 9, generator=gen, device=gpu_device).to(dtype)
+    b, bias = torch.randn(K, N, generator=gen, device=gpu_device).to(dtype), torch.randn(N, generator=gen, device=gpu_device).to(dtype)
+    weight = BlockScaledWeight(b)
+    x = wide[1:17, 3:K + 3]
+    each = torch.cat([block_scaled_matmul(x[m:m + 1], weight, bias=bias) for m in range(16)])
+    check_product(each, seen(_round(x.contiguous(), False, True, False)[0], 16, K)[0], weight.dequantized().cpu().double(), bias, "rows")
+    x[2, K - 1] = math.nan
+    for m in range(1, 17):
+        y = block_scaled_matmul(x[:m], weight, bias=bias)
+        keep = [r for r in range(m) if r != 2]
+        assert torch.equal(y[keep], each[keep]) and (m < 3 or bool(y[2].isnan().all()))
+
+
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("M, K, N", [(65, 2500, 70), (400, 700, 129), (500, 260, 1300), (520, 1100, 5130), (1030, 5000, 1290), (2100, 257, 2570), (4100, 600, 2500)])
 def test_every_tile(gpu_device, M, K, N, dtype):
