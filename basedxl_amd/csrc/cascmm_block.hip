@@ -88,7 +88,7 @@ template <int IODT> static hipError_t block_gemm(const BlockGemmParams& p, hipSt
 
 template <int IODT, int WAVES> static hipError_t block_rows_waves(const BlockRowsParams& p, hipStream_t s) {
   hipError_t err = hipSuccess;
-  const dim3 grid((unsigned)(p.N + 15) / 16), threads(64 * WAVES);
+  const dim3 grid((unsigned)(p.N + 15) / 16, (unsigned)(p.M + 15) / 16), threads(64 * WAVES);
   if (p.M <= 4) CASCMM_LAUNCH(err, (cascmm_block_rows_kernel<IODT, WAVES, 1>), grid, threads, 0, s, p);
   else if (p.M <= 8) CASCMM_LAUNCH(err, (cascmm_block_rows_kernel<IODT, WAVES, 2>), grid, threads, 0, s, p);
   else CASCMM_LAUNCH(err, (cascmm_block_rows_kernel<IODT, WAVES, 4>), grid, threads, 0, s, p);
@@ -96,11 +96,15 @@ template <int IODT, int WAVES> static hipError_t block_rows_waves(const BlockRow
 }
 // Sixteen waves where no CU gets a second workgroup, eight behind that (us, 16 waves / 8: 1 x 5120 x 1280 5.3 / 5.4, 16 x 5120 x 1280 8.2 / 9.2; 1 x 1280 x 10240 7.7 / 5.5, 16 x 1280 x 5120
 // 7.5 / 6.0, 8 x 10240 x 10240 33.5 / 29.9)
+static int64_t block_rows_groups(int64_t M, int64_t N) { return (M + 15) / 16 * ((N + 15) / 16); }
 template <int IODT> static hipError_t block_rows(const BlockRowsParams& p, hipStream_t s) {
-  return p.N <= 256 * 16 ? block_rows_waves<IODT, 16>(p, s) : block_rows_waves<IODT, 8>(p, s);
+  return block_rows_groups(p.M, p.N) <= 256 ? block_rows_waves<IODT, 16>(p, s) : block_rows_waves<IODT, 8>(p, s);
 }
-// (fp32 results come from the 16-bit instruction, which the kernel of few rows does not use)
-static bool block_few_rows(int64_t M, int64_t K, int dtype) { return M <= 16 && K > 0 && dtype != CASCMM_DT_F32; }
+// Which products take that one launch: those of sixteen rows, and of more while two workgroups fall to a CU (us, so / rounded in a launch of its own, then tiles: 48 x 5120 x 1280 8.3 / 13.9,
+// 90 x 640 x 640 3.8 / 6.4, 8192 x 640 x 16 4.4 / 9.5, 77 x 2048 x 1280 7.5 / 9.4, 64 x 40960 x 640 45 / 108, 128 x 10240 x 640 21.3 / 23.1; with three, 512 x 640 x 384 6.3 / 6.6 but
+// 154 x 1280 x 1280 9.8 / 8.1).  fp32 results come from the 16-bit instruction, which this kernel does not use.
+constexpr int64_t kBlockRowsMost = 512;
+static bool block_few_rows(int64_t M, int64_t N, int64_t K, int dtype) { return (M <= 16 || block_rows_groups(M, N) <= kBlockRowsMost) && K > 0 && dtype != CASCMM_DT_F32; }
 static size_t block_slice(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace cascmm
@@ -186,7 +190,7 @@ int cascmm_block_gemm(const void* a, const void* a_scales, const void* b, const 
 }
 
 size_t cascmm_block_linear_workspace_bytes(int64_t M, int64_t K, int dtype) {
-  if (M < 0 || K < 0 || M > INT32_MAX || K > kBlockMostK || !block_dtype(dtype) || block_few_rows(M, K, dtype)) return 0;
+  if (M < 0 || K < 0 || M > INT32_MAX || K > kBlockMostK || !block_dtype(dtype) || (M <= 16 && block_few_rows(M, 0, K, dtype))) return 0;
   return block_slice((size_t)(M * block_padded(K))) + (size_t)block_scale_bytes(M, K);
 }
 
@@ -196,7 +200,7 @@ int cascmm_block_linear(const void* x, const void* b, const void* b_scales, void
   if (M < 0 || N < 0 || K < 0 || ldx < K || ldc < N) return CASCMM_ERR_BAD_SHAPE;
   if (M > INT32_MAX || N > INT32_MAX || K > kBlockMostK) return CASCMM_ERR_TOO_LARGE;
   if (M == 0 || N == 0) return CASCMM_OK;
-  if (!block_few_rows(M, K, dtype)) {
+  if (!block_few_rows(M, N, K, dtype)) {
     if (!workspace && M * K > 0) return CASCMM_ERR_WORKSPACE;
     if (workspace_bytes < cascmm_block_linear_workspace_bytes(M, K, dtype)) return CASCMM_ERR_WORKSPACE;
     if (!block_aligned(workspace, 16)) return CASCMM_ERR_ALIGNMENT;

@@ -582,9 +582,9 @@ __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const Blo
 }
 
 // ---------------------------------------------------------------------------------------
-// few rows: c [M][N] of up to sixteen rows of x, rounded here
+// few rows: c [M][N], x rounded here
 // ---------------------------------------------------------------------------------------
-// Sixteen columns a workgroup, a block of k at a time a wave; every workgroup rounds the rows itself, which costs less than a launch in front of it (1 x 5120 x 1280 bf16 5.3 us a call in a
+// Sixteen columns and rows a workgroup, a block of k at a time a wave; every workgroup rounds the rows itself, which costs less than a launch in front of it (1 x 5120 x 1280 bf16 5.3 us a call in a
 // graph; a launch each 5 and 11).  Bound by what a CU's vector memory takes in: the weights' fragments come straight from memory, sixteen bytes a lane, and a load of the rows is four of
 // them whole, sixteen lanes a row, turned into fragments in the wave's own LDS (loaded as fragments, sixteen rows whatever M is, 6.9 us, and 43 instead of 30 for 8 x 10240 x 10240).  The
 // next block's loads are under way while one is multiplied, with no branch between them (a load that a branch may skip makes every wait one for all); two blocks ahead gain nothing (5.4).
@@ -608,11 +608,12 @@ __global__ __launch_bounds__(64 * WAVES) void cascmm_block_rows_kernel(const Blo
   const int n = blockIdx.x * 16 + l15, row_b = n < p.N ? n : p.N - 1;
   const unsigned char* const b = p.b + (int64_t)row_b * p.blocks * kBlock + part * 16;
   unsigned char* const mine = rounded[wave];
+  const int m0 = blockIdx.y * 16, rows = p.M - m0 < 16 ? p.M - m0 : 16;
   const E* x[QUADS];
 #pragma unroll
   for (int i = 0; i < QUADS; ++i) {
     const int row = 4 * i + part;
-    x[i] = (const E*)p.x + (row < p.M ? row : p.M - 1) * p.ldx + l15 * 8;
+    x[i] = (const E*)p.x + (m0 + (row < rows ? row : rows - 1)) * p.ldx + l15 * 8;
   }
   struct Piece {
     u32x4 b[2];
@@ -676,9 +677,9 @@ __global__ __launch_bounds__(64 * WAVES) void cascmm_block_rows_kernel(const Blo
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) s += ((const f32x4*)rounded[w])[from][e];
-    if (m < p.M && column < p.N) {
+    if (m < rows && column < p.N) {
       if (p.bias) s += IoType<IODT>::load((const E*)p.bias + column);
-      IoType<IODT>::store((E*)p.c + m * p.ldc + column, s);
+      IoType<IODT>::store((E*)p.c + (int64_t)(m0 + m) * p.ldc + column, s);
     }
   }
 }

@@ -458,8 +458,8 @@ int cascmm_block_round(const void* x, int64_t rows, int64_t cols, int64_t ldx, i
                        size_t workspace_bytes, void* stream);
 int cascmm_block_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, void* C, const void* bias,
                       int64_t M, int64_t N, int64_t K, int64_t ldc, int dtype, void* stream);
-/* cascmm_block_round of x [M, K] (leading dimension ldx, blocks along its rows) and cascmm_block_gemm with it, in one call; up to sixteen 16-bit rows in one launch.  The
- * workspace (16-byte aligned, no initialisation) holds cascmm_block_linear_workspace_bytes: the rounded x, nothing for few rows. */
+/* cascmm_block_round of x [M, K] (leading dimension ldx, blocks along its rows) and cascmm_block_gemm with it, in one call; small 16-bit ones in one launch.  The
+ * workspace (16-byte aligned, no initialisation) holds cascmm_block_linear_workspace_bytes: the rounded x, nothing for up to sixteen 16-bit rows. */
 size_t cascmm_block_linear_workspace_bytes(int64_t M, int64_t K, int dtype);
 int cascmm_block_linear(const void* x, const void* b, const void* b_scales, void* C, const void* bias, int64_t M, int64_t N,
                         int64_t K, int64_t ldx, int64_t ldc, int dtype, void* workspace, size_t workspace_bytes, void* stream);
