@@ -200,10 +200,11 @@ int cascmm_block_linear(const void* x, const void* b, const void* b_scales, void
   if (M < 0 || N < 0 || K < 0 || ldx < K || ldc < N) return CASCMM_ERR_BAD_SHAPE;
   if (M > INT32_MAX || N > INT32_MAX || K > kBlockMostK) return CASCMM_ERR_TOO_LARGE;
   if (M == 0 || N == 0) return CASCMM_OK;
+  // (whichever kernel takes the call: what a caller has to bring depends on M and K alone)
+  const size_t need = cascmm_block_linear_workspace_bytes(M, K, dtype);
+  if (need && (!workspace || workspace_bytes < need)) return CASCMM_ERR_WORKSPACE;
+  if (need && !block_aligned(workspace, 16)) return CASCMM_ERR_ALIGNMENT;
   if (!block_few_rows(M, N, K, dtype)) {
-    if (!workspace && M * K > 0) return CASCMM_ERR_WORKSPACE;
-    if (workspace_bytes < cascmm_block_linear_workspace_bytes(M, K, dtype)) return CASCMM_ERR_WORKSPACE;
-    if (!block_aligned(workspace, 16)) return CASCMM_ERR_ALIGNMENT;
     void* const scales = (char*)workspace + block_slice((size_t)(M * block_padded(K)));
     // (everything is checked before the first launch: the product's own checks see the same arguments)
     if (!C || (K > 0 && (!x || !b || !b_scales))) return CASCMM_ERR_NULL_POINTER;
