@@ -132,14 +132,12 @@ struct GatedHow { bool post; int64_t norm; double eps, alpha; };
 enum { kWeight, kBias, kGate, kScale, kPostWeight, kPostBias, kParameters };
 typedef std::array<at::Tensor, kParameters> Parameters;
 
-// whether a parameter is one row or one for each entry of x's first axis
-bool parameter_of(const at::Tensor& x, const at::Tensor& t, bool may_group, bool& grouped) {
+// whether a parameter is one row, or one for each entry of x's first axis at any distance from each other (parts of a wider row, as a conditioning's are)
+bool parameter_of(const at::Tensor& x, const at::Tensor& t, bool may_group) {
   const int64_t cols = x.size(-1);
-  grouped = false;
-  if ((t.scalar_type() != x.scalar_type() && t.scalar_type() != at::kFloat) || !t.is_contiguous() || t.dim() < 1 || t.size(-1) != cols) return false;
-  if (t.dim() == 1) return true;
-  grouped = true;
-  return may_group && t.dim() == x.dim() && t.size(0) == x.size(0) && x.size(0) > 1 && t.numel() == t.size(0) * cols;
+  if ((t.scalar_type() != x.scalar_type() && t.scalar_type() != at::kFloat) || t.dim() < 1 || t.size(-1) != cols || (cols > 1 && t.stride(-1) != 1)) return false;
+  if (t.numel() == cols) return t.dim() == 1 || t.dim() <= x.dim();
+  return may_group && t.dim() == x.dim() && t.size(0) == x.size(0) && t.numel() == t.size(0) * cols && t.stride(0) >= cols;
 }
 cascmm_gated_norm gated_arguments(const at::Tensor& s, const Parameters& p, const GatedHow& how) {
   cascmm_gated_norm a;
@@ -150,9 +148,9 @@ cascmm_gated_norm gated_arguments(const at::Tensor& s, const Parameters& p, cons
   for (const at::Tensor& t : p)
     if (t.defined()) {
       code = dtype_code(t);
-      grouped = grouped || t.dim() > 1;
+      grouped = grouped || t.numel() > cols;
     }
-  auto ld = [&](const at::Tensor& t) { return t.defined() && t.dim() > 1 ? cols : 0; };
+  auto ld = [&](const at::Tensor& t) { return t.defined() && t.numel() > cols ? t.stride(0) : 0; };
   a.weight = data_of(p[kWeight]); a.bias = data_of(p[kBias]); a.gate = data_of(p[kGate]); a.scale = data_of(p[kScale]);
   a.post_weight = data_of(p[kPostWeight]); a.post_bias = data_of(p[kPostBias]);
   a.rows = rows; a.cols = cols; a.group_rows = grouped ? rows / s.size(0) : rows;
@@ -297,10 +295,9 @@ PyObject* gated_add_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
     if (!(how.eps >= 0) || !(how.eps < 1e30) || !std::isfinite(how.alpha) || (!how.post && (p[kPostWeight].defined() || p[kPostBias].defined()))) Py_RETURN_NONE;
     at::ScalarType type = at::ScalarType::Undefined;
-    bool grouped;
     for (int i = 0; i < kParameters; ++i) {
       if (!p[i].defined()) continue;
-      if (!parameter_of(*x, p[i], i < kPostWeight, grouped) || (type != at::ScalarType::Undefined && p[i].scalar_type() != type) || dual({&p[i]})) Py_RETURN_NONE;
+      if (!parameter_of(*x, p[i], i < kPostWeight) || (type != at::ScalarType::Undefined && p[i].scalar_type() != type) || dual({&p[i]})) Py_RETURN_NONE;
       type = p[i].scalar_type();
     }
     if (differentiated({x, residual, &p[0], &p[1], &p[2], &p[3], &p[4], &p[5]})) {

@@ -39,7 +39,14 @@ def _parameter(t: Optional[torch.Tensor], name: str, x: torch.Tensor, grouped: b
 
 
 def _leading(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None or t.dim() == 1 else t.shape[1]
+    return 0 if t is None or t.dim() == 1 else t.stride(0)
+
+
+def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """``t`` itself where the kernels can read its rows as they lie, at any distance from each other."""
+    if t is None or (t.shape[-1] == 1 or t.stride(-1) == 1) and (t.dim() == 1 or t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
 
 
 def _arguments(x2, r2, s2, parameters, rows, cols, group_rows, how, weight_dtype):
@@ -74,7 +81,7 @@ def _forward(x, residual, parameters, how, keep):
     stats = torch.empty(4, rows, dtype=torch.float32, device=x.device) if keep else None
     if rows == 0 or cols == 0:
         return y, s, stats
-    x2, r2, parameters = _flat(x), _flat(residual), [None if t is None else t.contiguous() for t in parameters]
+    x2, r2, parameters = _flat(x), _flat(residual), [_rows(t) for t in parameters]
     with torch.cuda.device(x.device):
         a = _arguments(x2, r2, s.view(rows, cols), parameters, rows, cols, group_rows, how, _weight_dtype(x, parameters))
         a.y, a.ldy, a.stats = y.data_ptr(), cols, _ptr(stats)
@@ -114,7 +121,7 @@ class _GatedAddNorm(torch.autograd.Function):
         fresh = torch.empty_like if rows > 0 else torch.zeros_like
         grads = [fresh(t, memory_format=torch.contiguous_format) if w else None for t, w in zip(parameters, want[2:])]
         if rows > 0 and cols > 0:
-            parameters = [None if t is None else t.contiguous() for t in parameters]
+            parameters = [_rows(t) for t in parameters]
             l = _lib.lib()
             with torch.cuda.device(dev):
                 dy2, ds2, s2 = _flat(dy), None if ds is None else _flat(ds), _flat(s)

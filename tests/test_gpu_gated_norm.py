@@ -250,6 +250,31 @@ def test_strides(gpu_device, cols, dtype):
     assert torch.equal(mine[0].view(3, 7, cols), grads[0]) and mine[list(leaves).index("gate")].shape == (21, cols)
 
 
+@pytest.mark.parametrize("samples", [1, 4])
+@pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
+def test_parts_of_a_conditioning(gpu_device, samples, wdtype):
+    """Parameters of a sample as parts of one wide row, of one sample too: the same as parameters of their own, without a copy, and so are the gradients."""
+    gen = torch.Generator(device=gpu_device).manual_seed(samples)
+    draw = lambda *shape: torch.randn(*shape, generator=gen, device=gpu_device)   # noqa: E731
+    x, residual, dy, ds = (draw(samples, 9, 200).bfloat16() for _ in range(4))
+    wide = draw(samples, 1, 3 * 200).to(wdtype).requires_grad_()
+    how = dict(norm="rms", eps=1e-5)
+    weight, bias, gate = wide.chunk(3, dim=-1)
+    native = _lib.native().gated_add_norm(x, residual, weight, bias, gate, 1.0, None, None, False, 1, 1e-5)
+    assert native is not None
+    y, s = gated_add_norm(x, residual, weight, bias, gate=gate, **how)
+    own = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for t in (weight, bias, gate)]
+    y2, s2 = gated_add_norm(x, residual, own[0], own[1], gate=own[2], **how)
+    assert all(torch.equal(p, q) for p, q in ((native[0], y2), (native[1], s2), (y, y2), (s, s2)))
+    whole = torch.autograd.grad((y, s), wide, (dy, ds))[0]
+    parts = torch.autograd.grad((y2, s2), own, (dy, ds))
+    assert torch.equal(whole, torch.cat(parts, -1)) and all(g.shape == (samples, 1, 200) for g in parts)
+    with torch.no_grad():
+        # one gate for all samples, spread over them: read as it would be written out
+        spread = gate[:1].expand(samples, 1, 200)
+        assert all(torch.equal(p, q) for p, q in zip(gated_add_norm(x, residual, gate=spread, **how), gated_add_norm(x, residual, gate=spread.contiguous(), **how)))
+
+
 def test_scalars_and_mixed_types(gpu_device):
     t = make(HOWS["affine"], 2, 30, 128, torch.bfloat16, torch.float32, gpu_device, 6)
     gate, scale = torch.tensor(0.75, device=gpu_device, requires_grad=True), torch.tensor(1.5, device=gpu_device, requires_grad=True)
