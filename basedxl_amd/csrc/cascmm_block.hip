@@ -4,6 +4,7 @@
 #include <cstring>
 
 #include <algorithm>
+#include <cmath>
 
 #include "cascmm_norm_kernel.h"
 #include "cascmm_variants.h"
@@ -32,13 +33,17 @@ template <int IODT> static hipError_t block_round(const BlockRoundParams& p, boo
 // 31.2 / 7.9; 128 x 64, three stages deep, 640 / 68.2 / 42.8 / 17.4 / 6.7; 64 x 64, as deep, 825 / 90.5 / 51.3 / 18.8 / 5.7 (two deep 816 / 88.8 / 50.8 / 22.9 / 5.9 with the weights in the caches,
 // and 1.6 more of 154 x 5120 x 1280 with them in memory); 64 x 64 with k dealt to two groups of waves, four stages deep, 977 / 115 / 96.9 / 23.9 / 6.1, and for 640 x 640 x 8192 17.0 where the
 // others take 70, 42, 24 and 20.  Of 25 sizes the estimate's tile is the best or within 5 % for 24, 13 % behind for one.  In the terms: what a block of k and a tile's beginning and end take,
-// times the tiles that fall to a CU.
+// times the tiles that fall to a CU.  Where the last turn of 256 x 256 tiles would leave half of the CUs or more without one, its tiles are cut in pieces, four (128 x 128) up to a quarter of a
+// turn and two (128 x 256) up to a half: 2048 x 10240 x 1280 33.5 where 128 x 128 takes 35.2 and 256 x 256 38.9, 4096 x 5120 x 2560 51.1, 61.9 and 62.3, 2304 x 8192 x 4096 69.8, 88.8 and 90.6,
+// 8192 x 5120 x 1280, in twos, 59.2, 73 and 62.1; of twelve such sizes the rule's is the best for eleven, 9 % behind for one.
 typedef BlockTile<2, 2, 1, 1, 3, 1> BlockTile64;
 typedef BlockTile<2, 2, 1, 1, 4, 2> BlockTile64Shares;
 typedef BlockTile<2, 2, 2, 1, 3, 1> BlockTile128x64;
 typedef BlockTile<2, 2, 2, 2, 2, 1> BlockTile128;
 typedef BlockTile<2, 4, 4, 2, 2, 1> BlockTile256;
-enum { kTile64, kTile64Shares, kTile128x64, kTile128, kTile256, kTiles };
+typedef BlockTile<2, 4, 2, 1, 3, 1> BlockPiece128;     // (on the waves of a 256 x 256 tile)
+typedef BlockTile<2, 4, 2, 2, 2, 1> BlockPiece128x256;
+enum { kTile64, kTile64Shares, kTile128x64, kTile128, kTile256, kTile256Pieces, kTiles };
 static int block_tile(int64_t M, int64_t N, int64_t blocks, bool fine) {
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
   const double k = (double)blocks;
@@ -47,11 +52,12 @@ static int block_tile(int64_t M, int64_t N, int64_t blocks, bool fine) {
   cost[kTile64] = std::max(n64 * (0.22 * k + 0.9), 0.3 * k + 1.0);
   cost[kTile64Shares] = n64 * (0.23 * k + 1.9);
   cost[kTile128x64] = n128x64 <= 1 ? 0.36 * k + 1.2 : n128x64 * (0.31 * k + 1.0);
-  cost[kTile128] = n128 <= 1 ? 0.62 * k + 1.5 : n128 * (0.45 * k + 1.5);
-  cost[kTile256] = n256 * ((t256 <= 128 ? 1.05 : t256 <= 256 ? 1.2 : 1.45) * k + 3.5);
+  cost[kTile128] = n128 <= 1 ? 0.62 * k + 1.5 : n128 == 2 ? 2 * (0.45 * k + 1.5) : n128 * (0.5 * k + 2.0);
+  cost[kTile256] = t256 <= 256 ? (t256 <= 128 ? 1.05 : 1.2) * k + 3.5 : n256 * (1.4 * k + 5.5);
+  cost[kTile256Pieces] = t256 > 256 && t256 % 256 != 0 && t256 % 256 <= 128 ? (n256 - 1) * (1.4 * k + 5.5) + (t256 % 256 <= 64 ? 0.45 : 0.75) * k + 8.0 : INFINITY;
   int best = kTile64;
   for (int i = 0; i < kTiles; ++i)
-    if (cost[i] < cost[best] && !(fine && i == kTile256)) best = i;     // (widened fragments do not fit beside 128 x 64 sums of a wave)
+    if (cost[i] < cost[best] && !(fine && i >= kTile256)) best = i;     // (widened fragments do not fit beside 128 x 64 sums of a wave)
   return best;
 }
 
@@ -59,8 +65,8 @@ static int block_tile(int64_t M, int64_t N, int64_t blocks, bool fine) {
 static bool block_too_large(int64_t M, int64_t N, int64_t K, bool fine) {
   if (M > INT32_MAX || N > INT32_MAX || K > kBlockMostK || block_scale_bytes(std::max(M, N), K) > INT32_MAX) return true;
   const int tile = block_tile(M, N, block_padded(K) / kBlock, fine);
-  const int64_t bm = tile <= kTile64Shares ? 64 : tile == kTile256 ? 256 : 128, bn = tile <= kTile128x64 ? 64 : tile == kTile256 ? 256 : 128;
-  return ((M + bm - 1) / bm) * ((N + bn - 1) / bn) > (int64_t)UINT32_MAX / 512;
+  const int64_t bm = tile <= kTile64Shares ? 64 : tile >= kTile256 ? 256 : 128, bn = tile <= kTile128x64 ? 64 : tile >= kTile256 ? 256 : 128;
+  return ((M + bm - 1) / bm) * ((N + bn - 1) / bn) > (int64_t)UINT32_MAX / 512 - 256;     // (pieces: up to 192 more)
 }
 
 template <int IODT, typename T> static hipError_t block_gemm_tile(BlockGemmParams p, hipStream_t s) {
@@ -73,6 +79,18 @@ template <int IODT, typename T> static hipError_t block_gemm_tile(BlockGemmParam
   CASCMM_LAUNCH(err, (cascmm_block_gemm_kernel<IODT, T, FINE>), dim3((unsigned)p.tiles_m * (unsigned)p.tiles_n), dim3(T::THREADS), T::LDS, s, p);
   return err;
 }
+template <int IODT, typename T, typename R> static hipError_t block_gemm_pieces(BlockGemmParams p, hipStream_t s) {
+  hipError_t err = hipSuccess;
+  static LdsFlags done;
+  if (!ensure_lds((const void*)cascmm_block_gemm_pieces_kernel<IODT, T, R>, T::LDS, done)) return hipErrorInvalidValue;
+  p.tiles_m = (p.M + T::BM - 1) / T::BM;
+  p.tiles_n = (p.N + T::BN - 1) / T::BN;
+  const unsigned tiles = (unsigned)p.tiles_m * (unsigned)p.tiles_n;
+  p.whole = (int)(tiles / 256 * 256);
+  const unsigned pieces = (tiles - (unsigned)p.whole) * (T::BM / R::BM) * (T::BN / R::BN);
+  CASCMM_LAUNCH(err, (cascmm_block_gemm_pieces_kernel<IODT, T, R>), dim3((unsigned)p.whole + pieces), dim3(T::THREADS), T::LDS, s, p);
+  return err;
+}
 template <int IODT> static hipError_t block_gemm(const BlockGemmParams& p, hipStream_t s) {
   constexpr bool FINE = IODT == CASCMM_DT_F32;
   switch (block_tile(p.M, p.N, p.blocks, FINE)) {
@@ -80,8 +98,14 @@ template <int IODT> static hipError_t block_gemm(const BlockGemmParams& p, hipSt
     case kTile64Shares: return block_gemm_tile<IODT, BlockTile64Shares>(p, s);
     case kTile128x64: return block_gemm_tile<IODT, BlockTile128x64>(p, s);
     case kTile128: return block_gemm_tile<IODT, BlockTile128>(p, s);
-    default:
+    case kTile256:
       if constexpr (!FINE) return block_gemm_tile<IODT, BlockTile256>(p, s);
+      return hipErrorInvalidValue;
+    default:
+      if constexpr (!FINE) {
+        const int64_t left = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) % 256;
+        return left <= 64 ? block_gemm_pieces<IODT, BlockTile256, BlockPiece128>(p, s) : block_gemm_pieces<IODT, BlockTile256, BlockPiece128x256>(p, s);
+      }
       return hipErrorInvalidValue;
   }
 }

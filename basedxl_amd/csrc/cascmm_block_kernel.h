@@ -7,7 +7,7 @@
 // Infinities and NaN become NaN.
 //
 // The rounding is bound by memory, the product by the clock that the card holds under it: 8192 x 1280 x 5120 takes the same time on 160 CUs (256 x 256 tiles) as on all 256 (256 x 160), at 1.75 GHz
-// from the busy cycles.  Measured (us in a graph): 8192 x 8192 x 8192 bf16 409 (2.7 PF; registers alone reach 4.1 to 4.4), 8192 x 5120 x 1280 60, 2048 x 10240 x 1280 34.6, 154 x 5120 x 1280 5.7;
+// from the busy cycles.  Measured (us in a graph): 8192 x 8192 x 8192 bf16 409 (2.7 PF; registers alone reach 4.1 to 4.4), 8192 x 5120 x 1280 59, 2048 x 10240 x 1280 33.5, 154 x 5120 x 1280 5.7;
 // rounding 8192 x 5120 bf16 in both orders with its sums 37.5 (168 MB, 4.5 TB/s), 2048 x 1280 along rows 3.7 (a launch of 32 tiles, which turns them too, 5.4).  Tried and left out: four waves on 256 x 320 (the sums no longer fit the
 // accumulation registers and are moved about: 2.3 us a block of k for 1.25 of instructions), stages of half a block in deeper rings (8192 x 8192 x 8192 620), 256 x 128 tiles (490).
 //
@@ -314,6 +314,7 @@ struct BlockGemmParams {
   int64_t ldc;
   int M, N, blocks;                // blocks of 128 along k
   int tiles_m, tiles_n;
+  int whole;                       // (pieces) tiles that stay whole
 };
 
 typedef __attribute__((address_space(3))) void* block_lds_ptr;
@@ -342,9 +343,11 @@ template <int WM_, int WN_, int MT_, int NT_, int DEEP_, int SHARES_> struct Blo
 
 // Workgroup w runs on die w % 8, each with a cache of its own: a die takes tiles that follow each other, in bands of `band` tiles down and all the way across, so that those at work
 // at a time share rows of both operands
-__device__ __forceinline__ void block_place(unsigned w, int tiles_m, int tiles_n, int band, int& tile_m, int& tile_n) {
-  const unsigned total = gridDim.x, die = w & 7u, each = total >> 3, more = total & 7u;
-  const unsigned id = die * each + (die < more ? die : more) + (w >> 3);
+__device__ __forceinline__ unsigned block_order(unsigned w, unsigned total) {
+  const unsigned die = w & 7u, each = total >> 3, more = total & 7u;
+  return die * each + (die < more ? die : more) + (w >> 3);
+}
+__device__ __forceinline__ void block_place(unsigned id, int tiles_m, int tiles_n, int band, int& tile_m, int& tile_n) {
   const unsigned across = (unsigned)band * (unsigned)tiles_n, which = id / across, in = id % across;
   const unsigned down = (unsigned)tiles_m - which * band < (unsigned)band ? (unsigned)tiles_m - which * band : (unsigned)band;    // (the last band may be lower)
   tile_m = (int)(which * band + in % down);
@@ -441,15 +444,12 @@ __device__ __forceinline__ void block_store(const BlockGemmParams& p, const f32x
   }
 }
 
-template <int IODT, typename T, bool FINE>
-__global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const BlockGemmParams p) {
-  constexpr int MT = T::MT, NT = T::NT, BM = T::BM, BN = T::BN;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char block_smem[];
+// the tile of c at (m0, n0)
+template <int IODT, typename T, bool FINE> __device__ __forceinline__ void block_product(const BlockGemmParams& p, unsigned char* block_smem, int m0, int n0) {
+  constexpr int MT = T::MT, NT = T::NT, BM = T::BM;
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % T::WAVES, share = __builtin_amdgcn_readfirstlane(tid >> 6) / T::WAVES;
-  int tile_m, tile_n;
-  block_place(blockIdx.x, p.tiles_m, p.tiles_n, T::BAND, tile_m, tile_n);
-  const int m0 = tile_m * BM, n0 = tile_n * BN, wm = (wave / T::WN) * 32 * MT, wn = (wave % T::WN) * 32 * NT;
+  const int wm = (wave / T::WN) * 32 * MT, wn = (wave % T::WN) * 32 * NT;
   // this share's blocks; all shares take as many steps, those past the last block without products
   const int steps = (p.blocks + T::SHARES - 1) / T::SHARES, first = share * steps, live = p.blocks - first < steps ? p.blocks - first : steps;
   unsigned char* const ring = block_smem + share * T::DEEP * T::STAGE;
@@ -579,6 +579,29 @@ __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const Blo
     if (share > 0) return;
   }
   block_store<IODT, T>(p, acc, block_smem, m0, n0, wave, lane);
+}
+template <int IODT, typename T, bool FINE> __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_kernel(const BlockGemmParams p) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char block_smem[];
+  int tile_m, tile_n;
+  block_place(block_order(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, T::BAND, tile_m, tile_n);
+  block_product<IODT, T, FINE>(p, block_smem, tile_m * T::BM, tile_n * T::BN);
+}
+// The first p.whole tiles by a workgroup each, those behind them in pieces of R's size: where the last turn of tiles would leave most of the CUs without one
+template <int IODT, typename T, typename R> __global__ __launch_bounds__(T::THREADS) void cascmm_block_gemm_pieces_kernel(const BlockGemmParams p) {
+  static_assert(R::THREADS == T::THREADS && R::LDS <= T::LDS && T::BM % R::BM == 0 && T::BN % R::BN == 0, "pieces");
+  extern __shared__ __attribute__((aligned(1024))) unsigned char block_smem[];
+  constexpr unsigned PIECES = (T::BM / R::BM) * (T::BN / R::BN);
+  const unsigned whole = (unsigned)p.whole;
+  int tile_m, tile_n;
+  if (blockIdx.x < whole) {
+    block_place(block_order(blockIdx.x, whole), p.tiles_m, p.tiles_n, T::BAND, tile_m, tile_n);
+    block_product<IODT, T, false>(p, block_smem, tile_m * T::BM, tile_n * T::BN);
+  } else {
+    const unsigned id = block_order(blockIdx.x - whole, gridDim.x - whole), piece = id % PIECES;
+    block_place(whole + id / PIECES, p.tiles_m, p.tiles_n, T::BAND, tile_m, tile_n);
+    const int m0 = tile_m * T::BM + (int)(piece / (T::BN / R::BN)) * R::BM, n0 = tile_n * T::BN + (int)(piece % (T::BN / R::BN)) * R::BN;
+    if (m0 < p.M && n0 < p.N) block_product<IODT, R, false>(p, block_smem, m0, n0);
+  }
 }
 
 // ---------------------------------------------------------------------------------------

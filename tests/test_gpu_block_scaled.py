@@ -224,7 +224,7 @@ def test_few_rows(gpu_device, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("M, K, N", [(65, 2500, 70), (400, 700, 129), (300, 2500, 700), (500, 260, 1300), (520, 1100, 5130), (1030, 5000, 1290), (2100, 257, 2570), (4100, 600, 2500)])
+@pytest.mark.parametrize("M, K, N", [(65, 2500, 70), (400, 700, 129), (300, 2500, 700), (500, 260, 1300), (520, 1100, 5130), (1030, 5000, 1290), (2100, 257, 2570), (4100, 600, 2500), (3900, 1300, 5000), (4900, 1300, 4700)])
 def test_every_tile(gpu_device, M, K, N, dtype):
     """Sizes that the rule gives to each of its tiles, with rows, columns and k past their edges."""
     gen = torch.Generator(device=gpu_device).manual_seed(M)
