@@ -124,9 +124,9 @@ class _GatedAddNorm(torch.autograd.Function):
             parameters = [_rows(t) for t in parameters]
             l = _lib.lib()
             with torch.cuda.device(dev):
-                dy2, ds2, s2 = _flat(dy), None if ds is None else _flat(ds), _flat(s)
-                a = _arguments(None if x is None else _flat(x), None if residual is None else _flat(residual), s2, parameters, rows, cols, group_rows, ctx.how,
-                               _weight_dtype(s, parameters))
+                # (names of their own until the launch: a copy that is given back before the workspace is allocated is where the workspace may come to lie)
+                dy2, s2, (ds2, x2, r2) = _flat(dy), _flat(s), (None if t is None else _flat(t) for t in (ds, x, residual))
+                a = _arguments(x2, r2, s2, parameters, rows, cols, group_rows, ctx.how, _weight_dtype(s, parameters))
                 a.dy, a.ds, a.stats, a.dx, a.dresidual = dy2.data_ptr(), _ptr(ds2), stats.data_ptr(), _ptr(dx), _ptr(dr)
                 a.dweight, a.dbias, a.dgate, a.dscale, a.dpost_weight, a.dpost_bias = map(_ptr, grads)
                 a.lddy, a.ldds, a.lddx, a.lddr = _ld(dy2), 0 if ds2 is None else _ld(ds2), cols, cols

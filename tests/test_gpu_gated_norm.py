@@ -250,6 +250,26 @@ def test_strides(gpu_device, cols, dtype):
     assert torch.equal(mine[0].view(3, 7, cols), grads[0]) and mine[list(leaves).index("gate")].shape == (21, cols)
 
 
+@pytest.mark.parametrize("name", ["conditioned", "both_norms", "everything", "rms_everything"])
+@pytest.mark.parametrize("samples, tokens, cols", [(3, 7, 5), (4, 64, 640), (8, 33, 1000), (2, 9, 7000)])
+def test_gradients_of_rows_that_are_copied(gpu_device, samples, tokens, cols, name):
+    """x and the residual in orders that no rows describe (a channel-first image's tokens, samples behind tokens, one row for all tokens): the gradients of copies made beforehand.
+    A workspace of five rows of sums for each of up to 256 groups fits in what such a copy occupies."""
+    how = HOWS[name]
+    t = make(how, samples, tokens, cols, torch.float32, torch.float32, gpu_device, cols)
+    forms = {"columns": lambda v: v.transpose(1, 2).contiguous().transpose(1, 2), "turned": lambda v: v.transpose(0, 1).contiguous().transpose(0, 1),
+             "expanded": lambda v: v[:, :1].expand(v.shape)}
+    for of_x, of_residual in (("columns", "turned"), ("turned", "expanded"), ("expanded", "columns")):
+        given = dict(t, x=forms[of_x](t["x"]), residual=forms[of_residual](t["residual"]))
+        grads = []
+        for contiguous in (True, False):
+            leaves = {k: (v.contiguous() if contiguous else v).detach().requires_grad_() for k, v in given.items() if k not in ("dy", "ds")}
+            for _ in range(3):      # (again on memory that the last one gave back)
+                grads.append(torch.autograd.grad(call(leaves, how, 1e-5), list(leaves.values()), (t["dy"], t["ds"])))
+        for other in grads[1:]:
+            assert all(torch.equal(p, q) for p, q in zip(other, grads[0])), (of_x, of_residual)
+
+
 @pytest.mark.parametrize("samples", [1, 4])
 @pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
 def test_parts_of_a_conditioning(gpu_device, samples, wdtype):
