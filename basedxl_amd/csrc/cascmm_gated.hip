@@ -30,8 +30,8 @@ static int gated_plan(const cascmm_gated_norm& a, bool backward, GatedPlan& plan
   plan.lanes = gated_shape(a.cols, backward, 16 / gated_size(a.dtype)).lanes;
   plan.rich = a.scale || (a.post && a.post_bias);
   gated_parts(plan.groups, a.group_rows, plan.lanes, backward, plan.parts, plan.part_rows);
-  // (a launch has fewer than 2^32 threads; the sums of rows without registers are a grid's second axis)
-  if (plan.groups * plan.parts > (plan.lanes ? (1 << 24) - 1 : backward ? 65535 : INT32_MAX)) return CASCMM_ERR_TOO_LARGE;
+  // (a launch has fewer than 2^32 threads)
+  if (plan.groups * plan.parts > (plan.lanes ? (1 << 24) - 1 : INT32_MAX)) return CASCMM_ERR_TOO_LARGE;
   return CASCMM_OK;
 }
 static size_t gated_bytes(const cascmm_gated_norm& a, const GatedPlan& plan) {

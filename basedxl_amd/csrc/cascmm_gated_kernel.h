@@ -520,30 +520,32 @@ __global__ __launch_bounds__(kGatedWide) void cascmm_gated_norm_backward_wide_ke
     }
   }
 }
-// ... and the five sums with a thread a column over a part's rows (blockIdx.y: group and part)
+// ... and the five sums with a thread a column over a part's rows; `all` parts of all groups, which the grid's second axis goes through
 template <int IODT>
-__global__ __launch_bounds__(256) void cascmm_gated_norm_sums_kernel(const GatedParams p, int post) {
+__global__ __launch_bounds__(256) void cascmm_gated_norm_sums_kernel(const GatedParams p, int64_t all, int post) {
   typedef typename IoType<IODT>::T E;
   const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (col >= p.cols) return;
-  const int64_t group = blockIdx.y / p.parts, first = (int64_t)(blockIdx.y % p.parts) * p.part_rows;
-  const int64_t end = group * p.group_rows + (first + p.part_rows < p.group_rows ? first + p.part_rows : p.group_rows);
-  const int64_t wat = group * p.weight_ld + col;
-  const float w = !p.weight ? 1.f : p.f32 ? ((const float*)p.weight)[wat] : (float)((const E*)p.weight)[wat];
-  float sum[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int64_t row = group * p.group_rows + first; row < end; ++row) {
-    const float mean1 = p.stats[row], rstd1 = p.stats[p.rows + row], mean2 = p.stats[2 * p.rows + row], rstd2 = p.stats[3 * p.rows + row];
-    const float d = (float)((const E*)p.dy)[row * p.lddy + col], shat = ((float)((const E*)p.sum)[row * p.lds + col] - mean2) * rstd2;
-    float D = rstd2 * (d * w - p.row_means[row] - shat * p.row_means[p.rows + row]);
-    if (p.ds) D += (float)((const E*)p.ds)[row * p.ldds + col];
-    if (post || p.gate) sum[0] = __builtin_fmaf(D, ((float)((const E*)p.x)[row * p.ldx + col] - mean1) * rstd1, sum[0]);
-    sum[1] += D;
-    if (p.scale) sum[2] = __builtin_fmaf(D, (float)((const E*)p.residual)[row * p.ldr + col], sum[2]);
-    sum[3] = __builtin_fmaf(d, shat, sum[3]);
-    sum[4] += d;
-  }
+  for (int64_t at = blockIdx.y; at < all; at += gridDim.y) {
+    const int64_t group = at / p.parts, first = at % p.parts * p.part_rows;
+    const int64_t end = group * p.group_rows + (first + p.part_rows < p.group_rows ? first + p.part_rows : p.group_rows);
+    const int64_t wat = group * p.weight_ld + col;
+    const float w = !p.weight ? 1.f : p.f32 ? ((const float*)p.weight)[wat] : (float)((const E*)p.weight)[wat];
+    float sum[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int64_t row = group * p.group_rows + first; row < end; ++row) {
+      const float mean1 = p.stats[row], rstd1 = p.stats[p.rows + row], mean2 = p.stats[2 * p.rows + row], rstd2 = p.stats[3 * p.rows + row];
+      const float d = (float)((const E*)p.dy)[row * p.lddy + col], shat = ((float)((const E*)p.sum)[row * p.lds + col] - mean2) * rstd2;
+      float D = rstd2 * (d * w - p.row_means[row] - shat * p.row_means[p.rows + row]);
+      if (p.ds) D += (float)((const E*)p.ds)[row * p.ldds + col];
+      if (post || p.gate) sum[0] = __builtin_fmaf(D, ((float)((const E*)p.x)[row * p.ldx + col] - mean1) * rstd1, sum[0]);
+      sum[1] += D;
+      if (p.scale) sum[2] = __builtin_fmaf(D, (float)((const E*)p.residual)[row * p.ldr + col], sum[2]);
+      sum[3] = __builtin_fmaf(d, shat, sum[3]);
+      sum[4] += d;
+    }
 #pragma unroll
-  for (int i = 0; i < 5; ++i) p.partials[((int64_t)blockIdx.y * 5 + i) * p.cols + col] = sum[i];
+    for (int i = 0; i < 5; ++i) p.partials[(at * 5 + i) * p.cols + col] = sum[i];
+  }
 }
 
 // The gradients from the workgroups' sums.  Thirty-two columns a workgroup; of its 32 rows of threads `share` (a power of two) add a group's parts between them, so that

@@ -85,7 +85,7 @@ template <int IODT> hipError_t gated_backward(const GatedParams& p, int64_t grou
     CASCMM_LAUNCH(err, (p.cols < NormRow<IODT>::VEC ? cascmm_gated_norm_backward_wide_kernel<IODT, true> : cascmm_gated_norm_backward_wide_kernel<IODT, false>), grid, dim3(kGatedWide), 0, s,
                   p, post);
     if (p.partials && err == hipSuccess)
-      CASCMM_LAUNCH(err, cascmm_gated_norm_sums_kernel<IODT>, dim3((unsigned)((p.cols + 255) / 256), (unsigned)groups * (unsigned)p.parts), dim3(256), 0, s, p, post);
+      CASCMM_LAUNCH(err, cascmm_gated_norm_sums_kernel<IODT>, dim3((unsigned)((p.cols + 255) / 256), (unsigned)std::min<int64_t>(groups * p.parts, 4096)), dim3(256), 0, s, p, groups * p.parts, post);
     return err;
   }
   if (post) return rich ? gated_backward_of<IODT, true, true>(p, (unsigned)groups, s) : gated_backward_of<IODT, true, false>(p, (unsigned)groups, s);

@@ -58,6 +58,17 @@ def test_workspace():
     assert l.cascmm_gated_norm_forward(None, None) == -1 and l.cascmm_gated_norm_backward(None, None, 0, None) == -1
 
 
+@pytest.mark.parametrize("dtype, cols", [(F32, 3), (BF16, 7), (F32, 6145), (F16, 9000)])
+@pytest.mark.parametrize("rows, group_rows", [(65536, 1), (70000, 1), (1 << 21, 16)])
+def test_the_backward_pass_takes_the_groups_that_the_forward_pass_takes(dtype, cols, rows, group_rows):
+    """Rows that no registers hold, with parameters for more groups than a grid's second axis has places."""
+    lds = {k: cols for k in ("ldx", "ldr", "ldy", "lds", "lddy", "ldds", "lddx", "lddr", "gate_ld", "weight_ld")}
+    a, l = arguments(rows=rows, group_rows=group_rows, cols=cols, dtype=dtype, weight_dtype=dtype, dgate=P, dweight=P, dpost_weight=P, **lds), _lib.lib()
+    need = l.cascmm_gated_norm_workspace_bytes(ctypes.byref(a))
+    assert need >= rows // group_rows * 5 * cols * 4
+    assert l.cascmm_gated_norm_backward(ctypes.byref(a), P, need - 1, None) == -5      # (nothing but the workspace is wrong)
+
+
 def test_tensors_off_the_gpu_are_refused():
     x = torch.zeros(2, 8)
     with pytest.raises(RuntimeError, match="only runs on an AMD GPU"):

@@ -270,6 +270,18 @@ def test_gradients_of_rows_that_are_copied(gpu_device, samples, tokens, cols, na
             assert all(torch.equal(p, q) for p, q in zip(other, grads[0])), (of_x, of_residual)
 
 
+@pytest.mark.parametrize("name", ["conditioned", "everything"])
+@pytest.mark.parametrize("samples, tokens, cols, dtype", [(65537, 1, 3, torch.float32), (70001, 2, 7, torch.bfloat16), (5000, 3, 6147, torch.float16)])
+def test_more_groups_than_a_grid_has_rows(gpu_device, samples, tokens, cols, dtype, name):
+    """Rows that no registers hold, with parameters for each of many samples."""
+    how = HOWS[name]
+    t = make(how, samples, tokens, cols, dtype, dtype, gpu_device, cols)
+    leaves = {k: v.clone().requires_grad_() for k, v in t.items() if k not in ("dy", "ds")}
+    y, s = call(leaves, how, 1e-3)
+    grads = dict(zip(leaves, torch.autograd.grad((y, s), list(leaves.values()), (t["dy"], t["ds"]))))
+    check(t, how, 1e-3, y, s, grads)
+
+
 @pytest.mark.parametrize("samples", [1, 4])
 @pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
 def test_parts_of_a_conditioning(gpu_device, samples, wdtype):
