@@ -82,6 +82,7 @@ SIGNATURES = {
     "cascmm_layer_norm_backward": (c_int, [c_void_p] * 9 + [c_int64] * 6 + [c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "cascmm_gated_norm_forward": (c_int, [c_void_p, c_void_p]),
     "cascmm_gated_norm_workspace_bytes": (c_size_t, [c_void_p]),
+    "cascmm_gated_norm_backward_bytes": (c_size_t, [c_void_p]),
     "cascmm_gated_norm_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "cascmm_gradients_workspace_bytes": (c_size_t, [c_int, c_void_p]),
     "cascmm_clip_gradients": (c_int, [c_int, c_void_p, c_int, c_double, c_void_p, c_void_p, c_size_t, c_void_p]),

@@ -34,9 +34,13 @@ static int gated_plan(const cascmm_gated_norm& a, bool backward, GatedPlan& plan
   if (plan.groups * plan.parts > (plan.lanes ? (1 << 24) - 1 : INT32_MAX)) return CASCMM_ERR_TOO_LARGE;
   return CASCMM_OK;
 }
-static size_t gated_bytes(const cascmm_gated_norm& a, const GatedPlan& plan) {
-  const size_t sums = (size_t)plan.groups * (size_t)plan.parts * 5 * (size_t)a.cols * sizeof(float);
-  return sums + (plan.lanes ? 0 : 2 * (size_t)a.rows * sizeof(float)) + 16;
+static bool gated_sums(const cascmm_gated_norm& a) { return a.dgate || a.dscale || a.dpost_weight || a.dpost_bias || a.dweight || a.dbias; }
+// five sums where there is a row of the residual's scales or a bias of the first norm, and of rows without registers, else three
+static size_t gated_sum_bytes(const cascmm_gated_norm& a, const GatedPlan& plan) {
+  return (size_t)plan.groups * (size_t)plan.parts * (plan.lanes && !plan.rich ? 3 : 5) * (size_t)a.cols * sizeof(float);
+}
+static size_t gated_bytes(const cascmm_gated_norm& a, const GatedPlan& plan, bool sums) {
+  return (sums ? gated_sum_bytes(a, plan) + (plan.lanes ? 0 : 2 * (size_t)a.rows * sizeof(float)) : 0) + 16;
 }
 static bool gated_pointers(const cascmm_gated_norm& a) {
   const int64_t es = gated_size(a.dtype), ws = gated_size(a.weight_dtype);
@@ -95,7 +99,11 @@ int cascmm_gated_norm_forward(const cascmm_gated_norm* args, void* stream) {
 
 size_t cascmm_gated_norm_workspace_bytes(const cascmm_gated_norm* args) {
   GatedPlan plan;
-  return args && gated_plan(*args, true, plan) == CASCMM_OK ? gated_bytes(*args, plan) : 0;
+  return args && gated_plan(*args, true, plan) == CASCMM_OK ? gated_bytes(*args, plan, true) : 0;
+}
+size_t cascmm_gated_norm_backward_bytes(const cascmm_gated_norm* args) {
+  GatedPlan plan;
+  return args && gated_plan(*args, true, plan) == CASCMM_OK ? gated_bytes(*args, plan, gated_sums(*args)) : 0;
 }
 
 int cascmm_gated_norm_backward(const cascmm_gated_norm* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -104,7 +112,7 @@ int cascmm_gated_norm_backward(const cascmm_gated_norm* args, void* workspace, s
   GatedPlan plan;
   const int st = gated_plan(a, true, plan);
   if (st != CASCMM_OK) return st;
-  const bool sums = a.dgate || a.dscale || a.dpost_weight || a.dpost_bias || a.dweight || a.dbias, reads_x = a.post || a.gate;
+  const bool sums = gated_sums(a), reads_x = a.post || a.gate;
   if (a.lddy < a.cols || a.lds < a.cols || (reads_x && a.ldx < a.cols) || (a.scale && a.ldr < a.cols) || (a.ds && a.ldds < a.cols) || (a.dx && a.lddx < a.cols) ||
       (a.dresidual && a.lddr < a.cols))
     return CASCMM_ERR_BAD_SHAPE;
@@ -115,11 +123,11 @@ int cascmm_gated_norm_backward(const cascmm_gated_norm* args, void* workspace, s
   if (a.cols == 0 || (!a.dx && !a.dresidual && !sums) || (a.rows == 0 && !sums)) return CASCMM_OK;
   if (a.rows > 0 && (!a.dy || !a.sum || !a.stats || (reads_x && !a.x) || (a.scale && !a.residual))) return CASCMM_ERR_NULL_POINTER;
   if (!gated_pointers(a)) return CASCMM_ERR_ALIGNMENT;
-  if (!workspace || workspace_bytes < gated_bytes(a, plan)) return CASCMM_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < gated_bytes(a, plan, sums)) return CASCMM_ERR_WORKSPACE;
   if (!gated_aligned(workspace, 16)) return CASCMM_ERR_ALIGNMENT;
   GatedParams p = gated_params(a, plan);
   p.partials = sums ? (float*)workspace : nullptr;
-  if (!plan.lanes) p.row_means = (float*)workspace + (size_t)plan.groups * (size_t)plan.parts * 5 * (size_t)a.cols;
+  if (!plan.lanes && sums) p.row_means = (float*)((char*)workspace + gated_sum_bytes(a, plan));
   const hipStream_t s = (hipStream_t)stream;
   const bool post = a.post != 0;
   hipError_t err = hipSuccess;

@@ -218,7 +218,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     a.dx = ptr(dx); a.dresidual = ptr(dr);
     a.lddx = a.lddr = cols;
     if (residual.defined()) rows_of(residual, rows, cols, a.ldr);
-    const at::Tensor ws = scratch(cascmm_gated_norm_workspace_bytes(&a), s);
+    const at::Tensor ws = scratch(cascmm_gated_norm_backward_bytes(&a), s);
     check(cascmm_gated_norm_backward(&a, ws.data_ptr(), ws.nbytes(), stream_of(s)), "cascmm_gated_norm_backward");
     if (want_x) out[0] = same ? dr : dx;
     if (want_r) out[1] = dr;

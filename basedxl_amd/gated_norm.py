@@ -130,7 +130,7 @@ class _GatedAddNorm(torch.autograd.Function):
                 a.dy, a.ds, a.stats, a.dx, a.dresidual = dy2.data_ptr(), _ptr(ds2), stats.data_ptr(), _ptr(dx), _ptr(dr)
                 a.dweight, a.dbias, a.dgate, a.dscale, a.dpost_weight, a.dpost_bias = map(_ptr, grads)
                 a.lddy, a.ldds, a.lddx, a.lddr = _ld(dy2), 0 if ds2 is None else _ld(ds2), cols, cols
-                ws = torch.empty(l.cascmm_gated_norm_workspace_bytes(ctypes.byref(a)), dtype=torch.uint8, device=dev)   # (a temporary of the call)
+                ws = torch.empty(l.cascmm_gated_norm_backward_bytes(ctypes.byref(a)), dtype=torch.uint8, device=dev)   # (a temporary of the call)
                 _lib.check(l.cascmm_gated_norm_backward(ctypes.byref(a), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream),
                            "cascmm_gated_norm_backward")
         return (dr if same and want[0] else dx, dr if want[1] else None, *grads, None, None, None, None)
@@ -146,7 +146,7 @@ def gated_add_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[tor
 
     ``x`` and ``residual``: fp32, fp16 or bf16, alike, with any leading dimensions.  ``gate``, ``residual_scale`` (a number or a tensor), ``weight`` and ``bias`` are
     [C], or one row for each entry of the first axis of ``x``, ``(B, 1, .., C)``, as a conditioning gives them to its samples (made for many rows to a sample: the backward
-    pass holds five rows of sums for each); gate and scale may be scalars too; ``post_weight`` and ``post_bias`` are [C].  All of the dtype of ``x`` or fp32; None: ones, for a bias
+    pass holds three to five fp32 rows of sums for each while it runs, if any of their gradients is wanted); gate and scale may be scalars too; ``post_weight`` and ``post_bias`` are [C].  All of the dtype of ``x`` or fp32; None: ones, for a bias
     zeros.  The norm is of ``s`` as it is returned, rounded to the tensors' dtype; statistics and arithmetic are fp32, each result is rounded once.
     Differentiable once in all tensors, through both results; sums over rows are added in a fixed order, so the same call gives the same bits."""
     # the ordinary eager call in one native function; None: whatever is not ordinary about it is decided below

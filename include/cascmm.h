@@ -395,7 +395,8 @@ int cascmm_layer_norm_backward(const void* dy, const void* ds, const void* x, co
  * Backward, from the gradients dy of y and ds of s (NULL: zeros): dx, dresidual, and of those operands that are there dgate, dscale, dpost_weight, dpost_bias, dweight and
  * dbias, [cols] or, where the operand's leading dimension is not 0, [groups][cols]; each NULL if it is not wanted.  It reads sum and stats of the forward pass, x with
  * `post` or a gate, residual with a scale.  Sums over rows are fp32 in a fixed order, without atomics.  The workspace (16-byte aligned, no initialisation) holds
- * cascmm_gated_norm_workspace_bytes: five rows of sums for each of up to 1024 workgroups, and at least one workgroup to a group.
+ * cascmm_gated_norm_backward_bytes of these arguments: nothing but 16 bytes where none of dgate to dbias is wanted, else three rows of sums, or five with a scale, a post_bias or rows
+ * that registers do not hold, for each of up to 1024 workgroups and at least one workgroup to a group.  cascmm_gated_norm_workspace_bytes is what is enough whichever are wanted.
  * The struct is read during the call only.
  */
 typedef enum cascmm_norm_kind { CASCMM_NORM_LAYER = 0, CASCMM_NORM_RMS = 1 } cascmm_norm_kind;
@@ -413,6 +414,7 @@ typedef struct cascmm_gated_norm {
 } cascmm_gated_norm;
 int cascmm_gated_norm_forward(const cascmm_gated_norm* args, void* stream);
 size_t cascmm_gated_norm_workspace_bytes(const cascmm_gated_norm* args);
+size_t cascmm_gated_norm_backward_bytes(const cascmm_gated_norm* args);
 int cascmm_gated_norm_backward(const cascmm_gated_norm* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /*

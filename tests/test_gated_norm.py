@@ -69,6 +69,20 @@ def test_the_backward_pass_takes_the_groups_that_the_forward_pass_takes(dtype, c
     assert l.cascmm_gated_norm_backward(ctypes.byref(a), P, need - 1, None) == -5      # (nothing but the workspace is wrong)
 
 
+@pytest.mark.parametrize("cols, rich", [(8, False), (8, True), (1280, False), (1280, True), (3, False), (9000, True)])
+def test_a_backward_pass_asks_for_what_it_writes(cols, rich):
+    """No more than 16 bytes where no sum over rows is wanted; three rows of sums, or five, for each group of one row."""
+    lds = {k: cols for k in ("ldx", "ldr", "ldy", "lds", "lddy", "ldds", "lddx", "lddr", "gate_ld", "weight_ld")}
+    how = dict(rows=32768, group_rows=1, cols=cols, **lds, **({} if rich else dict(scale=None, post_bias=None)))
+    l, sums = _lib.lib(), 5 if rich or cols in (3, 9000) else 3
+    means = 2 * 32768 * 4 if cols in (3, 9000) else 0
+    for wanted, want in ((dict(), 16), (dict(dweight=P), 16 + 32768 * sums * cols * 4 + means), (dict(dgate=P, dbias=P), 16 + 32768 * sums * cols * 4 + means)):
+        a = arguments(**how, **wanted)
+        assert l.cascmm_gated_norm_backward_bytes(ctypes.byref(a)) == want <= l.cascmm_gated_norm_workspace_bytes(ctypes.byref(a))
+        assert l.cascmm_gated_norm_backward(ctypes.byref(a), P, want - 1, None) == -5 and l.cascmm_gated_norm_backward(ctypes.byref(a), None, want, None) == -5
+    assert l.cascmm_gated_norm_backward_bytes(None) == 0 and l.cascmm_gated_norm_backward_bytes(ctypes.byref(arguments(rows=7))) == 0
+
+
 def test_tensors_off_the_gpu_are_refused():
     x = torch.zeros(2, 8)
     with pytest.raises(RuntimeError, match="only runs on an AMD GPU"):

@@ -282,6 +282,26 @@ def test_more_groups_than_a_grid_has_rows(gpu_device, samples, tokens, cols, dty
     check(t, how, 1e-3, y, s, grads)
 
 
+@pytest.mark.parametrize("cols", [5, 640, 7000])
+@pytest.mark.parametrize("name", ["conditioned", "both_norms", "everything"])
+def test_gradients_of_the_streams_alone(gpu_device, cols, name):
+    """Parameters for every token that are not trained: the same gradients of x and the residual, without memory for sums that nobody wants."""
+    how, rows = HOWS[name], 2000
+    t = make(how, rows, 1, cols, torch.bfloat16, torch.bfloat16, gpu_device, cols)
+    both = []
+    for trained in (True, False):
+        leaves = {k: v.clone().requires_grad_(trained or k in ("x", "residual")) for k, v in t.items() if k not in ("dy", "ds")}
+        out = call(leaves, how, 1e-5)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        requested = lambda which: torch.cuda.memory_stats()["requested_bytes.all." + which]   # noqa: E731  (what was asked for: a block may be up to 1 MiB larger)
+        before = requested("current")
+        both.append(torch.autograd.grad(out, (leaves["x"], leaves["residual"]), (t["dy"], t["ds"])))
+        if not trained:
+            assert requested("peak") - before == 2 * rows * cols * 2 + 16      # (the two results, and the least workspace)
+    assert all(torch.equal(p, q) for p, q in zip(*both))
+
+
 @pytest.mark.parametrize("samples", [1, 4])
 @pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
 def test_parts_of_a_conditioning(gpu_device, samples, wdtype):
