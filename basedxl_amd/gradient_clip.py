@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import math
 from array import array
-from typing import Iterable, Optional, Sequence, Union
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -26,6 +26,74 @@ def _dense(t: torch.Tensor) -> bool:
             return False
         span *= size
     return True
+
+
+def _reach(terms: Sequence[Tuple[int, int, int]], low: int, high: int) -> bool:
+    """Whether some sum of c * stride, least <= c <= most for each of ``terms`` (stride, least, most), largest strides first, lies in [low, high]."""
+    if not terms:
+        return low <= 0 <= high
+    (stride, least, most), rest = terms[0], terms[1:]
+    down, up = sum(s * c for s, c, _ in rest), sum(s * c for s, _, c in rest)
+    return any(_reach(rest, low - c * stride, high - c * stride) for c in range(max(least, -((up - low) // stride)), min(most, (high - down) // stride) + 1))
+
+
+def _steps(t: torch.Tensor) -> List[Tuple[int, int]]:
+    """(distance in bytes, indices behind the first) of the axes that move."""
+    size = t.element_size()
+    return sorted(((st * size, n - 1) for n, st in zip(t.shape, t.stride()) if n > 1), reverse=True)
+
+
+def _overlap(p: torch.Tensor, q: torch.Tensor) -> bool:
+    """Whether two tensors, of any strides, share a byte."""
+    if p.numel() == 0 or q.numel() == 0:
+        return False
+    terms = {}
+    for t, sign in ((p, -1), (q, 1)):
+        for stride, most in _steps(t):
+            if stride:
+                least, up = terms.get(stride, (0, 0))
+                terms[stride] = (least - most, up) if sign < 0 else (least, up + most)
+    apart = q.data_ptr() - p.data_ptr()
+    return _reach([(s, *terms[s]) for s in sorted(terms, reverse=True)], 1 - q.element_size() - apart, p.element_size() - 1 - apart)
+
+
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two elements of a tensor share memory."""
+    if t.numel() == 0:
+        return False
+    steps = _steps(t)
+    if any(stride == 0 for stride, _ in steps):
+        return True
+    # (two elements whose first index that differs is the k-th)
+    return any(_reach([(steps[k][0], 1, steps[k][1])] + [(s, -n, n) for s, n in steps[k + 1:]], 0, 0) for k in range(len(steps)))
+
+
+def _direct(g: torch.Tensor, o: torch.Tensor) -> bool:
+    """Whether the kernels read ``g`` and write ``o`` as they lie (else the elements are copied)."""
+    return _dense(g) and (o is g or (_dense(o) and o.stride() == g.stride()))
+
+
+def _refuse_shared_memory(gradients: Sequence[torch.Tensor], results: Sequence[torch.Tensor]) -> None:
+    """Refuses a result that shares memory with another, with a gradient that is not its own or with itself, where one of the two is copied (the C entry point
+    sees copies in their places; of the others it sees all)."""
+    spans = []
+    for i, (g, o) in enumerate(zip(gradients, results)):
+        copied = not _direct(g, o)
+        if copied and _overlaps_itself(o):
+            raise ValueError(f"clip_gradients: elements of result {i} share memory")
+        for t, written in ((o, True),) if o is g else ((o, True), (g, False)):
+            if t.numel():
+                spans.append((t.data_ptr(), t.data_ptr() + sum(s * n for s, n in _steps(t)) + t.element_size(), i, written, copied, t))
+    spans.sort(key=lambda s: s[0])
+    behind = []      # those that reach beyond where the next one begins
+    for span in spans:
+        begin, _, i, written, copied, t = span
+        behind = [s for s in behind if s[1] > begin]
+        for _, _, k, w, c, other in behind:
+            if k != i and (written or w) and (copied or c) and _overlap(t, other):
+                which = "another" if written and w else f"gradient {k if written else i}"
+                raise ValueError(f"clip_gradients: result {i if written else k} shares memory with {which}")
+        behind.append(span)
 
 
 def _check(gradients: Sequence[torch.Tensor], norm_type: float, name: str) -> int:
@@ -81,7 +149,8 @@ def clip_gradients(gradients: Iterable[torch.Tensor], max_norm: float, *, norm_t
     """``g * min(1, max_norm / (norm + 1e-6))`` for every gradient, in place or into ``out`` (a tensor for each, of its shape and of its type or
     fp32), and the norm of all of them together as :func:`gradient_norm` returns it.  Nothing waits for the GPU: the factor stays there, and gradients
     in place that need no clipping are not written.  A NaN among the gradients makes all of them NaN; an infinity makes the factor 0 and itself NaN.  A result shares memory
-    with no other result and no gradient but its own (CascmmError): a tensor that is listed twice would be scaled twice."""
+    with no other result and no gradient but its own (CascmmError, ValueError where the elements of one of the two are copied: strides with gaps, or other than those of its
+    gradient): a tensor that is listed twice would be scaled twice.  Parts of a buffer whose elements lie between each other do not share memory."""
     gradients = list(gradients)
     results = gradients if out is None else list(out)
     norm = _lib.short_cut().clip_gradients(gradients, results, _NORM_TYPES.get(norm_type, -1), max_norm)
@@ -100,14 +169,14 @@ def clip_gradients(gradients: Iterable[torch.Tensor], max_norm: float, *, norm_t
                 raise ValueError(f"clip_gradients: out[{i}] must be {tuple(g.shape)}, {g.dtype} or float32, on {g.device}, got {tuple(o.shape)} {o.dtype} on {o.device}")
             if o.requires_grad and o.is_leaf:
                 raise ValueError(f"clip_gradients: out[{i}] is a leaf that requires a gradient")
-        if _dense(g) and (o is g or (_dense(o) and o.stride() == g.stride())):
+    direct = [_direct(g, o) for g, o in zip(gradients, results)]
+    if not all(direct):
+        _refuse_shared_memory(gradients, results)
+    for g, o, whole in zip(gradients, results, direct):
+        if whole:
             sources.append(g)
             targets.append(o)
         else:   # (orders of elements that differ, or gaps between them: the scaled elements are put in place behind the call)
-            if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
-                raise ValueError(f"clip_gradients: elements of result {i} share memory")
-            if any(o.data_ptr() == other.data_ptr() for k, other in enumerate(results) if k != i and other.numel() > 0) and o.numel() > 0:
-                raise ValueError(f"clip_gradients: result {i} shares memory with another")
             sources.append(g.contiguous())
             targets.append(torch.empty(g.shape, dtype=o.dtype, device=g.device))
             copied.append((o, targets[-1]))

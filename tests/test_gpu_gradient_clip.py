@@ -163,6 +163,21 @@ def test_refusals(gpu_device):
     assert torch.equal(gradient_norm([g, g]), gradient_norm([g, h]))                   # (a norm reads only)
 
 
+def test_columns_of_one_buffer(gpu_device):
+    """Views whose elements lie between each other are no overlap; views that share elements are one wherever they begin, and then nothing is written."""
+    c, far = torch.randn(40, 30, device=gpu_device), torch.randn(40, 30, device=gpu_device)
+    kept, views = c.clone(), [c[:, :7], c[:, 7:8], c[:, 8::2], c[:, 9::2]]
+    want = norm_of([kept], 2.0)
+    check_norm(clip_gradients(views, 0.5), want)
+    check_scaled(c, kept, want, 0.5)
+    c.copy_(kept)
+    for gradients, out in (([c[:, :3], c[:, 2:5]], None), ([far[:, 1:3], far], [c[:, 1:3], c]), ([far, far[:, 1:3]], [c, c[:, 1:3]]), ([far[:, :5], c[:, 4:9]], [c[:, :5], far[:, 4:9]]),
+                           ([far[:, :5], c], [c[:, 3:8], torch.empty_like(c)]), ([far[:, :5], c.bfloat16()[:, :2]], [c[:, ::7], c[:, 6:8]]), ([far[:6, :3]], [c.as_strided((6, 3), (1, 1))])):
+        with pytest.raises(ValueError, match="share"):
+            clip_gradients(gradients, 1e-3, out=out)
+        assert torch.equal(c, kept)
+
+
 def test_ordinary_calls_are_one_native_function(gpu_device):
     g, h = torch.ones(8, 3, device=gpu_device), torch.ones(8, 3, device=gpu_device, dtype=torch.bfloat16)
     f = _lib.native().clip_gradients
