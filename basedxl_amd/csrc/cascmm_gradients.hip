@@ -117,7 +117,7 @@ int cascmm_clip_gradients(int count, const cascmm_gradient* gradients, int norm_
   memset(&b, 0, sizeof(b));
   b.chunk = plan.chunk;
   b.parts = (double*)((char*)workspace + 16);
-  b.head = (float*)workspace;
+  b.head = (double*)workspace;
   b.max_norm = max_norm;
   b.norm = norm;
   b.type = norm_type;

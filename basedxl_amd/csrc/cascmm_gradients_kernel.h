@@ -4,7 +4,8 @@
 //
 // Sums are fp64 from the first square on: nothing overflows or vanishes between 1e-45 and 3e38, and the norm is good to fp32's last bit whatever
 // the number of elements.  The tensors are cut into chunks, one to a workgroup; each chunk's sum goes to a place of its own and the places are added
-// in a fixed order, so that the same call gives the same bits.  Results are rounded once, from fp32.
+// in a fixed order, so that the same call gives the same bits.  Results are rounded once, from fp32.  A factor below fp32's normal numbers (gradients of 1e38 and more) would lose its
+// bits, or be zero where results are not: it is multiplied in fp64 then.
 //
 // Bound by memory: the gradients are read for the norm and again to be scaled, 12 bytes an fp32 element with the store.  The tensors' addresses travel in the
 // kernels' arguments, as many to a launch as fit: there is no table in memory to be kept, copied or outlived by a recorded graph.
@@ -22,7 +23,7 @@ constexpr int kGradMerged = 2560;         // partial sums that every workgroup o
 struct GradBatch {
   int64_t chunk;
   double* parts;        // of all chunks of the call
-  float* head;          // [0]: factor
+  double* head;         // the factor
   double max_norm;
   float* norm;
   unsigned part0, all_parts;   // the first chunk of this launch; of all launches
@@ -120,19 +121,19 @@ template <int UNUSED> __global__ __launch_bounds__(256) void cascmm_gradient_par
 }
 
 // norm and factor from all parts, in every thread of a workgroup of NT
-template <int NT> __device__ __forceinline__ float grad_factor(const double* parts, unsigned count, int type, double max_norm, double* slots, double& norm) {
+template <int NT> __device__ __forceinline__ double grad_factor(const double* parts, unsigned count, int type, double max_norm, double* slots, double& norm) {
   double v = 0;
   for (unsigned i = threadIdx.x; i < count; i += NT) v = grad_join(v, parts[i], type);
   v = grad_meet<NT>(v, type, slots);
   norm = type == 2 ? __builtin_sqrt(v) : v;
   const double f = max_norm / (norm + 1e-6);
-  return (float)(f > 1.0 ? 1.0 : f);   // (a NaN stays one)
+  return f > 1.0 ? 1.0 : f;   // (a NaN stays one)
 }
 template <int UNUSED>
-__global__ __launch_bounds__(1024) void cascmm_gradient_norm_kernel(const double* __restrict__ parts, unsigned count, int type, double max_norm, float* norm_out, float* head) {
+__global__ __launch_bounds__(1024) void cascmm_gradient_norm_kernel(const double* __restrict__ parts, unsigned count, int type, double max_norm, float* norm_out, double* head) {
   __shared__ double slots[16];
   double norm;
-  const float f = grad_factor<1024>(parts, count, type, max_norm, slots, norm);
+  const double f = grad_factor<1024>(parts, count, type, max_norm, slots, norm);
   if (threadIdx.x == 0) {
     *norm_out = (float)norm;
     *head = f;
@@ -168,20 +169,34 @@ template <int DT, int ODT> __device__ __forceinline__ void grad_scale(const void
   }
 }
 
+// ... by a factor below fp32's normal numbers: of any types, an element at a time
+__device__ __forceinline__ void grad_scale_finely(const GradBatch& b, int t, int64_t at, int64_t len, double f) {
+  const int dt = b.dtype[t];
+  for (int64_t i = at + threadIdx.x; i < at + len; i += 256) {
+    const float g = dt == CASCMM_DT_F32 ? ((const float*)b.g[t])[i] : dt == CASCMM_DT_F16 ? (float)((const _Float16*)b.g[t])[i] : (float)((const __bf16*)b.g[t])[i];
+    const float o = (float)((double)g * f);
+    if (b.out_dtype[t] == CASCMM_DT_F32) ((float*)b.out[t])[i] = o;
+    else if (b.out_dtype[t] == CASCMM_DT_F16) ((_Float16*)b.out[t])[i] = (_Float16)o;
+    else ((__bf16*)b.out[t])[i] = (__bf16)o;
+  }
+}
+
 // the second pass.  Gradients that stay where they are and are not clipped are not touched.
 template <int UNUSED> __global__ __launch_bounds__(256) void cascmm_gradient_scale_kernel(const GradBatch b) {
   __shared__ double slots[4];
   const int t = grad_tensor(b, blockIdx.x);
-  float f;
+  double factor;
   if (b.merged) {
     double norm;
-    f = grad_factor<256>(b.parts, b.all_parts, b.type, b.max_norm, slots, norm);
+    factor = grad_factor<256>(b.parts, b.all_parts, b.type, b.max_norm, slots, norm);
     if (b.part0 + blockIdx.x == 0 && threadIdx.x == 0) *b.norm = (float)norm;
   } else {
-    f = *b.head;
+    factor = *b.head;
   }
+  const float f = (float)factor;
   if (f == 1.f && b.out[t] == b.g[t]) return;
   const int64_t at = (int64_t)(blockIdx.x - b.first[t]) * b.chunk, left = b.n[t] - at, len = left < b.chunk ? left : b.chunk;
+  if (factor < 0x1p-126) return grad_scale_finely(b, t, at, len, factor);
   const int dt = b.dtype[t], odt = b.out_dtype[t];
   if (dt == CASCMM_DT_F32) grad_scale<CASCMM_DT_F32, CASCMM_DT_F32>(b.g[t], b.out[t], at, len, f);
   else if (dt == CASCMM_DT_F16 && odt == CASCMM_DT_F16) grad_scale<CASCMM_DT_F16, CASCMM_DT_F16>(b.g[t], b.out[t], at, len, f);

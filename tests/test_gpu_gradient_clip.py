@@ -91,6 +91,21 @@ def test_squares_beyond_fp32(gpu_device, scale):
         check_scaled(o, g, want, 0.5 * scale)
 
 
+@pytest.mark.parametrize("dtypes", [(torch.float32,), (torch.bfloat16,), (torch.bfloat16, torch.float32, torch.float16)])
+@pytest.mark.parametrize("sizes", [[(1000,), (333,)], [(1 + i % 9,) for i in range(2700)]])        # (the factor made by every workgroup, and by a kernel of its own)
+@pytest.mark.parametrize("max_norm", [2.0, 1e-3, 1e-20, 3e-38, 1e-60])
+def test_factors_below_the_normal_numbers(gpu_device, max_norm, sizes, dtypes):
+    """Gradients as large as their type holds: the factor is far below fp32's normal numbers, and the results are not."""
+    gradients = [(g.float().tanh() * (6e4 if g.dtype == torch.float16 else 3e38)).to(g.dtype) for g in make(sizes, dtypes, gpu_device)]
+    want = norm_of(gradients, 2.0)
+    for out in ([torch.empty_like(g) for g in gradients], [torch.empty_like(g, dtype=torch.float32) for g in gradients], None):
+        into = [g.clone() for g in gradients] if out is None else gradients
+        norm = clip_gradients(into, max_norm, out=out)
+        assert float(norm) == math.inf if float(want) > 3.5e38 else abs(float(norm) - float(want)) <= float(want) * U
+        for o, g in zip(into if out is None else out, gradients):
+            check_scaled(o, g, want, max_norm)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("where", [0, 4099, 9999])
