@@ -312,6 +312,24 @@ def test_scales_far_apart(gpu_device, ea, eb):
     check_product(block_scaled_matmul(a16.to(gpu_device), b16.to(gpu_device)), held(a16, "rows")[0], held(b16, "square")[0], None, "bf16")
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("K", [16, 128, 300, 5000])
+def test_large_products_that_cancel(gpu_device, K, dtype):
+    """Two products of the largest size in every few neighbours, of which nothing is left: what small ones add up to is good to 2^-10 of the large ones in 16 bits, and exact in fp32."""
+    gen = torch.Generator().manual_seed(K)
+    a, b = torch.randint(1, 8, (5, K), generator=gen) * 2.0 ** -6, torch.randint(-7, 8, (K, 9), generator=gen) * 2.0 ** -3
+    for at in range(0, K - 8, 37):
+        a[:, at], a[:, at + 5] = 448.0, 448.0
+        b[at], b[at + 5] = 1.0, -1.0
+    a, b = a.to(dtype), b.to(dtype)
+    ha, hb = held(a, "rows")[0], held(b, "square")[0]
+    assert torch.equal(ha, a.double()) and torch.equal(hb, b.double())         # (whole numbers of up to three bits: held as they are)
+    y = block_scaled_matmul(a.to(gpu_device), b.to(gpu_device))
+    check_product(y, ha, hb, None, "y")
+    if dtype == torch.float32:
+        assert torch.equal(y.cpu().double(), ha @ hb)                          # (multiples of 2^-9, and sums of less than 2^15)
+
+
 def test_ordinary_calls_are_one_native_function(gpu_device):
     x, w, b = (torch.ones(s, device=gpu_device, dtype=torch.bfloat16) for s in ((4, 20, 64), (64, 32), (32,)))
     held = BlockScaledWeight(w)
