@@ -137,7 +137,8 @@ def block_scaled_matmul(a: torch.Tensor, b, *, bias: Optional[torch.Tensor] = No
     result (of the dtype of ``a``) is rounded once.  16-bit results come from the 8-bit matrix instruction, which cuts products at about 2^-15 of the largest of their neighbours: of ordinary
     data 1.5e-5 of a result's usual size (rms; less than its rounding, but results far below the usual size show it), and at worst 2^-10 of the largest product of every sixteen
     neighbouring k, to which alone what large products that cancel leave is good.
-    fp32 results have products and sums to fp32's accuracy (at about half the rate, 1272 against 2798 TFLOP/s at 8192 x 8192 x 8192; rounded elements below 2^-126 count as zeros there).  K and the rows of ``a`` up to 2^22.
+    fp32 results have products and sums to fp32's accuracy (at about half the rate, 1272 against 2798 TFLOP/s at 8192 x 8192 x 8192; rounded elements below 2^-126 count as zeros there, and
+    those that round to 2^128, from 1.9375 * 2^127 on, as infinite).  K and the rows of ``a`` up to 2^22.
 
     Differentiable once in ``a``, ``b`` (a tensor: a held weight is a constant that no gradient passes through) and ``bias``, by products of the same kind, with the
     rounding passed over: ``dy`` in blocks of 128 along N times the same rounded ``b``; ``a`` and ``dy`` both in blocks of 128 rows; ``dbias`` from ``dy`` itself."""

@@ -451,7 +451,7 @@ int cascmm_clip_gradients(int count, const cascmm_gradient* gradients, int norm_
  * aligned, no initialisation) holds cascmm_block_round_workspace_bytes.  values and values_t are 16-byte aligned.
  * cascmm_block_gemm: a [M rows][K], b [N rows][K], C [M, N] (leading dimension ldc) and bias (NULL or [N]) of `dtype`.  16-bit results come from the 8-bit matrix
  * instruction, which cuts products at about 2^-15 of the largest of their neighbours (of ordinary data 1.5e-5 rms of a result's size; at worst 2^-10 of the largest product of every
- * sixteen neighbouring k), fp32 results from the 16-bit one on the same values, with fp32's accuracy (rounded elements below 2^-126 count as zeros).  K up to 2^22.
+ * sixteen neighbouring k), fp32 results from the 16-bit one on the same values, with fp32's accuracy (rounded elements below 2^-126 count as zeros, those of 2^128 as infinite).  K up to 2^22.
  */
 size_t cascmm_block_values_bytes(int64_t rows, int64_t k);
 size_t cascmm_block_scales_bytes(int64_t rows, int64_t k);

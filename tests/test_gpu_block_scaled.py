@@ -330,6 +330,25 @@ def test_large_products_that_cancel(gpu_device, K, dtype):
         assert torch.equal(y.cpu().double(), ha @ hb)                          # (multiples of 2^-9, and sums of less than 2^15)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+def test_the_largest_numbers(gpu_device, dtype):
+    """The type's lowest value, as a mask has it: a finite number like others in 16 bits; in fp32, where it rounds to -2^128, infinite, and it alone."""
+    gen = torch.Generator().manual_seed(4)
+    a, b = stream(gen, 12, 260, dtype), (0.02 * torch.randn(260, 70, generator=gen)).to(dtype)
+    b[7, 5] = 0.0
+    clean = block_scaled_matmul(a.to(gpu_device), b.to(gpu_device))
+    a[3, 7], a[6, 7], a[6, 200] = torch.finfo(dtype).min, 0.96 * torch.finfo(dtype).max, -0.9 * torch.finfo(dtype).max
+    y = block_scaled_matmul(a.to(gpu_device), b.to(gpu_device))
+    rest = [r for r in range(12) if r not in (3, 6)]
+    assert torch.equal(y[rest], clean[rest])
+    ha, hb = held(a, "rows")[0], held(b, "square")[0]
+    if dtype == torch.float32:
+        row, zero = y[3].cpu().double(), hb[7] == 0
+        assert ha[3, 7] == -2.0 ** 128 and bool(row[zero].isnan().all()) and torch.equal(row[~zero], -math.inf * hb[7][~zero])
+        ha, y = ha[[r for r in range(12) if r != 3]], y[[r for r in range(12) if r != 3]]
+    check_product(y, ha, hb, None, "y")
+
+
 def test_ordinary_calls_are_one_native_function(gpu_device):
     x, w, b = (torch.ones(s, device=gpu_device, dtype=torch.bfloat16) for s in ((4, 20, 64), (64, 32), (32,)))
     held = BlockScaledWeight(w)
