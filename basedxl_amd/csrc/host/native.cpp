@@ -47,8 +47,7 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (st != CASCMM_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 
@@ -100,8 +99,7 @@ PyObject* prepared(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (st != CASCMM_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 
@@ -159,8 +157,7 @@ PyObject* fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (st != CASCMM_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 

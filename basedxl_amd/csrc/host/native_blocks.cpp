@@ -267,8 +267,7 @@ PyObject* block_scaled(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     return THPVariable_Wrap(std::move(out));
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 
@@ -308,8 +307,7 @@ PyObject* gated_add_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Gated g = gated_forward(*x, *residual, p, how, false);
     return pair(std::move(g.y), std::move(g.s));
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 
@@ -353,8 +351,7 @@ PyObject* clip_gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     for (const at::Tensor* o : written) o->unsafeGetTensorImpl()->bump_version();   // (written behind autograd's back)
     return THPVariable_Wrap(std::move(norm));
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 

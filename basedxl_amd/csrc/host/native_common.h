@@ -7,6 +7,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -64,6 +65,20 @@ inline int products_code(PyObject* s) {
   if (PyUnicode_CompareWithASCIIString(s, "tri") == 0) return CASCMM_PROD_TRI;
   if (PyUnicode_CompareWithASCIIString(s, "full") == 0) return CASCMM_PROD_FULL;
   return -1;
+}
+
+// A native function's answer to an exception, in its handler: None, so that the Python code decides, but for one that Python code raised within the call (a hook of saved tensors, by which
+// activation checkpointing ends its second run; a dispatch mode): that is the caller's, and Python code behind it would run the hook once more.
+inline PyObject* not_ordinary() {
+  try {
+    throw;
+  } catch (python_error& e) {
+    e.restore();
+    if (PyErr_Occurred()) return nullptr;
+  } catch (...) {
+  }
+  PyErr_Clear();
+  Py_RETURN_NONE;
 }
 
 // a plain torch.Tensor or Parameter on the current GPU (no subclass: those may not own memory)

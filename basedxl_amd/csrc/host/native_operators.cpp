@@ -282,8 +282,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     at::Tensor y = differentiated({x, &weight, &bias}) ? LayerNormNode::apply(*x, optional_of(weight), optional_of(bias), eps) : norm_forward(*x, at::Tensor(), weight, bias, eps, false).y;
     return THPVariable_Wrap(std::move(y));
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 
@@ -316,8 +315,7 @@ PyObject* add_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Py_XDECREF(ps);
     return both;
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 
@@ -342,8 +340,7 @@ PyObject* epilogue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const at::Tensor weight = kernel_rows(*b, N, ldb, copied_weight(*b, p.K, N) > INT32_MAX);
     return run_product(p, weight.const_data_ptr(), 0, copied_weight(weight, p.K, N), N, fmt, terms, products, device);
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 
@@ -370,8 +367,7 @@ PyObject* epilogue_prepared(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
     }
     return run_product(p, slots->const_data_ptr(), 1, 0, N, fmt, terms, products, device);
   } catch (...) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
+    return not_ordinary();
   }
 }
 
