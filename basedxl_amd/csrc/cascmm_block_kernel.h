@@ -6,8 +6,10 @@
 // applies it by itself (one E8M0 byte a lane), so that all blocks of a row meet in one fp32 accumulator and nothing is added to the loop for the scales.
 // Infinities and NaN become NaN.
 //
-// The rounding is bound by memory, the product by the clock that the card holds under it: 8192 x 1280 x 5120 takes the same time on 160 CUs (256 x 256 tiles) as on all 256 (256 x 160), at 1.75 GHz
-// from the busy cycles.  Measured (us in a graph): 8192 x 8192 x 8192 bf16 409 (2.7 PF; registers alone reach 4.1 to 4.4), 8192 x 5120 x 1280 59, 2048 x 10240 x 1280 33.5, 154 x 5120 x 1280 5.7;
+// The rounding is bound by memory.  The product, over 8192 k, by the matrix units at the clock that the card holds under them (82 % of the busy cycles of the CUs at 1.6 GHz); over 1280 k by
+// tiles that begin and end every ten blocks, while nothing else runs on their CU (46 to 53 % busy; 76 % over 5120 k on 160 CUs), at 1.75 to 1.85 GHz: 8192 x 1280 x 5120 takes the same time on 160 CUs
+// (256 x 256 tiles) as on all 256 (256 x 160).  Measured (us in a graph): 8192 x 8192 x 8192 bf16 393 to 409 (2.7 PF; registers alone reach 4.1 to 4.4), 8192 x 5120 x 1280 59 to 61,
+// 2048 x 10240 x 1280 33.5 to 34.4, 154 x 5120 x 1280 5.7; fp32 8192 x 8192 x 8192 865 (1.27 PF), 8192 x 5120 x 1280 112, 8192 x 1280 x 1280 35.6 (bf16 20.3);
 // rounding 8192 x 5120 bf16 in both orders with its sums 37.5 (168 MB, 4.5 TB/s), 2048 x 1280 along rows 3.7 (a launch of 32 tiles, which turns them too, 5.4).  Tried and left out: four waves on 256 x 320 (the sums no longer fit the
 // accumulation registers and are moved about: 2.3 us a block of k for 1.25 of instructions), stages of half a block in deeper rings (8192 x 8192 x 8192 620), 256 x 128 tiles (490).
 //
@@ -489,7 +491,7 @@ template <int IODT, typename T, bool FINE> __device__ __forceinline__ void block
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(half, MT + j), whole(half, i), acc[i][j], 0, 0, 0, (int)scale[MT + j], 0, (int)scale[i]);
     } else {
       typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-      auto wide = [&](int g, int part) {     // eight values, scaled
+      auto wide = [&](int g, int part) {     // eight values, scaled (once for a half, whatever the products it enters: 128 conversions beside 32 products of a 128 x 128 tile's block)
         const float s = __builtin_bit_cast(float, (scale[g] & 255u) << 23);
         u32x4 w;
 #pragma unroll
